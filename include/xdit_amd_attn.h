@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define XDIT_ATTN_ABI_VERSION 8
+#define XDIT_ATTN_ABI_VERSION 9
 
 typedef enum {
   XDIT_OK = 0,
@@ -410,6 +410,102 @@ int xdit_qk_prologue(const xdit_prologue_args* args);
  * kernels).  All jobs share dtype and stream; XDIT_NORM_TOKEN jobs cannot be batched.
  */
 int xdit_qk_prologue_batch(const xdit_prologue_args* jobs, int32_t count);
+
+/* ---- around the attention call: the rest of a DiT block ------------------------------------------ */
+
+/*
+ * Norms before and after a block fused with its gate and residual scale.  Rows are (b, s), columns C:
+ *     v = y | rms(y) | layer(y), times y_weight                    (y_norm)
+ *     h = x + residual_scale * gate * v                            (y == NULL: h = x)
+ *     n = (rms(h) | layer(h)) * weight + bias, times (1 + scale), plus shift   (norm)
+ * with layer(h) = (h - mean) / sqrt(var + eps) and rms(h) = h / sqrt(mean(h^2) + eps) over C.  What is NULL is
+ * left out.  Everything is computed in fp32 from the inputs; h and n are rounded once, n from the unrounded h.
+ * `fp8 != 0`: n is written as e4m3 bytes with one fp32 scale per block of 128 columns of a row, as
+ * xdit_fp8_block_quant would quantise the unrounded n; n_scale[kb * B*S + b*S + s] holds the scale of columns
+ * [128 kb, 128 kb + 128).  `stats` (optional) receives (mean, 1/deviation) of h and of y, four floats a row
+ * (0 and 1 for a norm that is absent; an RMS norm's mean is 0): what the backward call reads.
+ * gate, scale and shift are (B, 1 or S, C): s stride 0 for one row per batch entry.  C: a multiple of 8, at most 8192.
+ * h may be NULL (not wanted) and may be x or y themselves; n may be x or y.  norm == XDIT_ROWNORM_NONE: n is not written.
+ * Replaces: the AdaLayerNormZero modulation, the gated residual addition and the sandwich norms that diffusers'
+ * transformer blocks run around the processors of xfuser/model_executor/models/transformers/ as separate kernels.
+ */
+enum xdit_rownorm { XDIT_ROWNORM_NONE = 0, XDIT_ROWNORM_RMS = 1, XDIT_ROWNORM_LAYER = 2 };
+
+typedef struct {
+  int64_t b, s;                /* element strides of a (B, S, C) tensor; the C stride is 1 */
+} xdit_row_strides;
+
+typedef struct {
+  uint32_t struct_size;        /* = sizeof(xdit_gated_norm_args) */
+  int32_t dtype;               /* x, y, h, n: bf16, fp16 or fp32 */
+  int32_t mod_dtype;           /* gate, scale, shift: dtype or fp32 */
+  int32_t weight_dtype;        /* weight, bias, y_weight: dtype or fp32 */
+  int32_t norm, y_norm;        /* xdit_rownorm */
+  int32_t fp8;
+  int32_t B, C;
+  float eps, y_eps, residual_scale;
+  int64_t S;
+  const void* x;
+  const void* y;               /* may be NULL */
+  void* h;                     /* may be NULL */
+  void* n;
+  float* n_scale;              /* fp8 only */
+  float* stats;                /* (B,S,4) contiguous, may be NULL */
+  const void* gate;            /* each may be NULL */
+  const void* scale;
+  const void* shift;
+  const void* weight;
+  const void* bias;
+  const void* y_weight;
+  xdit_row_strides x_stride, y_stride, h_stride, n_stride, gate_stride, scale_stride, shift_stride;
+  void* stream;
+} xdit_gated_norm_args;
+
+int xdit_gated_norm(const xdit_gated_norm_args* args);
+
+/*
+ * Gradients of xdit_gated_norm from dh and dn (either may be NULL), the h, y and stats of the forward call and its
+ * parameters.  dx is the gradient of x (and the running gradient of the residual stream).  dgate / dscale / dshift have the
+ * forms of gate / scale / shift (contiguous, one row per batch entry or per token; scale and shift must agree in that),
+ * dweight, dbias and dy_weight have C entries; each output may be NULL.  Column sums are taken in fp32 in a fixed order.
+ * `workspace`: xdit_gated_norm_backward_workspace_bytes(args) bytes, 16-byte aligned, private to the stream until the
+ * call's kernels finish (0 bytes where no column sum is asked for).
+ */
+typedef struct {
+  uint32_t struct_size;        /* = sizeof(xdit_gated_norm_backward_args) */
+  int32_t dtype, mod_dtype, weight_dtype;
+  int32_t norm, y_norm;
+  int32_t gate_per_token, mod_per_token;   /* != 0: gate (scale and shift) have a row per token */
+  int32_t B, C;
+  float residual_scale;
+  int32_t reserved0;
+  int64_t S;
+  const void* dh;
+  const void* dn;
+  const void* h;
+  const void* y;
+  const float* stats;
+  const void* gate;
+  const void* scale;
+  const void* weight;
+  const void* bias;
+  const void* y_weight;
+  void* dx;
+  void* dy;
+  void* dgate;
+  void* dscale;
+  void* dshift;
+  void* dweight;
+  void* dbias;
+  void* dy_weight;
+  xdit_row_strides dh_stride, dn_stride, h_stride, y_stride, gate_stride, scale_stride, dx_stride, dy_stride;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} xdit_gated_norm_backward_args;
+
+int64_t xdit_gated_norm_backward_workspace_bytes(const xdit_gated_norm_backward_args* args);
+int xdit_gated_norm_backward(const xdit_gated_norm_backward_args* args);
 
 /* Message of the last error on the calling thread ("" if none). Never NULL. */
 const char* xdit_attn_last_error(void);

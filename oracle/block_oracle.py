@@ -1,0 +1,137 @@
+"""Float64 restatement of the operators around the attention call of a DiT block, from their formulas.
+
+Every function takes tensors of any floating dtype and returns float64 results (unrounded: what a kernel
+rounds once at its end), together with the magnitudes that its rounding errors scale with where a test needs them.
+"""
+import torch
+
+
+def _d(t):
+    return None if t is None else t.double()
+
+
+def _tokens(m):
+    """(B, C) modulation -> (B, 1, C)."""
+    return None if m is None else (m.double()[:, None] if m.ndim == 2 else m.double())
+
+
+def row_norm(x, kind, eps):
+    """-> normed x, mean (zero for "rms"), 1 / deviation, over the last dimension."""
+    mean = x.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(x[..., :1])
+    r = 1.0 / torch.sqrt((x - mean).pow(2).mean(-1, keepdim=True) + eps)
+    return (x - mean) * r, mean, r
+
+
+def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=None, norm="layer", eps=1e-6, y_norm=None,
+               y_weight=None, y_eps=1e-6, residual_scale=1.0):
+    """-> h, n, stats (B,S,4), and a row-wise size of the terms n is made of."""
+    x, y = _d(x), _d(y)
+    ym, yr = torch.zeros_like(x[..., :1]), torch.ones_like(x[..., :1])
+    h, terms = x, x.abs()
+    if y is not None:
+        v = y
+        if y_norm is not None:
+            v, ym, yr = row_norm(y, y_norm, y_eps)
+        if y_weight is not None:
+            v = v * _d(y_weight)
+        if gate is not None:
+            v = v * _tokens(gate)
+        h = x + residual_scale * v
+        terms = terms + abs(residual_scale) * v.abs()
+    if norm is None:
+        return h, None, torch.cat([torch.zeros_like(ym), torch.ones_like(yr), ym, yr], -1), terms
+    n, m, r = row_norm(h, norm, eps)
+    size = terms.amax(-1, keepdim=True) * r
+    if weight is not None:
+        n, size = n * _d(weight), size * _d(weight).abs()
+    if bias is not None:
+        n, size = n + _d(bias), size + _d(bias).abs()
+    if scale is not None:
+        n, size = n * (1 + _tokens(scale)), size * (1 + _tokens(scale).abs())
+    if shift is not None:
+        n, size = n + _tokens(shift), size + _tokens(shift).abs()
+    return h, n, torch.cat([m, r, ym, yr], -1), size
+
+
+def gated_norm_backward(dh, dn, h, stats, y=None, gate=None, scale=None, shift=None, weight=None, bias=None, norm="layer", y_norm=None,
+                        y_weight=None, residual_scale=1.0):
+    """-> gradients, and for each the size of the terms it is the sum of."""
+    h = _d(h)
+    B, S, C = h.shape
+    m, r, ym, yr = stats.double().split(1, -1)
+    t = torch.zeros_like(h) if dh is None else _d(dh)
+    size = t.abs()
+    g, big = {}, {}
+
+    def put(name, like, terms, elementwise):
+        """Sums `terms` over the rows that share an entry of `like`."""
+        if like is None:
+            return
+        if elementwise:
+            g[name], big[name] = terms, terms.abs()
+            return
+        dims = (0, 1) if like.ndim == 1 else (1,)
+        g[name], big[name] = terms.sum(dims).view(like.shape), terms.abs().sum(dims).view(like.shape)
+
+    def per_token(m):
+        return m is not None and m.ndim == 3 and m.shape[1] == S and S > 1
+
+    if dn is not None:
+        dn = _d(dn)
+        u = (h - m) * r
+        us = (h.abs() + m.abs()) * r
+        w = 1.0 if weight is None else _d(weight)
+        b = 0.0 if bias is None else _d(bias)
+        one = 1.0 if scale is None else 1 + _tokens(scale)
+        put("dshift", shift, dn, per_token(shift))
+        put("dscale", scale, dn * (u * w + b), per_token(scale))
+        if scale is not None:   # the sum is formed as w * sum(dn u) + b * sum(dn)
+            s2 = dn.abs() * (us * abs(w) + abs(b))
+            big["dscale"] = s2 if per_token(scale) else s2.sum(1).view(scale.shape)
+        put("dweight", weight, dn * one * u, False)
+        if weight is not None:
+            big["dweight"] = (dn * one * us).abs().sum((0, 1))
+        put("dbias", bias, dn * one + torch.zeros_like(h), False)
+        du = dn * one * w
+        dot = (du * u).mean(-1, keepdim=True)
+        flat = du.mean(-1, keepdim=True) if norm == "layer" else 0.0
+        t = t + r * (du - flat - u * dot)
+        size = size + r * (du.abs() + du.abs().mean(-1, keepdim=True) + us * (du.abs() * us).mean(-1, keepdim=True))
+    g["dx"], big["dx"] = t, size
+    if y is not None:
+        z = (_d(y) - ym) * yr
+        zs = (_d(y).abs() + ym.abs()) * yr
+        yw = 1.0 if y_weight is None else _d(y_weight)
+        ga = 1.0 if gate is None else _tokens(gate)
+        put("dgate", gate, residual_scale * t * z * yw, per_token(gate))
+        if gate is not None:
+            s2 = (residual_scale * size * zs * yw).abs()
+            big["dgate"] = s2 if per_token(gate) else s2.sum(1).view(gate.shape)
+        e = residual_scale * ga * t
+        put("dy_weight", y_weight, e * z, False)
+        if y_weight is not None:
+            big["dy_weight"] = (residual_scale * ga * size * zs).abs().sum((0, 1))
+        e = e * yw
+        es = (residual_scale * ga * yw * size).abs() if isinstance(ga, torch.Tensor) or isinstance(yw, torch.Tensor) else abs(residual_scale) * size
+        if y_norm is not None:
+            dot = (e * z).mean(-1, keepdim=True)
+            flat = e.mean(-1, keepdim=True) if y_norm == "layer" else 0.0
+            e = yr * (e - flat - z * dot)
+            es = yr * (es + es.mean(-1, keepdim=True) + zs * (es * zs).mean(-1, keepdim=True))
+        g["dy"], big["dy"] = e, es
+    return g, big
+
+
+def block_scales(x, rows):
+    """Exact scale of every rows x 128 block of (M, K)."""
+    M, K = x.shape
+    mb, kb = -(-M // rows), -(-K // 128)
+    p = torch.zeros(mb * rows, kb * 128, dtype=torch.float64, device=x.device)
+    p[:M, :K] = x.double().abs()
+    top = p.view(mb, rows, kb, 128).amax((1, 3))
+    return torch.where(top > 0, (top / 448.0).clamp(min=2.0 ** -126), torch.ones_like(top))
+
+
+def spread(scale, rows, M, K):
+    """Block scales -> one per element of (M, K)."""
+    return scale.repeat_interleave(rows, 0)[:M].repeat_interleave(128, 1)[:, :K]

@@ -9,7 +9,7 @@ import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libxdit_amd_attn.so")
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 XDIT_OK = 0
 XDIT_ERR_INVALID_ARG = -1
@@ -193,10 +193,38 @@ class PrologueArgs(ctypes.Structure):
     ]
 
 
+class RowStrides(ctypes.Structure):
+    _fields_ = [("b", ctypes.c_int64), ("s", ctypes.c_int64)]
+
+
+class GatedNormArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", ctypes.c_uint32)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "mod_dtype", "weight_dtype", "norm", "y_norm", "fp8", "B", "C")]
+                + [(n, ctypes.c_float) for n in ("eps", "y_eps", "residual_scale")]
+                + [("S", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("x", "y", "h", "n", "n_scale", "stats", "gate", "scale", "shift", "weight", "bias", "y_weight")]
+                + [(n + "_stride", RowStrides) for n in ("x", "y", "h", "n", "gate", "scale", "shift")]
+                + [("stream", ctypes.c_void_p)])
+
+
+class GatedNormBackwardArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", ctypes.c_uint32)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "mod_dtype", "weight_dtype", "norm", "y_norm", "gate_per_token", "mod_per_token", "B", "C")]
+                + [("residual_scale", ctypes.c_float), ("reserved0", ctypes.c_int32), ("S", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("dh", "dn", "h", "y", "stats", "gate", "scale", "weight", "bias", "y_weight",
+                                                  "dx", "dy", "dgate", "dscale", "dshift", "dweight", "dbias", "dy_weight")]
+                + [(n + "_stride", RowStrides) for n in ("dh", "dn", "h", "y", "gate", "scale", "dx", "dy")]
+                + [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
+
+
+ROWNORM_NONE, ROWNORM_RMS, ROWNORM_LAYER = 0, 1, 2
+
 NORM_NONE, NORM_HEAD, NORM_TOKEN = 0, 1, 2
 ROPE_NONE, ROPE_INTERLEAVED, ROPE_SPLIT_HALF, ROPE_WAN = 0, 1, 2, 3
 
-EXPORTS = ("xdit_attn_fwd", "xdit_attn_fwd_two_queries", "xdit_attn_fwd_noalloc", "xdit_attn_fwd_accumulate", "xdit_attn_workspace_bytes", "xdit_attn_launch_plan", "xdit_lse_merge", "xdit_fp8_quant", "xdit_fp8_quant_batch", "xdit_qk_prologue", "xdit_qk_prologue_batch", "xdit_attn_last_error", "xdit_attn_abi_version")
+EXPORTS = ("xdit_attn_fwd", "xdit_attn_fwd_two_queries", "xdit_attn_fwd_noalloc", "xdit_attn_fwd_accumulate", "xdit_attn_workspace_bytes", "xdit_attn_launch_plan", "xdit_lse_merge", "xdit_fp8_quant", "xdit_fp8_quant_batch", "xdit_qk_prologue", "xdit_qk_prologue_batch",
+           "xdit_gated_norm", "xdit_gated_norm_backward", "xdit_gated_norm_backward_workspace_bytes",
+           "xdit_attn_last_error", "xdit_attn_abi_version")
 
 _lib = None
 _lock = threading.Lock()
@@ -238,6 +266,11 @@ def lib():
         L.xdit_qk_prologue.restype = ctypes.c_int
         L.xdit_qk_prologue_batch.argtypes = [ctypes.POINTER(PrologueArgs), ctypes.c_int32]
         L.xdit_qk_prologue_batch.restype = ctypes.c_int
+        for name, args, result in (("xdit_gated_norm", GatedNormArgs, ctypes.c_int),
+                                   ("xdit_gated_norm_backward", GatedNormBackwardArgs, ctypes.c_int),
+                                   ("xdit_gated_norm_backward_workspace_bytes", GatedNormBackwardArgs, ctypes.c_int64)):
+            f = getattr(L, name)
+            f.argtypes, f.restype = [ctypes.POINTER(args)], result
         L.xdit_attn_last_error.argtypes = []
         L.xdit_attn_last_error.restype = ctypes.c_char_p
         L.xdit_attn_abi_version.argtypes = []

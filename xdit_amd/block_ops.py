@@ -1,0 +1,254 @@
+"""Tensor-level entry points of the operators around the attention call of a DiT block: the norms with
+their modulation, gate and residual, forward and backward.
+
+Hidden states are (B, S, C) with any B and S strides (multiples of 16 bytes) and a unit C stride; PyTorch is
+used for device memory and the current stream only.  Argument structs are kept per call signature and thread,
+as those of `ops.attn_fwd` are.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import _RETIRED, _PLANS_MAX, _TLS, _code, _on_device, _sig, _stream, _stream_lock
+
+_ROWNORM = {None: _lib.ROWNORM_NONE, "rms": _lib.ROWNORM_RMS, "layer": _lib.ROWNORM_LAYER}
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_SCRATCH = {}
+
+
+def _scratch(device, stream, nbytes):
+    """Scratch of the calls of one (device, stream), which are ordered; taken under the stream's lock.  One that a call
+    has outgrown stays allocated: a graph captured on the stream may hold its address."""
+    buf = _SCRATCH.get((device, stream))
+    if buf is None or buf.numel() < nbytes:
+        if buf is not None:
+            _RETIRED.append(buf)
+        buf = _SCRATCH[(device, stream)] = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+    return buf.data_ptr()
+
+
+def _plan(key, build):
+    plans = _TLS.__dict__.setdefault("plans", {})
+    plan = plans.get(key)
+    if plan is None:
+        plan = build()
+        if len(plans) >= _PLANS_MAX:
+            plans.clear()
+        plans[key] = plan
+    return plan
+
+
+def _check(name, t, shape, dtypes, device):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError("%s must be a tensor" % name)
+    if t.device != device:
+        raise ValueError("%s is on %s, expected %s" % (name, t.device, device))
+    if not t.is_cuda:
+        raise RuntimeError("%s is not on a GPU: the kernels are HIP-only, there is no CPU path" % name)
+    if t.dtype not in dtypes:
+        raise ValueError("%s has dtype %s, expected one of %s" % (name, t.dtype, ", ".join(str(d) for d in dtypes)))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.ndim and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError("%s must have a unit stride over its last dimension" % name)
+
+
+def _hidden(x):
+    if not isinstance(x, torch.Tensor) or x.ndim != 3:
+        raise ValueError("hidden states must be a 3-D tensor (B, S, C)")
+    _check("hidden states", x, None, _FLOATS, x.device)
+    return x.shape
+
+
+def _rows(t):
+    return _lib.RowStrides(t.stride(0), t.stride(1))
+
+
+def _mod(name, t, B, S, C, dtype, device):
+    """A modulation tensor (B or 1, S or 1, C) or (B or 1, C) -> (row strides, whether it has a row per token)."""
+    _check(name, t, None, (dtype, torch.float32), device)
+    s = t.shape
+    if t.ndim not in (2, 3) or s[-1] != C or s[0] not in (B, 1) or (t.ndim == 3 and s[1] not in (S, 1)):
+        raise ValueError("%s has shape %s, expected (%d or 1, [%d or 1,] %d)" % (name, tuple(s), B, S, C))
+    per_token = t.ndim == 3 and s[1] == S and S > 1
+    return _lib.RowStrides(t.stride(0) if s[0] > 1 else 0, t.stride(1) if per_token else 0), per_token
+
+
+def _shared(name, tensors, dtype):
+    """The one dtype of those of `tensors` that are given (`dtype` if none is)."""
+    found = {t.dtype for t in tensors if t is not None}
+    if len(found) > 1:
+        raise ValueError("%s must share a dtype" % name)
+    return found.pop() if found else dtype
+
+
+def _norm_code(name, kind):
+    try:
+        return _ROWNORM[kind]
+    except (KeyError, TypeError):
+        raise ValueError("%s must be None, 'rms' or 'layer'" % name) from None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=None, norm="layer", eps=1e-6, y_norm=None,
+               y_weight=None, y_eps=1e-6, residual_scale=1.0, fp8=False, return_stats=False, out_h=None):
+    """The residual addition behind a block and the modulated norm in front of the next one, in one pass -> (h, n):
+
+        v = y, or its "rms" / "layer" norm times y_weight        (`y_norm`)
+        h = x + residual_scale * gate * v                        (x itself where y is None)
+        n = norm(h) * weight + bias, times (1 + scale), plus shift
+
+    x, y: (B, S, C), bf16 / fp16 / fp32, C a multiple of 8 up to 8192.  gate, scale, shift: (B, C), (B, 1, C) or one row per
+    token (B, S, C); weight, bias, y_weight: (C,); each in x's dtype or fp32, or None.  `norm` None leaves out n (returned as
+    None).  All arithmetic is fp32, h and n are rounded once.  `fp8`: n is a pair (e4m3 tensor, scales (B, S, ceil(C / 128))
+    fp32), what `fp8_block_quant` makes of the unrounded n.  `return_stats` appends the (B, S, 4) fp32 statistics that
+    `gated_norm_backward` takes.  `out_h` receives h (it may be x: the residual stream is then updated in place)."""
+    B, S, C = _hidden(x)
+    device, dtype = x.device, x.dtype
+    key = ("gnorm", _sig(x), _sig(y), _sig(gate), _sig(scale), _sig(shift), _sig(weight), _sig(bias), _sig(y_weight), _sig(out_h), norm, y_norm, fp8,
+           eps, y_eps, residual_scale)
+
+    def build():
+        a = _lib.GatedNormArgs()
+        a.struct_size = ctypes.sizeof(a)
+        a.dtype = _code(dtype)
+        a.mod_dtype = _code(_shared("gate, scale and shift", (gate, scale, shift), dtype))
+        a.weight_dtype = _code(_shared("weight, bias and y_weight", (weight, bias, y_weight), dtype))
+        a.norm, a.y_norm, a.fp8 = _norm_code("norm", norm), _norm_code("y_norm", y_norm), 1 if fp8 else 0
+        a.B, a.S, a.C = B, S, C
+        a.eps, a.y_eps, a.residual_scale = float(eps), float(y_eps), float(residual_scale)
+        a.x_stride = _rows(x)
+        if y is not None:
+            _check("y", y, x.shape, (dtype,), device)
+            a.y_stride = _rows(y)
+        elif gate is not None or y_weight is not None or y_norm is not None:
+            raise ValueError("gate, y_weight and y_norm need y")
+        if norm is None and (fp8 or any(t is not None for t in (scale, shift, weight, bias))):
+            raise ValueError("fp8, scale, shift, weight and bias need a norm")
+        for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+            if t is not None:
+                setattr(a, name + "_stride", _mod(name, t, B, S, C, dtype, device)[0])
+        for name, t in (("weight", weight), ("bias", bias), ("y_weight", y_weight)):
+            if t is not None:
+                _check(name, t, (C,), (dtype, torch.float32), device)
+        if out_h is not None:
+            _check("out_h", out_h, x.shape, (dtype,), device)
+        a.h_stride = _lib.RowStrides(S * C, C) if out_h is None else _rows(out_h)
+        a.n_stride = _lib.RowStrides(S * C, C)
+        return a
+
+    a = _plan(key, build)
+    h = out_h
+    if h is None:
+        h = x if y is None else torch.empty((B, S, C), dtype=dtype, device=device)
+    n = n_scale = stats = None
+    if norm is not None:
+        n = torch.empty((B, S, C), dtype=torch.float8_e4m3fn if fp8 else dtype, device=device)
+    if fp8:
+        n_scale = torch.empty(((C + 127) // 128, B, S), dtype=torch.float32, device=device)
+    if return_stats:
+        stats = torch.empty((B, S, 4), dtype=torch.float32, device=device)
+    if B * S * C and (y is not None or norm is not None or out_h is not None):
+        a.x, a.y, a.n = x.data_ptr(), _ptr(y), _ptr(n)
+        a.h = h.data_ptr() if y is not None or out_h is not None else None
+        a.n_scale, a.stats = _ptr(n_scale), _ptr(stats)
+        a.gate, a.scale, a.shift, a.weight, a.bias, a.y_weight = _ptr(gate), _ptr(scale), _ptr(shift), _ptr(weight), _ptr(bias), _ptr(y_weight)
+        a.stream = _stream(device)
+        with _on_device(device):
+            rc = _lib.lib().xdit_gated_norm(ctypes.byref(a))
+        if rc != 0:
+            _lib.check(rc)
+    if fp8:
+        n = (n, n_scale.permute(1, 2, 0))
+    return (h, n, stats) if return_stats else (h, n)
+
+
+def gated_norm_backward(dh, dn, h, stats, y=None, gate=None, scale=None, shift=None, weight=None, bias=None, norm="layer", y_norm=None,
+                        y_weight=None, residual_scale=1.0):
+    """Gradients of `gated_norm` from dh and dn (either may be None), its results h and stats, its y and its
+    parameters -> a dict of dx and of those of dy, dgate, dscale, dshift, dweight, dbias and dy_weight whose operand was given.
+    dgate, dscale and dshift have the shapes of gate, scale and shift (a batch dimension of 1 that was broadcast is refused:
+    expand it); scale and shift must agree on having a row per token.  Sums over rows are fp32, in a fixed order."""
+    B, S, C = _hidden(h)
+    device, dtype = h.device, h.dtype
+    key = ("gnorm_bwd", _sig(dh), _sig(dn), _sig(h), _sig(stats), _sig(y), _sig(gate), _sig(scale), _sig(shift), _sig(weight), _sig(bias), _sig(y_weight),
+           norm, y_norm, residual_scale)
+
+    def build():
+        if dh is None and dn is None:
+            raise ValueError("dh and dn are both None")
+        a = _lib.GatedNormBackwardArgs()
+        a.struct_size = ctypes.sizeof(a)
+        a.dtype = _code(dtype)
+        mod = _shared("gate, scale and shift", (gate, scale, shift), dtype)
+        wt = _shared("weight, bias and y_weight", (weight, bias, y_weight), dtype)
+        a.mod_dtype, a.weight_dtype = _code(mod), _code(wt)
+        a.norm, a.y_norm = _norm_code("norm", norm), _norm_code("y_norm", y_norm)
+        a.B, a.S, a.C = B, S, C
+        a.residual_scale = float(residual_scale)
+        _check("stats", stats, (B, S, 4), (torch.float32,), device)
+        if not stats.is_contiguous():
+            raise ValueError("stats must be contiguous")
+        for name, t in (("dh", dh), ("dn", dn), ("y", y)):
+            if t is not None:
+                _check(name, t, h.shape, (dtype,), device)
+                setattr(a, name + "_stride", _rows(t))
+        a.h_stride = _rows(h)
+        if dn is not None and norm is None:
+            raise ValueError("dn needs a norm")
+        if y is None and (gate is not None or y_weight is not None or y_norm is not None):
+            raise ValueError("gate, y_weight and y_norm need y")
+        per = {}
+        for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+            if t is not None:
+                strides, per[name] = _mod(name, t, B, S, C, dtype, device)
+                if t.shape[0] != B:
+                    raise ValueError("%s is broadcast over the batch: expand it, its gradient has a row per batch entry" % name)
+                if name != "shift":
+                    setattr(a, name + "_stride", strides)
+        if "scale" in per and "shift" in per and per["scale"] != per["shift"]:
+            raise ValueError("scale and shift must both have a row per token or neither")
+        a.gate_per_token = 1 if per.get("gate") else 0
+        a.mod_per_token = 1 if per.get("scale") or per.get("shift") else 0
+        for name, t in (("weight", weight), ("bias", bias), ("y_weight", y_weight)):
+            if t is not None:
+                _check(name, t, (C,), (dtype, torch.float32), device)
+        a.dx_stride = a.dy_stride = _lib.RowStrides(S * C, C)
+        outs = [("dx", (B, S, C), dtype)]
+        if y is not None:
+            outs.append(("dy", (B, S, C), dtype))
+            outs += [("dgate", tuple(gate.shape), mod)] if gate is not None else []
+            outs += [("dy_weight", (C,), wt)] if y_weight is not None else []
+        if dn is not None:
+            outs += [("d" + name, tuple(t.shape), mod) for name, t in (("scale", scale), ("shift", shift)) if t is not None]
+            outs += [("d" + name, (C,), wt) for name, t in (("weight", weight), ("bias", bias)) if t is not None]
+        for name, _, _ in outs:
+            setattr(a, name, 16)   # any aligned address: the size of the workspace depends on which outputs there are
+        with _on_device(device):
+            need = _lib.lib().xdit_gated_norm_backward_workspace_bytes(ctypes.byref(a)) if B * S * C else 0
+        if need < 0:
+            _lib.check(need)
+        return a, outs, need
+
+    a, outs, need = _plan(key, build)
+    result = {name: torch.empty(shape, dtype=dt, device=device) for name, shape, dt in outs}
+    if B * S * C == 0:
+        for t in result.values():
+            t.zero_()
+        return result
+    for name, t in result.items():
+        setattr(a, name, t.data_ptr())
+    a.dh, a.dn, a.h, a.y, a.stats = _ptr(dh), _ptr(dn), h.data_ptr(), _ptr(y), stats.data_ptr()
+    a.gate, a.scale, a.weight, a.bias, a.y_weight = _ptr(gate), _ptr(scale), _ptr(weight), _ptr(bias), _ptr(y_weight)
+    a.stream = stream = _stream(device)
+    with _stream_lock(device, stream), _on_device(device):
+        if need:
+            a.workspace, a.workspace_bytes = _scratch(device, stream, need), need
+        rc = _lib.lib().xdit_gated_norm_backward(ctypes.byref(a))
+    if rc != 0:
+        _lib.check(rc)
+    return result

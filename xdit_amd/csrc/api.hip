@@ -9,6 +9,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "api_error.h"
 #include "attn_split.h"
 #include "launchers.h"
 #include "resident_walk.h"
@@ -309,6 +310,20 @@ int fill_quant(const xdit_quant_args* a, xdit::QuantParams& p) {
 }
 
 }  // namespace
+
+namespace xdit {
+
+void api_clear_error() { g_err[0] = 0; }
+
+int api_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+}  // namespace xdit
 
 extern "C" {
 

@@ -1,0 +1,176 @@
+// C ABI of the operators around the attention call: argument validation and launch.
+// Nothing here allocates device memory or synchronises; every launch goes to the caller's stream.
+#include "../../include/xdit_amd_attn.h"
+
+#include <cmath>
+#include <cstring>
+
+#include "api_error.h"
+#include "block_params.h"
+
+namespace {
+
+using xdit::api_fail;
+
+bool multiple_of(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+bool float_dtype(int d) { return d == XDIT_DTYPE_BF16 || d == XDIT_DTYPE_FP16 || d == XDIT_DTYPE_FP32; }
+int size_of(int d) { return d == XDIT_DTYPE_FP32 ? 4 : 2; }
+
+// A (B, S, C) tensor whose rows are read or written 8 elements at a time.  `written`: rows must not overlap.
+int check_rows(const char* name, const void* p, const xdit_row_strides& st, int esize, int64_t B, int64_t S, int64_t C, bool written) {
+  if (p == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "%s is NULL", name);
+  const unsigned align = esize == 1 ? 8 : 16;
+  const int64_t m = align / esize;
+  if (!multiple_of(p, align)) return api_fail(XDIT_ERR_INVALID_ARG, "%s is not %u-byte aligned", name, align);
+  if ((B > 1 && st.b % m) || (S > 1 && st.s % m))
+    return api_fail(XDIT_ERR_INVALID_ARG, "%s: strides (%lld,%lld) must be multiples of %lld elements", name, (long long)st.b, (long long)st.s, (long long)m);
+  if (st.b < 0 || st.s < 0) return api_fail(XDIT_ERR_INVALID_ARG, "%s: negative stride", name);
+  if (written && ((S > 1 && st.s < C) || (B > 1 && st.b < C)))
+    return api_fail(XDIT_ERR_INVALID_ARG, "%s: strides (%lld,%lld) make its rows of %lld overlap", name, (long long)st.b, (long long)st.s, (long long)C);
+  return 0;
+}
+
+int check_vector(const char* name, const void* p) {
+  if (p != nullptr && !multiple_of(p, 16)) return api_fail(XDIT_ERR_INVALID_ARG, "%s is not 16-byte aligned", name);
+  return 0;
+}
+
+// What both directions of the gated norm share.
+int check_norm_problem(int dtype, int mod_dtype, int weight_dtype, int norm, int y_norm, int B, int C, int64_t S, float alpha) {
+  if (!float_dtype(dtype)) return api_fail(XDIT_ERR_INVALID_ARG, "dtype %d must be bf16, fp16 or fp32", dtype);
+  if (mod_dtype != dtype && mod_dtype != XDIT_DTYPE_FP32) return api_fail(XDIT_ERR_INVALID_ARG, "mod_dtype %d must be dtype or fp32", mod_dtype);
+  if (weight_dtype != dtype && weight_dtype != XDIT_DTYPE_FP32) return api_fail(XDIT_ERR_INVALID_ARG, "weight_dtype %d must be dtype or fp32", weight_dtype);
+  if (norm < XDIT_ROWNORM_NONE || norm > XDIT_ROWNORM_LAYER || y_norm < XDIT_ROWNORM_NONE || y_norm > XDIT_ROWNORM_LAYER)
+    return api_fail(XDIT_ERR_INVALID_ARG, "unknown norm %d or y_norm %d", norm, y_norm);
+  if (B <= 0 || S <= 0 || C <= 0) return api_fail(XDIT_ERR_INVALID_ARG, "B, S, C must be positive");
+  if (B > 65535 || S > (int64_t(1) << 30) || B * S > 0x7fffffffLL) return api_fail(XDIT_ERR_INVALID_ARG, "too many rows for one launch");
+  if (C % 8 != 0 || C > xdit::kNormMaxC) return api_fail(XDIT_ERR_UNSUPPORTED, "C = %d: need a multiple of 8, at most %d", C, xdit::kNormMaxC);
+  if (!std::isfinite(alpha)) return api_fail(XDIT_ERR_INVALID_ARG, "residual_scale must be finite");
+  return 0;
+}
+
+xdit::RowStrides rs(const xdit_row_strides& s) { return {s.b, s.s}; }
+
+}  // namespace
+
+extern "C" {
+
+int xdit_gated_norm(const xdit_gated_norm_args* a) {
+  xdit::api_clear_error();
+  if (a == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "args is NULL");
+  if (a->struct_size != sizeof(xdit_gated_norm_args))
+    return api_fail(XDIT_ERR_INVALID_ARG, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(xdit_gated_norm_args));
+  int rc = check_norm_problem(a->dtype, a->mod_dtype, a->weight_dtype, a->norm, a->y_norm, a->B, a->C, a->S, a->residual_scale);
+  if (rc) return rc;
+  const int es = size_of(a->dtype), ms = size_of(a->mod_dtype);
+  const int64_t B = a->B, S = a->S, C = a->C;
+  if ((rc = check_rows("x", a->x, a->x_stride, es, B, S, C, false))) return rc;
+  if (a->y != nullptr && (rc = check_rows("y", a->y, a->y_stride, es, B, S, C, false))) return rc;
+  if (a->h != nullptr && (rc = check_rows("h", a->h, a->h_stride, es, B, S, C, true))) return rc;
+  if (a->y == nullptr && (a->gate != nullptr || a->y_weight != nullptr || a->y_norm != XDIT_ROWNORM_NONE))
+    return api_fail(XDIT_ERR_INVALID_ARG, "gate, y_weight and y_norm need y");
+  if (a->norm == XDIT_ROWNORM_NONE) {
+    if (a->h == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "without a norm there is only h to write, and h is NULL");
+    if (a->weight != nullptr || a->bias != nullptr || a->scale != nullptr || a->shift != nullptr || a->fp8)
+      return api_fail(XDIT_ERR_INVALID_ARG, "weight, bias, scale, shift and fp8 need a norm");
+  } else if ((rc = check_rows("n", a->n, a->n_stride, a->fp8 ? 1 : es, B, S, C, true))) {
+    return rc;
+  }
+  if (a->fp8 && a->n_scale == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "n_scale is NULL");
+  if ((a->norm != XDIT_ROWNORM_NONE && !(a->eps >= 0.f && std::isfinite(a->eps))) || (a->y_norm != XDIT_ROWNORM_NONE && !(a->y_eps >= 0.f && std::isfinite(a->y_eps))))
+    return api_fail(XDIT_ERR_INVALID_ARG, "eps must be finite and >= 0");
+  if (a->gate != nullptr && (rc = check_rows("gate", a->gate, a->gate_stride, ms, B, S, C, false))) return rc;
+  if (a->scale != nullptr && (rc = check_rows("scale", a->scale, a->scale_stride, ms, B, S, C, false))) return rc;
+  if (a->shift != nullptr && (rc = check_rows("shift", a->shift, a->shift_stride, ms, B, S, C, false))) return rc;
+  if ((rc = check_vector("weight", a->weight)) || (rc = check_vector("bias", a->bias)) || (rc = check_vector("y_weight", a->y_weight)) ||
+      (rc = check_vector("stats", a->stats)))
+    return rc;
+  xdit::GatedNormParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.x = a->x; p.y = a->y; p.h = a->h; p.n = a->n; p.n_scale = a->n_scale; p.stats = a->stats;
+  p.gate = a->gate; p.scale = a->scale; p.shift = a->shift; p.weight = a->weight; p.bias = a->bias; p.y_weight = a->y_weight;
+  p.xs = rs(a->x_stride); p.ys = rs(a->y_stride); p.hs = rs(a->h_stride); p.ns = rs(a->n_stride);
+  p.gs = rs(a->gate_stride); p.ss = rs(a->scale_stride); p.fs = rs(a->shift_stride);
+  p.B = a->B; p.S = (int)S; p.C = a->C; p.rows = B * S;
+  p.norm = a->norm; p.y_norm = a->y_norm; p.fp8 = a->fp8 != 0;
+  p.mod_wide = a->mod_dtype == XDIT_DTYPE_FP32; p.weight_wide = a->weight_dtype == XDIT_DTYPE_FP32;
+  p.eps = a->eps; p.y_eps = a->y_eps; p.alpha = a->residual_scale; p.inv_c = 1.0f / (float)C;
+  const hipError_t e = xdit::launch_gated_norm(p, a->dtype, (hipStream_t)a->stream);
+  if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "gated norm launch failed: %s", hipGetErrorString(e));
+  return XDIT_OK;
+}
+
+static int fill_norm_backward(const xdit_gated_norm_backward_args* a, xdit::GatedNormBwdParams& p, bool pointers) {
+  if (a == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "args is NULL");
+  if (a->struct_size != sizeof(xdit_gated_norm_backward_args))
+    return api_fail(XDIT_ERR_INVALID_ARG, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(xdit_gated_norm_backward_args));
+  int rc = check_norm_problem(a->dtype, a->mod_dtype, a->weight_dtype, a->norm, a->y_norm, a->B, a->C, a->S, a->residual_scale);
+  if (rc) return rc;
+  std::memset(&p, 0, sizeof(p));
+  p.dh = a->dh; p.dn = a->dn; p.h = a->h; p.y = a->y; p.stats = a->stats;
+  p.gate = a->gate; p.scale = a->scale; p.weight = a->weight; p.bias = a->bias; p.y_weight = a->y_weight;
+  p.dx = a->dx; p.dy = a->dy; p.dgate = a->dgate; p.dscale = a->dscale; p.dshift = a->dshift;
+  p.dweight = a->dweight; p.dbias = a->dbias; p.dy_weight = a->dy_weight;
+  p.dhs = rs(a->dh_stride); p.dns = rs(a->dn_stride); p.hs = rs(a->h_stride); p.ys = rs(a->y_stride);
+  p.gs = rs(a->gate_stride); p.ss = rs(a->scale_stride); p.dxs = rs(a->dx_stride); p.dys = rs(a->dy_stride);
+  p.B = a->B; p.S = (int)a->S; p.C = a->C;
+  p.norm = a->norm; p.y_norm = a->y_norm;
+  p.mod_wide = a->mod_dtype == XDIT_DTYPE_FP32; p.weight_wide = a->weight_dtype == XDIT_DTYPE_FP32;
+  p.gate_per_token = a->gate_per_token != 0; p.mod_per_token = a->mod_per_token != 0;
+  p.alpha = a->residual_scale; p.inv_c = 1.0f / (float)a->C;
+  xdit::gated_norm_bwd_plan(p);
+  if (!pointers) return 0;
+  const int es = size_of(a->dtype), ms = size_of(a->mod_dtype);
+  const int64_t B = a->B, S = a->S, C = a->C;
+  if (a->dh == nullptr && a->dn == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "dh and dn are both NULL");
+  if (a->dh != nullptr && (rc = check_rows("dh", a->dh, a->dh_stride, es, B, S, C, false))) return rc;
+  if (a->stats == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "stats is NULL");
+  if (a->dn != nullptr) {
+    if (a->norm == XDIT_ROWNORM_NONE) return api_fail(XDIT_ERR_INVALID_ARG, "dn needs a norm");
+    if ((rc = check_rows("dn", a->dn, a->dn_stride, es, B, S, C, false))) return rc;
+    if ((rc = check_rows("h", a->h, a->h_stride, es, B, S, C, false))) return rc;
+  } else if (a->dscale != nullptr || a->dshift != nullptr || a->dweight != nullptr || a->dbias != nullptr) {
+    return api_fail(XDIT_ERR_INVALID_ARG, "dscale, dshift, dweight and dbias need dn");
+  }
+  if (a->y != nullptr) {
+    if ((rc = check_rows("y", a->y, a->y_stride, es, B, S, C, false))) return rc;
+  } else if (a->dy != nullptr || a->dgate != nullptr || a->dy_weight != nullptr) {
+    return api_fail(XDIT_ERR_INVALID_ARG, "dy, dgate and dy_weight need y");
+  }
+  if (a->dx != nullptr && (rc = check_rows("dx", a->dx, a->dx_stride, es, B, S, C, true))) return rc;
+  if (a->dy != nullptr && (rc = check_rows("dy", a->dy, a->dy_stride, es, B, S, C, true))) return rc;
+  if (a->gate != nullptr && (rc = check_rows("gate", a->gate, a->gate_stride, ms, B, a->gate_per_token ? S : 1, C, false))) return rc;
+  if (a->scale != nullptr && (rc = check_rows("scale", a->scale, a->scale_stride, ms, B, a->mod_per_token ? S : 1, C, false))) return rc;
+  if (!a->gate_per_token) p.gs.s = 0;
+  if (!a->mod_per_token) p.ss.s = 0;
+  const struct { const char* name; const void* p; } vec[] = {{"weight", a->weight}, {"bias", a->bias}, {"y_weight", a->y_weight}, {"stats", a->stats},
+      {"dgate", a->dgate}, {"dscale", a->dscale}, {"dshift", a->dshift}, {"dweight", a->dweight}, {"dbias", a->dbias}, {"dy_weight", a->dy_weight}};
+  for (const auto& v : vec)
+    if ((rc = check_vector(v.name, v.p))) return rc;
+  return 0;
+}
+
+static int64_t norm_backward_bytes(const xdit::GatedNormBwdParams& p) { return p.sums ? (int64_t)p.B * p.parts * 3 * p.C * 4 : 0; }
+
+int64_t xdit_gated_norm_backward_workspace_bytes(const xdit_gated_norm_backward_args* a) {
+  xdit::api_clear_error();
+  xdit::GatedNormBwdParams p;
+  const int rc = fill_norm_backward(a, p, false);
+  return rc ? rc : norm_backward_bytes(p);
+}
+
+int xdit_gated_norm_backward(const xdit_gated_norm_backward_args* a) {
+  xdit::api_clear_error();
+  xdit::GatedNormBwdParams p;
+  if (int rc = fill_norm_backward(a, p, true)) return rc;
+  const int64_t need = norm_backward_bytes(p);
+  if (need > 0 && (a->workspace == nullptr || !multiple_of(a->workspace, 16) || a->workspace_bytes < need))
+    return api_fail(XDIT_ERR_INVALID_ARG, "workspace of %lld bytes (16-byte aligned) is needed, %lld given", (long long)need, (long long)a->workspace_bytes);
+  p.partial = (float*)a->workspace;
+  const hipError_t e = xdit::launch_gated_norm_bwd(p, a->dtype, (hipStream_t)a->stream);
+  if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "gated norm backward launch failed: %s", hipGetErrorString(e));
+  return XDIT_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,69 @@
+// Parameters and host-side launch functions of the operators around the attention call.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace xdit {
+
+struct RowStrides { int64_t b, s; };
+
+// dtype codes are the C ABI's (0 bf16, 1 fp16, 2 fp32); norms 0 none, 1 RMS, 2 layer.
+struct GatedNormParams {
+  const void* x;
+  const void* y;
+  void* h;
+  void* n;
+  float* n_scale;
+  float* stats;
+  const void* gate;
+  const void* scale;
+  const void* shift;
+  const void* weight;
+  const void* bias;
+  const void* y_weight;
+  RowStrides xs, ys, hs, ns, gs, ss, fs;  // gs: gate, ss: scale, fs: shift
+  int B, S, C;
+  int64_t rows;  // B * S
+  int norm, y_norm, fp8;
+  int mod_wide, weight_wide;  // those parameters are fp32 beside 16-bit tensors
+  float eps, y_eps, alpha, inv_c;
+};
+
+struct GatedNormBwdParams {
+  const void* dh;
+  const void* dn;
+  const void* h;
+  const void* y;
+  const float* stats;
+  const void* gate;
+  const void* scale;
+  const void* weight;
+  const void* bias;
+  const void* y_weight;
+  void* dx;
+  void* dy;
+  void* dgate;
+  void* dscale;
+  void* dshift;
+  void* dweight;
+  void* dbias;
+  void* dy_weight;
+  RowStrides dhs, dns, hs, ys, gs, ss, dxs, dys;
+  int B, S, C;
+  int norm, y_norm;
+  int mod_wide, weight_wide;
+  int gate_per_token, mod_per_token;
+  float alpha, inv_c;
+  float* partial;     // [B][parts][3][C]: sums over the rows of a part (dn u, dn, t z), see the kernel
+  int parts;          // parts the rows of a batch entry are cut into
+  int rows_per_part;
+  int sums;           // column sums are asked for
+};
+
+constexpr int kNormMaxC = 8192;
+
+hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, hipStream_t stream);
+hipError_t launch_gated_norm_bwd(const GatedNormBwdParams& p, int dtype, hipStream_t stream);
+void gated_norm_bwd_plan(GatedNormBwdParams& p);  // fills parts, rows_per_part and sums
+
+}  // namespace xdit

@@ -1,0 +1,123 @@
+// Pieces of the row-wise kernels (norms, rotations, block quantiser): 8-element loads and stores, sums over a
+// wavefront and over a workgroup, the scale and cast of a 1 x 128 fp8 block.
+#pragma once
+#include "common.h"
+#include "fp8_cast.h"
+
+namespace xdit {
+
+// Eight consecutive elements as they are in memory (16 bytes, or 32 in fp32).
+template <typename T> struct Raw8 {
+  static constexpr int N = sizeof(T) / 2;
+  typedef __attribute__((ext_vector_type(8 / N))) T vec;
+  vec x[N];
+  __device__ __forceinline__ float operator[](int i) const { return (float)x[i / (8 / N)][i % (8 / N)]; }
+};
+template <typename T>
+__device__ __forceinline__ void get8(const Raw8<T>& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = r[i];
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const void* p, int64_t off) { return *(const Raw8<T>*)((const T*)p + off); }
+template <typename T>
+__device__ __forceinline__ void store8(void* p, int64_t off, const float (&v)[8]) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; i++) r.x[i / (8 / Raw8<T>::N)][i % (8 / Raw8<T>::N)] = (T)v[i];
+  *(Raw8<T>*)((T*)p + off) = r;
+}
+// Eight parameters held as T or as fp32 (`wide`, uniform).
+template <typename T>
+__device__ __forceinline__ void load_param8(const void* p, int64_t off, bool wide, float (&v)[8]) {
+  if (wide) get8(load_raw8<float>(p, off), v);
+  else get8(load_raw8<T>(p, off), v);
+}
+template <typename T>
+__device__ __forceinline__ void store_param8(void* p, int64_t off, bool wide, const float (&v)[8]) {
+  if (wide) store8<float>(p, off, v);
+  else store8<T>(p, off, v);
+}
+
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_bits(unsigned x) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_plus(float x) { return x + __uint_as_float(dpp_bits<CTRL>(__float_as_uint(x))); }
+// Sum over the 16 lanes of a DPP row, to all of them: quad permutes, then the half-row and row mirrors.
+__device__ __forceinline__ float row16_sum(float x) {
+  x = dpp_plus<0xB1>(x);
+  x = dpp_plus<0x4E>(x);
+  x = dpp_plus<0x141>(x);
+  return dpp_plus<0x140>(x);
+}
+// Sum over the 64 lanes, to all of them, in a fixed order.
+__device__ __forceinline__ float wave_sum(float x) {
+  x = row16_sum(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  return sum_halves(x);
+}
+// Largest of the 16 lanes' values, as bit patterns of non-negative floats: infinities above numbers, NaN above all.
+__device__ __forceinline__ unsigned row16_max(unsigned x) {
+  x = max(x, dpp_bits<0xB1>(x));
+  x = max(x, dpp_bits<0x4E>(x));
+  x = max(x, dpp_bits<0x141>(x));
+  return max(x, dpp_bits<0x140>(x));
+}
+
+// Sums of K values over the NW wavefronts of a workgroup, to every thread, with one barrier.  `part` holds K * NW floats;
+// two consecutive calls must be given different arrays (the first's readers may still be at it).
+template <int K, int NW>
+__device__ __forceinline__ void block_sums(float (&x)[K], float* part) {
+#pragma unroll
+  for (int k = 0; k < K; k++) x[k] = wave_sum(x[k]);
+  if constexpr (NW > 1) {
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; k++) part[k * NW + (threadIdx.x >> 6)] = x[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      float s = part[k * NW];
+#pragma unroll
+      for (int w = 1; w < NW; w++) s += part[k * NW + w];
+      x[k] = s;
+    }
+  }
+}
+
+// Scale of an fp8 block from the bits of its abs-max: absmax / 448, at least the smallest normal number, 1 for a block
+// of zeros; NaN and infinities pass through (a block with one of them has no finite scale).
+__device__ __forceinline__ float block_scale(unsigned amax_bits) {
+  const float s = __uint_as_float(amax_bits) / kFp8Max;
+  return amax_bits == 0 ? 1.0f : (s < 0x1p-126f ? 0x1p-126f : s);
+}
+// The largest absolute value of 8 elements, as bits.
+__device__ __forceinline__ unsigned absmax8(const float (&v)[8]) {
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+// Eight quotients as e4m3 bytes.
+__device__ __forceinline__ i32x2 cast8(const float (&v)[8], const Divider& div) {
+  float q[8];
+  if (div.plain) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) q[j] = v[j] / div.scale;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) q[j] = div(v[j]);
+  }
+  i32x2 w;
+  w[0] = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  w[0] = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w[0], true);
+  w[1] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+  w[1] = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], w[1], true);
+  return w;
+}
+
+}  // namespace xdit
