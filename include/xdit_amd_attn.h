@@ -507,6 +507,62 @@ typedef struct {
 int64_t xdit_gated_norm_backward_workspace_bytes(const xdit_gated_norm_backward_args* args);
 int xdit_gated_norm_backward(const xdit_gated_norm_backward_args* args);
 
+/*
+ * Rotary positions on several axes (time, height, width, ...) for q and k in one launch, after an optional RMSNorm over
+ * head_dim.  Pair p of the P = pairs[0] + pairs[1] + ... rotated pairs belongs to the axis whose range of `pairs` it lies in:
+ *     phi = positions[b, s, axis(p)] * inv_freq[p]
+ *     (y1, y2) = (x1 cos phi - x2 sin phi, x1 sin phi + x2 cos phi)
+ * with the pair's elements 2p and 2p + 1 (XDIT_ROPE_INTERLEAVED) or p and p + P (XDIT_ROPE_SPLIT_HALF); columns from 2P on
+ * are not rotated.  norm != 0: x is first divided by sqrt(mean(x^2) + eps) over head_dim and multiplied by `weight`.
+ * Angles are reduced in fp64, everything else is fp32, the result is rounded once.  No tables: a token's sines and cosines
+ * are computed once for all of its heads.  head_dim: a multiple of 8 up to 512; P a multiple of 4.
+ * Replaces: the position embedding modules that build (cos, sin) tables and the rotation of the processors
+ * (transformer_flux.py:146-147, transformer_hunyuan_video.py:60-83, transformer_wan.py:108-120).
+ *
+ * xdit_axes_rope_backward: dy is the gradient of the rotated tensor, y receives that of x; x (the forward call's
+ * input) is read only where norm != 0.  `dweight` (norm != 0; D entries, may be NULL) receives the sum over rows, taken in
+ * fp32 in a fixed order through `workspace` (xdit_axes_rope_backward_workspace_bytes, 16-byte aligned, private to the
+ * stream until the call's kernels finish).
+ */
+#define XDIT_ROPE_MAX_AXES 4
+
+typedef struct {
+  const void* x;               /* (B,H,S,D) */
+  const void* dy;              /* backward only */
+  void* y;                     /* may be x (forward) or dy (backward) with the same strides */
+  const void* weight;          /* may be NULL */
+  void* dweight;               /* backward only, may be NULL */
+  xdit_strides x_stride, dy_stride, y_stride;
+  int32_t H, reserved0;
+} xdit_axes_rope_tensor;
+
+typedef struct {
+  uint32_t struct_size;        /* = sizeof(xdit_axes_rope_args) */
+  int32_t dtype;               /* bf16, fp16 or fp32 */
+  int32_t weight_dtype;        /* weight, dweight: dtype or fp32 */
+  int32_t rope;                /* XDIT_ROPE_INTERLEAVED or XDIT_ROPE_SPLIT_HALF */
+  int32_t norm;
+  int32_t pos_bits;            /* positions: -32 fp32, 32 int32, 64 int64 */
+  int32_t freq_bits;           /* inv_freq: 32 fp32, 64 fp64 */
+  int32_t B, D;
+  int32_t tensors;             /* 1 or 2 of `t` are there */
+  int32_t axes;
+  int32_t pairs[XDIT_ROPE_MAX_AXES];
+  float eps;
+  int64_t S;
+  const void* positions;       /* (B, S, axes), axis stride 1 */
+  int64_t pos_stride_b, pos_stride_s;
+  const void* inv_freq;        /* P entries, radians per unit of position */
+  xdit_axes_rope_tensor t[2];  /* q and k */
+  void* workspace;             /* backward only */
+  int64_t workspace_bytes;
+  void* stream;
+} xdit_axes_rope_args;
+
+int xdit_axes_rope(const xdit_axes_rope_args* args);
+int64_t xdit_axes_rope_backward_workspace_bytes(const xdit_axes_rope_args* args);
+int xdit_axes_rope_backward(const xdit_axes_rope_args* args);
+
 /* Message of the last error on the calling thread ("" if none). Never NULL. */
 const char* xdit_attn_last_error(void);
 

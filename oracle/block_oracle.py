@@ -135,3 +135,42 @@ def block_scales(x, rows):
 def spread(scale, rows, M, K):
     """Block scales -> one per element of (M, K)."""
     return scale.repeat_interleave(rows, 0)[:M].repeat_interleave(128, 1)[:, :K]
+
+
+def turn(x, positions, inv_freq, pairs, rope, sign=1):
+    """Every pair of (B,H,S,D) columns as a complex number times exp(i sign phi)."""
+    B, H, S, D = x.shape
+    axis = torch.tensor([a for a, n in enumerate(pairs) for _ in range(n)], dtype=torch.long, device=x.device)
+    phi = sign * positions.double()[..., axis] * inv_freq.double()            # ([B,] S, P)
+    phi = phi[:, None] if phi.ndim == 3 else phi
+    P = axis.numel()
+    a, b = (x[..., 0:2 * P:2], x[..., 1:2 * P:2]) if rope == "interleaved" else (x[..., :P], x[..., P:2 * P])
+    z = torch.complex(a.contiguous(), b.contiguous()) * torch.complex(torch.cos(phi), torch.sin(phi))
+    y = x.clone()
+    if rope == "interleaved":
+        y[..., 0:2 * P:2], y[..., 1:2 * P:2] = z.real, z.imag
+    else:
+        y[..., :P], y[..., P:2 * P] = z.real, z.imag
+    return y
+
+
+def axes_rope(x, weight, positions, inv_freq, pairs, norm, eps, rope):
+    x = _d(x)
+    if norm:
+        x = row_norm(x, "rms", eps)[0]
+        x = x if weight is None else x * _d(weight)
+    return turn(x, positions, inv_freq, pairs, rope)
+
+
+def axes_rope_backward(dy, x, weight, positions, inv_freq, pairs, norm, eps, rope):
+    """-> dx, dweight, and the sizes of the terms of both."""
+    d = turn(_d(dy), positions, inv_freq, pairs, rope, -1)
+    size = _d(dy).abs().amax(-1, keepdim=True) * 1.5
+    if not norm:
+        return d, None, size, None
+    u, _, r = row_norm(_d(x), "rms", eps)
+    w = 1.0 if weight is None else _d(weight)
+    g = d * w
+    dx = r * (g - u * (g * u).mean(-1, keepdim=True))
+    top = size * (1.0 if weight is None else w.abs())
+    return dx, (d * u).sum((0, 1, 2)), r * (top + u.abs() * (top * u.abs()).mean(-1, keepdim=True)), (size * u.abs()).sum((0, 1, 2))

@@ -217,6 +217,23 @@ class GatedNormBackwardArgs(ctypes.Structure):
                 + [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
 
 
+ROPE_MAX_AXES = 4
+
+
+class AxesRopeTensor(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "dy", "y", "weight", "dweight")]
+                + [(n + "_stride", Strides) for n in ("x", "dy", "y")]
+                + [("H", ctypes.c_int32), ("reserved0", ctypes.c_int32)])
+
+
+class AxesRopeArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", ctypes.c_uint32)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "weight_dtype", "rope", "norm", "pos_bits", "freq_bits", "B", "D", "tensors", "axes")]
+                + [("pairs", ctypes.c_int32 * ROPE_MAX_AXES), ("eps", ctypes.c_float), ("S", ctypes.c_int64), ("positions", ctypes.c_void_p),
+                   ("pos_stride_b", ctypes.c_int64), ("pos_stride_s", ctypes.c_int64), ("inv_freq", ctypes.c_void_p), ("t", AxesRopeTensor * 2),
+                   ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
+
+
 ROWNORM_NONE, ROWNORM_RMS, ROWNORM_LAYER = 0, 1, 2
 
 NORM_NONE, NORM_HEAD, NORM_TOKEN = 0, 1, 2
@@ -224,6 +241,7 @@ ROPE_NONE, ROPE_INTERLEAVED, ROPE_SPLIT_HALF, ROPE_WAN = 0, 1, 2, 3
 
 EXPORTS = ("xdit_attn_fwd", "xdit_attn_fwd_two_queries", "xdit_attn_fwd_noalloc", "xdit_attn_fwd_accumulate", "xdit_attn_workspace_bytes", "xdit_attn_launch_plan", "xdit_lse_merge", "xdit_fp8_quant", "xdit_fp8_quant_batch", "xdit_qk_prologue", "xdit_qk_prologue_batch",
            "xdit_gated_norm", "xdit_gated_norm_backward", "xdit_gated_norm_backward_workspace_bytes",
+           "xdit_axes_rope", "xdit_axes_rope_backward", "xdit_axes_rope_backward_workspace_bytes",
            "xdit_attn_last_error", "xdit_attn_abi_version")
 
 _lib = None
@@ -268,7 +286,10 @@ def lib():
         L.xdit_qk_prologue_batch.restype = ctypes.c_int
         for name, args, result in (("xdit_gated_norm", GatedNormArgs, ctypes.c_int),
                                    ("xdit_gated_norm_backward", GatedNormBackwardArgs, ctypes.c_int),
-                                   ("xdit_gated_norm_backward_workspace_bytes", GatedNormBackwardArgs, ctypes.c_int64)):
+                                   ("xdit_gated_norm_backward_workspace_bytes", GatedNormBackwardArgs, ctypes.c_int64),
+                                   ("xdit_axes_rope", AxesRopeArgs, ctypes.c_int),
+                                   ("xdit_axes_rope_backward", AxesRopeArgs, ctypes.c_int),
+                                   ("xdit_axes_rope_backward_workspace_bytes", AxesRopeArgs, ctypes.c_int64)):
             f = getattr(L, name)
             f.argtypes, f.restype = [ctypes.POINTER(args)], result
         L.xdit_attn_last_error.argtypes = []

@@ -1,8 +1,9 @@
 """Tensor-level entry points of the operators around the attention call of a DiT block: the norms with
-their modulation, gate and residual, forward and backward.
+their modulation, gate and residual and the rotation of q and k by positions on several axes, forward and
+backward.
 
-Hidden states are (B, S, C) with any B and S strides (multiples of 16 bytes) and a unit C stride; PyTorch is
-used for device memory and the current stream only.  Argument structs are kept per call signature and thread,
+Hidden states are (B, S, C), q and k logical (B, H, S, D), with any outer strides (multiples of 16 bytes) and a
+unit stride over the last dimension; PyTorch is used for device memory and the current stream only.  Argument structs are kept per call signature and thread,
 as those of `ops.attn_fwd` are.
 """
 import ctypes
@@ -252,3 +253,164 @@ def gated_norm_backward(dh, dn, h, stats, y=None, gate=None, scale=None, shift=N
     if rc != 0:
         _lib.check(rc)
     return result
+
+
+def rope_frequencies(axes_dim, theta=10000.0, device=None):
+    """Frequencies of a rotation in which every axis turns its own part of head_dim, `axes_dim[a]` columns of it ->
+    (inv_freq fp64, pairs): theta ** (-2 i / axes_dim[a]) for the pairs i of axis a; `theta` may be one per axis."""
+    thetas = theta if isinstance(theta, (tuple, list)) else (theta,) * len(axes_dim)
+    if len(thetas) != len(axes_dim) or any(d % 2 or d < 0 for d in axes_dim):
+        raise ValueError("axes_dim must be even numbers, with one theta or one per axis")
+    parts = [t ** (-torch.arange(0, d, 2, dtype=torch.float64) / max(d, 1)) for d, t in zip(axes_dim, thetas)]
+    return torch.cat(parts).to(device), tuple(d // 2 for d in axes_dim)
+
+
+_ROPE = {"interleaved": _lib.ROPE_INTERLEAVED, "split_half": _lib.ROPE_SPLIT_HALF}
+_POS_BITS = {torch.float32: -32, torch.int32: 32, torch.int64: 64}
+
+
+def _bhsd(name, t, B, S, D, dtype, device):
+    if not isinstance(t, torch.Tensor) or t.ndim != 4:
+        raise ValueError("%s must be a 4-D tensor (B, H, S, D)" % name)
+    _check(name, t, (B, t.shape[1], S, D), (dtype,), device)
+    return _lib.Strides(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _rope_args(first, tensors, positions, inv_freq, pairs, norm, eps, rope):
+    """The fields that forward and backward share.  `tensors`: (name, x, dy, y, weight) of q and, if it is there, k."""
+    B, _, S, D = first.shape
+    device, dtype = first.device, first.dtype
+    if rope not in _ROPE:
+        raise ValueError("rope must be one of %s" % (sorted(_ROPE),))
+    if not 1 <= len(pairs) <= _lib.ROPE_MAX_AXES:
+        raise ValueError("between 1 and %d axes are supported" % _lib.ROPE_MAX_AXES)
+    a = _lib.AxesRopeArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.dtype, a.rope, a.norm, a.eps = _code(dtype), _ROPE[rope], 1 if norm else 0, float(eps)
+    a.weight_dtype = _code(_shared("q_weight and k_weight", [t[4] for t in tensors], dtype))
+    _check("positions", positions, None, tuple(_POS_BITS), device)
+    A = len(pairs)
+    if positions.ndim not in (2, 3) or tuple(positions.shape[-2:]) != (S, A) or (positions.ndim == 3 and positions.shape[0] not in (B, 1)):
+        raise ValueError("positions has shape %s, expected ([%d or 1,] %d, %d)" % (tuple(positions.shape), B, S, A))
+    _check("inv_freq", inv_freq, (sum(pairs),), (torch.float32, torch.float64), device)
+    a.pos_bits, a.freq_bits = _POS_BITS[positions.dtype], 64 if inv_freq.dtype == torch.float64 else 32
+    a.pos_stride_s = positions.stride(-2)
+    a.pos_stride_b = positions.stride(0) if positions.ndim == 3 and positions.shape[0] > 1 else 0
+    a.B, a.S, a.D = B, S, D
+    a.tensors, a.axes = len(tensors), A
+    for i, n in enumerate(pairs):
+        a.pairs[i] = int(n)
+    for i, (name, x, dy, y, weight) in enumerate(tensors):
+        t = a.t[i]
+        t.H = (x if x is not None else dy).shape[1]
+        for kind, v in (("x", x), ("dy", dy), ("y", y)):
+            if v is not None:
+                strides = _bhsd(name if kind == "x" else "%s of %s" % (kind, name), v, B, S, D, dtype, device)
+                if v.shape[1] != t.H:
+                    raise ValueError("%s: the tensors have %d and %d heads" % (name, v.shape[1], t.H))
+                setattr(t, kind + "_stride", strides)
+        if y is None:
+            t.y_stride = _lib.Strides(t.H * S * D, S * D, D)
+        if weight is not None:
+            if not norm:
+                raise ValueError("%s has a weight but no norm" % name)
+            _check(name + "_weight", weight, (D,), (dtype, torch.float32), device)
+    return a
+
+
+def axes_rope(q, k, positions, inv_freq, pairs, norm=False, q_weight=None, k_weight=None, eps=1e-6, rope="interleaved", out_q=None, out_k=None):
+    """Rotates q and k (logical (B, H, S, D), any strides; k may be None or have other heads than q) by positions on up to
+    four axes, after an RMSNorm over head_dim with gains `q_weight` / `k_weight` (D entries, q's dtype or fp32, or None) where
+    `norm` is set -> (q, k), new BHSD-contiguous tensors or `out_q` / `out_k` (which may be q and k themselves).
+
+    positions: (S, A) or (B, S, A), fp32, int32 or int64.  Pair p belongs to the axis whose part of `pairs` (pairs per axis) it
+    lies in and turns by position * inv_freq[p] (`rope_frequencies` makes both; sum(pairs) a multiple of 4).  `rope`: a pair is
+    the columns (2p, 2p + 1), "interleaved", or (p, p + sum(pairs)), "split_half"; columns from 2 sum(pairs) on are not rotated.
+    Angles are reduced in fp64, the rest is fp32, the result is rounded once."""
+    if not isinstance(q, torch.Tensor) or q.ndim != 4:
+        raise ValueError("q must be a 4-D tensor (B, H, S, D)")
+    device, dtype = q.device, q.dtype
+    B, H, S, D = q.shape
+    key = ("arope", _sig(q), _sig(k), _sig(positions), _sig(inv_freq), pairs, norm, _sig(q_weight), _sig(k_weight), eps, rope, _sig(out_q), _sig(out_k))
+
+    def build():
+        _check("q", q, None, _FLOATS, device)
+        if k is None and (k_weight is not None or out_k is not None):
+            raise ValueError("k_weight and out_k need k")
+        if k is not None and not isinstance(k, torch.Tensor):
+            raise ValueError("k must be a 4-D tensor (B, H, S, D)")
+        return _rope_args(q, [("q", q, None, out_q, q_weight)] + ([("k", k, None, out_k, k_weight)] if k is not None else []),
+                          positions, inv_freq, pairs, norm, eps, rope)
+
+    a = _plan(key, build)
+    oq = torch.empty((B, H, S, D), dtype=dtype, device=device) if out_q is None else out_q
+    ok = out_k
+    if k is not None and ok is None:
+        ok = torch.empty((B, k.shape[1], S, D), dtype=dtype, device=device)
+    if B * S * D == 0:
+        return oq, ok
+    t = a.t[0]
+    t.x, t.y, t.weight = q.data_ptr(), oq.data_ptr(), _ptr(q_weight)
+    if k is not None:
+        t = a.t[1]
+        t.x, t.y, t.weight = k.data_ptr(), ok.data_ptr(), _ptr(k_weight)
+    a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+    a.stream = _stream(device)
+    with _on_device(device):
+        rc = _lib.lib().xdit_axes_rope(ctypes.byref(a))
+    if rc != 0:
+        _lib.check(rc)
+    return oq, ok
+
+
+def axes_rope_backward(dq, dk, positions, inv_freq, pairs, q=None, k=None, norm=False, q_weight=None, k_weight=None, eps=1e-6, rope="interleaved"):
+    """Gradients of `axes_rope` from those of its results -> (dq, dk, dq_weight, dk_weight), new BHSD-contiguous tensors;
+    None for what was not there (dk may be None).  With the norm q and k are the inputs of the forward call.  The gains'
+    gradients are summed in fp32 in a fixed order."""
+    if not isinstance(dq, torch.Tensor) or dq.ndim != 4:
+        raise ValueError("dq must be a 4-D tensor (B, H, S, D)")
+    device, dtype = dq.device, dq.dtype
+    B, H, S, D = dq.shape
+    if not norm:
+        q = k = None
+    key = ("arope_bwd", _sig(dq), _sig(dk), _sig(positions), _sig(inv_freq), pairs, _sig(q), _sig(k), norm, _sig(q_weight), _sig(k_weight), eps, rope)
+
+    def build():
+        _check("dq", dq, None, _FLOATS, device)
+        if norm and (q is None or (dk is not None and k is None)):
+            raise ValueError("the gradient of the norm needs q (and k)")
+        if dk is None and (k is not None or k_weight is not None):
+            raise ValueError("k and k_weight need dk")
+        if dk is not None and not isinstance(dk, torch.Tensor):
+            raise ValueError("dk must be a 4-D tensor (B, H, S, D)")
+        a = _rope_args(dq, [("q", q, dq, None, q_weight)] + ([("k", k, dk, None, k_weight)] if dk is not None else []),
+                       positions, inv_freq, pairs, norm, eps, rope)
+        for i, w in enumerate((q_weight, k_weight)):
+            a.t[i].dweight = None if w is None else 16   # any aligned address: only what is asked for decides the size
+        with _on_device(device):
+            need = _lib.lib().xdit_axes_rope_backward_workspace_bytes(ctypes.byref(a)) if B * S * D else 0
+        if need < 0:
+            _lib.check(need)
+        return a, need
+
+    a, need = _plan(key, build)
+    outs, grads = [], []
+    for d, w in ((dq, q_weight), (dk, k_weight)):
+        outs.append(None if d is None else torch.empty(d.shape, dtype=dtype, device=device))
+        grads.append(None if w is None else torch.empty((D,), dtype=w.dtype, device=device))
+    if B * S * D == 0:
+        for g in grads:
+            if g is not None:
+                g.zero_()
+        return (*outs, *grads)
+    for t, d, x, w, y, g in zip(a.t, (dq, dk), (q, k), (q_weight, k_weight), outs, grads):
+        t.dy, t.x, t.weight, t.y, t.dweight = _ptr(d), _ptr(x), _ptr(w), _ptr(y), _ptr(g)
+    a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+    a.stream = stream = _stream(device)
+    with _stream_lock(device, stream), _on_device(device):
+        if need:
+            a.workspace, a.workspace_bytes = _scratch(device, stream, need), need
+        rc = _lib.lib().xdit_axes_rope_backward(ctypes.byref(a))
+    if rc != 0:
+        _lib.check(rc)
+    return (*outs, *grads)

@@ -173,4 +173,99 @@ int xdit_gated_norm_backward(const xdit_gated_norm_backward_args* a) {
   return XDIT_OK;
 }
 
+static int fill_axes_rope(const xdit_axes_rope_args* a, xdit::AxesRopeParams& p, bool backward, bool pointers) {
+  if (a == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "args is NULL");
+  if (a->struct_size != sizeof(xdit_axes_rope_args))
+    return api_fail(XDIT_ERR_INVALID_ARG, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(xdit_axes_rope_args));
+  if (!float_dtype(a->dtype)) return api_fail(XDIT_ERR_INVALID_ARG, "dtype %d must be bf16, fp16 or fp32", a->dtype);
+  if (a->weight_dtype != a->dtype && a->weight_dtype != XDIT_DTYPE_FP32) return api_fail(XDIT_ERR_INVALID_ARG, "weight_dtype %d must be dtype or fp32", a->weight_dtype);
+  if (a->rope != XDIT_ROPE_INTERLEAVED && a->rope != XDIT_ROPE_SPLIT_HALF) return api_fail(XDIT_ERR_INVALID_ARG, "rope %d must be interleaved or split_half", a->rope);
+  if (a->pos_bits != -32 && a->pos_bits != 32 && a->pos_bits != 64) return api_fail(XDIT_ERR_INVALID_ARG, "pos_bits %d must be -32 (fp32), 32 or 64", a->pos_bits);
+  if (a->freq_bits != 32 && a->freq_bits != 64) return api_fail(XDIT_ERR_INVALID_ARG, "freq_bits %d must be 32 or 64", a->freq_bits);
+  if (a->B <= 0 || a->S <= 0) return api_fail(XDIT_ERR_INVALID_ARG, "B and S must be positive");
+  if (a->S > (int64_t(1) << 30) || (int64_t)a->B * a->S > 0x7fffffffLL) return api_fail(XDIT_ERR_INVALID_ARG, "too many tokens for one launch");
+  if (a->D <= 0 || a->D % 8 != 0 || a->D > 512) return api_fail(XDIT_ERR_UNSUPPORTED, "head_dim %d: need a multiple of 8, at most 512", a->D);
+  if (a->tensors != 1 && a->tensors != 2) return api_fail(XDIT_ERR_INVALID_ARG, "tensors %d must be 1 or 2", a->tensors);
+  if (a->axes < 1 || a->axes > XDIT_ROPE_MAX_AXES) return api_fail(XDIT_ERR_INVALID_ARG, "axes %d must be between 1 and %d", a->axes, XDIT_ROPE_MAX_AXES);
+  if (a->norm && !(a->eps >= 0.f && std::isfinite(a->eps))) return api_fail(XDIT_ERR_INVALID_ARG, "eps must be finite and >= 0");
+  std::memset(&p, 0, sizeof(p));
+  int64_t P = 0;
+  for (int i = 0; i < XDIT_ROPE_MAX_AXES; i++) {
+    if (i < a->axes) {
+      if (a->pairs[i] < 0 || a->pairs[i] > a->D) return api_fail(XDIT_ERR_INVALID_ARG, "pairs[%d] = %d is out of range", i, a->pairs[i]);
+      P += a->pairs[i];
+    }
+    p.axis_end[i] = (int)P;
+  }
+  if (2 * P > a->D) return api_fail(XDIT_ERR_INVALID_ARG, "%lld pairs do not fit head_dim %d", (long long)P, a->D);
+  if (P % 4 != 0) return api_fail(XDIT_ERR_UNSUPPORTED, "%lld rotated pairs: need a multiple of 4", (long long)P);
+  p.P = (int)P;
+  p.tensors = a->tensors; p.B = a->B; p.S = (int)a->S; p.D = a->D; p.axes = a->axes;
+  p.split_half = a->rope == XDIT_ROPE_SPLIT_HALF; p.norm = a->norm != 0;
+  p.pos_bits = a->pos_bits; p.freq_wide = a->freq_bits == 64; p.weight_wide = a->weight_dtype == XDIT_DTYPE_FP32;
+  p.positions = a->positions; p.ps_b = a->pos_stride_b; p.ps_s = a->pos_stride_s; p.inv_freq = a->inv_freq;
+  p.eps = a->eps; p.inv_d = 1.0f / (float)a->D;
+  const int es = size_of(a->dtype);
+  int rc;
+  for (int i = 0; i < a->tensors; i++) {
+    const xdit_axes_rope_tensor& t = a->t[i];
+    xdit::RopeTensor& o = p.t[i];
+    if (t.H <= 0 || t.H > 65535) return api_fail(XDIT_ERR_INVALID_ARG, "t[%d]: H = %d must be between 1 and 65535", i, t.H);
+    o.x = t.x; o.dy = t.dy; o.y = t.y; o.weight = t.weight; o.dweight = backward && p.norm ? t.dweight : nullptr; o.H = t.H;
+    o.xs_b = t.x_stride.b; o.xs_h = t.x_stride.h; o.xs_s = t.x_stride.s;
+    o.ds_b = t.dy_stride.b; o.ds_h = t.dy_stride.h; o.ds_s = t.dy_stride.s;
+    o.ys_b = t.y_stride.b; o.ys_h = t.y_stride.h; o.ys_s = t.y_stride.s;
+    p.sums |= o.dweight != nullptr;
+    if (!pointers) continue;
+    const struct { const char* name; const void* ptr; const xdit_strides* st; bool used, written; } rows[] = {
+        {"x", t.x, &t.x_stride, !backward || p.norm, false}, {"dy", t.dy, &t.dy_stride, backward, false}, {"y", t.y, &t.y_stride, true, true}};
+    for (const auto& r : rows) {
+      if (!r.used) continue;
+      const xdit_row_strides bs = {r.st->b, r.st->s}, bh = {r.st->b, r.st->h};
+      if ((rc = check_rows(r.name, r.ptr, bs, es, a->B, a->S, a->D, r.written)) || (rc = check_rows(r.name, r.ptr, bh, es, a->B, t.H, a->D, r.written))) return rc;
+    }
+    if (t.weight != nullptr && !p.norm) return api_fail(XDIT_ERR_INVALID_ARG, "a weight needs the norm");
+    if ((rc = check_vector("weight", t.weight))) return rc;
+    if (o.dweight != nullptr && t.weight == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "dweight needs weight");
+  }
+  if (pointers) {
+    if (a->positions == nullptr || !multiple_of(a->positions, a->pos_bits == 64 ? 8 : 4)) return api_fail(XDIT_ERR_INVALID_ARG, "positions is NULL or not aligned to its elements");
+    if (a->inv_freq == nullptr || !multiple_of(a->inv_freq, a->freq_bits / 8)) return api_fail(XDIT_ERR_INVALID_ARG, "inv_freq is NULL or not aligned to its elements");
+    if (a->pos_stride_b < 0 || a->pos_stride_s < 0) return api_fail(XDIT_ERR_INVALID_ARG, "positions: negative stride");
+  }
+  xdit::axes_rope_plan(p, backward);
+  return 0;
+}
+
+int xdit_axes_rope(const xdit_axes_rope_args* a) {
+  xdit::api_clear_error();
+  xdit::AxesRopeParams p;
+  if (int rc = fill_axes_rope(a, p, false, true)) return rc;
+  const hipError_t e = xdit::launch_axes_rope(p, a->dtype, false, (hipStream_t)a->stream);
+  if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "rotation launch failed: %s", hipGetErrorString(e));
+  return XDIT_OK;
+}
+
+static int64_t rope_backward_bytes(const xdit::AxesRopeParams& p) { return p.sums ? (int64_t)p.head_groups * p.token_groups * 2 * p.D * 4 : 0; }
+
+int64_t xdit_axes_rope_backward_workspace_bytes(const xdit_axes_rope_args* a) {
+  xdit::api_clear_error();
+  xdit::AxesRopeParams p;
+  const int rc = fill_axes_rope(a, p, true, false);
+  return rc ? rc : rope_backward_bytes(p);
+}
+
+int xdit_axes_rope_backward(const xdit_axes_rope_args* a) {
+  xdit::api_clear_error();
+  xdit::AxesRopeParams p;
+  if (int rc = fill_axes_rope(a, p, true, true)) return rc;
+  const int64_t need = rope_backward_bytes(p);
+  if (need > 0 && (a->workspace == nullptr || !multiple_of(a->workspace, 16) || a->workspace_bytes < need))
+    return api_fail(XDIT_ERR_INVALID_ARG, "workspace of %lld bytes (16-byte aligned) is needed, %lld given", (long long)need, (long long)a->workspace_bytes);
+  p.partial = (float*)a->workspace;
+  const hipError_t e = xdit::launch_axes_rope(p, a->dtype, true, (hipStream_t)a->stream);
+  if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "rotation backward launch failed: %s", hipGetErrorString(e));
+  return XDIT_OK;
+}
+
 }  // extern "C"

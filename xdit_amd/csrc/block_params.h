@@ -66,4 +66,41 @@ hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, hipStream_t st
 hipError_t launch_gated_norm_bwd(const GatedNormBwdParams& p, int dtype, hipStream_t stream);
 void gated_norm_bwd_plan(GatedNormBwdParams& p);  // fills parts, rows_per_part and sums
 
+// Rotation of q and k by positions on several axes.
+struct RopeTensor {
+  const void* x;
+  const void* dy;
+  void* y;
+  const void* weight;
+  void* dweight;
+  int64_t xs_b, xs_h, xs_s;
+  int64_t ds_b, ds_h, ds_s;
+  int64_t ys_b, ys_h, ys_s;
+  int H;
+};
+
+struct AxesRopeParams {
+  RopeTensor t[2];
+  int tensors;
+  int B, S, D;
+  int P;              // rotated pairs
+  int axis_end[4];    // first pair behind the axis' range (P for the axes that are not there)
+  int axes;
+  int split_half, norm;
+  int pos_bits, freq_wide, weight_wide;
+  const void* positions;
+  int64_t ps_b, ps_s;
+  const void* inv_freq;
+  float eps, inv_d;
+  int lpr;             // lanes per row: smallest power of two >= D / 8
+  int heads_per_wave;  // of the heads of q and k, laid end to end
+  int head_groups;
+  int token_groups;    // workgroups the tokens are dealt to (backward; forward: four tokens each)
+  float* partial;      // backward: [head group][token group][2][D]
+  int sums;
+};
+
+hipError_t launch_axes_rope(const AxesRopeParams& p, int dtype, bool backward, hipStream_t stream);
+void axes_rope_plan(AxesRopeParams& p, bool backward);  // fills lpr, heads_per_wave, head_groups, token_groups
+
 }  // namespace xdit
