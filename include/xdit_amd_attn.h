@@ -563,6 +563,64 @@ int xdit_axes_rope(const xdit_axes_rope_args* args);
 int64_t xdit_axes_rope_backward_workspace_bytes(const xdit_axes_rope_args* args);
 int xdit_axes_rope_backward(const xdit_axes_rope_args* args);
 
+/*
+ * fp8 (e4m3) quantiser with an fp32 scale per block of 1 x 128 (block_rows 1: activations) or 128 x 128 elements (block_rows
+ * 128: weights), the blocks at the end cut off by the tensor:
+ *     scale = absmax / 448, at least 2^-126, 1 for a block of zeros ;  y = e4m3(x / scale)
+ * y has the bytes of a true fp32 division.  A block that holds a NaN is NaN, one with an infinity has an infinite scale.
+ * scale: block_rows 1: scale[kb * B*S + b*S + s]; 128 (B must be 1): scale[(s / 128) * ceil(K / 128) + kb].
+ */
+typedef struct {
+  uint32_t struct_size;        /* = sizeof(xdit_block_quant_args) */
+  int32_t dtype;               /* x: bf16, fp16 or fp32 */
+  int32_t block_rows;          /* 1 or 128 */
+  int32_t B;
+  int64_t S, K;                /* x is (B, S, K); K a multiple of 8 */
+  const void* x;
+  void* y;                     /* (B, S, K) e4m3 bytes */
+  float* scale;
+  xdit_row_strides x_stride, y_stride;
+  void* stream;
+} xdit_block_quant_args;
+
+int xdit_fp8_block_quant(const xdit_block_quant_args* args);
+
+/*
+ * Product of block-scaled fp8 (e4m3) matrices, out = x w^T + bias:
+ *     out[m, n] = sum_kb x_scale[m, kb] w_scale[n / 128, kb] sum_{k in block kb} x[m, k] w[n, k]  + bias[n]
+ * x (M, K) with a scale per 1 x 128 block, w (N, K) with one per 128 x 128 block (what xdit_fp8_block_quant makes), K a
+ * multiple of 16, rows 16-byte aligned.  The scaled sums of the blocks are held in fp32 and the result is rounded once to
+ * out_dtype.  Within a block, exact_sums != 0: products are exact and summed in fp32 (the operands are widened to fp16 on their
+ * way into the matrix cores); 0: the fp8 matrix instructions, twice as fast, which add eight consecutive k at a time and cut
+ * every product of those at 2^-13 of the largest one's binade.  `workspace` (optional, xdit_fp8_block_matmul_workspace_bytes, 16-byte
+ * aligned, private to the stream until the call's kernels finish) lets a product of few rows cut K over the chip; without it
+ * K is not cut.  Results are reproducible bit for bit for the same arguments and workspace.
+ */
+typedef struct {
+  uint32_t struct_size;        /* = sizeof(xdit_block_matmul_args) */
+  int32_t out_dtype;           /* bf16, fp16 or fp32 */
+  int32_t bias_dtype;          /* out_dtype or fp32 */
+  int32_t cu_count;            /* 0 = plan for the compute units of the current device; > 0 = for that many (tests, tuning) */
+  int32_t exact_sums;
+  int32_t reserved0;
+  int64_t M, N, K;
+  const void* x;
+  const float* x_scale;
+  const void* w;
+  const float* w_scale;
+  const void* bias;            /* N entries, may be NULL */
+  void* out;                   /* (M, N) */
+  int64_t x_stride, w_stride, out_stride;       /* elements from row to row */
+  int64_t x_scale_stride_m, x_scale_stride_k;   /* of (M, ceil(K / 128)) */
+  int64_t w_scale_stride_n, w_scale_stride_k;   /* of (ceil(N / 128), ceil(K / 128)) */
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} xdit_block_matmul_args;
+
+int64_t xdit_fp8_block_matmul_workspace_bytes(const xdit_block_matmul_args* args);
+int xdit_fp8_block_matmul(const xdit_block_matmul_args* args);
+
 /* Message of the last error on the calling thread ("" if none). Never NULL. */
 const char* xdit_attn_last_error(void);
 

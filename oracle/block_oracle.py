@@ -174,3 +174,28 @@ def axes_rope_backward(dy, x, weight, positions, inv_freq, pairs, norm, eps, rop
     dx = r * (g - u * (g * u).mean(-1, keepdim=True))
     top = size * (1.0 if weight is None else w.abs())
     return dx, (d * u).sum((0, 1, 2)), r * (top + u.abs() * (top * u.abs()).mean(-1, keepdim=True)), (size * u.abs()).sum((0, 1, 2))
+
+
+def block_matmul(x, x_scale, w, w_scale, bias=None):
+    """-> (M, N) product of the values the operands stand for, and the sum of its terms' sizes."""
+    M, K = x.shape
+    N = w.shape[0]
+    a = x.double() * spread(x_scale.double(), 1, M, K)
+    b = w.double() * spread(w_scale.double(), 128, N, K)
+    y, size = a @ b.t(), a.abs() @ b.t().abs()
+    if bias is not None:
+        y, size = y + bias.double(), size + bias.double().abs()
+    return y, size
+
+
+def largest_of_eights(x, x_scale, w, w_scale):
+    """Sum over the groups of eight consecutive k of the largest |x w| of the group."""
+    a = x.float() * spread(x_scale.float(), 1, *x.shape)
+    b = w.float() * spread(w_scale.float(), 128, *w.shape)
+    total = torch.zeros(x.shape[0], w.shape[0], device=x.device)
+    for k in range(0, x.shape[1], 8):
+        top = torch.zeros_like(total)
+        for j in range(k, k + 8):
+            top = torch.maximum(top, torch.outer(a[:, j].abs(), b[:, j].abs()))
+        total += top
+    return total.double()

@@ -234,6 +234,22 @@ class AxesRopeArgs(ctypes.Structure):
                    ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
 
 
+class BlockQuantArgs(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("block_rows", ctypes.c_int32), ("B", ctypes.c_int32),
+                ("S", ctypes.c_int64), ("K", ctypes.c_int64), ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("x_stride", RowStrides), ("y_stride", RowStrides), ("stream", ctypes.c_void_p)]
+
+
+class BlockMatmulArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", ctypes.c_uint32), ("out_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32), ("cu_count", ctypes.c_int32),
+                 ("exact_sums", ctypes.c_int32), ("reserved0", ctypes.c_int32)]
+                + [(n, ctypes.c_int64) for n in ("M", "N", "K")]
+                + [(n, ctypes.c_void_p) for n in ("x", "x_scale", "w", "w_scale", "bias", "out")]
+                + [(n, ctypes.c_int64) for n in ("x_stride", "w_stride", "out_stride", "x_scale_stride_m", "x_scale_stride_k",
+                                                 "w_scale_stride_n", "w_scale_stride_k")]
+                + [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
+
+
 ROWNORM_NONE, ROWNORM_RMS, ROWNORM_LAYER = 0, 1, 2
 
 NORM_NONE, NORM_HEAD, NORM_TOKEN = 0, 1, 2
@@ -242,6 +258,7 @@ ROPE_NONE, ROPE_INTERLEAVED, ROPE_SPLIT_HALF, ROPE_WAN = 0, 1, 2, 3
 EXPORTS = ("xdit_attn_fwd", "xdit_attn_fwd_two_queries", "xdit_attn_fwd_noalloc", "xdit_attn_fwd_accumulate", "xdit_attn_workspace_bytes", "xdit_attn_launch_plan", "xdit_lse_merge", "xdit_fp8_quant", "xdit_fp8_quant_batch", "xdit_qk_prologue", "xdit_qk_prologue_batch",
            "xdit_gated_norm", "xdit_gated_norm_backward", "xdit_gated_norm_backward_workspace_bytes",
            "xdit_axes_rope", "xdit_axes_rope_backward", "xdit_axes_rope_backward_workspace_bytes",
+           "xdit_fp8_block_quant", "xdit_fp8_block_matmul", "xdit_fp8_block_matmul_workspace_bytes",
            "xdit_attn_last_error", "xdit_attn_abi_version")
 
 _lib = None
@@ -289,7 +306,10 @@ def lib():
                                    ("xdit_gated_norm_backward_workspace_bytes", GatedNormBackwardArgs, ctypes.c_int64),
                                    ("xdit_axes_rope", AxesRopeArgs, ctypes.c_int),
                                    ("xdit_axes_rope_backward", AxesRopeArgs, ctypes.c_int),
-                                   ("xdit_axes_rope_backward_workspace_bytes", AxesRopeArgs, ctypes.c_int64)):
+                                   ("xdit_axes_rope_backward_workspace_bytes", AxesRopeArgs, ctypes.c_int64),
+                                   ("xdit_fp8_block_quant", BlockQuantArgs, ctypes.c_int),
+                                   ("xdit_fp8_block_matmul", BlockMatmulArgs, ctypes.c_int),
+                                   ("xdit_fp8_block_matmul_workspace_bytes", BlockMatmulArgs, ctypes.c_int64)):
             f = getattr(L, name)
             f.argtypes, f.restype = [ctypes.POINTER(args)], result
         L.xdit_attn_last_error.argtypes = []

@@ -1,6 +1,6 @@
 """Tensor-level entry points of the operators around the attention call of a DiT block: the norms with
 their modulation, gate and residual and the rotation of q and k by positions on several axes, forward and
-backward.
+backward, and the projections' fp8 product with a scale per block of 128 and its quantiser.
 
 Hidden states are (B, S, C), q and k logical (B, H, S, D), with any outer strides (multiples of 16 bytes) and a
 unit stride over the last dimension; PyTorch is used for device memory and the current stream only.  Argument structs are kept per call signature and thread,
@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _RETIRED, _PLANS_MAX, _TLS, _code, _on_device, _sig, _stream, _stream_lock
+from .ops import TUNING, _PLANS_MAX, _RETIRED, _TLS, _code, _on_device, _sig, _stream, _stream_lock
 
 _ROWNORM = {None: _lib.ROWNORM_NONE, "rms": _lib.ROWNORM_RMS, "layer": _lib.ROWNORM_LAYER}
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -414,3 +414,110 @@ def axes_rope_backward(dq, dk, positions, inv_freq, pairs, q=None, k=None, norm=
     if rc != 0:
         _lib.check(rc)
     return (*outs, *grads)
+
+
+def fp8_block_quant(x, block_rows=1):
+    """fp8 (e4m3) values and fp32 scales of x, a scale per 1 x 128 block (`block_rows` 1: activations) or 128 x 128 block
+    (128: weights) -> (y, scale), x about y * scale:  scale = absmax / 448 (1 for a block of zeros), y = e4m3(x / scale).
+
+    x: (M, K), or (B, S, K) with `block_rows` 1, bf16 / fp16 / fp32, any row strides that are multiples of 16 bytes, K a multiple of 8;
+    the last blocks are cut off by the tensor.  y is contiguous; scale is (M, ceil(K / 128)) or (B, S, ceil(K / 128)), the scales
+    of one block of columns side by side in memory, or contiguous (ceil(M / 128), ceil(K / 128))."""
+    if not isinstance(x, torch.Tensor) or x.ndim not in (2, 3) or (x.ndim == 3 and block_rows != 1):
+        raise ValueError("x must be (M, K), or (B, S, K) with blocks of one row")
+    device = x.device
+    key = ("bquant", _sig(x), block_rows)
+    B, S, K = x.shape if x.ndim == 3 else (1, *x.shape)
+    kb = (K + 127) // 128
+
+    def build():
+        _check("x", x, None, _FLOATS, device)
+        a = _lib.BlockQuantArgs()
+        a.struct_size = ctypes.sizeof(a)
+        a.dtype, a.block_rows = _code(x.dtype), int(block_rows)
+        a.B, a.S, a.K = B, S, K
+        a.x_stride = _lib.RowStrides(x.stride(0) if x.ndim == 3 else 0, x.stride(-2))
+        a.y_stride = _lib.RowStrides(S * K, K)
+        return a
+
+    a = _plan(key, build)
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty((kb, B, S) if block_rows == 1 else ((S + 127) // 128, kb), dtype=torch.float32, device=device)
+    if B * S * K:
+        a.x, a.y, a.scale, a.stream = x.data_ptr(), y.data_ptr(), scale.data_ptr(), _stream(device)
+        with _on_device(device):
+            rc = _lib.lib().xdit_fp8_block_quant(ctypes.byref(a))
+        if rc != 0:
+            _lib.check(rc)
+    if block_rows != 1:
+        return y, scale
+    return y, (scale.permute(1, 2, 0) if x.ndim == 3 else scale.view(kb, S).t())
+
+
+def fp8_block_matmul(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, out=None, exact_sums=None):
+    """x w^T + bias of block-scaled fp8 matrices -> (M, N) (or (B, S, N)) in `out_dtype`:
+
+        out[m, n] = sum over blocks kb of  x_scale[m, kb] * w_scale[n // 128, kb] * (x[m, kb] . w[n, kb])  + bias[n]
+
+    x: (M, K) or (B, S, K) e4m3 with scales (M, ceil(K / 128)) or (B, S, ceil(K / 128)); w: (N, K) with scales (ceil(N / 128),
+    ceil(K / 128)) (`fp8_block_quant` of both; scales may have any strides); K a multiple of 16; bias (N,) in out_dtype or fp32.
+    The blocks' sums are held in fp32 and the result is rounded once; the same call gives the same bits.  `exact_sums` True:
+    products are exact and summed in fp32; False: the fp8 matrix instructions, twice as fast, which add eight consecutive k at a
+    time with every product cut at 2^-13 of the largest one's binade; None: exact for fp32 results, where that shows."""
+    for name, t in (("x", x), ("x_scale", x_scale), ("w", w), ("w_scale", w_scale)):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("%s must be a tensor" % name)
+    device, shape = x.device, x.shape
+    if x.ndim == 3:
+        if x_scale.ndim != 3 or x_scale.shape[:2] != shape[:2]:
+            raise ValueError("x_scale has shape %s, expected (%d, %d, ceil(K / 128))" % (tuple(x_scale.shape), shape[0], shape[1]))
+        x, x_scale = x.flatten(0, 1), x_scale.flatten(0, 1)
+    key = ("bmm", _sig(x), _sig(x_scale), _sig(w), _sig(w_scale), _sig(bias), out_dtype, _sig(out), exact_sums, TUNING["cu_count"])
+    if x.ndim != 2 or w.ndim != 2:
+        raise ValueError("x must be (M, K) or (B, S, K), w (N, K)")
+    (M, K), N = x.shape, w.shape[0]
+
+    def build():
+        kb = (K + 127) // 128
+        _check("x", x, None, (torch.float8_e4m3fn,), device)
+        _check("w", w, (N, K), (torch.float8_e4m3fn,), device)
+        for name, t, rows in (("x_scale", x_scale, M), ("w_scale", w_scale, (N + 127) // 128)):
+            if t.device != device or t.dtype != torch.float32 or tuple(t.shape) != (rows, kb):
+                raise ValueError("%s must be a (%d, %d) fp32 tensor on %s" % (name, rows, kb, device))
+        if out_dtype not in _FLOATS:
+            raise ValueError("out_dtype must be bf16, fp16 or fp32")
+        if bias is not None:
+            _check("bias", bias, (N,), (out_dtype, torch.float32), device)
+        a = _lib.BlockMatmulArgs()
+        a.struct_size = ctypes.sizeof(a)
+        a.out_dtype, a.bias_dtype = _code(out_dtype), _code(out_dtype if bias is None else bias.dtype)
+        a.cu_count = int(TUNING["cu_count"])
+        a.exact_sums = int(out_dtype == torch.float32 if exact_sums is None else bool(exact_sums))
+        a.M, a.N, a.K = M, N, K
+        a.x_stride, a.w_stride, a.out_stride = x.stride(0), w.stride(0), N
+        if out is not None:
+            _check("out", out, (*shape[:-1], N), (out_dtype,), device)
+            flat = out.view(-1, N) if out.ndim == 3 else out
+            a.out_stride = flat.stride(0)
+        a.x_scale_stride_m, a.x_scale_stride_k = x_scale.stride()
+        a.w_scale_stride_n, a.w_scale_stride_k = w_scale.stride()
+        with _on_device(device):
+            need = _lib.lib().xdit_fp8_block_matmul_workspace_bytes(ctypes.byref(a)) if M * N * K else 0
+        if need < 0:
+            _lib.check(need)
+        return a, need
+
+    a, need = _plan(key, build)
+    y = torch.empty((*shape[:-1], N), dtype=out_dtype, device=device) if out is None else out
+    if M * N == 0:
+        return y
+    if K == 0:
+        return y.zero_() if bias is None else y.copy_(bias)
+    a.x, a.x_scale, a.w, a.w_scale, a.bias, a.out = x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), _ptr(bias), y.data_ptr()
+    a.stream = stream = _stream(device)
+    with _stream_lock(device, stream), _on_device(device):
+        a.workspace, a.workspace_bytes = (_scratch(device, stream, need), need) if need else (None, 0)
+        rc = _lib.lib().xdit_fp8_block_matmul(ctypes.byref(a))
+    if rc != 0:
+        _lib.check(rc)
+    return y

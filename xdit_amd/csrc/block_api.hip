@@ -268,4 +268,79 @@ int xdit_axes_rope_backward(const xdit_axes_rope_args* a) {
   return XDIT_OK;
 }
 
+int xdit_fp8_block_quant(const xdit_block_quant_args* a) {
+  xdit::api_clear_error();
+  if (a == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "args is NULL");
+  if (a->struct_size != sizeof(xdit_block_quant_args))
+    return api_fail(XDIT_ERR_INVALID_ARG, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(xdit_block_quant_args));
+  if (!float_dtype(a->dtype)) return api_fail(XDIT_ERR_INVALID_ARG, "dtype %d must be bf16, fp16 or fp32", a->dtype);
+  if (a->block_rows != 1 && a->block_rows != 128) return api_fail(XDIT_ERR_INVALID_ARG, "block_rows %d must be 1 or 128", a->block_rows);
+  if (a->B <= 0 || a->S <= 0 || a->K <= 0) return api_fail(XDIT_ERR_INVALID_ARG, "B, S, K must be positive");
+  if (a->S > (int64_t(1) << 30) || a->B * a->S > 0x7fffffffLL || a->K > (int64_t(1) << 30)) return api_fail(XDIT_ERR_INVALID_ARG, "tensor too large for one launch");
+  if (a->K % 8 != 0) return api_fail(XDIT_ERR_UNSUPPORTED, "K = %lld: need a multiple of 8", (long long)a->K);
+  if (a->block_rows == 128 && a->B != 1) return api_fail(XDIT_ERR_INVALID_ARG, "blocks of 128 rows need B = 1");
+  int rc;
+  if ((rc = check_rows("x", a->x, a->x_stride, size_of(a->dtype), a->B, a->S, a->K, false))) return rc;
+  if ((rc = check_rows("y", a->y, a->y_stride, 1, a->B, a->S, a->K, true))) return rc;
+  if (a->scale == nullptr || !multiple_of(a->scale, 4)) return api_fail(XDIT_ERR_INVALID_ARG, "scale is NULL or not 4-byte aligned");
+  xdit::BlockQuantParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.x = a->x; p.y = (unsigned char*)a->y; p.scale = a->scale; p.xs = rs(a->x_stride); p.ys = rs(a->y_stride);
+  p.rows = a->B * a->S; p.S = (int)a->S; p.K = (int)a->K; p.kblocks = (p.K + 127) / 128;
+  const hipError_t e = xdit::launch_fp8_block_quant(p, a->dtype, a->block_rows, (hipStream_t)a->stream);
+  if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "block quantiser launch failed: %s", hipGetErrorString(e));
+  return XDIT_OK;
+}
+
+static int fill_block_matmul(const xdit_block_matmul_args* a, xdit::BlockMatmulParams& p, bool pointers) {
+  if (a == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "args is NULL");
+  if (a->struct_size != sizeof(xdit_block_matmul_args))
+    return api_fail(XDIT_ERR_INVALID_ARG, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(xdit_block_matmul_args));
+  if (!float_dtype(a->out_dtype)) return api_fail(XDIT_ERR_INVALID_ARG, "out_dtype %d must be bf16, fp16 or fp32", a->out_dtype);
+  if (a->bias_dtype != a->out_dtype && a->bias_dtype != XDIT_DTYPE_FP32) return api_fail(XDIT_ERR_INVALID_ARG, "bias_dtype %d must be out_dtype or fp32", a->bias_dtype);
+  if (a->M <= 0 || a->N <= 0 || a->K <= 0) return api_fail(XDIT_ERR_INVALID_ARG, "M, N, K must be positive");
+  if (a->M > (1 << 30) || a->N > (1 << 24) || a->K > (1 << 24)) return api_fail(XDIT_ERR_INVALID_ARG, "M is limited to 2^30, N and K to 2^24");
+  if (a->K % 16 != 0) return api_fail(XDIT_ERR_UNSUPPORTED, "K = %lld: need a multiple of 16", (long long)a->K);
+  if (a->cu_count < 0 || a->cu_count > 4096) return api_fail(XDIT_ERR_INVALID_ARG, "cu_count %d must be between 0 and 4096", a->cu_count);
+  std::memset(&p, 0, sizeof(p));
+  p.x = (const unsigned char*)a->x; p.xsc = a->x_scale; p.w = (const unsigned char*)a->w; p.wsc = a->w_scale; p.bias = a->bias; p.out = a->out;
+  p.xs = a->x_stride; p.ws = a->w_stride; p.os = a->out_stride;
+  p.xsc_m = a->x_scale_stride_m; p.xsc_k = a->x_scale_stride_k; p.wsc_n = a->w_scale_stride_n; p.wsc_k = a->w_scale_stride_k;
+  p.M = (int)a->M; p.N = (int)a->N; p.K = (int)a->K; p.kblocks = (p.K + 127) / 128;
+  p.bias_wide = a->bias_dtype == XDIT_DTYPE_FP32;
+  p.cu_count = a->cu_count;
+  p.exact = a->exact_sums != 0;
+  if (!pointers) return 0;
+  if (a->x == nullptr || a->w == nullptr || a->x_scale == nullptr || a->w_scale == nullptr || a->out == nullptr)
+    return api_fail(XDIT_ERR_INVALID_ARG, "x, x_scale, w, w_scale or out is NULL");
+  if (!multiple_of(a->x, 16) || !multiple_of(a->w, 16)) return api_fail(XDIT_ERR_INVALID_ARG, "x and w must be 16-byte aligned");
+  if ((a->M > 1 && (a->x_stride % 16 || a->x_stride < a->K)) || (a->N > 1 && (a->w_stride % 16 || a->w_stride < a->K)))
+    return api_fail(XDIT_ERR_INVALID_ARG, "rows of x and w must be multiples of 16 bytes apart, at least K = %lld", (long long)a->K);
+  if (a->x_stride >= (1 << 24) || a->w_stride >= (1 << 24)) return api_fail(XDIT_ERR_INVALID_ARG, "row strides of 2^24 bytes or more are not supported");
+  if (!multiple_of(a->out, size_of(a->out_dtype)) || (a->M > 1 && a->out_stride < a->N))
+    return api_fail(XDIT_ERR_INVALID_ARG, "out is not aligned to its elements or its rows overlap");
+  if (a->x_scale_stride_m < 0 || a->x_scale_stride_k < 0 || a->w_scale_stride_n < 0 || a->w_scale_stride_k < 0)
+    return api_fail(XDIT_ERR_INVALID_ARG, "negative scale stride");
+  if (a->bias != nullptr && !multiple_of(a->bias, size_of(a->bias_dtype))) return api_fail(XDIT_ERR_INVALID_ARG, "bias is not aligned to its elements");
+  if (a->workspace != nullptr && (!multiple_of(a->workspace, 16) || a->workspace_bytes < 0)) return api_fail(XDIT_ERR_INVALID_ARG, "workspace is not 16-byte aligned");
+  p.partial = (float*)a->workspace;
+  return 0;
+}
+
+int64_t xdit_fp8_block_matmul_workspace_bytes(const xdit_block_matmul_args* a) {
+  xdit::api_clear_error();
+  xdit::BlockMatmulParams p;
+  const int rc = fill_block_matmul(a, p, false);
+  return rc ? rc : (int64_t)xdit::fp8_block_matmul_workspace(p);
+}
+
+int xdit_fp8_block_matmul(const xdit_block_matmul_args* a) {
+  xdit::api_clear_error();
+  xdit::BlockMatmulParams p;
+  if (int rc = fill_block_matmul(a, p, true)) return rc;
+  const hipError_t e = xdit::launch_fp8_block_matmul(p, a->out_dtype, a->workspace != nullptr ? (size_t)a->workspace_bytes : 0, (hipStream_t)a->stream);
+  if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "block-scaled product launch failed: %s", hipGetErrorString(e));
+  return XDIT_OK;
+}
+
 }  // extern "C"

@@ -103,4 +103,37 @@ struct AxesRopeParams {
 hipError_t launch_axes_rope(const AxesRopeParams& p, int dtype, bool backward, hipStream_t stream);
 void axes_rope_plan(AxesRopeParams& p, bool backward);  // fills lpr, heads_per_wave, head_groups, token_groups
 
+// Block-wise fp8 quantiser and the block-scaled product.
+struct BlockQuantParams {
+  const void* x;
+  unsigned char* y;
+  float* scale;
+  RowStrides xs, ys;
+  int64_t rows;  // B * S
+  int S, K, kblocks;
+};
+
+hipError_t launch_fp8_block_quant(const BlockQuantParams& p, int dtype, int block_rows, hipStream_t stream);
+
+struct BlockMatmulParams {
+  const unsigned char* x;
+  const float* xsc;
+  const unsigned char* w;
+  const float* wsc;
+  const void* bias;
+  void* out;
+  int64_t xs, ws, os;            // row strides of x, w and out
+  int64_t xsc_m, xsc_k, wsc_n, wsc_k;
+  int M, N, K, kblocks;
+  int bias_wide;
+  int exact;
+  int cu_count;
+  float* partial;                // split K: [split][M][N] sums
+  int splits;                    // parts K is cut into
+  int blocks_per_split;
+};
+
+size_t fp8_block_matmul_workspace(const BlockMatmulParams& p);
+hipError_t launch_fp8_block_matmul(const BlockMatmulParams& p, int out_dtype, size_t workspace_bytes, hipStream_t stream);
+
 }  // namespace xdit
