@@ -32,7 +32,8 @@ def _hipcc():
 
 
 # per-file additions; the prologue reproduces separately rounded fp32 products and sums
-EXTRA_FLAGS = {"qk_prologue.hip": ["-ffp-contract=off"]}
+# the block-scaled product's sums leave the matrix cores for a multiply-add, which reads no accumulation registers
+EXTRA_FLAGS = {"qk_prologue.hip": ["-ffp-contract=off"], "fp8_block_matmul.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _compile(src):

@@ -11,6 +11,11 @@
 // 16x16x32 form does the same, at a third of the rate): on random bytes a block's sum is off by 305 units of 2^-24 of its terms'
 // sizes on average, 2900 at most.  Behind a rounding to bf16 or fp16 that is out of sight; for fp32 results, or where the
 // caller asks for it, both operands are widened to fp16, which is exact, and the fp16 instructions sum within 5 units.
+#include <atomic>
+#include <type_traits>
+
+#include "attn_split.h"
+#include "attn_tiles.h"
 #include "block_params.h"
 #include "row_ops.h"
 
@@ -18,92 +23,247 @@ namespace xdit {
 
 namespace bmm {
 
-// The 32 bytes at k of a row, zeros from K on (K is a multiple of 16).
-__device__ __forceinline__ i32x8 load_k32(const unsigned char* row, int k, int K) {
-  i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-  if (k < K) lo = *(const i32x4*)(row + k);
-  if (k + 16 < K) hi = *(const i32x4*)(row + k + 16);
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-// Sum over the 128 k of a block: 16 x 16 outputs.
+// Eight bytes as fp16, exactly.
 __device__ __forceinline__ f16x8 widen8(int lo, int hi) {
   const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
   const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
   return (f16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-template <bool EXACT>
-__device__ __forceinline__ f32x4 block_sum(const i32x8& a, const i32x8& b) {
-  f32x4 d = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (!EXACT) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, d, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-  for (int t = 0; t < 4; t++) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(a[2 * t], a[2 * t + 1]), widen8(b[2 * t], b[2 * t + 1]), d, 0, 0, 0);
-  return d;
-}
-
 __device__ __forceinline__ float bias_at(const BlockMatmulParams& p, int out_dtype_bits, int n) {
   if (p.bias_wide) return ((const float*)p.bias)[n];
   return out_dtype_bits == 0 ? (float)((const __bf16*)p.bias)[n] : (float)((const _Float16*)p.bias)[n];
 }
 template <typename T> constexpr int kIsHalf = __is_same(T, _Float16) ? 1 : 0;
 
-// Four wavefronts, 64 x 64 outputs, operands straight from global memory.
-template <typename T, bool EXACT>
-__global__ __launch_bounds__(256) void matmul_simple_kernel(const BlockMatmulParams p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// ---- the tiled kernel --------------------------------------------------------------------------------
+// A workgroup of WN x WM wavefronts computes BN x BM outputs (n x m), a wavefront 16 TN x 16 TM of them.  The operands'
+// 128-byte row pieces of a block of K stream through LDS in STAGES buffers, filled by direct global -> LDS loads of 16 bytes
+// a lane; the scales of the block (BM of x, one or two of w) travel with them.  A buffer is a plain array of 128-byte
+// rows whose eight 16-byte chunks are stored in the order chunk ^ (row / 2 % 8): sixteen consecutive rows' equal chunks, what a
+// fragment read fetches at a time, then lie in sixteen different places of the 256 bytes that LDS serves per clock.
+template <int BN_, int BM_, int WN_, int WM_, int STAGES_>
+struct Shape {
+  static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, STAGES = STAGES_;
+  static constexpr int NW = WN * WM;                  // wavefronts
+  static constexpr int TN = BN / WN / 16, TM = BM / WM / 16;
+  static constexpr int PIECES = (BN + BM) / 8;        // 1 KiB pieces of 8 rows per stage
+  static constexpr int LOADS = PIECES / NW;           // ... per wavefront
+  static constexpr int W_BYTES = BN * 128, X_BYTES = BM * 128;
+  static constexpr int SC_X = W_BYTES + X_BYTES;      // scales of x
+  static constexpr int SC_W = SC_X + BM * 4;          // scales of w, 64 of them (lane % (BN / 128))
+  static constexpr int STAGE_BYTES = SC_W + 256;
+  static constexpr int LDS = STAGES * STAGE_BYTES;
+  static_assert(BN % (32 * WN) == 0 && BM % (32 * WM) == 0 && BM % 64 == 0 && PIECES % NW == 0 && (BN / 8) % NW == 0, "pieces are of one operand");
+  static_assert(BM / 64 < NW && NW % 2 == 0, "the wavefronts behind the first BM / 64 fetch the scales of w");
+  static_assert(BN >= 128 ? (BN / WN) <= 128 : true, "a wavefront's n lie in one block of 128");
+};
+
+// 4 bytes a lane from 64-bit addresses straight into LDS at lds + 4 lane.
+__device__ __forceinline__ void load_lds_4(const void* p, unsigned lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, off"
+      :
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p)
+      : "memory", "m0");
+}
+// At most N of this wavefront's loads are under way, and all of its LDS reads are done.
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ i32x8 zero_from(const i32x8& v, int valid) {  // keeps the first `valid` (0, 16 or 32) bytes
+  i32x8 r = v;
+#pragma unroll
+  for (int i = 0; i < 4; i++) { r[i] = valid > 0 ? r[i] : 0; r[4 + i] = valid > 16 ? r[4 + i] : 0; }
+  return r;
+}
+
+// The 128 k of 16 rows as a matrix instruction takes them: bytes, or widened to fp16.
+template <bool EXACT> struct Operand;
+template <> struct Operand<false> {
+  i32x8 v;
+  __device__ __forceinline__ void set(const i32x8& x) { v = x; }
+};
+template <> struct Operand<true> {
+  f16x8 v[4];
+  __device__ __forceinline__ void set(const i32x8& x) {
+#pragma unroll
+    for (int t = 0; t < 4; t++) v[t] = widen8(x[2 * t], x[2 * t + 1]);
+  }
+};
+// 16 x 16 outputs summed over a block.
+__device__ __forceinline__ f32x4 block_sum(const Operand<false>& a, const Operand<false>& b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 block_sum(const Operand<true>& a, const Operand<true>& b) {
+  f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < 4; t++) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[t], b.v[t], d, 0, 0, 0);
+  return d;
+}
+
+// Tile of the problem that workgroup `w` computes.  Workgroups go round-robin to the 8 XCDs; each XCD takes a contiguous
+// range of an order in which 32 consecutive tiles, what it runs at once, are a patch of 8 x 4 tiles (m x n), so that its L2
+// serves every row panel to 4 and every column panel to 8 of them.
+__device__ __forceinline__ bool tile_of(int w, int tiles_n, int tiles_m, int& tn, int& tm) {
+  const int total = tiles_n * tiles_m;
+  const int i = xcd_tile_index(w, (total + 7) / 8);
+  if (i >= total) return false;
+  const int band = i / (8 * tiles_n);
+  const int height = min(8, tiles_m - 8 * band);
+  const int r = i - band * 8 * tiles_n;
+  tn = r / height;
+  tm = 8 * band + r - tn * height;
+  return true;
+}
+
+template <typename T, bool EXACT, typename S>
+__global__ __launch_bounds__(64 * S::NW) void matmul_tiled_kernel(const BlockMatmulParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int l16 = lane & 15, quad = lane >> 4;
-  const int n0 = blockIdx.x * 64 + (wave & 1) * 32, m0 = blockIdx.y * 64 + (wave >> 1) * 32;
-  const unsigned char* wrow[2];
-  const unsigned char* xrow[2];
-  int m[2];
-  f32x4 acc[2][2] = {};
+  int tile_n, tile_m;
+  if (!tile_of(blockIdx.x, (p.N + S::BN - 1) / S::BN, (p.M + S::BM - 1) / S::BM, tile_n, tile_m)) return;
+  const int n0 = tile_n * S::BN, m0 = tile_m * S::BM;
+  const int kb0 = blockIdx.y * p.blocks_per_split, kb1 = min(p.kblocks, kb0 + p.blocks_per_split);
+
+  // ---- loads of a stage: piece g = wave + NW i holds rows 8 g .. 8 g + 7 of [w tile; x tile]
+  const unsigned lds0 = (unsigned)(uintptr_t)(XDIT_LDS unsigned char*)smem;
+  const int piece_row = lane >> 3;
+  const unsigned chunk = (unsigned)((lane & 7) ^ ((4 * wave + (lane >> 4)) & 7)) * 16;   // NW is even: a wavefront's pieces have one parity
+  const unsigned char* wbase = p.w + (int64_t)n0 * p.ws + (int64_t)kb0 * 128;
+  const unsigned char* xbase = p.x + (int64_t)m0 * p.xs + (int64_t)kb0 * 128;
+  const int wlast = min(S::BN, p.N - n0) - 1, xlast = min(S::BM, p.M - m0) - 1;  // rows beyond the matrix re-read its last one
+  const bool xscale = wave < S::BM / 64;
+  const float* sc = xscale ? p.xsc + (int64_t)(m0 + min(64 * wave + lane, xlast)) * p.xsc_m + (int64_t)kb0 * p.xsc_k
+                           : p.wsc + (int64_t)min((n0 >> 7) + (lane % (S::BN > 128 ? S::BN / 128 : 1)), (p.N - 1) >> 7) * p.wsc_n + (int64_t)kb0 * p.wsc_k;
+  const int64_t sc_step = xscale ? p.xsc_k : p.wsc_k;
+  const unsigned sc_dst = xscale ? S::SC_X + 256 * wave : S::SC_W;
+  int k_left = p.K - kb0 * 128;   // of the next stage to be requested
+  auto request = [&](int stage) {
+    const unsigned dst = lds0 + stage * S::STAGE_BYTES;
+    const int kmax = k_left >= 128 ? 112 : k_left - 16;   // chunks beyond K re-read the last one (and are not used)
+    const unsigned c = min((int)chunk, kmax);
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    wrow[i] = p.w + (int64_t)min(n0 + 16 * i + l16, p.N - 1) * p.ws;
-    m[i] = min(m0 + 16 * i + l16, p.M - 1);
-    xrow[i] = p.x + (int64_t)m[i] * p.xs;
-  }
-  const int nb[2] = {min(n0, p.N - 1) >> 7, min(n0 + 16, p.N - 1) >> 7};
-  for (int kb = 0; kb < p.kblocks; kb++) {
-    const int k = kb * 128 + quad * 32;
-    i32x8 a[2], b[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) { a[i] = load_k32(wrow[i], k, p.K); b[i] = load_k32(xrow[i], k, p.K); }
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const float xs = p.xsc[m[j] * p.xsc_m + kb * p.xsc_k];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const float s = xs * p.wsc[nb[i] * p.wsc_n + kb * p.wsc_k];
-        const f32x4 d = block_sum<EXACT>(a[i], b[j]);
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(d[e], s, acc[i][j][e]);
-      }
+    for (int i = 0; i < S::LOADS; i++) {
+      const int g = wave + S::NW * i;
+      const bool second = S::NW * i >= S::BN / 8;
+      const int row = 8 * g + piece_row - (second ? S::BN : 0);
+      if (!second) load_lds_16(wbase, __umul24((unsigned)min(row, wlast), (unsigned)p.ws) + c, dst + g * 1024);
+      else load_lds_16(xbase, __umul24((unsigned)min(row, xlast), (unsigned)p.xs) + c, dst + g * 1024);
     }
+    load_lds_4(sc, dst + sc_dst);
+    wbase += 128;
+    xbase += 128;
+    sc += sc_step;
+    k_left -= 128;
+  };
+
+  // ---- fragments: lane (l16, quad) holds bytes 32 quad .. + 31 of its row
+  const int wn = wave % S::WN, wm = wave / S::WN;
+  const int swz = (l16 >> 1) & 7;
+  const int off0 = l16 * 128 + (((2 * quad) ^ swz) << 4), off1 = l16 * 128 + (((2 * quad + 1) ^ swz) << 4);
+  const int a_row = wn * S::TN * 16 * 128, b_row = S::W_BYTES + wm * S::TM * 16 * 128;
+  auto fragment = [&](const unsigned char* rows) {
+    const i32x4 lo = *(const i32x4*)(rows + off0), hi = *(const i32x4*)(rows + off1);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+
+  f32x4 acc[S::TN][S::TM] = {};
+  // The sums of row i + 1 of the tile are under way while those of row i are scaled and added: a wavefront issues in order, and
+  // a result is there some ten instructions after its matrix instruction.
+  auto compute = [&](const unsigned char* buf, int valid, auto tail) {
+    Operand<EXACT> b[S::TM], a;
+    float s[S::TM];
+    f32x4 d[2][S::TM];
+    a.set(fragment(buf + a_row));
+    const float ws = *(const float*)(buf + S::SC_W + 4 * (S::BN > 128 ? (wn * S::TN * 16) >> 7 : 0));
+#pragma unroll
+    for (int j = 0; j < S::TM; j++) {
+      i32x8 v = fragment(buf + b_row + j * 2048);
+      if constexpr (decltype(tail)::value) v = zero_from(v, valid - 32 * quad);
+      b[j].set(v);
+    }
+#pragma unroll
+    for (int j = 0; j < S::TM; j++) s[j] = *(const float*)(buf + S::SC_X + 4 * ((wm * S::TM + j) * 16 + l16)) * ws;
+#pragma unroll
+    for (int i = 0; i <= S::TN; i++) {
+      i32x8 next;
+      if (i + 1 < S::TN) next = fragment(buf + a_row + (i + 1) * 2048);
+#pragma unroll
+      for (int j = 0; j < S::TM; j++) {
+        if (i < S::TN) d[i & 1][j] = block_sum(a, b[j]);
+        if (i > 0) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[i - 1][j][e] = __builtin_fmaf(d[(i - 1) & 1][j][e], s[j], acc[i - 1][j][e]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (i + 1 < S::TN) a.set(next);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < S::STAGES - 1; i++)
+    if (kb0 + i < kb1) request(i);
+  int stage = 0;
+  auto arrive = [&](int kb) {   // block kb is in its buffer for every wavefront, the buffer before it is requested anew
+    if (S::STAGES > 2 && kb + S::STAGES - 2 < kb1) wait_loads<(S::LOADS + 1) * (S::STAGES - 2)>();
+    else wait_loads<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (kb + S::STAGES - 1 < kb1) request(stage == 0 ? S::STAGES - 1 : stage - 1);
+  };
+  const int whole = min(kb1, p.K >> 7);
+  for (int kb = kb0; kb < whole; kb++) {
+    arrive(kb);
+    compute(smem + stage * S::STAGE_BYTES, 128, std::false_type{});
+    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
   }
+  if (whole < kb1) {   // the last block, cut off by K
+    arrive(whole);
+    compute(smem + stage * S::STAGE_BYTES, p.K - whole * 128, std::true_type{});
+  }
+
+  // ---- accumulator element e of lane (l16, quad): m = l16, n = 4 quad + e
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
-    const int row = m0 + 16 * j + l16;
-    if (row >= p.M) continue;
+  for (int j = 0; j < S::TM; j++) {
+    const int m = m0 + (wm * S::TM + j) * 16 + l16;
+    if (m >= p.M) continue;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < S::TN; i++) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int n = n0 + 16 * i + 4 * quad + e;
-        if (n < p.N) ((T*)p.out)[(int64_t)row * p.os + n] = (T)(acc[i][j][e] + (p.bias != nullptr ? bias_at(p, kIsHalf<T>, n) : 0.f));
+        const int n = n0 + (wn * S::TN + i) * 16 + 4 * quad + e;
+        if (n >= p.N) continue;
+        if (p.splits > 1) p.partial[((int64_t)blockIdx.y * p.M + m) * p.N + n] = acc[i][j][e];
+        else ((T*)p.out)[(int64_t)m * p.os + n] = (T)(acc[i][j][e] + (p.bias != nullptr ? bias_at(p, kIsHalf<T>, n) : 0.f));
       }
     }
   }
 }
 
-template <typename T>
-static hipError_t run(const BlockMatmulParams& p, size_t workspace_bytes, hipStream_t stream) {
-  const int64_t down = ((int64_t)p.M + 63) / 64;
-  if (down > 65535) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)((p.N + 63) / 64), (unsigned)down), block(256);
-  if (p.exact) hipLaunchKernelGGL((matmul_simple_kernel<T, true>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((matmul_simple_kernel<T, false>), grid, block, 0, stream, p);
+template <typename T, bool EXACT, typename S>
+static hipError_t launch_tiled(const BlockMatmulParams& p, hipStream_t stream) {
+  const int64_t tiles = (int64_t)((p.N + S::BN - 1) / S::BN) * ((p.M + S::BM - 1) / S::BM);
+  if (tiles > 0x3fffffff) return hipErrorInvalidValue;
+  static std::atomic<bool> lds_ready[kMaxDevices];
+  const int slot = current_device_slot();
+  if (S::LDS > 65536 && !lds_ready[slot].load(std::memory_order_relaxed)) {  // > 64 KiB of dynamic LDS must be enabled once per kernel and device
+    const hipError_t e = hipFuncSetAttribute((const void*)matmul_tiled_kernel<T, EXACT, S>, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
+    if (e != hipSuccess) return e;
+    lds_ready[slot].store(true, std::memory_order_relaxed);
+  }
+  hipLaunchKernelGGL((matmul_tiled_kernel<T, EXACT, S>), dim3((unsigned)((tiles + 7) / 8 * 8), (unsigned)p.splits), dim3(64 * S::NW), S::LDS, stream, p);
   return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t run(BlockMatmulParams p, size_t workspace_bytes, hipStream_t stream) {
+  p.splits = 1;
+  p.blocks_per_split = p.kblocks;
+  if (p.exact) return launch_tiled<T, true, Shape<128, 128, 2, 2, 2>>(p, stream);
+  return launch_tiled<T, false, Shape<256, 256, 2, 4, 2>>(p, stream);
 }
 
 }  // namespace bmm
