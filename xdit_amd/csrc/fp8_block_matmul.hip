@@ -202,8 +202,7 @@ __global__ __launch_bounds__(64 * S::NW) void matmul_tiled_kernel(const BlockMat
   int k_left = p.K - kb0 * 128;   // of the next stage to be requested
   auto request = [&](int stage) {
     const unsigned dst = lds0 + stage * S::STAGE_BYTES;
-    const int kmax = k_left >= 128 ? 112 : k_left - 16;   // chunks beyond K re-read the last one (and are not used)
-    const unsigned c = min((int)chunk, kmax);
+    const unsigned c = min((int)chunk, k_left >= 128 ? 112 : k_left - 16);   // chunks beyond K re-read the last one (and are not used)
 #pragma unroll
     for (int i = 0; i < S::LOADS; i++) {
       const int g = wave + S::NW * i;
@@ -233,7 +232,7 @@ __global__ __launch_bounds__(64 * S::NW) void matmul_tiled_kernel(const BlockMat
   f32x4 acc[S::TN][S::TM] = {};
   // The sums of row i + 1 of the tile are under way while those of row i are scaled and added: a wavefront issues in order, and
   // a result is there some ten instructions after its matrix instruction.
-  auto compute = [&](const unsigned char* buf, int valid, auto tail) {
+  auto compute = [&](const unsigned char* buf, int valid, auto tail, int into) {
     Operand<EXACT> b[S::TM], a;
     float s[S::TM];
     f32x4 d[2][S::TM];
@@ -251,6 +250,7 @@ __global__ __launch_bounds__(64 * S::NW) void matmul_tiled_kernel(const BlockMat
     for (int i = 0; i <= S::TN; i++) {
       i32x8 next;
       if (i + 1 < S::TN) next = fragment(buf + a_row + (i + 1) * 2048);
+      if (i == 0 && into >= 0) request(into);   // uniform
 #pragma unroll
       for (int j = 0; j < S::TM; j++) {
         if (i < S::TN) d[i & 1][j] = block_sum(a, b[j]);
@@ -267,26 +267,27 @@ __global__ __launch_bounds__(64 * S::NW) void matmul_tiled_kernel(const BlockMat
   for (int i = 0; i < S::STAGES - 1; i++)
     if (kb0 + i < kb1) request(i);
   int stage = 0;
-  auto arrive = [&](int kb) {   // block kb is in its buffer for every wavefront, the buffer before it is requested anew
+  auto arrive = [&](int kb) {   // block kb is in its buffer for every wavefront -> the buffer that is free now, -1: no further block
     if (S::STAGES > 2 && kb + S::STAGES - 2 < kb1) wait_loads<(S::LOADS + 1) * (S::STAGES - 2)>();
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (kb + S::STAGES - 1 < kb1) request(stage == 0 ? S::STAGES - 1 : stage - 1);
+    return kb + S::STAGES - 1 < kb1 ? (stage == 0 ? S::STAGES - 1 : stage - 1) : -1;
   };
   const int whole = min(kb1, p.K >> 7);
   for (int kb = kb0; kb < whole; kb++) {
-    arrive(kb);
-    compute(smem + stage * S::STAGE_BYTES, 128, std::false_type{});
+    const int into = arrive(kb);
+    compute(smem + stage * S::STAGE_BYTES, 128, std::false_type{}, into);
     stage = stage + 1 == S::STAGES ? 0 : stage + 1;
   }
   if (whole < kb1) {   // the last block, cut off by K
     arrive(whole);
-    compute(smem + stage * S::STAGE_BYTES, p.K - whole * 128, std::true_type{});
+    compute(smem + stage * S::STAGE_BYTES, p.K - whole * 128, std::true_type{}, -1);
   }
 
   // ---- accumulator element e of lane (l16, quad): m = l16, n = 4 quad + e.  Sixteen rows at a time go through LDS, so
   // that they leave as whole lines (element by element this end took a third of a 5120-deep product).
+  wait_loads<0>();
   __builtin_amdgcn_s_barrier();   // no wavefront reads its buffers any more
   if (p.splits > 1) put_rows<float, S>(acc, smem, p.partial + (int64_t)blockIdx.y * p.M * p.N, p.N, nullptr, 0, p, n0 + wn * S::TN * 16, m0 + wm * S::TM * 16, wave, lane);
   else put_rows<T, S>(acc, smem, (T*)p.out, p.os, p.bias, kIsHalf<T>, p, n0 + wn * S::TN * 16, m0 + wm * S::TM * 16, wave, lane);
@@ -307,17 +308,162 @@ static hipError_t launch_tiled(const BlockMatmulParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// ---- few rows ----------------------------------------------------------------------------------------
+// Up to 16 MT rows: what counts is reading w once.  A workgroup takes 16 n, its NW wavefronts the blocks of K in turn, so
+// that together they read NW whole lines of a row of w; straight into registers, four blocks ahead.  Sums are exact here: the
+// matrix cores are idle anyway.  The wavefronts' sums are joined in LDS, in their order.
+template <typename T, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void matmul_rows_kernel(const BlockMatmulParams p) {
+  __shared__ __align__(16) float part[NW][16 * MT][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int l16 = lane & 15, quad = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int kb0 = blockIdx.y * p.blocks_per_split, kb1 = min(p.kblocks, kb0 + p.blocks_per_split);
+  const unsigned char* w = p.w + (int64_t)min(n0 + l16, p.N - 1) * p.ws + 16 * quad;
+  const unsigned char* x[MT];
+  const float* xsc[MT];
+#pragma unroll
+  for (int j = 0; j < MT; j++) {
+    const int m = min(16 * j + l16, p.M - 1);
+    x[j] = p.x + (int64_t)m * p.xs + 16 * quad;
+    xsc[j] = p.xsc + m * p.xsc_m;
+  }
+  const float* wsc = p.wsc + (n0 >> 7) * p.wsc_n;
+  f32x4 acc[MT] = {};
+  constexpr int AHEAD = 4;
+  struct Block { i32x8 a, b[MT]; float s[MT], ws; };
+  auto load = [&](Block& t, int kb) {
+    auto chunks = [&](const unsigned char* r) {
+      const i32x4 lo = *(const i32x4*)(r + (int64_t)kb * 128), hi = *(const i32x4*)(r + (int64_t)kb * 128 + 64);
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    t.a = chunks(w);
+    t.ws = wsc[kb * p.wsc_k];
+#pragma unroll
+    for (int j = 0; j < MT; j++) { t.b[j] = chunks(x[j]); t.s[j] = xsc[j][kb * p.xsc_k]; }
+  };
+  auto add = [&](const Block& t) {
+    Operand<true> a, b;
+    a.set(t.a);
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+      b.set(t.b[j]);
+      const f32x4 d = block_sum(a, b);
+      const float s = t.s[j] * t.ws;
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[j][e] = __builtin_fmaf(d[e], s, acc[j][e]);
+    }
+  };
+  const int whole = min(kb1, p.K >> 7);
+  int kb = kb0 + wave;
+  for (; kb + (AHEAD - 1) * NW < whole; kb += AHEAD * NW) {
+    Block t[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) load(t[u], kb + u * NW);
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) add(t[u]);
+  }
+  for (; kb < whole; kb += NW) {
+    Block t;
+    load(t, kb);
+    add(t);
+  }
+  if (kb < kb1) {   // the last block, cut off by K: its chunks beyond re-read the first and count as zeros of x
+    const int valid = p.K - kb * 128 - 16 * quad;   // bytes from this lane's first chunk on
+    Block t;
+    auto chunks = [&](const unsigned char* r) {
+      const unsigned char* at = r + (int64_t)kb * 128;
+      const i32x4 lo = *(const i32x4*)(at - (valid > 0 ? 0 : 16 * quad)), hi = *(const i32x4*)(at + (valid > 64 ? 64 : -16 * quad));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    t.a = chunks(w);
+    t.ws = wsc[kb * p.wsc_k];
+#pragma unroll
+    for (int j = 0; j < MT; j++) { t.b[j] = zero_from(chunks(x[j]), valid); t.s[j] = xsc[j][kb * p.xsc_k]; }
+    add(t);
+  }
+#pragma unroll
+  for (int j = 0; j < MT; j++) *(f32x4*)&part[wave][16 * j + l16][4 * quad] = acc[j];
+  __syncthreads();
+  for (int t = threadIdx.x; t < 256 * MT; t += 64 * NW) {
+    const int m = t >> 4, n = n0 + (t & 15);
+    if (m >= p.M || n >= p.N) continue;
+    float v = part[0][m][t & 15];
+#pragma unroll
+    for (int u = 1; u < NW; u++) v += part[u][m][t & 15];
+    if (p.splits > 1) p.partial[((int64_t)blockIdx.y * p.M + m) * p.N + n] = v;
+    else ((T*)p.out)[m * p.os + n] = (T)(v + (p.bias != nullptr ? bias_at(p, kIsHalf<T>, n) : 0.f));
+  }
+}
+
+// The parts' sums in their order, plus bias.
+template <typename T>
+__global__ __launch_bounds__(256) void matmul_join_kernel(const BlockMatmulParams p) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int m = blockIdx.y;
+  if (n >= p.N) return;
+  const float* in = p.partial + (int64_t)m * p.N + n;
+  float v = 0.f;
+  for (int i = 0; i < p.splits; i++) v += in[(int64_t)i * p.M * p.N];
+  ((T*)p.out)[m * p.os + n] = (T)(v + (p.bias != nullptr ? bias_at(p, kIsHalf<T>, (int)n) : 0.f));
+}
+
+template <typename T, int MT, int NW>
+static void launch_rows(const BlockMatmulParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL((matmul_rows_kernel<T, MT, NW>), dim3((unsigned)((p.N + 15) / 16), (unsigned)p.splits), dim3(64 * NW), 0, stream, p);
+}
+
+// How a product is run.
+enum Kernel { ROWS16, ROWS32, ROWS64, TILE64, TILE128, TILE256 };
+struct Plan { Kernel kernel; int splits; };
+
+static Plan plan_of(const BlockMatmulParams& p) {
+  const int cus = resident_cus(p.cu_count);
+  Plan r = {TILE256, 1};
+  if (p.M <= 64) {
+    r.kernel = p.M <= 16 ? ROWS16 : p.M <= 32 ? ROWS32 : ROWS64;
+    const int64_t groups = (p.N + 15) / 16;
+    r.splits = (int)(2 * cus / groups);
+  } else if ((int64_t)p.M * p.N < (int64_t)cus * 64 * 64 * 2) {
+    r.kernel = TILE64;
+  } else if ((int64_t)p.M * p.N < (int64_t)cus * 128 * 128 * 2 || p.exact) {
+    r.kernel = TILE128;
+  }
+  if (r.splits > p.kblocks / 8) r.splits = p.kblocks / 8;
+  if (r.splits < 1) r.splits = 1;
+  return r;
+}
+
+template <typename T, bool EXACT>
+static hipError_t launch_tile(const BlockMatmulParams& p, Kernel k, hipStream_t stream) {
+  if (k == TILE64) return launch_tiled<T, EXACT, Shape<64, 64, 2, 2, 4>>(p, stream);
+  if (k == TILE128 || EXACT) return launch_tiled<T, EXACT, Shape<128, 128, 2, 2, 2>>(p, stream);
+  return launch_tiled<T, false, Shape<256, 256, 2, 4, 2>>(p, stream);
+}
+
 template <typename T>
 static hipError_t run(BlockMatmulParams p, size_t workspace_bytes, hipStream_t stream) {
-  p.splits = 1;
-  p.blocks_per_split = p.kblocks;
-  if (p.exact) return launch_tiled<T, true, Shape<128, 128, 2, 2, 2>>(p, stream);
-  return launch_tiled<T, false, Shape<256, 256, 2, 4, 2>>(p, stream);
+  const Plan plan = plan_of(p);
+  p.splits = (size_t)plan.splits * p.M * p.N * 4 <= workspace_bytes ? plan.splits : 1;
+  p.blocks_per_split = (p.kblocks + p.splits - 1) / p.splits;
+  p.splits = (p.kblocks + p.blocks_per_split - 1) / p.blocks_per_split;
+  hipError_t e = hipSuccess;
+  if (plan.kernel == ROWS16) launch_rows<T, 1, 8>(p, stream);
+  else if (plan.kernel == ROWS32) launch_rows<T, 2, 8>(p, stream);
+  else if (plan.kernel == ROWS64) launch_rows<T, 4, 8>(p, stream);
+  else e = p.exact ? launch_tile<T, true>(p, plan.kernel, stream) : launch_tile<T, false>(p, plan.kernel, stream);
+  if (e == hipSuccess) e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  hipLaunchKernelGGL((matmul_join_kernel<T>), dim3((unsigned)((p.N + 255) / 256), (unsigned)p.M), dim3(256), 0, stream, p);
+  return hipGetLastError();
 }
 
 }  // namespace bmm
 
-size_t fp8_block_matmul_workspace(const BlockMatmulParams& p) { return 0; }
+size_t fp8_block_matmul_workspace(const BlockMatmulParams& p) {
+  const int splits = bmm::plan_of(p).splits;
+  return splits > 1 ? (size_t)splits * p.M * p.N * 4 : 0;
+}
 
 hipError_t launch_fp8_block_matmul(const BlockMatmulParams& p, int out_dtype, size_t workspace_bytes, hipStream_t stream) {
   if (out_dtype == 0) return bmm::run<__bf16>(p, workspace_bytes, stream);
