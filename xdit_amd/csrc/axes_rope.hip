@@ -198,21 +198,22 @@ __global__ __launch_bounds__(256) void axes_rope_bwd_kernel(const AxesRopeParams
   }
 }
 
-// The workgroups' sums in their order: 8 columns x 32 runs of them per workgroup.
+// The workgroups' sums in a fixed order, 64 runs of every 64th and then the runs; 4 columns per workgroup.
 template <typename T>
 __global__ __launch_bounds__(256) void axes_rope_bwd_finish_kernel(const AxesRopeParams p) {
-  __shared__ float part[32][9];
+  __shared__ float part[64][5];
   const int t = blockIdx.y;
   const RopeTensor& q = p.t[t];
-  const int col = blockIdx.x * 8 + (threadIdx.x & 7), run = threadIdx.x >> 3;
+  if (q.dweight == nullptr) return;
+  const int col = blockIdx.x * 4 + (threadIdx.x & 3), run = threadIdx.x >> 2;
   const int n = p.head_groups * p.token_groups;
   float s = 0.f;
-  for (int i = run; i < n; i += 32) s += p.partial[((int64_t)i * 2 + t) * p.D + col];
-  part[run][threadIdx.x & 7] = s;
+#pragma unroll 8
+  for (int i = run; i < n; i += 64) s += p.partial[((int64_t)i * 2 + t) * p.D + col];
+  part[run][threadIdx.x & 3] = s;
   __syncthreads();
-  if (run != 0 || q.dweight == nullptr) return;
-  s = 0.f;
-  for (int i = 0; i < 32; i++) s += part[i][threadIdx.x & 7];
+  if (run != 0) return;
+  for (int i = 1; i < 64; i++) s += part[i][threadIdx.x & 3];
   if (p.weight_wide) ((float*)q.dweight)[col] = s;
   else ((T*)q.dweight)[col] = (T)s;
 }
@@ -231,14 +232,15 @@ static hipError_t run(const AxesRopeParams& p, bool backward, hipStream_t stream
   else hipLaunchKernelGGL((axes_rope_bwd_kernel<T, false>), grid, block, 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.sums) return e;
-  hipLaunchKernelGGL((axes_rope_bwd_finish_kernel<T>), dim3((unsigned)(p.D / 8), (unsigned)p.tensors), block, 0, stream, p);
+  hipLaunchKernelGGL((axes_rope_bwd_finish_kernel<T>), dim3((unsigned)(p.D / 4), (unsigned)p.tensors), block, 0, stream, p);
   return hipGetLastError();
 }
 
 }  // namespace axrope
 
 // A wavefront takes all heads of its token where that leaves the chip some 4096 wavefronts, fewer heads otherwise
-// (one instruction's worth at least): the sines are computed again by each of them.
+// (one instruction's worth at least): the sines are computed again by each of them.  Backward: at most the 1024 workgroups
+// that the chip holds at once, each going over its tokens, so that there are few sums to add up.
 void axes_rope_plan(AxesRopeParams& p, bool backward) {
   int lpr = 1;
   while (lpr * 8 < p.D) lpr <<= 1;
@@ -253,7 +255,7 @@ void axes_rope_plan(AxesRopeParams& p, bool backward) {
   p.heads_per_wave = ((total + groups - 1) / groups + slots - 1) / slots * slots;
   p.head_groups = (total + p.heads_per_wave - 1) / p.heads_per_wave;
   const int64_t wgs = (tokens + 3) / 4;
-  p.token_groups = (int)(backward && wgs * p.head_groups > 2048 ? (2048 + p.head_groups - 1) / p.head_groups : wgs);
+  p.token_groups = (int)(backward && wgs * p.head_groups > 1024 ? (1024 + p.head_groups - 1) / p.head_groups : wgs);
 }
 
 hipError_t launch_axes_rope(const AxesRopeParams& p, int dtype, bool backward, hipStream_t stream) {

@@ -27,6 +27,7 @@ struct GatedNormParams {
   int norm, y_norm, fp8;
   int mod_wide, weight_wide;  // those parameters are fp32 beside 16-bit tensors
   float eps, y_eps, alpha, inv_c;
+  int rows_per_part;  // filled by the launcher
 };
 
 struct GatedNormBwdParams {

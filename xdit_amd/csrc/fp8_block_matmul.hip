@@ -12,6 +12,7 @@
 // sizes on average, 2900 at most.  Behind a rounding to bf16 or fp16 that is out of sight; for fp32 results, or where the
 // caller asks for it, both operands are widened to fp16, which is exact, and the fp16 instructions sum within 5 units.
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "attn_split.h"
@@ -46,16 +47,19 @@ struct Shape {
   static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, STAGES = STAGES_;
   static constexpr int NW = WN * WM;                  // wavefronts
   static constexpr int TN = BN / WN / 16, TM = BM / WM / 16;
-  static constexpr int PIECES = (BN + BM) / 8;        // 1 KiB pieces of 8 rows per stage
-  static constexpr int LOADS = PIECES / NW;           // ... per wavefront
+  static constexpr int W_LOADS = BN / 8 / NW;         // 1 KiB pieces of 8 rows per stage and wavefront, of w
+  static constexpr int X_LOADS = BM / 8 > NW ? BM / 8 / NW : 1;   // ... and of x (few rows: some pieces are fetched twice)
+  static constexpr int LOADS = W_LOADS + X_LOADS + 1; // ... and a load of scales
   static constexpr int W_BYTES = BN * 128, X_BYTES = BM * 128;
   static constexpr int SC_X = W_BYTES + X_BYTES;      // scales of x
-  static constexpr int SC_W = SC_X + BM * 4;          // scales of w, 64 of them (lane % (BN / 128))
+  static constexpr int SC_W = SC_X + (BM > 64 ? BM : 64) * 4;   // scales of w, 64 of them (lane % (BN / 128))
   static constexpr int STAGE_BYTES = SC_W + 256;
   static constexpr int LDS = STAGES * STAGE_BYTES;
-  static_assert(BN % (32 * WN) == 0 && BM % (32 * WM) == 0 && BM % 64 == 0 && PIECES % NW == 0 && (BN / 8) % NW == 0, "pieces are of one operand");
-  static_assert(BM / 64 < NW && NW % 2 == 0, "the wavefronts behind the first BM / 64 fetch the scales of w");
-  static_assert(BN >= 128 ? (BN / WN) <= 128 : true, "a wavefront's n lie in one block of 128");
+  static constexpr int SC_PIECES = BM > 64 ? BM / 64 : 1;
+  static_assert(BN % (16 * WN) == 0 && BM % (16 * WM) == 0 && (BN / 8) % NW == 0 && (BM / 8 % NW == 0 || NW % (BM / 8) == 0), "pieces");
+  static_assert(NW % 2 == 0 && (BM / 8) % 2 == 0, "a wavefront's pieces have one parity");
+  static_assert(SC_PIECES < NW, "the wavefronts behind the first fetch the scales of w");
+  static_assert(BN / WN <= 128 && 128 % (BN / WN) == 0, "a wavefront's n lie in one block of 128");
 };
 
 // 4 bytes a lane from 64-bit addresses straight into LDS at lds + 4 lane.
@@ -154,10 +158,10 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[S::TN][S::TM], unsig
     if (lines) {
       constexpr int E = 16 / sizeof(T), PER_ROW = WIDE / E;   // 16-byte pieces
 #pragma unroll
-      for (int k = 0; k < 16 * PER_ROW / 64; k++) {
+      for (int k = 0; k < (16 * PER_ROW + 63) / 64; k++) {
         const int r = (64 * k + lane) / PER_ROW, n = (64 * k + lane) % PER_ROW * E;
+        if (r >= rows) continue;   // at most 16
         const i32x4 v = *(const i32x4*)(mine + r * PITCH + n * sizeof(T));
-        if (r >= rows) continue;
         if (n + E <= width) {
           *(i32x4*)(dst + r * os + n) = v;
         } else {
@@ -187,14 +191,14 @@ __global__ __launch_bounds__(64 * S::NW) void matmul_tiled_kernel(const BlockMat
   const int n0 = tile_n * S::BN, m0 = tile_m * S::BM;
   const int kb0 = blockIdx.y * p.blocks_per_split, kb1 = min(p.kblocks, kb0 + p.blocks_per_split);
 
-  // ---- loads of a stage: piece g = wave + NW i holds rows 8 g .. 8 g + 7 of [w tile; x tile]
+  // ---- loads of a stage: piece g = wave + NW i holds rows 8 g .. 8 g + 7 of the tile of w (x)
   const unsigned lds0 = (unsigned)(uintptr_t)(XDIT_LDS unsigned char*)smem;
   const int piece_row = lane >> 3;
   const unsigned chunk = (unsigned)((lane & 7) ^ ((4 * wave + (lane >> 4)) & 7)) * 16;   // NW is even: a wavefront's pieces have one parity
   const unsigned char* wbase = p.w + (int64_t)n0 * p.ws + (int64_t)kb0 * 128;
   const unsigned char* xbase = p.x + (int64_t)m0 * p.xs + (int64_t)kb0 * 128;
   const int wlast = min(S::BN, p.N - n0) - 1, xlast = min(S::BM, p.M - m0) - 1;  // rows beyond the matrix re-read its last one
-  const bool xscale = wave < S::BM / 64;
+  const bool xscale = wave < S::SC_PIECES;
   const float* sc = xscale ? p.xsc + (int64_t)(m0 + min(64 * wave + lane, xlast)) * p.xsc_m + (int64_t)kb0 * p.xsc_k
                            : p.wsc + (int64_t)min((n0 >> 7) + (lane % (S::BN > 128 ? S::BN / 128 : 1)), (p.N - 1) >> 7) * p.wsc_n + (int64_t)kb0 * p.wsc_k;
   const int64_t sc_step = xscale ? p.xsc_k : p.wsc_k;
@@ -204,12 +208,14 @@ __global__ __launch_bounds__(64 * S::NW) void matmul_tiled_kernel(const BlockMat
     const unsigned dst = lds0 + stage * S::STAGE_BYTES;
     const unsigned c = min((int)chunk, k_left >= 128 ? 112 : k_left - 16);   // chunks beyond K re-read the last one (and are not used)
 #pragma unroll
-    for (int i = 0; i < S::LOADS; i++) {
+    for (int i = 0; i < S::W_LOADS; i++) {
       const int g = wave + S::NW * i;
-      const bool second = S::NW * i >= S::BN / 8;
-      const int row = 8 * g + piece_row - (second ? S::BN : 0);
-      if (!second) load_lds_16(wbase, __umul24((unsigned)min(row, wlast), (unsigned)p.ws) + c, dst + g * 1024);
-      else load_lds_16(xbase, __umul24((unsigned)min(row, xlast), (unsigned)p.xs) + c, dst + g * 1024);
+      load_lds_16(wbase, __umul24((unsigned)min(8 * g + piece_row, wlast), (unsigned)p.ws) + c, dst + g * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < S::X_LOADS; i++) {
+      const int g = S::BM / 8 >= S::NW ? wave + S::NW * i : wave % (S::BM / 8);
+      load_lds_16(xbase, __umul24((unsigned)min(8 * g + piece_row, xlast), (unsigned)p.xs) + c, dst + S::W_BYTES + g * 1024);
     }
     load_lds_4(sc, dst + sc_dst);
     wbase += 128;
@@ -268,7 +274,7 @@ __global__ __launch_bounds__(64 * S::NW) void matmul_tiled_kernel(const BlockMat
     if (kb0 + i < kb1) request(i);
   int stage = 0;
   auto arrive = [&](int kb) {   // block kb is in its buffer for every wavefront -> the buffer that is free now, -1: no further block
-    if (S::STAGES > 2 && kb + S::STAGES - 2 < kb1) wait_loads<(S::LOADS + 1) * (S::STAGES - 2)>();
+    if (S::STAGES > 2 && kb + S::STAGES - 2 < kb1) wait_loads<S::LOADS * (S::STAGES - 2)>();
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -308,137 +314,81 @@ static hipError_t launch_tiled(const BlockMatmulParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// ---- few rows ----------------------------------------------------------------------------------------
-// Up to 16 MT rows: what counts is reading w once.  A workgroup takes 16 n, its NW wavefronts the blocks of K in turn, so
-// that together they read NW whole lines of a row of w; straight into registers, four blocks ahead.  Sums are exact here: the
-// matrix cores are idle anyway.  The wavefronts' sums are joined in LDS, in their order.
-template <typename T, int MT, int NW>
-__global__ __launch_bounds__(64 * NW) void matmul_rows_kernel(const BlockMatmulParams p) {
-  __shared__ __align__(16) float part[NW][16 * MT][16];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int l16 = lane & 15, quad = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int kb0 = blockIdx.y * p.blocks_per_split, kb1 = min(p.kblocks, kb0 + p.blocks_per_split);
-  const unsigned char* w = p.w + (int64_t)min(n0 + l16, p.N - 1) * p.ws + 16 * quad;
-  const unsigned char* x[MT];
-  const float* xsc[MT];
-#pragma unroll
-  for (int j = 0; j < MT; j++) {
-    const int m = min(16 * j + l16, p.M - 1);
-    x[j] = p.x + (int64_t)m * p.xs + 16 * quad;
-    xsc[j] = p.xsc + m * p.xsc_m;
-  }
-  const float* wsc = p.wsc + (n0 >> 7) * p.wsc_n;
-  f32x4 acc[MT] = {};
-  constexpr int AHEAD = 4;
-  struct Block { i32x8 a, b[MT]; float s[MT], ws; };
-  auto load = [&](Block& t, int kb) {
-    auto chunks = [&](const unsigned char* r) {
-      const i32x4 lo = *(const i32x4*)(r + (int64_t)kb * 128), hi = *(const i32x4*)(r + (int64_t)kb * 128 + 64);
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    t.a = chunks(w);
-    t.ws = wsc[kb * p.wsc_k];
-#pragma unroll
-    for (int j = 0; j < MT; j++) { t.b[j] = chunks(x[j]); t.s[j] = xsc[j][kb * p.xsc_k]; }
-  };
-  auto add = [&](const Block& t) {
-    Operand<true> a, b;
-    a.set(t.a);
-#pragma unroll
-    for (int j = 0; j < MT; j++) {
-      b.set(t.b[j]);
-      const f32x4 d = block_sum(a, b);
-      const float s = t.s[j] * t.ws;
-#pragma unroll
-      for (int e = 0; e < 4; e++) acc[j][e] = __builtin_fmaf(d[e], s, acc[j][e]);
-    }
-  };
-  const int whole = min(kb1, p.K >> 7);
-  int kb = kb0 + wave;
-  for (; kb + (AHEAD - 1) * NW < whole; kb += AHEAD * NW) {
-    Block t[AHEAD];
-#pragma unroll
-    for (int u = 0; u < AHEAD; u++) load(t[u], kb + u * NW);
-#pragma unroll
-    for (int u = 0; u < AHEAD; u++) add(t[u]);
-  }
-  for (; kb < whole; kb += NW) {
-    Block t;
-    load(t, kb);
-    add(t);
-  }
-  if (kb < kb1) {   // the last block, cut off by K: its chunks beyond re-read the first and count as zeros of x
-    const int valid = p.K - kb * 128 - 16 * quad;   // bytes from this lane's first chunk on
-    Block t;
-    auto chunks = [&](const unsigned char* r) {
-      const unsigned char* at = r + (int64_t)kb * 128;
-      const i32x4 lo = *(const i32x4*)(at - (valid > 0 ? 0 : 16 * quad)), hi = *(const i32x4*)(at + (valid > 64 ? 64 : -16 * quad));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    t.a = chunks(w);
-    t.ws = wsc[kb * p.wsc_k];
-#pragma unroll
-    for (int j = 0; j < MT; j++) { t.b[j] = zero_from(chunks(x[j]), valid); t.s[j] = xsc[j][kb * p.xsc_k]; }
-    add(t);
-  }
-#pragma unroll
-  for (int j = 0; j < MT; j++) *(f32x4*)&part[wave][16 * j + l16][4 * quad] = acc[j];
-  __syncthreads();
-  for (int t = threadIdx.x; t < 256 * MT; t += 64 * NW) {
-    const int m = t >> 4, n = n0 + (t & 15);
-    if (m >= p.M || n >= p.N) continue;
-    float v = part[0][m][t & 15];
-#pragma unroll
-    for (int u = 1; u < NW; u++) v += part[u][m][t & 15];
-    if (p.splits > 1) p.partial[((int64_t)blockIdx.y * p.M + m) * p.N + n] = v;
-    else ((T*)p.out)[m * p.os + n] = (T)(v + (p.bias != nullptr ? bias_at(p, kIsHalf<T>, n) : 0.f));
-  }
-}
-
 // The parts' sums in their order, plus bias.
 template <typename T>
 __global__ __launch_bounds__(256) void matmul_join_kernel(const BlockMatmulParams p) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int m = blockIdx.y;
-  if (n >= p.N) return;
-  const float* in = p.partial + (int64_t)m * p.N + n;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, count = (int64_t)p.M * p.N;
+  if (i >= count) return;
+  const int64_t m = i / p.N;
+  const int n = (int)(i - m * p.N);
+  const float* in = p.partial + i;
   float v = 0.f;
-  for (int i = 0; i < p.splits; i++) v += in[(int64_t)i * p.M * p.N];
-  ((T*)p.out)[m * p.os + n] = (T)(v + (p.bias != nullptr ? bias_at(p, kIsHalf<T>, (int)n) : 0.f));
+#pragma unroll 4
+  for (int k = 0; k < p.splits; k++) v += in[k * count];
+  ((T*)p.out)[m * p.os + n] = (T)(v + (p.bias != nullptr ? bias_at(p, kIsHalf<T>, n) : 0.f));
 }
 
-template <typename T, int MT, int NW>
-static void launch_rows(const BlockMatmulParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL((matmul_rows_kernel<T, MT, NW>), dim3((unsigned)((p.N + 15) / 16), (unsigned)p.splits), dim3(64 * NW), 0, stream, p);
-}
+// ---- how a product is run ---------------------------------------------------------------------------
+// Seven shapes (with exact sums the first four and 128 x 128 in two buffers), each with K uncut or cut into some parts;
+// the one with the shortest estimated time is taken:
+//     start + sum over the rounds of workgroups [fix + blocks of K a workgroup * max(lat, workgroups on a compute unit * busy)],
+//     at least the bytes of x, w and out at the memory's rate, and for a cut K the second kernel's launch and its traffic.
+// lat is what a block takes a workgroup alone (its loads' way), busy what it costs a compute unit (its products), both in us.  The
+// constants are fitted to 4009 times of every option at 190 problems (1 to 12000 rows, 64 to 30720 columns, K 320 to
+// 13824; 16-bit results) and 1161 at 70 (exact sums); there the choice is 1.4 % (0.9 %) slower than the fastest option on
+// average, 14 % (10 %) at worst.  Shapes of 128 x 16, 128 x 32 and 128 x 256 would give another 0.2 %.
+struct Option { int bn, bm, per_cu; double lat, busy, fix; };
+static const Option kFast[] = {{64, 16, 3, 0.181, 0.118, 1.162}, {64, 32, 3, 0.226, 0.222, 1.044}, {64, 64, 2, 0.122, 0.231, 1.054}, {128, 64, 2, 0.393, 0.472, 0.935},
+                               {128, 128, 2, 0.763, 0.524, 0.328}, {128, 128, 1, 0.702, 0.400, 1.060}, {256, 256, 1, 0.559, 1.410, 2.624}};
+static const Option kExact[] = {{64, 16, 3, 0.201, 0.160, 0.962}, {64, 32, 3, 0.277, 0.305, 1.192}, {64, 64, 2, 0.363, 0.341, 0.898}, {128, 64, 2, 0.653, 0.594, 0.924},
+                                {128, 128, 2, 1.187, 0.938, 1.506}};
+constexpr int kMostSplits = 16;
 
-// How a product is run.
-enum Kernel { ROWS16, ROWS32, ROWS64, TILE64, TILE128, TILE256 };
-struct Plan { Kernel kernel; int splits; };
+struct Plan { int shape, splits; };
 
 static Plan plan_of(const BlockMatmulParams& p) {
-  const int cus = resident_cus(p.cu_count);
-  Plan r = {TILE256, 1};
-  if (p.M <= 64) {
-    r.kernel = p.M <= 16 ? ROWS16 : p.M <= 32 ? ROWS32 : ROWS64;
-    const int64_t groups = (p.N + 15) / 16;
-    r.splits = (int)(2 * cus / groups);
-  } else if ((int64_t)p.M * p.N < (int64_t)cus * 64 * 64 * 2) {
-    r.kernel = TILE64;
-  } else if ((int64_t)p.M * p.N < (int64_t)cus * 128 * 128 * 2 || p.exact) {
-    r.kernel = TILE128;
+  const Option* options = p.exact ? kExact : kFast;
+  const int count = p.exact ? 5 : 7;
+  const int64_t cus = resident_cus(p.cu_count);
+  const double moved = ((double)p.N + p.M) * p.K, written = (double)p.M * p.N;
+  const double rate = p.exact ? 7.3e6 : 8.4e6, join = p.exact ? 4.0 : 4.6, join_bytes = p.exact ? 0.67e-6 : 1.2e-6;   // bytes per us; us; us per sum
+  Plan best = {0, 1};
+  double best_us = 0.0;
+  for (int i = 0; i < count; i++) {
+    const Option& o = options[i];
+    const int64_t tiles = (int64_t)((p.N + o.bn - 1) / o.bn) * ((p.M + o.bm - 1) / o.bm);
+    static const int kCuts[] = {1, 2, 3, 4, 6, 8, 12, kMostSplits};
+    for (int cut : kCuts) {
+      if (cut > 1 && (cut > p.kblocks / 2 || tiles * cut > 6 * cus)) break;   // two blocks a part at least, and no cut where the chip is full
+      const int blocks = (p.kblocks + cut - 1) / cut, splits = (p.kblocks + blocks - 1) / blocks;
+      const int64_t groups = tiles * splits, round = cus * o.per_cu, rest = groups % round;
+      double us = (double)(groups / round) * (o.fix + blocks * fmax(o.lat, o.per_cu * o.busy));
+      if (rest > 0) us += o.fix + blocks * fmax(o.lat, (double)((rest + cus - 1) / cus) * o.busy);
+      us = fmax(us, (moved + (splits == 1 ? 2.0 * written : 0.0)) / rate + o.fix);
+      if (splits > 1) us += join + join_bytes * splits * written;
+      if (best_us == 0.0 || us < best_us) {
+        best_us = us;
+        best = {i, splits};
+      }
+    }
   }
-  if (r.splits > p.kblocks / 8) r.splits = p.kblocks / 8;
-  if (r.splits < 1) r.splits = 1;
-  return r;
+  return best;
 }
 
 template <typename T, bool EXACT>
-static hipError_t launch_tile(const BlockMatmulParams& p, Kernel k, hipStream_t stream) {
-  if (k == TILE64) return launch_tiled<T, EXACT, Shape<64, 64, 2, 2, 4>>(p, stream);
-  if (k == TILE128 || EXACT) return launch_tiled<T, EXACT, Shape<128, 128, 2, 2, 2>>(p, stream);
-  return launch_tiled<T, false, Shape<256, 256, 2, 4, 2>>(p, stream);
+static hipError_t launch_shape(const BlockMatmulParams& p, int shape, hipStream_t stream) {
+  switch (shape) {
+    case 0: return launch_tiled<T, EXACT, Shape<64, 16, 4, 1, 4>>(p, stream);
+    case 1: return launch_tiled<T, EXACT, Shape<64, 32, 4, 1, 4>>(p, stream);
+    case 2: return launch_tiled<T, EXACT, Shape<64, 64, 2, 2, 4>>(p, stream);
+    case 3: return launch_tiled<T, EXACT, Shape<128, 64, 4, 1, 3>>(p, stream);
+    case 4: return launch_tiled<T, EXACT, Shape<128, 128, 2, 2, 2>>(p, stream);
+  }
+  if constexpr (!EXACT) {
+    if (shape == 5) return launch_tiled<T, EXACT, Shape<128, 128, 2, 2, 4>>(p, stream);
+    if (shape == 6) return launch_tiled<T, EXACT, Shape<256, 256, 2, 4, 2>>(p, stream);
+  }
+  return hipErrorInvalidValue;
 }
 
 template <typename T>
@@ -447,14 +397,9 @@ static hipError_t run(BlockMatmulParams p, size_t workspace_bytes, hipStream_t s
   p.splits = (size_t)plan.splits * p.M * p.N * 4 <= workspace_bytes ? plan.splits : 1;
   p.blocks_per_split = (p.kblocks + p.splits - 1) / p.splits;
   p.splits = (p.kblocks + p.blocks_per_split - 1) / p.blocks_per_split;
-  hipError_t e = hipSuccess;
-  if (plan.kernel == ROWS16) launch_rows<T, 1, 8>(p, stream);
-  else if (plan.kernel == ROWS32) launch_rows<T, 2, 8>(p, stream);
-  else if (plan.kernel == ROWS64) launch_rows<T, 4, 8>(p, stream);
-  else e = p.exact ? launch_tile<T, true>(p, plan.kernel, stream) : launch_tile<T, false>(p, plan.kernel, stream);
-  if (e == hipSuccess) e = hipGetLastError();
+  const hipError_t e = p.exact ? launch_shape<T, true>(p, plan.shape, stream) : launch_shape<T, false>(p, plan.shape, stream);
   if (e != hipSuccess || p.splits == 1) return e;
-  hipLaunchKernelGGL((matmul_join_kernel<T>), dim3((unsigned)((p.N + 255) / 256), (unsigned)p.M), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((matmul_join_kernel<T>), dim3((unsigned)(((int64_t)p.M * p.N + 255) / 256)), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 

@@ -14,6 +14,7 @@
 // (with a scale or a gate per token the factor goes into the sum, and dscale, dshift, dgate are elementwise).
 // HBM-bound: forward one read of x and y and one write of h and n, backward one read of dh, dn, h, y and one
 // write of dx and dy.
+#include "attn_split.h"
 #include "block_params.h"
 #include "row_ops.h"
 
@@ -21,293 +22,339 @@ namespace xdit {
 
 namespace gnorm {
 
-// One workgroup of four wavefronts per row; a thread holds up to N chunks of 8 columns (thread, thread + 256, ...).
-template <typename T, int N>
-__global__ __launch_bounds__(256) void gated_norm_row_kernel(const GatedNormParams p) {
-  __shared__ float part[4][8];
-  const int64_t row = blockIdx.x;
-  const int b = (int)(row / p.S);
-  const int s = (int)(row - (int64_t)b * p.S);
-  const int chunks = p.C >> 3;
-  float h[N][8];
-  float ym = 0.f, yr = 1.f, m = 0.f, r = 1.f;
-  bool live[N];
-  int col[N];
+// A row is held by as many wavefronts as it has 512 columns, eight columns a thread, and a workgroup goes over the rows of one
+// part of one batch entry: modulation and gains stay in registers, folded to three vectors (gate alpha w_y, (1 + scale) w and
+// b (1 + scale) + shift), where fetching them for every row was two thirds of all traffic from the L2.  The next rows are on their
+// way while these are worked on.
+
+// Sums over the wavefronts of a workgroup of up to four values (k = 0 .. K-1) a wavefront has posted at part[k][wave]: sixteen
+// lanes read a value's entries, a DPP row adds them, and the total is broadcast from there.
+constexpr int kMaxWaves = 16;
+struct Posted { float v[4][kMaxWaves]; };
+
+__device__ __forceinline__ float from_lane(float x, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane)); }
+
+// Mean and reciprocal deviation of R rows of C elements, of which a thread holds eight of each (zeros beyond the row).  One
+// barrier: a wavefront sums its 512 elements and the squares of their differences to ITS mean, and the squares about the
+// row's mean follow from those and the means (Chan, Golub and LeVeque, 1979), so that no digits cancel.
+template <int R>
+__device__ __forceinline__ void row_stats(const float (&v)[R][8], bool layer, bool live, int waves, int wave, int lane, float inv_c, float eps, Posted& sums,
+                                          Posted& squares, float (&mean)[R], float (&rstd)[R], int chunks) {
+  const int mine = min(64, chunks - 64 * wave) * 8;   // this wavefront's elements
+  float s[R], q[R];
 #pragma unroll
-  for (int k = 0; k < N; k++) {
-    const int c = threadIdx.x + 256 * k;
-    live[k] = c < chunks;
-    col[k] = (live[k] ? c : 0) * 8;
-    get8(load_raw8<T>(p.x, b * p.xs.b + s * p.xs.s + col[k]), h[k]);
+  for (int r = 0; r < R; r++) {
+    float x = 0.f;
+    if (layer) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x += v[r][i];
+      x = wave_sum(x);
+    }
+    s[r] = x;
+    const float m = x / (float)mine;
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) { const float d = v[r][i] - m; y += d * d; }
+    q[r] = wave_sum(live ? y : 0.f);
   }
-  if (p.y != nullptr) {
-    float v[N][8];
+  if (waves > 1) {
+    if (lane == 0) {
 #pragma unroll
-    for (int k = 0; k < N; k++) get8(load_raw8<T>(p.y, b * p.ys.b + s * p.ys.s + col[k]), v[k]);
-    if (p.y_norm == 2) {
-      float a[1] = {0.f};
-#pragma unroll
-      for (int k = 0; k < N; k++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) a[0] += live[k] ? v[k][i] : 0.f;
-      block_sums<1, 4>(a, part[0]);
-      ym = a[0] * p.inv_c;
+      for (int r = 0; r < R; r++) { sums.v[r][wave] = s[r]; squares.v[r][wave] = q[r]; }
     }
-    if (p.y_norm != 0) {
-      float a[1] = {0.f};
+    __syncthreads();
+    const int r = lane >> 4, w = lane & 15;
+    const bool there = w < waves && r < R;
+    const float ws = there ? sums.v[r][w] : 0.f, wq = there ? squares.v[r][w] : 0.f;
+    const float total = row16_sum(ws);
+    const float n = (float)(min(64, chunks - 64 * w) * 8);
+    const float d = there && layer ? ws / n - total * inv_c : 0.f;
+    const float all = row16_sum(there ? wq + n * d * d : 0.f);
 #pragma unroll
-      for (int k = 0; k < N; k++)
+    for (int k = 0; k < R; k++) { s[k] = from_lane(total, 16 * k); q[k] = from_lane(all, 16 * k); }
+  }
 #pragma unroll
-        for (int i = 0; i < 8; i++) { const float d = v[k][i] - ym; a[0] += live[k] ? d * d : 0.f; }
-      block_sums<1, 4>(a, part[1]);
-      yr = 1.0f / sqrtf(a[0] * p.inv_c + p.y_eps);
+  for (int r = 0; r < R; r++) {
+    mean[r] = s[r] * inv_c;
+    rstd[r] = 1.0f / sqrtf(q[r] * inv_c + eps);
+  }
+}
+
+// TOKEN: modulation has a row per token and is fetched with it.
+template <typename T, int R, bool TOKEN>
+__global__ __launch_bounds__(1024) void gated_norm_kernel(const GatedNormParams p) {
+  __shared__ Posted post[2][4];   // by turns: [y sums, y squares, h sums, h squares]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int chunks = p.C >> 3, waves = (int)blockDim.x >> 6;
+  const bool live = (int)threadIdx.x < chunks;
+  const int col = (live ? (int)threadIdx.x : 0) * 8;
+  const int b = blockIdx.y;
+  const int s0 = blockIdx.x * p.rows_per_part, s1 = min(p.S, s0 + p.rows_per_part);
+  const bool has_y = p.y != nullptr;
+  Raw8<T> x[R], y[R];
+  auto load = [&](int s) {
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int sr = min(s + r, s1 - 1);   // rows past the part re-read its last
+      x[r] = load_raw8<T>(p.x, b * p.xs.b + sr * p.xs.s + col);
+      if (has_y) y[r] = load_raw8<T>(p.y, b * p.ys.b + sr * p.ys.s + col);
     }
+  };
+  load(s0);
+  float g[8], sc[8], sh[8];
+  auto fill = [](float (&v)[8], float c) {
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-      float g[8], w[8];
+    for (int i = 0; i < 8; i++) v[i] = c;
+  };
+  auto fold_gate = [&](int s) {   // g = gate alpha w_y
+    float yw[8];
+    fill(g, 1.f); fill(yw, 1.f);
+    if (p.gate != nullptr) load_param8<T>(p.gate, b * p.gs.b + s * p.gs.s + col, p.mod_wide, g);
+    if (p.y_weight != nullptr) load_param8<T>(p.y_weight, col, p.weight_wide, yw);
+#pragma unroll
+    for (int i = 0; i < 8; i++) g[i] *= p.alpha * yw[i];
+  };
+  auto fold_scale = [&](int s) {   // sc = (1 + scale) w, sh = b (1 + scale) + shift
+    float w[8], bi[8];
+    fill(sc, 0.f); fill(sh, 0.f); fill(w, 1.f); fill(bi, 0.f);
+    if (p.scale != nullptr) load_param8<T>(p.scale, b * p.ss.b + s * p.ss.s + col, p.mod_wide, sc);
+    if (p.shift != nullptr) load_param8<T>(p.shift, b * p.fs.b + s * p.fs.s + col, p.mod_wide, sh);
+    if (p.weight != nullptr) load_param8<T>(p.weight, col, p.weight_wide, w);
+    if (p.bias != nullptr) load_param8<T>(p.bias, col, p.weight_wide, bi);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      sh[i] = __builtin_fmaf(bi[i], 1.f + sc[i], sh[i]);
+      sc[i] = w[i] * (1.f + sc[i]);
+    }
+  };
+  if constexpr (!TOKEN) {
+    fold_gate(0);
+    fold_scale(0);
+  }
+  for (int s = s0, turn = 0; s < s1; s += R, turn ^= 1) {
+    float h[R][8], v[R][8];
+    float ym[R], yr[R], m[R], rs[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      get8(x[r], h[r]);
+      if (has_y) get8(y[r], v[r]);
+      ym[r] = m[r] = 0.f;
+      yr[r] = rs[r] = 1.f;
+      if (!live) { fill(h[r], 0.f); fill(v[r], 0.f); }
+    }
+    if (s + R < s1) load(s + R);
+    if (has_y) {
       if (p.y_norm != 0) {
+        row_stats<R>(v, p.y_norm == 2, live, waves, wave, lane, p.inv_c, p.y_eps, post[turn][0], post[turn][1], ym, yr, chunks);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[k][i] = (v[k][i] - ym) * yr;
-      }
-      if (p.y_weight != nullptr) {
-        load_param8<T>(p.y_weight, col[k], p.weight_wide, w);
+        for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[k][i] *= w[i];
-      }
-      if (p.gate != nullptr) {
-        load_param8<T>(p.gate, b * p.gs.b + s * p.gs.s + col[k], p.mod_wide, g);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[k][i] *= g[i];
+          for (int i = 0; i < 8; i++) v[r][i] = (v[r][i] - ym[r]) * yr[r];
       }
 #pragma unroll
-      for (int i = 0; i < 8; i++) h[k][i] += p.alpha * v[k][i];
+      for (int r = 0; r < R; r++) {
+        if constexpr (TOKEN) fold_gate(min(s + r, s1 - 1));
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[r][i] = live ? __builtin_fmaf(g[i], v[r][i], h[r][i]) : 0.f;
+      }
     }
-  }
-  if (p.h != nullptr) {
+    if (p.h != nullptr) {
 #pragma unroll
-    for (int k = 0; k < N; k++)
-      if (live[k]) store8<T>(p.h, b * p.hs.b + s * p.hs.s + col[k], h[k]);
-  }
-  if (p.norm == 2) {
-    float a[1] = {0.f};
-#pragma unroll
-    for (int k = 0; k < N; k++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) a[0] += live[k] ? h[k][i] : 0.f;
-    block_sums<1, 4>(a, part[2]);
-    m = a[0] * p.inv_c;
-  }
-  if (p.norm != 0) {
-    float a[1] = {0.f};
-#pragma unroll
-    for (int k = 0; k < N; k++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) { const float d = h[k][i] - m; a[0] += live[k] ? d * d : 0.f; }
-    block_sums<1, 4>(a, part[3]);
-    r = 1.0f / sqrtf(a[0] * p.inv_c + p.eps);
-  }
-  if (p.stats != nullptr && threadIdx.x == 0) *(f32x4*)(p.stats + row * 4) = (f32x4){m, r, ym, yr};
-  if (p.norm == 0) return;
-#pragma unroll
-  for (int k = 0; k < N; k++) {
-    float v[8], w[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (h[k][i] - m) * r;
-    if (p.weight != nullptr) {
-      load_param8<T>(p.weight, col[k], p.weight_wide, w);
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] *= w[i];
+      for (int r = 0; r < R; r++)
+        if (live && s + r < s1) store8<T>(p.h, b * p.hs.b + (s + r) * p.hs.s + col, h[r]);
     }
-    if (p.bias != nullptr) {
-      load_param8<T>(p.bias, col[k], p.weight_wide, w);
+    if (p.norm != 0) row_stats<R>(h, p.norm == 2, live, waves, wave, lane, p.inv_c, p.eps, post[turn][2], post[turn][3], m, rs, chunks);
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] += w[i];
-    }
-    if (p.scale != nullptr) {
-      load_param8<T>(p.scale, b * p.ss.b + s * p.ss.s + col[k], p.mod_wide, w);
+    for (int r = 0; r < R; r++) {
+      if (s + r >= s1) continue;   // uniform
+      const int64_t row = (int64_t)b * p.S + s + r;
+      if (p.stats != nullptr && threadIdx.x == 0) *(f32x4*)(p.stats + row * 4) = (f32x4){m[r], rs[r], ym[r], yr[r]};
+      if (p.norm == 0) continue;
+      if constexpr (TOKEN) fold_scale(s + r);
+      float n[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] *= 1.0f + w[i];
-    }
-    if (p.shift != nullptr) {
-      load_param8<T>(p.shift, b * p.fs.b + s * p.fs.s + col[k], p.mod_wide, w);
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] += w[i];
-    }
-    if (!p.fp8) {
-      if (live[k]) store8<T>(p.n, b * p.ns.b + s * p.ns.s + col[k], v);
-    } else {  // a block of 128 columns is a DPP row: 16 lanes of 8 columns
-      const Divider div(block_scale(row16_max(live[k] ? absmax8(v) : 0)));
-      const i32x2 q = cast8(v, div);
-      if (live[k]) {
-        *(i32x2*)((unsigned char*)p.n + b * p.ns.b + s * p.ns.s + col[k]) = q;
-        if ((threadIdx.x & 15) == 0) p.n_scale[(int64_t)(col[k] >> 7) * p.rows + row] = div.scale;
+      for (int i = 0; i < 8; i++) n[i] = __builtin_fmaf((h[r][i] - m[r]) * rs[r], sc[i], sh[i]);
+      if (!p.fp8) {
+        if (live) store8<T>(p.n, b * p.ns.b + (s + r) * p.ns.s + col, n);
+      } else {  // a block of 128 columns is a DPP row: 16 lanes of 8 columns
+        const Divider div(block_scale(row16_max(live ? absmax8(n) : 0)));
+        const i32x2 q = cast8(n, div);
+        if (live) {
+          *(i32x2*)((unsigned char*)p.n + b * p.ns.b + (s + r) * p.ns.s + col) = q;
+          if ((lane & 15) == 0) p.n_scale[(int64_t)(col >> 7) * p.rows + row] = div.scale;
+        }
       }
     }
   }
 }
 
+// Parts of a batch entry's rows: as many workgroups as the chip holds at once (16 wavefronts a compute unit at these
+// registers), one row each where there are fewer rows than that.
 template <typename T>
-static hipError_t run(const GatedNormParams& p, hipStream_t stream) {
-  const int n = (p.C + 2047) / 2048;
-  const dim3 grid((unsigned)p.rows), block(256);
-  if (n <= 1) hipLaunchKernelGGL((gated_norm_row_kernel<T, 1>), grid, block, 0, stream, p);
-  else if (n <= 2) hipLaunchKernelGGL((gated_norm_row_kernel<T, 2>), grid, block, 0, stream, p);
-  else if (n <= 3) hipLaunchKernelGGL((gated_norm_row_kernel<T, 3>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((gated_norm_row_kernel<T, 4>), grid, block, 0, stream, p);
+static hipError_t run(GatedNormParams p, hipStream_t stream) {
+  const int waves = (p.C + 511) / 512;
+  const int64_t at_once = (int64_t)resident_cus() * (16 / waves > 0 ? 16 / waves : 1);
+  p.rows_per_part = (int)((p.rows + at_once - 1) / at_once);
+  const dim3 grid((unsigned)((p.S + p.rows_per_part - 1) / p.rows_per_part), (unsigned)p.B), block(64 * waves);
+  const bool token = (p.gate != nullptr && p.gs.s != 0) || (p.scale != nullptr && p.ss.s != 0) || (p.shift != nullptr && p.fs.s != 0);
+  if (token) hipLaunchKernelGGL((gated_norm_kernel<T, 1, true>), grid, block, 0, stream, p);
+  else if (p.rows_per_part == 1) hipLaunchKernelGGL((gated_norm_kernel<T, 1, false>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((gated_norm_kernel<T, sizeof(T) == 2 ? 2 : 1, false>), grid, block, 0, stream, p);  // two rows of fp32 do not fit the registers
   return hipGetLastError();
 }
 
 // ---- backward --------------------------------------------------------------------------------
 
-// A workgroup runs over the rows of one part of one batch entry; a thread keeps the column sums of its chunks.
-template <typename T, int N>
-__global__ __launch_bounds__(256) void gated_norm_bwd_kernel(const GatedNormBwdParams p) {
-  __shared__ float part[4][8];
+// The two totals over a workgroup of values x, one barrier.
+__device__ __forceinline__ void two_sums(float& a, float& b, int waves, int wave, int lane, Posted& post) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if (waves == 1) return;
+  if (lane == 0) { post.v[0][wave] = a; post.v[1][wave] = b; }
+  __syncthreads();
+  const int k = lane >> 4, w = lane & 15;
+  const float t = row16_sum(w < waves && k < 2 ? post.v[k][w] : 0.f);
+  a = from_lane(t, 0);
+  b = from_lane(t, 16);
+}
+
+// A workgroup runs over the rows of one part of one batch entry; a thread keeps the sums of its eight columns.
+template <typename T, bool TOKEN>
+__global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwdParams p) {
+  __shared__ Posted post[2][2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int chunks = p.C >> 3, waves = (int)blockDim.x >> 6;
+  const bool live = (int)threadIdx.x < chunks;
+  const int col = (live ? (int)threadIdx.x : 0) * 8;
   const int b = blockIdx.y;
-  const int s0 = blockIdx.x * p.rows_per_part;
-  const int s1 = min(p.S, s0 + p.rows_per_part);
-  const int chunks = p.C >> 3;
-  float sa[N][8] = {}, sf[N][8] = {}, sg[N][8] = {};
-  bool live[N];
-  int col[N];
+  const int s0 = blockIdx.x * p.rows_per_part, s1 = min(p.S, s0 + p.rows_per_part);
+  const bool has_n = p.dn != nullptr, has_y = p.y != nullptr;
+  Raw8<T> rdh, rdn, rh, ry;
+  f32x4 st;
+  auto load = [&](int s) {
+    st = *(const f32x4*)(p.stats + ((int64_t)b * p.S + s) * 4);
+    if (p.dh != nullptr) rdh = load_raw8<T>(p.dh, b * p.dhs.b + s * p.dhs.s + col);
+    if (has_n) {
+      rdn = load_raw8<T>(p.dn, b * p.dns.b + s * p.dns.s + col);
+      rh = load_raw8<T>(p.h, b * p.hs.b + s * p.hs.s + col);
+    }
+    if (has_y) ry = load_raw8<T>(p.y, b * p.ys.b + s * p.ys.s + col);
+  };
+  constexpr bool AHEAD = sizeof(T) == 2 && !TOKEN;   // the next row is requested ahead where the registers allow it
+  if constexpr (AHEAD) load(s0);
+  float scw[8], gyw[8], sa[8] = {}, sf[8] = {}, sg[8] = {};   // (1 + scale) w, alpha gate w_y, column sums
+  auto fill = [](float (&v)[8], float c) {
 #pragma unroll
-  for (int k = 0; k < N; k++) {
-    const int c = threadIdx.x + 256 * k;
-    live[k] = c < chunks;
-    col[k] = (live[k] ? c : 0) * 8;
+    for (int i = 0; i < 8; i++) v[i] = c;
+  };
+  auto times = [&](const void* q, int64_t off, bool wide, float plus, float (&v)[8]) {   // v *= plus + q
+    if (q == nullptr) return;
+    float w[8];
+    load_param8<T>(q, off, wide, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] *= plus + w[i];
+  };
+  if constexpr (!TOKEN) {
+    fill(scw, 1.f);
+    times(p.scale, b * p.ss.b + col, p.mod_wide, 1.f, scw);
+    times(p.weight, col, p.weight_wide, 0.f, scw);
+    fill(gyw, p.alpha);
+    times(p.gate, b * p.gs.b + col, p.mod_wide, 0.f, gyw);
+    times(p.y_weight, col, p.weight_wide, 0.f, gyw);
   }
-  for (int s = s0; s < s1; s++) {
+  for (int s = s0, turn = 0; s < s1; s++, turn ^= 1) {
     const int64_t row = (int64_t)b * p.S + s;
-    const f32x4 st = *(const f32x4*)(p.stats + row * 4);
-    float t[N][8], du[N][8], u[N][8];
-    float a[2] = {0.f, 0.f};
+    if constexpr (!AHEAD) load(s);
+    const f32x4 now = st;
+    float t[8], du[8], u[8];
+    fill(t, 0.f);
+    if (p.dh != nullptr) get8(rdh, t);
+    if (has_n) { get8(rdn, du); get8(rh, u); }
+    const Raw8<T> y_now = ry;
+    if (AHEAD && s + 1 < s1) load(s + 1);
+    if (has_n) {
 #pragma unroll
-    for (int k = 0; k < N; k++) {
+      for (int i = 0; i < 8; i++) u[i] = (u[i] - now[0]) * now[1];
+      if constexpr (!TOKEN) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) t[k][i] = 0.f;
-      if (p.dh != nullptr) get8(load_raw8<T>(p.dh, b * p.dhs.b + s * p.dhs.s + col[k]), t[k]);
-      if (p.dn != nullptr) {
-        float w[8], bi[8];
-        get8(load_raw8<T>(p.dn, b * p.dns.b + s * p.dns.s + col[k]), du[k]);
-        get8(load_raw8<T>(p.h, b * p.hs.b + s * p.hs.s + col[k]), u[k]);
+        for (int i = 0; i < 8; i++) { sa[i] += du[i] * u[i]; sf[i] += du[i]; du[i] *= scw[i]; }
+      } else {
+        if (p.mod_per_token && live && p.dshift != nullptr) store_param8<T>(p.dshift, row * p.C + col, p.mod_wide, du);
+        if (p.mod_per_token && live && p.dscale != nullptr) {
+          float d[8], bi[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) u[k][i] = (u[k][i] - st[0]) * st[1];
-        if (p.mod_per_token) {
-          if (live[k] && p.dshift != nullptr) store_param8<T>(p.dshift, row * p.C + col[k], p.mod_wide, du[k]);
-          if (live[k] && p.dscale != nullptr) {
-            float d[8];
+          for (int i = 0; i < 8; i++) d[i] = u[i];
+          times(p.weight, col, p.weight_wide, 0.f, d);
+          fill(bi, 0.f);
+          if (p.bias != nullptr) load_param8<T>(p.bias, col, p.weight_wide, bi);
 #pragma unroll
-            for (int i = 0; i < 8; i++) d[i] = u[k][i];
-            if (p.weight != nullptr) {
-              load_param8<T>(p.weight, col[k], p.weight_wide, w);
-#pragma unroll
-              for (int i = 0; i < 8; i++) d[i] *= w[i];
-            }
-            if (p.bias != nullptr) {
-              load_param8<T>(p.bias, col[k], p.weight_wide, bi);
-#pragma unroll
-              for (int i = 0; i < 8; i++) d[i] += bi[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) d[i] *= du[k][i];
-            store_param8<T>(p.dscale, row * p.C + col[k], p.mod_wide, d);
-          }
+          for (int i = 0; i < 8; i++) d[i] = du[i] * (d[i] + bi[i]);
+          store_param8<T>(p.dscale, row * p.C + col, p.mod_wide, d);
         }
-        float sc[8];
-        if (p.scale != nullptr) load_param8<T>(p.scale, b * p.ss.b + s * p.ss.s + col[k], p.mod_wide, sc);
-        if (p.scale != nullptr && p.mod_per_token) {
+        if (p.mod_per_token) times(p.scale, b * p.ss.b + s * p.ss.s + col, p.mod_wide, 1.f, du);
 #pragma unroll
-          for (int i = 0; i < 8; i++) du[k][i] *= 1.0f + sc[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) { sa[k][i] += du[k][i] * u[k][i]; sf[k][i] += du[k][i]; }
-        if (p.scale != nullptr && !p.mod_per_token) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) du[k][i] *= 1.0f + sc[i];
-        }
-        if (p.weight != nullptr) {
-          load_param8<T>(p.weight, col[k], p.weight_wide, w);
-#pragma unroll
-          for (int i = 0; i < 8; i++) du[k][i] *= w[i];
-        }
-        if (live[k]) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) { a[0] += du[k][i]; a[1] += du[k][i] * u[k][i]; }
-        }
+        for (int i = 0; i < 8; i++) { sa[i] += du[i] * u[i]; sf[i] += du[i]; }
+        if (!p.mod_per_token) times(p.scale, b * p.ss.b + col, p.mod_wide, 1.f, du);
+        times(p.weight, col, p.weight_wide, 0.f, du);
       }
+      float a = 0.f, d = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) { a += du[i]; d += du[i] * u[i]; }
+      a = live ? a : 0.f;
+      d = live ? d : 0.f;
+      two_sums(a, d, waves, wave, lane, post[turn][0]);
+      const float mean = p.norm == 2 ? a * p.inv_c : 0.f, dot = d * p.inv_c;
+#pragma unroll
+      for (int i = 0; i < 8; i++) t[i] += now[1] * (du[i] - mean - u[i] * dot);
     }
-    if (p.dn != nullptr) {
-      block_sums<2, 4>(a, part[(s - s0) & 1]);
-      const float mean = p.norm == 2 ? a[0] * p.inv_c : 0.f, dot = a[1] * p.inv_c;
+    if (p.dx != nullptr && live) store8<T>(p.dx, b * p.dxs.b + s * p.dxs.s + col, t);
+    if (!has_y) continue;
+    float z[8];   // t becomes e
+    get8(y_now, z);
 #pragma unroll
-      for (int k = 0; k < N; k++)
+    for (int i = 0; i < 8; i++) z[i] = (z[i] - now[2]) * now[3];
+    if constexpr (!TOKEN) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) t[k][i] += st[1] * (du[k][i] - mean - u[k][i] * dot);
-    }
-    if (p.dx != nullptr) {
-#pragma unroll
-      for (int k = 0; k < N; k++)
-        if (live[k]) store8<T>(p.dx, b * p.dxs.b + s * p.dxs.s + col[k], t[k]);
-    }
-    if (p.y == nullptr) continue;
-    // t becomes e, u becomes z
-    a[0] = a[1] = 0.f;
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-      float g[8], w[8];
-      get8(load_raw8<T>(p.y, b * p.ys.b + s * p.ys.s + col[k]), u[k]);
-#pragma unroll
-      for (int i = 0; i < 8; i++) u[k][i] = (u[k][i] - st[2]) * st[3];
-      if (p.y_weight != nullptr) load_param8<T>(p.y_weight, col[k], p.weight_wide, w);
-      if (p.gate_per_token && p.dgate != nullptr && live[k]) {
+      for (int i = 0; i < 8; i++) { sg[i] += t[i] * z[i]; t[i] *= gyw[i]; }
+    } else {
+      if (p.gate_per_token && live && p.dgate != nullptr) {
         float d[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) d[i] = p.alpha * t[k][i] * (p.y_weight != nullptr ? u[k][i] * w[i] : u[k][i]);
-        store_param8<T>(p.dgate, row * p.C + col[k], p.mod_wide, d);
+        for (int i = 0; i < 8; i++) d[i] = p.alpha * t[i] * z[i];
+        times(p.y_weight, col, p.weight_wide, 0.f, d);
+        store_param8<T>(p.dgate, row * p.C + col, p.mod_wide, d);
       }
-      if (p.gate != nullptr) load_param8<T>(p.gate, b * p.gs.b + s * p.gs.s + col[k], p.mod_wide, g);
       if (!p.gate_per_token) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) sg[k][i] += t[k][i] * u[k][i];
+        for (int i = 0; i < 8; i++) sg[i] += t[i] * z[i];
       }
 #pragma unroll
-      for (int i = 0; i < 8; i++) t[k][i] *= p.gate != nullptr ? p.alpha * g[i] : p.alpha;
+      for (int i = 0; i < 8; i++) t[i] *= p.alpha;
+      times(p.gate, b * p.gs.b + s * p.gs.s + col, p.mod_wide, 0.f, t);
       if (p.gate_per_token) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) sg[k][i] += t[k][i] * u[k][i];
+        for (int i = 0; i < 8; i++) sg[i] += t[i] * z[i];
       }
-      if (p.y_weight != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) t[k][i] *= w[i];
-      }
-      if (live[k]) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) { a[0] += t[k][i]; a[1] += t[k][i] * u[k][i]; }
-      }
+      times(p.y_weight, col, p.weight_wide, 0.f, t);
     }
     if (p.y_norm != 0) {
-      block_sums<2, 4>(a, part[2 + ((s - s0) & 1)]);
-      const float mean = p.y_norm == 2 ? a[0] * p.inv_c : 0.f, dot = a[1] * p.inv_c;
+      float a = 0.f, d = 0.f;
 #pragma unroll
-      for (int k = 0; k < N; k++)
+      for (int i = 0; i < 8; i++) { a += t[i]; d += t[i] * z[i]; }
+      a = live ? a : 0.f;
+      d = live ? d : 0.f;
+      two_sums(a, d, waves, wave, lane, post[turn][1]);
+      const float mean = p.y_norm == 2 ? a * p.inv_c : 0.f, dot = d * p.inv_c;
 #pragma unroll
-        for (int i = 0; i < 8; i++) t[k][i] = st[3] * (t[k][i] - mean - u[k][i] * dot);
+      for (int i = 0; i < 8; i++) t[i] = now[3] * (t[i] - mean - z[i] * dot);
     }
-    if (p.dy != nullptr) {
-#pragma unroll
-      for (int k = 0; k < N; k++)
-        if (live[k]) store8<T>(p.dy, b * p.dys.b + s * p.dys.s + col[k], t[k]);
-    }
+    if (p.dy != nullptr && live) store8<T>(p.dy, b * p.dys.b + s * p.dys.s + col, t);
   }
-  if (!p.sums) return;
+  if (!p.sums || !live) return;
   float* out = p.partial + ((int64_t)b * p.parts + blockIdx.x) * 3 * p.C;
-#pragma unroll
-  for (int k = 0; k < N; k++) {
-    if (!live[k]) continue;
-    store8<float>(out, col[k], sa[k]);
-    store8<float>(out, p.C + col[k], sf[k]);
-    store8<float>(out, 2 * (int64_t)p.C + col[k], sg[k]);
-  }
+  store8<float>(out, col, sa);
+  store8<float>(out, p.C + col, sf);
+  store8<float>(out, 2 * (int64_t)p.C + col, sg);
 }
 
 template <typename T>
@@ -318,24 +365,34 @@ __device__ __forceinline__ void put_param(void* p, int64_t i, bool wide, float v
   else ((T*)p)[i] = (T)v;
 }
 
-// The parts' sums, added in their order, and from them the parameters' gradients; one thread per column.
+// The parts' sums, added in a fixed order (sixteen runs of every sixteenth part, then the runs), and from them the
+// parameters' gradients; 16 columns per workgroup.
 template <typename T>
 __global__ __launch_bounds__(256) void gated_norm_bwd_finish_kernel(const GatedNormBwdParams p) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= p.C) return;
-  const float w = p.weight != nullptr ? param_at<T>(p.weight, c, p.weight_wide) : 1.f;
-  const float bi = p.bias != nullptr ? param_at<T>(p.bias, c, p.weight_wide) : 0.f;
-  const float yw = p.y_weight != nullptr ? param_at<T>(p.y_weight, c, p.weight_wide) : 1.f;
+  __shared__ float runs[3][16][17];
+  const int k = threadIdx.x & 15, run = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + k;
+  const bool live = c < p.C;
+  const int cc = live ? c : 0;
   float dw = 0.f, db = 0.f, dyw = 0.f;
   for (int b = 0; b < p.B; b++) {
     float a = 0.f, f = 0.f, g = 0.f;
-    const float* in = p.partial + (int64_t)b * p.parts * 3 * p.C + c;
-    for (int i = 0; i < p.parts; i++, in += 3 * (int64_t)p.C) { a += in[0]; f += in[p.C]; g += in[2 * (int64_t)p.C]; }
+    const float* in = p.partial + ((int64_t)b * p.parts + run) * 3 * p.C + cc;
+#pragma unroll 4
+    for (int i = run; i < p.parts; i += 16, in += 48 * (int64_t)p.C) { a += in[0]; f += in[p.C]; g += in[2 * (int64_t)p.C]; }
+    __syncthreads();   // the sums of the batch entry before have been read
+    runs[0][run][k] = a;
+    runs[1][run][k] = f;
+    runs[2][run][k] = g;
+    __syncthreads();
+    if (run != 0 || !live) continue;
+    for (int i = 1; i < 16; i++) { a += runs[0][i][k]; f += runs[1][i][k]; g += runs[2][i][k]; }
     if (p.mod_per_token) {
       dw += a;
       db += f;
     } else {
       const float sc = p.scale != nullptr ? 1.f + param_at<T>(p.scale, b * p.ss.b + c, p.mod_wide) : 1.f;
+      const float w = p.weight != nullptr ? param_at<T>(p.weight, c, p.weight_wide) : 1.f, bi = p.bias != nullptr ? param_at<T>(p.bias, c, p.weight_wide) : 0.f;
       if (p.dshift != nullptr) put_param<T>(p.dshift, (int64_t)b * p.C + c, p.mod_wide, f);
       if (p.dscale != nullptr) put_param<T>(p.dscale, (int64_t)b * p.C + c, p.mod_wide, w * a + bi * f);
       dw += sc * a;
@@ -344,11 +401,12 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_finish_kernel(const GatedN
     if (p.gate_per_token) {
       dyw += g;
     } else {
-      const float ga = p.gate != nullptr ? param_at<T>(p.gate, b * p.gs.b + c, p.mod_wide) : 1.f;
-      if (p.dgate != nullptr) put_param<T>(p.dgate, (int64_t)b * p.C + c, p.mod_wide, p.alpha * yw * g);
-      dyw += p.alpha * ga * g;
+      const float ga = p.alpha * (p.gate != nullptr ? param_at<T>(p.gate, b * p.gs.b + c, p.mod_wide) : 1.f);
+      if (p.dgate != nullptr) put_param<T>(p.dgate, (int64_t)b * p.C + c, p.mod_wide, p.alpha * (p.y_weight != nullptr ? param_at<T>(p.y_weight, c, p.weight_wide) : 1.f) * g);
+      dyw += ga * g;
     }
   }
+  if (run != 0 || !live) return;
   if (p.dweight != nullptr) put_param<T>(p.dweight, c, p.weight_wide, dw);
   if (p.dbias != nullptr) put_param<T>(p.dbias, c, p.weight_wide, db);
   if (p.dy_weight != nullptr) put_param<T>(p.dy_weight, c, p.weight_wide, dyw);
@@ -356,15 +414,12 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_finish_kernel(const GatedN
 
 template <typename T>
 static hipError_t run_bwd(const GatedNormBwdParams& p, hipStream_t stream) {
-  const int n = (p.C + 2047) / 2048;
-  const dim3 grid((unsigned)p.parts, (unsigned)p.B), block(256);
-  if (n <= 1) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, 1>), grid, block, 0, stream, p);
-  else if (n <= 2) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, 2>), grid, block, 0, stream, p);
-  else if (n <= 3) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, 3>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, 4>), grid, block, 0, stream, p);
-  hipError_t e = hipGetLastError();
+  const dim3 grid((unsigned)p.parts, (unsigned)p.B), block(64 * ((p.C + 511) / 512));
+  if (p.mod_per_token || p.gate_per_token) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, false>), grid, block, 0, stream, p);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.sums) return e;
-  hipLaunchKernelGGL((gated_norm_bwd_finish_kernel<T>), dim3((unsigned)((p.C + 255) / 256)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((gated_norm_bwd_finish_kernel<T>), dim3((unsigned)((p.C + 15) / 16)), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -377,12 +432,15 @@ hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, hipStream_t st
   return hipErrorInvalidValue;
 }
 
-// Parts: enough workgroups to fill the chip (4 per compute unit), at least 16 rows each where there are that many.
+// Parts: as many workgroups as the chip holds at once (16 wavefronts a compute unit); with column sums at least 8 rows
+// each, so that writing and reading a part's sums (24 C bytes) stays beside the rows' 12 C and more.
 void gated_norm_bwd_plan(GatedNormBwdParams& p) {
   const bool mods = !p.mod_per_token && (p.dscale != nullptr || p.dshift != nullptr);
   p.sums = mods || (!p.gate_per_token && p.dgate != nullptr) || p.dweight != nullptr || p.dbias != nullptr || p.dy_weight != nullptr;
-  int per = (int)(((int64_t)p.B * p.S + 1023) / 1024);
-  if (p.sums && per < 16) per = 16;
+  const int waves = (p.C + 511) / 512;
+  const int64_t at_once = (int64_t)resident_cus() * (16 / waves > 0 ? 16 / waves : 1);
+  int per = (int)(((int64_t)p.B * p.S + at_once - 1) / at_once);
+  if (p.sums && per < 8) per = 8;
   if (per > p.S) per = p.S;
   p.rows_per_part = per;
   p.parts = (p.S + per - 1) / per;
