@@ -40,7 +40,7 @@ __device__ __forceinline__ float from_lane(float x, int lane) { return __uint_as
 template <int R>
 __device__ __forceinline__ void row_stats(const float (&v)[R][8], bool layer, bool live, int waves, int wave, int lane, float inv_c, float eps, Posted& sums,
                                           Posted& squares, float (&mean)[R], float (&rstd)[R], int chunks) {
-  const int mine = min(64, chunks - 64 * wave) * 8;   // this wavefront's elements
+  const float inv_mine = 1.f / (float)(min(64, chunks - 64 * wave) * 8);   // of this wavefront's elements
   float s[R], q[R];
 #pragma unroll
   for (int r = 0; r < R; r++) {
@@ -51,7 +51,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[R][8], bool layer, bo
       x = wave_sum(x);
     }
     s[r] = x;
-    const float m = x / (float)mine;
+    const float m = x * inv_mine;
     float y = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) { const float d = v[r][i] - m; y += d * d; }
@@ -68,7 +68,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[R][8], bool layer, bo
     const float ws = there ? sums.v[r][w] : 0.f, wq = there ? squares.v[r][w] : 0.f;
     const float total = row16_sum(ws);
     const float n = (float)(min(64, chunks - 64 * w) * 8);
-    const float d = there && layer ? ws / n - total * inv_c : 0.f;
+    const float d = there && layer ? ws * __builtin_amdgcn_rcpf(n) - total * inv_c : 0.f;
     const float all = row16_sum(there ? wq + n * d * d : 0.f);
 #pragma unroll
     for (int k = 0; k < R; k++) { s[k] = from_lane(total, 16 * k); q[k] = from_lane(all, 16 * k); }
@@ -76,13 +76,35 @@ __device__ __forceinline__ void row_stats(const float (&v)[R][8], bool layer, bo
 #pragma unroll
   for (int r = 0; r < R; r++) {
     mean[r] = s[r] * inv_c;
-    rstd[r] = 1.0f / sqrtf(q[r] * inv_c + eps);
+    rstd[r] = inv_sqrt(q[r] * inv_c + eps);
+  }
+}
+
+// Eight columns of a row of n as T or as part of an fp8 block: 16 lanes, a DPP row, hold its 128 columns.
+template <typename T>
+__device__ __forceinline__ void put_row8(const GatedNormParams& p, float (&n)[8], void* to, int col, int64_t row, bool live, int lane) {
+  if (!p.fp8) {
+    if (live) store8<T>(to, 0, n);
+    return;
+  }
+  // n has no bits of its own to keep (it is not stored): a product with the reciprocal, within two units of the quotient, in place
+  // of the division (which with its scale took 40 % of the time: VALU instructions)
+  const float top = __uint_as_float(row16_max(live ? absmax8(n) : 0));
+  float scale = top * (1.f / kFp8Max);
+  scale = top == 0.f ? 1.f : (scale < 0x1p-126f ? 0x1p-126f : scale);
+  const float inv = __builtin_amdgcn_rcpf(scale);
+#pragma unroll
+  for (int i = 0; i < 8; i++) n[i] *= inv;
+  if (live) {
+    *(i32x2*)to = to_fp8(n);
+    if ((lane & 15) == 0) p.n_scale[(int64_t)(col >> 7) * p.rows + row] = scale;
   }
 }
 
 // TOKEN: modulation has a row per token and is fetched with it.
-template <typename T, int R, bool TOKEN>
-__global__ __launch_bounds__(1024) void gated_norm_kernel(const GatedNormParams p) {
+template <typename T, bool TOKEN>
+__global__ __launch_bounds__(1024, TOKEN ? 4 : 6) void gated_norm_kernel(const GatedNormParams p) {
+  constexpr int R = 1;   // rows at a time
   __shared__ Posted post[2][4];   // by turns: [y sums, y squares, h sums, h squares]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int chunks = p.C >> 3, waves = (int)blockDim.x >> 6;
@@ -174,32 +196,193 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(const GatedNormParams 
       float n[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) n[i] = __builtin_fmaf((h[r][i] - m[r]) * rs[r], sc[i], sh[i]);
-      if (!p.fp8) {
-        if (live) store8<T>(p.n, b * p.ns.b + (s + r) * p.ns.s + col, n);
-      } else {  // a block of 128 columns is a DPP row: 16 lanes of 8 columns
-        const Divider div(block_scale(row16_max(live ? absmax8(n) : 0)));
-        const i32x2 q = cast8(n, div);
-        if (live) {
-          *(i32x2*)((unsigned char*)p.n + b * p.ns.b + (s + r) * p.ns.s + col) = q;
-          if ((lane & 15) == 0) p.n_scale[(int64_t)(col >> 7) * p.rows + row] = div.scale;
-        }
-      }
+      const int64_t at = b * p.ns.b + (s + r) * p.ns.s + col;
+      put_row8<T>(p, n, p.fp8 ? (void*)((unsigned char*)p.n + at) : (void*)((T*)p.n + at), col, row, live, lane);
     }
   }
 }
 
-// Parts of a batch entry's rows: as many workgroups as the chip holds at once (16 wavefronts a compute unit at these
-// registers), one row each where there are fewer rows than that.
+// Many rows: a wavefront to a row, 64 N chunks of 8 columns; the three parameter vectors of the batch entry lie in LDS, as
+// halves of chunks so that a lane's 16-byte reads are consecutive.  Nothing is exchanged between wavefronts, so twelve to
+// thirty-two of them on a compute unit keep 150 KB of rows on their way.
+template <typename T, int N>
+__global__ __launch_bounds__(256, N >= 6 ? 3 : 4) void gated_norm_wave_kernel(const GatedNormParams p) {
+  extern __shared__ __align__(16) f32x4 vectors[];   // [vector][N][2][64]: sc, sh and, with y, g
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int chunks = p.C >> 3, b = blockIdx.y;
+  const bool has_y = p.y != nullptr;
+  for (int c = threadIdx.x; c < 64 * N; c += 256) {
+    const int col = (c < chunks ? c : 0) * 8;
+    float v[8], sc[8], sh[8], w[8];
+    auto fill = [](float (&v)[8], float c) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = c;
+    };
+    auto put = [&](int vec, const float (&v)[8]) {
+#pragma unroll
+      for (int q = 0; q < 2; q++) vectors[((vec * N + (c >> 6)) * 2 + q) * 64 + (c & 63)] = (f32x4){v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+    };
+    fill(sc, 0.f); fill(sh, 0.f); fill(w, 1.f); fill(v, 0.f);
+    if (p.scale != nullptr) load_param8<T>(p.scale, b * p.ss.b + col, p.mod_wide, sc);
+    if (p.shift != nullptr) load_param8<T>(p.shift, b * p.fs.b + col, p.mod_wide, sh);
+    if (p.weight != nullptr) load_param8<T>(p.weight, col, p.weight_wide, w);
+    if (p.bias != nullptr) load_param8<T>(p.bias, col, p.weight_wide, v);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      sh[i] = __builtin_fmaf(v[i], 1.f + sc[i], sh[i]);
+      sc[i] = w[i] * (1.f + sc[i]);
+    }
+    put(0, sc);
+    put(1, sh);
+    if (!has_y) continue;
+    fill(v, 1.f); fill(w, 1.f);
+    if (p.gate != nullptr) load_param8<T>(p.gate, b * p.gs.b + col, p.mod_wide, v);
+    if (p.y_weight != nullptr) load_param8<T>(p.y_weight, col, p.weight_wide, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] *= p.alpha * w[i];
+    put(2, v);
+  }
+  __syncthreads();
+  auto vec8 = [&](int vec, int k, float (&v)[8]) {
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      const f32x4 t = vectors[((vec * N + k) * 2 + q) * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[4 * q + i] = t[i];
+    }
+  };
+  const bool last = lane + 64 * (N - 1) < chunks;   // the chunks before the last are whole
+  const int col_last = last ? (lane + 64 * (N - 1)) * 8 : 0;
+  auto col = [&](int k) { return (unsigned)(k < N - 1 ? lane * 8 + 512 * k : col_last); };   // 32-bit offsets from a row's uniform start
+  for (int s = blockIdx.x * 4 + wave; s < p.S; s += gridDim.x * 4) {
+    Raw8<T> x[N], y[N];
+    auto row_of = [&](const void* p, const RowStrides& st) { return (const char*)((const T*)p + b * st.b + s * st.s); };
+    const char* xrow = row_of(p.x, p.xs);
+#pragma unroll
+    for (int k = 0; k < N; k++) x[k] = *(const Raw8<T>*)(xrow + col(k) * (unsigned)sizeof(T));
+    if (has_y) {
+      const char* yrow = row_of(p.y, p.ys);
+#pragma unroll
+      for (int k = 0; k < N; k++) y[k] = *(const Raw8<T>*)(yrow + col(k) * (unsigned)sizeof(T));
+    }
+    float h[N][8];
+    float ym = 0.f, yr = 1.f, m = 0.f, rs = 1.f;
+    if (has_y) {
+      if (p.y_norm != 0) {
+        if (p.y_norm == 2) {
+          float a = 0.f;
+#pragma unroll
+          for (int k = 0; k < N; k++) {
+            float c = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) c += y[k][i];
+            a += k < N - 1 || last ? c : 0.f;
+          }
+          ym = wave_sum(a) * p.inv_c;
+        }
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+          float c = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) { const float d = y[k][i] - ym; c = __builtin_fmaf(d, d, c); }
+          a += k < N - 1 || last ? c : 0.f;
+        }
+        yr = inv_sqrt(wave_sum(a) * p.inv_c + p.y_eps);
+      }
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        float g[8];
+        vec8(2, k, g);
+        asm volatile("" : "+v"(x[k].x[0]), "+v"(y[k].x[0]));   // as loaded: no conversion is kept from the sums above
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[k][i] = __builtin_fmaf(g[i], (y[k][i] - ym) * yr, x[k][i]);
+        __builtin_amdgcn_sched_barrier(0);   // chunk by chunk: h takes the registers that x and y leave
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; k++) get8(x[k], h[k]);
+    }
+    if (p.h != nullptr) {
+      char* hrow = (char*)row_of(p.h, p.hs);
+#pragma unroll
+      for (int k = 0; k < N; k++)
+        if (k < N - 1 || last) store8<T>(hrow + col(k) * (unsigned)sizeof(T), 0, h[k]);
+    }
+    if (p.norm == 2) {
+      float a = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        float c = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) c += h[k][i];
+        a += k < N - 1 || last ? c : 0.f;
+      }
+      m = wave_sum(a) * p.inv_c;
+    }
+    if (p.norm != 0) {
+      float a = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        float c = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) { const float d = h[k][i] - m; c = __builtin_fmaf(d, d, c); }
+        a += k < N - 1 || last ? c : 0.f;
+      }
+      rs = inv_sqrt(wave_sum(a) * p.inv_c + p.eps);
+    }
+    const int64_t row = (int64_t)b * p.S + s;
+    if (p.stats != nullptr && lane == 0) *(f32x4*)(p.stats + row * 4) = (f32x4){m, rs, ym, yr};
+    if (p.norm == 0) continue;
+    char* nrow = p.fp8 ? (char*)p.n + b * p.ns.b + s * p.ns.s : (char*)row_of(p.n, p.ns);
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      float n[8], sc[8], sh[8];
+      vec8(0, k, sc);
+      vec8(1, k, sh);
+#pragma unroll
+      for (int i = 0; i < 8; i++) n[i] = __builtin_fmaf((h[k][i] - m) * rs, sc[i], sh[i]);
+      put_row8<T>(p, n, nrow + col(k) * (p.fp8 ? 1u : (unsigned)sizeof(T)), col(k), row, k < N - 1 || last, lane);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// Rows are spread over wavefronts (a workgroup to a row) where there are fewer rows than the chip holds wavefronts, where
+// the modulation changes with the row, and where a row does not fit a wavefront's registers.
+template <typename T, int N>
+static hipError_t launch_wave(const GatedNormParams& p, hipStream_t stream) {
+  static std::atomic<int> residency[kMaxDevices];
+  const int lds = (p.y != nullptr ? 3 : 2) * N * 2048;
+  std::atomic<int>& known = residency[current_device_slot()];
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {   // asked with the three vectors of a call with y
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, (const void*)gated_norm_wave_kernel<T, N>, 256, 3 * N * 2048) != hipSuccess || n <= 0) n = 1;
+    known.store(n, std::memory_order_relaxed);
+  }
+  int64_t groups = ((int64_t)resident_cus() * n + p.B - 1) / p.B;
+  if (groups > (p.S + 3) / 4) groups = (p.S + 3) / 4;
+  hipLaunchKernelGGL((gated_norm_wave_kernel<T, N>), dim3((unsigned)groups, (unsigned)p.B), dim3(256), lds, stream, p);
+  return hipGetLastError();
+}
+
 template <typename T>
 static hipError_t run(GatedNormParams p, hipStream_t stream) {
+  const bool token = (p.gate != nullptr && p.gs.s != 0) || (p.scale != nullptr && p.ss.s != 0) || (p.shift != nullptr && p.fs.s != 0);
   const int waves = (p.C + 511) / 512;
-  const int64_t at_once = (int64_t)resident_cus() * (16 / waves > 0 ? 16 / waves : 1);
+  if (!token && waves <= 6 && p.rows >= (int64_t)resident_cus() * 16) {
+    if (waves <= 1) return launch_wave<T, 1>(p, stream);
+    if (waves <= 2) return launch_wave<T, 2>(p, stream);
+    if (waves <= 3) return launch_wave<T, 3>(p, stream);
+    if (waves <= 4) return launch_wave<T, 4>(p, stream);
+    return launch_wave<T, 6>(p, stream);
+  }
+  const int per_simd = (waves + 3) / 4;   // of the six wavefronts (with modulation per token four) that fit a SIMD by registers
+  const int64_t at_once = (int64_t)resident_cus() * ((token ? 4 : 6) / per_simd);
   p.rows_per_part = (int)((p.rows + at_once - 1) / at_once);
   const dim3 grid((unsigned)((p.S + p.rows_per_part - 1) / p.rows_per_part), (unsigned)p.B), block(64 * waves);
-  const bool token = (p.gate != nullptr && p.gs.s != 0) || (p.scale != nullptr && p.ss.s != 0) || (p.shift != nullptr && p.fs.s != 0);
-  if (token) hipLaunchKernelGGL((gated_norm_kernel<T, 1, true>), grid, block, 0, stream, p);
-  else if (p.rows_per_part == 1) hipLaunchKernelGGL((gated_norm_kernel<T, 1, false>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((gated_norm_kernel<T, sizeof(T) == 2 ? 2 : 1, false>), grid, block, 0, stream, p);  // two rows of fp32 do not fit the registers
+  if (token) hipLaunchKernelGGL((gated_norm_kernel<T, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((gated_norm_kernel<T, false>), grid, block, 0, stream, p);
   return hipGetLastError();
 }
 

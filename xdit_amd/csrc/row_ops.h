@@ -95,14 +95,29 @@ __device__ __forceinline__ float block_scale(unsigned amax_bits) {
   const float s = __uint_as_float(amax_bits) / kFp8Max;
   return amax_bits == 0 ? 1.0f : (s < 0x1p-126f ? 0x1p-126f : s);
 }
-// The largest absolute value of 8 elements, as bits.
+// The largest absolute value of 8 elements, as bits; NaN where one of them is (v_maximum3_f32: four instructions).
 __device__ __forceinline__ unsigned absmax8(const float (&v)[8]) {
-  unsigned m = 0;
+  float m = __builtin_fabsf(v[0]);
 #pragma unroll
-  for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
+  for (int i = 1; i < 8; i++) m = __builtin_elementwise_maximum(m, __builtin_fabsf(v[i]));
+  return __float_as_uint(m) & 0x7fffffffu;
 }
-// Eight quotients as e4m3 bytes.
+// 1 / sqrt(x) within a unit: the hardware's estimate and one Newton step; numbers too small for that by division.
+__device__ __forceinline__ float inv_sqrt(float x) {
+  if (x < 0x1p-100f) return 1.0f / sqrtf(x);
+  const float r = __builtin_amdgcn_rsqf(x);
+  return r * __builtin_fmaf(-0.5f * x * r, r, 1.5f);
+}
+// Eight numbers as e4m3 bytes.
+__device__ __forceinline__ i32x2 to_fp8(const float (&q)[8]) {
+  i32x2 w;
+  w[0] = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  w[0] = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w[0], true);
+  w[1] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+  w[1] = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], w[1], true);
+  return w;
+}
+// Eight quotients as the bytes of a true division.
 __device__ __forceinline__ i32x2 cast8(const float (&v)[8], const Divider& div) {
   float q[8];
   if (div.plain) {
@@ -112,12 +127,7 @@ __device__ __forceinline__ i32x2 cast8(const float (&v)[8], const Divider& div) 
 #pragma unroll
     for (int j = 0; j < 8; j++) q[j] = div(v[j]);
   }
-  i32x2 w;
-  w[0] = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-  w[0] = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w[0], true);
-  w[1] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
-  w[1] = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], w[1], true);
-  return w;
+  return to_fp8(q);
 }
 
 }  // namespace xdit
