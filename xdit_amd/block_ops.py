@@ -91,6 +91,11 @@ def _norm_code(name, kind):
         raise ValueError("%s must be None, 'rms' or 'layer'" % name) from None
 
 
+def _new_like(t):
+    """A new contiguous tensor of t's shape, dtype and device."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -108,12 +113,16 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
     None).  All arithmetic is fp32, h and n are rounded once.  `fp8`: n is a pair (e4m3 tensor, scales (B, S, ceil(C / 128))
     fp32), what `fp8_block_quant` makes of the unrounded n.  `return_stats` appends the (B, S, 4) fp32 statistics that
     `gated_norm_backward` takes.  `out_h` receives h (it may be x: the residual stream is then updated in place)."""
-    B, S, C = _hidden(x)
+    try:
+        B, S, C = x.shape
+    except (AttributeError, TypeError, ValueError):
+        raise ValueError("hidden states must be a 3-D tensor (B, S, C)") from None
     device, dtype = x.device, x.dtype
     key = ("gnorm", _sig(x), _sig(y), _sig(gate), _sig(scale), _sig(shift), _sig(weight), _sig(bias), _sig(y_weight), _sig(out_h), norm, y_norm, fp8,
            eps, y_eps, residual_scale)
 
     def build():
+        _hidden(x)
         a = _lib.GatedNormArgs()
         a.struct_size = ctypes.sizeof(a)
         a.dtype = _code(dtype)
@@ -145,14 +154,15 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
     a = _plan(key, build)
     h = out_h
     if h is None:
-        h = x if y is None else torch.empty((B, S, C), dtype=dtype, device=device)
+        h = x if y is None else _new_like(x)
     n = n_scale = stats = None
-    if norm is not None:
-        n = torch.empty((B, S, C), dtype=torch.float8_e4m3fn if fp8 else dtype, device=device)
     if fp8:
-        n_scale = torch.empty(((C + 127) // 128, B, S), dtype=torch.float32, device=device)
+        n = x.new_empty((B, S, C), dtype=torch.float8_e4m3fn)
+        n_scale = x.new_empty(((C + 127) // 128, B, S), dtype=torch.float32)
+    elif norm is not None:
+        n = _new_like(x)
     if return_stats:
-        stats = torch.empty((B, S, 4), dtype=torch.float32, device=device)
+        stats = x.new_empty((B, S, 4), dtype=torch.float32)
     if B * S * C and (y is not None or norm is not None or out_h is not None):
         a.x, a.y, a.n = x.data_ptr(), _ptr(y), _ptr(n)
         a.h = h.data_ptr() if y is not None or out_h is not None else None
@@ -236,7 +246,7 @@ def gated_norm_backward(dh, dn, h, stats, y=None, gate=None, scale=None, shift=N
         return a, outs, need
 
     a, outs, need = _plan(key, build)
-    result = {name: torch.empty(shape, dtype=dt, device=device) for name, shape, dt in outs}
+    result = {name: h.new_empty(shape, dtype=dt) for name, shape, dt in outs}
     if B * S * C == 0:
         for t in result.values():
             t.zero_()
@@ -343,10 +353,10 @@ def axes_rope(q, k, positions, inv_freq, pairs, norm=False, q_weight=None, k_wei
                           positions, inv_freq, pairs, norm, eps, rope)
 
     a = _plan(key, build)
-    oq = torch.empty((B, H, S, D), dtype=dtype, device=device) if out_q is None else out_q
+    oq = _new_like(q) if out_q is None else out_q
     ok = out_k
     if k is not None and ok is None:
-        ok = torch.empty((B, k.shape[1], S, D), dtype=dtype, device=device)
+        ok = _new_like(k)
     if B * S * D == 0:
         return oq, ok
     t = a.t[0]
@@ -396,8 +406,8 @@ def axes_rope_backward(dq, dk, positions, inv_freq, pairs, q=None, k=None, norm=
     a, need = _plan(key, build)
     outs, grads = [], []
     for d, w in ((dq, q_weight), (dk, k_weight)):
-        outs.append(None if d is None else torch.empty(d.shape, dtype=dtype, device=device))
-        grads.append(None if w is None else torch.empty((D,), dtype=w.dtype, device=device))
+        outs.append(None if d is None else _new_like(d))
+        grads.append(None if w is None else w.new_empty((D,)))
     if B * S * D == 0:
         for g in grads:
             if g is not None:
@@ -441,8 +451,8 @@ def fp8_block_quant(x, block_rows=1):
         return a
 
     a = _plan(key, build)
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
-    scale = torch.empty((kb, B, S) if block_rows == 1 else ((S + 127) // 128, kb), dtype=torch.float32, device=device)
+    y = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty((kb, B, S) if block_rows == 1 else ((S + 127) // 128, kb), dtype=torch.float32)
     if B * S * K:
         a.x, a.y, a.scale, a.stream = x.data_ptr(), y.data_ptr(), scale.data_ptr(), _stream(device)
         with _on_device(device):
@@ -508,7 +518,7 @@ def fp8_block_matmul(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16
         return a, need
 
     a, need = _plan(key, build)
-    y = torch.empty((*shape[:-1], N), dtype=out_dtype, device=device) if out is None else out
+    y = x.new_empty((*shape[:-1], N), dtype=out_dtype) if out is None else out
     if M * N == 0:
         return y
     if K == 0:
