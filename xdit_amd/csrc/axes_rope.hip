@@ -15,18 +15,32 @@ namespace xdit {
 namespace axrope {
 
 template <typename T> struct Four { typedef __attribute__((ext_vector_type(4))) T vec; };
+template <typename T> struct Pair { typename Four<T>::vec lo, hi; };
 
 // What a lane holds of a row: four pairs, as two groups of four consecutive elements at columns `a` and `b` (one group
 // of eight where they touch: interleaved pairs, and the columns behind the rotated ones).
-template <typename T, bool SPLIT>
-__device__ __forceinline__ void load_row(const void* p, int64_t off, int a, int b, float (&v)[8]) {
-  if constexpr (SPLIT) {
-    const auto lo = *(const typename Four<T>::vec*)((const T*)p + off + a), hi = *(const typename Four<T>::vec*)((const T*)p + off + b);
+template <typename T, bool SPLIT> struct RowPart {   // as loaded
+  typename Four<T>::vec lo, hi;
+  __device__ __forceinline__ void load(const void* p, int64_t off, int a, int b) {
+    if constexpr (SPLIT) {
+      lo = *(const typename Four<T>::vec*)((const T*)p + off + a);
+      hi = *(const typename Four<T>::vec*)((const T*)p + off + b);
+    } else {
+      const Raw8<T> r = load_raw8<T>(p, off + a);
+      lo = __builtin_bit_cast(Pair<T>, r).lo;
+      hi = __builtin_bit_cast(Pair<T>, r).hi;
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
     for (int i = 0; i < 4; i++) { v[i] = (float)lo[i]; v[4 + i] = (float)hi[i]; }
-  } else {
-    get8(load_raw8<T>(p, off + a), v);
   }
+};
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void load_row(const void* p, int64_t off, int a, int b, float (&v)[8]) {
+  RowPart<T, SPLIT> r;
+  r.load(p, off, a, b);
+  r.get(v);
 }
 template <typename T, bool SPLIT>
 __device__ __forceinline__ void store_row(void* p, int64_t off, int a, int b, const float (&v)[8]) {
@@ -57,14 +71,23 @@ __device__ __forceinline__ void rotate(float (&v)[8], const float (&cs)[4], cons
   }
 }
 
-// Sum over the `lpr` consecutive lanes (a power of two) that hold a row.
+// Sum over the `lpr` consecutive lanes (a power of two, uniform) that hold a row, to all of them.
 __device__ __forceinline__ float row_sum(float x, int lpr) {
-  if (lpr == 16) return row16_sum(x);
-  for (int m = 1; m < lpr; m <<= 1) x += __shfl_xor(x, m);
+  if (lpr >= 2) x = dpp_plus<0xB1>(x);    // quad_perm [1,0,3,2]
+  if (lpr >= 4) x = dpp_plus<0x4E>(x);    // quad_perm [2,3,0,1]
+  if (lpr >= 8) x = dpp_plus<0x141>(x);   // row_half_mirror
+  if (lpr >= 16) x = dpp_plus<0x140>(x);  // row_mirror
+  if (lpr >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (lpr >= 64) x = sum_halves(x);
   return x;
 }
 
-// Sines and cosines of the four pairs of lane chunk c at token (b, s); sign -1 turns back.
+// Sines and cosines of the four pairs of lane chunk c at token (b, s); sign -1 turns back.  16-bit tensors take the hardware's
+// sine and cosine of a part of a turn (off by at most 1.3e-7, against the 2^-9 or 2^-12 of the result's rounding).
+template <bool EXACT>
 __device__ __forceinline__ void turn(const AxesRopeParams& p, int b, int s, int c, float sign, float (&cs)[4], float (&sn)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; j++) { cs[j] = 1.f; sn[j] = 0.f; }
@@ -78,7 +101,12 @@ __device__ __forceinline__ void turn(const AxesRopeParams& p, int b, int s, int 
     const double f = p.freq_wide ? ((const double*)p.inv_freq)[q] : (double)((const float*)p.inv_freq)[q];
     const double turns = pos * (f * 0.15915494309189533577);  // 1 / (2 pi)
     const float r = (float)(turns - rint(turns));
-    sincospif(2.f * r, &sn[j], &cs[j]);
+    if constexpr (EXACT) {
+      sincospif(2.f * r, &sn[j], &cs[j]);
+    } else {
+      sn[j] = __builtin_amdgcn_sinf(r);
+      cs[j] = __builtin_amdgcn_cosf(r);
+    }
     sn[j] *= sign;
   }
 }
@@ -96,7 +124,7 @@ __global__ __launch_bounds__(256) void axes_rope_kernel(const AxesRopeParams p) 
   const int ca = apart ? 4 * cc : 8 * cc, cb = apart ? p.P + 4 * cc : 8 * cc + 4;
   const int b = (int)(tok / p.S), s = (int)(tok - (int64_t)b * p.S);
   float cs[4], sn[4];
-  turn(p, b, s, cc, 1.f, cs, sn);
+  turn<sizeof(T) == 4>(p, b, s, cc, 1.f, cs, sn);
   const int g0 = blockIdx.y * p.heads_per_wave, g1 = g0 + p.heads_per_wave;
   int base = 0;
   for (int t = 0; t < p.tensors; t++) {
@@ -116,7 +144,7 @@ __global__ __launch_bounds__(256) void axes_rope_kernel(const AxesRopeParams p) 
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) ss += v[i] * v[i];
-        const float r = 1.0f / sqrtf(row_sum(live ? ss : 0.f, p.lpr) * p.inv_d + p.eps);
+        const float r = inv_sqrt(row_sum(live ? ss : 0.f, p.lpr) * p.inv_d + p.eps);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] *= r * w[i];
       }
@@ -129,7 +157,7 @@ __global__ __launch_bounds__(256) void axes_rope_kernel(const AxesRopeParams p) 
 // Backward: a workgroup's wavefronts go over the tokens (token group, token group + groups, ...), four at a time, and
 // keep the sums of d x^ of their lanes' columns.
 template <typename T, bool SPLIT>
-__global__ __launch_bounds__(256) void axes_rope_bwd_kernel(const AxesRopeParams p) {
+__global__ __launch_bounds__(256, 4) void axes_rope_bwd_kernel(const AxesRopeParams p) {
   __shared__ float part[4][2][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = lane & (p.lpr - 1), slot = lane / p.lpr, slots = 64 / p.lpr;
@@ -142,7 +170,7 @@ __global__ __launch_bounds__(256) void axes_rope_bwd_kernel(const AxesRopeParams
   for (int64_t tok = (int64_t)blockIdx.x * 4 + wave; tok < (int64_t)p.B * p.S; tok += (int64_t)p.token_groups * 4) {
     const int b = (int)(tok / p.S), s = (int)(tok - (int64_t)b * p.S);
     float cs[4], sn[4];
-    turn(p, b, s, cc, -1.f, cs, sn);
+    turn<sizeof(T) == 4>(p, b, s, cc, -1.f, cs, sn);
     int base = 0;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
@@ -154,19 +182,27 @@ __global__ __launch_bounds__(256) void axes_rope_bwd_kernel(const AxesRopeParams
 #pragma unroll
       for (int i = 0; i < 8; i++) w[i] = 1.f;
       if (q.weight != nullptr && h_begin < h_end) load_gain<T, SPLIT>(q.weight, p.weight_wide, ca, cb, w);
+      RowPart<T, SPLIT> next_d, next_x;   // the heads after these are on their way while these are worked on
+      auto request = [&](int h0) {
+        const int h = min(h0 + slot, h_end - 1);
+        next_d.load(q.dy, b * q.ds_b + h * q.ds_h + s * q.ds_s, ca, cb);
+        if (p.norm) next_x.load(q.x, b * q.xs_b + h * q.xs_h + s * q.xs_s, ca, cb);
+      };
+      if (h_begin < h_end) request(h_begin);
       for (int h0 = h_begin; h0 < h_end; h0 += slots) {
         const int h = h0 + slot;
         const bool there = live && h < h_end;
         const int hc = h < h_end ? h : h_end - 1;
-        float d[8];
-        load_row<T, SPLIT>(q.dy, b * q.ds_b + hc * q.ds_h + s * q.ds_s, ca, cb, d);
+        float d[8], x[8];
+        next_d.get(d);
+        if (p.norm) next_x.get(x);
+        if (h0 + slots < h_end) request(h0 + slots);
         rotate<SPLIT>(d, cs, sn);
         if (p.norm) {
-          float x[8], ss = 0.f, dot = 0.f;
-          load_row<T, SPLIT>(q.x, b * q.xs_b + hc * q.xs_h + s * q.xs_s, ca, cb, x);
+          float ss = 0.f, dot = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; i++) ss += x[i] * x[i];
-          const float r = 1.0f / sqrtf(row_sum(live ? ss : 0.f, p.lpr) * p.inv_d + p.eps);
+          const float r = inv_sqrt(row_sum(live ? ss : 0.f, p.lpr) * p.inv_d + p.eps);
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             x[i] *= r;
@@ -205,15 +241,16 @@ __global__ __launch_bounds__(256) void axes_rope_bwd_finish_kernel(const AxesRop
   const int t = blockIdx.y;
   const RopeTensor& q = p.t[t];
   if (q.dweight == nullptr) return;
-  const int col = blockIdx.x * 4 + (threadIdx.x & 3), run = threadIdx.x >> 2;
+  const int run = threadIdx.x >> 2;
   const int n = p.head_groups * p.token_groups;
   float s = 0.f;
 #pragma unroll 8
-  for (int i = run; i < n; i += 64) s += p.partial[((int64_t)i * 2 + t) * p.D + col];
+  for (int i = run; i < n; i += 64) s += p.partial[((int64_t)i * 2 + t) * p.D + blockIdx.x * 4 + (threadIdx.x & 3)];
   part[run][threadIdx.x & 3] = s;
   __syncthreads();
-  if (run != 0) return;
-  for (int i = 1; i < 64; i++) s += part[i][threadIdx.x & 3];
+  s = wave_sum(part[threadIdx.x & 63][threadIdx.x >> 6]);   // a wavefront adds the runs of a column
+  if ((threadIdx.x & 63) != 0) return;
+  const int col = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (p.weight_wide) ((float*)q.dweight)[col] = s;
   else ((T*)q.dweight)[col] = (T)s;
 }

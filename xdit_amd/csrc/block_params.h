@@ -58,6 +58,7 @@ struct GatedNormBwdParams {
   float* partial;     // [B][parts][3][C]: sums over the rows of a part (dn u, dn, t z), see the kernel
   int parts;          // parts the rows of a batch entry are cut into
   int rows_per_part;
+  int teams;          // rows a workgroup works on at a time
   int sums;           // column sums are asked for
 };
 

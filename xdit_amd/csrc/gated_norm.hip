@@ -401,14 +401,17 @@ __device__ __forceinline__ void two_sums(float& a, float& b, int waves, int wave
   b = from_lane(t, 16);
 }
 
-// A workgroup runs over the rows of one part of one batch entry; a thread keeps the sums of its eight columns.
+// A workgroup runs over the rows of one part of one batch entry, as many at a time as it has teams of wavefronts (short rows
+// leave room for several); a thread keeps the sums of its eight columns, and the teams' sums are added in LDS at the end.
 template <typename T, bool TOKEN>
 __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwdParams p) {
-  __shared__ Posted post[2][2];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int chunks = p.C >> 3, waves = (int)blockDim.x >> 6;
-  const bool live = (int)threadIdx.x < chunks;
-  const int col = (live ? (int)threadIdx.x : 0) * 8;
+  __shared__ Posted posts[kMaxWaves][2][2];
+  extern __shared__ __align__(16) float joined[];   // [3][C] where there are several teams
+  const int lane = threadIdx.x & 63, waves = (p.C + 511) >> 9;
+  const int team = __builtin_amdgcn_readfirstlane((int)threadIdx.x / (64 * waves)), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) - team * waves;
+  const int chunks = p.C >> 3, place = 64 * wave + lane;   // of this thread's chunk
+  Posted (&post)[2][2] = posts[team];
+  const int col = (place < chunks ? place : 0) * 8;
   const int b = blockIdx.y;
   const int s0 = blockIdx.x * p.rows_per_part, s1 = min(p.S, s0 + p.rows_per_part);
   const bool has_n = p.dn != nullptr, has_y = p.y != nullptr;
@@ -424,7 +427,7 @@ __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwd
     if (has_y) ry = load_raw8<T>(p.y, b * p.ys.b + s * p.ys.s + col);
   };
   constexpr bool AHEAD = sizeof(T) == 2 && !TOKEN;   // the next row is requested ahead where the registers allow it
-  if constexpr (AHEAD) load(s0);
+  if constexpr (AHEAD) load(min(s0 + team, s1 - 1));
   float scw[8], gyw[8], sa[8] = {}, sf[8] = {}, sg[8] = {};   // (1 + scale) w, alpha gate w_y, column sums
   auto fill = [](float (&v)[8], float c) {
 #pragma unroll
@@ -445,7 +448,10 @@ __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwd
     times(p.gate, b * p.gs.b + col, p.mod_wide, 0.f, gyw);
     times(p.y_weight, col, p.weight_wide, 0.f, gyw);
   }
-  for (int s = s0, turn = 0; s < s1; s++, turn ^= 1) {
+  for (int first = s0, turn = 0; first < s1; first += p.teams, turn ^= 1) {
+    const bool there = first + team < s1;            // a team without a row goes through the motions: the barriers are everybody's
+    const bool live = there && place < chunks;
+    const int s = min(first + team, s1 - 1);
     const int64_t row = (int64_t)b * p.S + s;
     if constexpr (!AHEAD) load(s);
     const f32x4 now = st;
@@ -454,13 +460,13 @@ __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwd
     if (p.dh != nullptr) get8(rdh, t);
     if (has_n) { get8(rdn, du); get8(rh, u); }
     const Raw8<T> y_now = ry;
-    if (AHEAD && s + 1 < s1) load(s + 1);
+    if (AHEAD && first + p.teams < s1) load(min(first + p.teams + team, s1 - 1));
     if (has_n) {
 #pragma unroll
       for (int i = 0; i < 8; i++) u[i] = (u[i] - now[0]) * now[1];
       if constexpr (!TOKEN) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) { sa[i] += du[i] * u[i]; sf[i] += du[i]; du[i] *= scw[i]; }
+        for (int i = 0; i < 8; i++) { sa[i] += there ? du[i] * u[i] : 0.f; sf[i] += there ? du[i] : 0.f; du[i] *= scw[i]; }
       } else {
         if (p.mod_per_token && live && p.dshift != nullptr) store_param8<T>(p.dshift, row * p.C + col, p.mod_wide, du);
         if (p.mod_per_token && live && p.dscale != nullptr) {
@@ -476,7 +482,7 @@ __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwd
         }
         if (p.mod_per_token) times(p.scale, b * p.ss.b + s * p.ss.s + col, p.mod_wide, 1.f, du);
 #pragma unroll
-        for (int i = 0; i < 8; i++) { sa[i] += du[i] * u[i]; sf[i] += du[i]; }
+        for (int i = 0; i < 8; i++) { sa[i] += there ? du[i] * u[i] : 0.f; sf[i] += there ? du[i] : 0.f; }
         if (!p.mod_per_token) times(p.scale, b * p.ss.b + col, p.mod_wide, 1.f, du);
         times(p.weight, col, p.weight_wide, 0.f, du);
       }
@@ -498,7 +504,7 @@ __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwd
     for (int i = 0; i < 8; i++) z[i] = (z[i] - now[2]) * now[3];
     if constexpr (!TOKEN) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) { sg[i] += t[i] * z[i]; t[i] *= gyw[i]; }
+      for (int i = 0; i < 8; i++) { sg[i] += there ? t[i] * z[i] : 0.f; t[i] *= gyw[i]; }
     } else {
       if (p.gate_per_token && live && p.dgate != nullptr) {
         float d[8];
@@ -509,14 +515,14 @@ __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwd
       }
       if (!p.gate_per_token) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) sg[i] += t[i] * z[i];
+        for (int i = 0; i < 8; i++) sg[i] += there ? t[i] * z[i] : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 8; i++) t[i] *= p.alpha;
       times(p.gate, b * p.gs.b + s * p.gs.s + col, p.mod_wide, 0.f, t);
       if (p.gate_per_token) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) sg[i] += t[i] * z[i];
+        for (int i = 0; i < 8; i++) sg[i] += there ? t[i] * z[i] : 0.f;
       }
       times(p.y_weight, col, p.weight_wide, 0.f, t);
     }
@@ -533,7 +539,28 @@ __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwd
     }
     if (p.dy != nullptr && live) store8<T>(p.dy, b * p.dys.b + s * p.dys.s + col, t);
   }
-  if (!p.sums || !live) return;
+  if (!p.sums) return;
+  for (int t = 1; t < p.teams; t++) {   // the last team's sums, plus the one's before, and so on
+    if (t > 1) __syncthreads();
+    if (team == p.teams - t && place < chunks) {
+      store8<float>(joined, col, sa);
+      store8<float>(joined, p.C + col, sf);
+      store8<float>(joined, 2 * p.C + col, sg);
+    }
+    __syncthreads();
+    if (team == p.teams - t - 1 && place < chunks) {
+      float v[8];
+      auto add = [&](int vec, float (&sum)[8]) {
+        get8(load_raw8<float>(joined, vec * p.C + col), v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum[i] += v[i];
+      };
+      add(0, sa);
+      add(1, sf);
+      add(2, sg);
+    }
+  }
+  if (team != 0 || place >= chunks) return;
   float* out = p.partial + ((int64_t)b * p.parts + blockIdx.x) * 3 * p.C;
   store8<float>(out, col, sa);
   store8<float>(out, p.C + col, sf);
@@ -548,34 +575,45 @@ __device__ __forceinline__ void put_param(void* p, int64_t i, bool wide, float v
   else ((T*)p)[i] = (T)v;
 }
 
-// The parts' sums, added in a fixed order (sixteen runs of every sixteenth part, then the runs), and from them the
-// parameters' gradients; 16 columns per workgroup.
+// The parts' sums, added in a fixed order (64 runs of every 64th part, then the runs), and from them the parameters'
+// gradients; 16 columns per workgroup.
 template <typename T>
-__global__ __launch_bounds__(256) void gated_norm_bwd_finish_kernel(const GatedNormBwdParams p) {
-  __shared__ float runs[3][16][17];
+__global__ __launch_bounds__(1024) void gated_norm_bwd_finish_kernel(const GatedNormBwdParams p) {
+  constexpr int RUNS = 64;
+  __shared__ float runs[3][RUNS][17], totals[3][16];
   const int k = threadIdx.x & 15, run = threadIdx.x >> 4;
   const int c = blockIdx.x * 16 + k;
   const bool live = c < p.C;
   const int cc = live ? c : 0;
+  // parameters are requested ahead of the sums that they are multiplied with
+  const float w = p.weight != nullptr ? param_at<T>(p.weight, cc, p.weight_wide) : 1.f, bi = p.bias != nullptr ? param_at<T>(p.bias, cc, p.weight_wide) : 0.f;
+  const float yw = p.y_weight != nullptr ? param_at<T>(p.y_weight, cc, p.weight_wide) : 1.f;
   float dw = 0.f, db = 0.f, dyw = 0.f;
   for (int b = 0; b < p.B; b++) {
+    const float sc = p.scale != nullptr && !p.mod_per_token ? 1.f + param_at<T>(p.scale, b * p.ss.b + cc, p.mod_wide) : 1.f;
+    const float ga = p.alpha * (p.gate != nullptr && !p.gate_per_token ? param_at<T>(p.gate, b * p.gs.b + cc, p.mod_wide) : 1.f);
     float a = 0.f, f = 0.f, g = 0.f;
     const float* in = p.partial + ((int64_t)b * p.parts + run) * 3 * p.C + cc;
-#pragma unroll 4
-    for (int i = run; i < p.parts; i += 16, in += 48 * (int64_t)p.C) { a += in[0]; f += in[p.C]; g += in[2 * (int64_t)p.C]; }
+#pragma unroll 8
+    for (int i = run; i < p.parts; i += RUNS, in += RUNS * 3 * (int64_t)p.C) { a += in[0]; f += in[p.C]; g += in[2 * (int64_t)p.C]; }
     __syncthreads();   // the sums of the batch entry before have been read
     runs[0][run][k] = a;
     runs[1][run][k] = f;
     runs[2][run][k] = g;
     __syncthreads();
+    for (int i = threadIdx.x >> 6; i < 48; i += 16) {   // a wavefront adds the 64 runs of a column
+      const float t = wave_sum(runs[i >> 4][threadIdx.x & 63][i & 15]);
+      if ((threadIdx.x & 63) == 0) totals[i >> 4][i & 15] = t;
+    }
+    __syncthreads();
     if (run != 0 || !live) continue;
-    for (int i = 1; i < 16; i++) { a += runs[0][i][k]; f += runs[1][i][k]; g += runs[2][i][k]; }
+    a = totals[0][k];
+    f = totals[1][k];
+    g = totals[2][k];
     if (p.mod_per_token) {
       dw += a;
       db += f;
     } else {
-      const float sc = p.scale != nullptr ? 1.f + param_at<T>(p.scale, b * p.ss.b + c, p.mod_wide) : 1.f;
-      const float w = p.weight != nullptr ? param_at<T>(p.weight, c, p.weight_wide) : 1.f, bi = p.bias != nullptr ? param_at<T>(p.bias, c, p.weight_wide) : 0.f;
       if (p.dshift != nullptr) put_param<T>(p.dshift, (int64_t)b * p.C + c, p.mod_wide, f);
       if (p.dscale != nullptr) put_param<T>(p.dscale, (int64_t)b * p.C + c, p.mod_wide, w * a + bi * f);
       dw += sc * a;
@@ -584,8 +622,7 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_finish_kernel(const GatedN
     if (p.gate_per_token) {
       dyw += g;
     } else {
-      const float ga = p.alpha * (p.gate != nullptr ? param_at<T>(p.gate, b * p.gs.b + c, p.mod_wide) : 1.f);
-      if (p.dgate != nullptr) put_param<T>(p.dgate, (int64_t)b * p.C + c, p.mod_wide, p.alpha * (p.y_weight != nullptr ? param_at<T>(p.y_weight, c, p.weight_wide) : 1.f) * g);
+      if (p.dgate != nullptr) put_param<T>(p.dgate, (int64_t)b * p.C + c, p.mod_wide, p.alpha * yw * g);
       dyw += ga * g;
     }
   }
@@ -597,12 +634,13 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_finish_kernel(const GatedN
 
 template <typename T>
 static hipError_t run_bwd(const GatedNormBwdParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)p.parts, (unsigned)p.B), block(64 * ((p.C + 511) / 512));
-  if (p.mod_per_token || p.gate_per_token) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, true>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, false>), grid, block, 0, stream, p);
+  const dim3 grid((unsigned)p.parts, (unsigned)p.B), block(64 * ((p.C + 511) / 512) * p.teams);
+  const int lds = p.teams > 1 ? 12 * p.C : 0;   // several teams: rows of up to 4096 columns
+  if (p.mod_per_token || p.gate_per_token) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, true>), grid, block, lds, stream, p);
+  else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, false>), grid, block, lds, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.sums) return e;
-  hipLaunchKernelGGL((gated_norm_bwd_finish_kernel<T>), dim3((unsigned)((p.C + 15) / 16)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((gated_norm_bwd_finish_kernel<T>), dim3((unsigned)((p.C + 15) / 16)), dim3(1024), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -615,18 +653,20 @@ hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, hipStream_t st
   return hipErrorInvalidValue;
 }
 
-// Parts: as many workgroups as the chip holds at once (16 wavefronts a compute unit); with column sums at least 8 rows
-// each, so that writing and reading a part's sums (24 C bytes) stays beside the rows' 12 C and more.
+// Workgroups of up to 16 wavefronts, one on a compute unit (by registers), each with as many teams as fit; a part has two rows
+// for every team at least, so that writing and reading a part's sums (24 C bytes) stays beside the rows' 12 C and more.
 void gated_norm_bwd_plan(GatedNormBwdParams& p) {
   const bool mods = !p.mod_per_token && (p.dscale != nullptr || p.dshift != nullptr);
   p.sums = mods || (!p.gate_per_token && p.dgate != nullptr) || p.dweight != nullptr || p.dbias != nullptr || p.dy_weight != nullptr;
   const int waves = (p.C + 511) / 512;
-  const int64_t at_once = (int64_t)resident_cus() * (16 / waves > 0 ? 16 / waves : 1);
-  int per = (int)(((int64_t)p.B * p.S + at_once - 1) / at_once);
-  if (p.sums && per < 8) per = 8;
+  p.teams = 16 / waves;
+  const int64_t cus = resident_cus();
+  int64_t per = ((int64_t)p.B * p.S + cus - 1) / cus;
+  while (p.teams > 1 && p.teams > per) p.teams /= 2;   // few rows: smaller workgroups, more of them
+  if (p.sums && per < 2 * p.teams) per = 2 * p.teams;
   if (per > p.S) per = p.S;
-  p.rows_per_part = per;
-  p.parts = (p.S + per - 1) / per;
+  p.rows_per_part = (int)per;
+  p.parts = (int)((p.S + per - 1) / per);
 }
 
 hipError_t launch_gated_norm_bwd(const GatedNormBwdParams& p, int dtype, hipStream_t stream) {
