@@ -339,7 +339,7 @@ def axes_rope(q, k, positions, inv_freq, pairs, norm=False, q_weight=None, k_wei
     Angles are reduced in fp64, the rest is fp32, the result is rounded once."""
     if not isinstance(q, torch.Tensor) or q.ndim != 4:
         raise ValueError("q must be a 4-D tensor (B, H, S, D)")
-    device, dtype = q.device, q.dtype
+    device, dtype, pairs = q.device, q.dtype, tuple(pairs)
     B, H, S, D = q.shape
     key = ("arope", _sig(q), _sig(k), _sig(positions), _sig(inv_freq), pairs, norm, _sig(q_weight), _sig(k_weight), eps, rope, _sig(out_q), _sig(out_k))
 
@@ -379,7 +379,7 @@ def axes_rope_backward(dq, dk, positions, inv_freq, pairs, q=None, k=None, norm=
     gradients are summed in fp32 in a fixed order."""
     if not isinstance(dq, torch.Tensor) or dq.ndim != 4:
         raise ValueError("dq must be a 4-D tensor (B, H, S, D)")
-    device, dtype = dq.device, dq.dtype
+    device, dtype, pairs = dq.device, dq.dtype, tuple(pairs)
     B, H, S, D = dq.shape
     if not norm:
         q = k = None

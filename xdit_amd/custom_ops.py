@@ -20,15 +20,30 @@ The reference wraps a vendor kernel the same way (xfuser/core/distributed/attent
     xdit_amd::norm_rope       (x, weight, cos, sin, eps, norm, rope,
                                rope_row0, rope_rows)                        -> y (BHSD-contiguous)
 
-All tensors are logical BHSD (any B/H/S strides); outputs are BHSD-contiguous, lse is (B,H,Sq)
+and the operators around the attention call (`xdit_amd.block_ops`), with their gradients:
+
+    xdit_amd::gated_norm      (x, y?, gate?, scale?, shift?, weight?, bias?, y_weight?, norm, eps,
+                               y_norm, y_eps, residual_scale)          -> (h, n, stats)
+    xdit_amd::gated_norm_fp8  (the same)                               -> (h, n, n_scale)
+    xdit_amd::gated_norm_backward (dh?, dn?, h, stats, y?, gate?, scale?, shift?, weight?, bias?,
+                               y_weight?, norm, y_norm, residual_scale) -> list of gradients
+    xdit_amd::axes_rope       (q, k?, positions, inv_freq, pairs, norm, q_weight?, k_weight?, eps,
+                               rope)                                   -> (q, k)
+    xdit_amd::axes_rope_backward (dq, dk?, positions, inv_freq, pairs, q?, k?, norm, q_weight?,
+                               k_weight?, eps, rope)                   -> list of gradients
+    xdit_amd::fp8_block_quant (x, block_rows)                          -> (y, scale)
+    xdit_amd::fp8_block_matmul (x, x_scale, w, w_scale, bias?, out_dtype, exact_sums?) -> y
+    xdit_amd::fp8_linear      (x, w, w_scale, w_t?, w_t_scale?, bias?) -> y
+
+Attention's tensors are logical BHSD (any B/H/S strides); outputs are BHSD-contiguous, lse is (B,H,Sq)
 fp32.  The ops are registered for GPU tensors only: there is no CPU implementation.
 """
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
-from torch.library import custom_op, register_fake
+from torch.library import custom_op, register_autograd, register_fake
 
-from . import ops
+from . import block_ops, ops
 
 Tensor = torch.Tensor
 
@@ -169,3 +184,197 @@ def norm_rope(x: Tensor, weight: Tensor, cos: Tensor, sin: Tensor, eps: float, n
 @register_fake("xdit_amd::norm_rope")
 def _norm_rope_fake(x, weight, cos, sin, eps, norm, rope, rope_row0, rope_rows):
     return x.new_empty(tuple(x.shape))
+
+
+# ---------------------------------------------------------------------------- around the attention call
+def _or_none(kind: str):
+    return None if kind == "none" else kind
+
+
+def _rows16(t):
+    """A gradient as the kernels take it: autograd may pass one that was expanded from a scalar."""
+    if t is None or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1])):
+        return t
+    return t.contiguous()
+
+
+@custom_op("xdit_amd::gated_norm", mutates_args=(), device_types="cuda")
+def gated_norm(x: Tensor, y: Optional[Tensor], gate: Optional[Tensor], scale: Optional[Tensor], shift: Optional[Tensor],
+               weight: Optional[Tensor], bias: Optional[Tensor], y_weight: Optional[Tensor], norm: str, eps: float, y_norm: str,
+               y_eps: float, residual_scale: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """`block_ops.gated_norm` with its statistics; `norm` and `y_norm` are "none", "rms" or "layer".  Without `y` the first
+    result has no rows (it would be x itself), with norm "none" the second has none."""
+    h, n, stats = block_ops.gated_norm(x, y, gate, scale, shift, weight, bias, _or_none(norm), eps, _or_none(y_norm), y_weight, y_eps,
+                                       residual_scale, return_stats=True)
+    B, S, C = x.shape
+    return x.new_empty((B, 0, C)) if y is None else h, x.new_empty((B, 0, C)) if n is None else n, stats
+
+
+@register_fake("xdit_amd::gated_norm")
+def _gated_norm_fake(x, y, gate, scale, shift, weight, bias, y_weight, norm, eps, y_norm, y_eps, residual_scale):
+    B, S, C = x.shape
+    return (x.new_empty((B, 0 if y is None else S, C)), x.new_empty((B, 0 if norm == "none" else S, C)),
+            x.new_empty((B, S, 4), dtype=torch.float32))
+
+
+@custom_op("xdit_amd::gated_norm_fp8", mutates_args=(), device_types="cuda")
+def gated_norm_fp8(x: Tensor, y: Optional[Tensor], gate: Optional[Tensor], scale: Optional[Tensor], shift: Optional[Tensor],
+                   weight: Optional[Tensor], bias: Optional[Tensor], y_weight: Optional[Tensor], norm: str, eps: float, y_norm: str,
+                   y_eps: float, residual_scale: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """The same with n as fp8 values and scales, and no gradient."""
+    h, (n, n_scale) = block_ops.gated_norm(x, y, gate, scale, shift, weight, bias, norm, eps, _or_none(y_norm), y_weight, y_eps,
+                                           residual_scale, fp8=True)
+    return x.new_empty((x.shape[0], 0, x.shape[2])) if y is None else h, n, n_scale
+
+
+@register_fake("xdit_amd::gated_norm_fp8")
+def _gated_norm_fp8_fake(x, y, gate, scale, shift, weight, bias, y_weight, norm, eps, y_norm, y_eps, residual_scale):
+    B, S, C = x.shape
+    return (x.new_empty((B, 0 if y is None else S, C)), x.new_empty((B, S, C), dtype=torch.float8_e4m3fn),
+            x.new_empty(((C + 127) // 128, B, S), dtype=torch.float32).permute(1, 2, 0))
+
+
+_NORM_GRADS = ("dx", "dy", "dgate", "dscale", "dshift", "dweight", "dbias", "dy_weight")
+
+
+def _norm_grad_shapes(dn, h, y, gate, scale, shift, weight, bias, y_weight):
+    """The operand whose shape and dtype each gradient has, None where there is none (as `block_ops.gated_norm_backward`)."""
+    def seen(t):
+        return t if dn is not None else None
+    return (h, y, gate, seen(scale), seen(shift), seen(weight), seen(bias), y_weight)
+
+
+@custom_op("xdit_amd::gated_norm_backward", mutates_args=(), device_types="cuda")
+def gated_norm_backward(dh: Optional[Tensor], dn: Optional[Tensor], h: Tensor, stats: Tensor, y: Optional[Tensor], gate: Optional[Tensor],
+                        scale: Optional[Tensor], shift: Optional[Tensor], weight: Optional[Tensor], bias: Optional[Tensor],
+                        y_weight: Optional[Tensor], norm: str, y_norm: str, residual_scale: float) -> List[Tensor]:
+    """`block_ops.gated_norm_backward`: those of dx, dy, dgate, dscale, dshift, dweight, dbias and dy_weight that there are."""
+    r = block_ops.gated_norm_backward(_rows16(dh), _rows16(dn), h, stats, y, gate, scale, shift, weight, bias, _or_none(norm),
+                                      _or_none(y_norm), y_weight, residual_scale)
+    return [r[name] for name in _NORM_GRADS if name in r]
+
+
+@register_fake("xdit_amd::gated_norm_backward")
+def _gated_norm_backward_fake(dh, dn, h, stats, y, gate, scale, shift, weight, bias, y_weight, norm, y_norm, residual_scale):
+    return [t.new_empty(t.shape) for t in _norm_grad_shapes(dn, h, y, gate, scale, shift, weight, bias, y_weight) if t is not None]
+
+
+def _gated_norm_setup(ctx, inputs, output):
+    x, y, gate, scale, shift, weight, bias, y_weight, norm, _, y_norm, _, residual_scale = inputs
+    h, _, stats = output
+    ctx.save_for_backward(x if y is None else h, stats, y, gate, scale, shift, weight, bias, y_weight)
+    ctx.kinds = (norm, y_norm, residual_scale)
+
+
+def _gated_norm_grad(ctx, dh, dn, dstats):
+    h, stats, y, gate, scale, shift, weight, bias, y_weight = ctx.saved_tensors
+    norm, y_norm, residual_scale = ctx.kinds
+    dh = None if y is None else dh
+    dn = None if norm == "none" else dn
+    if dh is None and dn is None:
+        return (None,) * 13
+    out = iter(torch.ops.xdit_amd.gated_norm_backward(dh, dn, h, stats, y, gate, scale, shift, weight, bias, y_weight, norm, y_norm, residual_scale))
+    of = _norm_grad_shapes(dn, h, y, gate, scale, shift, weight, bias, y_weight)
+    return (*(None if t is None else next(out) for t in of), None, None, None, None, None)
+
+
+register_autograd("xdit_amd::gated_norm", _gated_norm_grad, setup_context=_gated_norm_setup)
+
+
+@custom_op("xdit_amd::axes_rope", mutates_args=(), device_types="cuda")
+def axes_rope(q: Tensor, k: Optional[Tensor], positions: Tensor, inv_freq: Tensor, pairs: List[int], norm: bool, q_weight: Optional[Tensor],
+              k_weight: Optional[Tensor], eps: float, rope: str) -> Tuple[Tensor, Tensor]:
+    """`block_ops.axes_rope`; without `k` the second result has no heads."""
+    oq, ok = block_ops.axes_rope(q, k, positions, inv_freq, pairs, norm, q_weight, k_weight, eps, rope)
+    return oq, q.new_empty((q.shape[0], 0, *q.shape[2:])) if k is None else ok
+
+
+@register_fake("xdit_amd::axes_rope")
+def _axes_rope_fake(q, k, positions, inv_freq, pairs, norm, q_weight, k_weight, eps, rope):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], 0 if k is None else k.shape[1], *q.shape[2:]))
+
+
+@custom_op("xdit_amd::axes_rope_backward", mutates_args=(), device_types="cuda")
+def axes_rope_backward(dq: Tensor, dk: Optional[Tensor], positions: Tensor, inv_freq: Tensor, pairs: List[int], q: Optional[Tensor],
+                       k: Optional[Tensor], norm: bool, q_weight: Optional[Tensor], k_weight: Optional[Tensor], eps: float,
+                       rope: str) -> List[Tensor]:
+    """`block_ops.axes_rope_backward`: those of dq, dk, dq_weight and dk_weight that there are."""
+    r = block_ops.axes_rope_backward(_rows16(dq), _rows16(dk), positions, inv_freq, pairs, q, k, norm, q_weight, k_weight, eps, rope)
+    return [t for t in r if t is not None]
+
+
+@register_fake("xdit_amd::axes_rope_backward")
+def _axes_rope_backward_fake(dq, dk, positions, inv_freq, pairs, q, k, norm, q_weight, k_weight, eps, rope):
+    return [t.new_empty(t.shape) for t in (dq, dk, q_weight, k_weight) if t is not None]
+
+
+def _axes_rope_setup(ctx, inputs, output):
+    q, k, positions, inv_freq, pairs, norm, q_weight, k_weight, eps, rope = inputs
+    ctx.save_for_backward(*((q, k) if norm else (None, None)), positions, inv_freq, q_weight, k_weight)
+    ctx.kinds = (list(pairs), norm, eps, rope, k is not None)
+
+
+def _axes_rope_grad(ctx, dq, dk):
+    q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
+    pairs, norm, eps, rope, has_k = ctx.kinds
+    dk = dk if has_k else None
+    out = iter(torch.ops.xdit_amd.axes_rope_backward(dq, dk, positions, inv_freq, pairs, q, k, norm, q_weight, k_weight, eps, rope))
+    gq, gk, gqw, gkw = (None if t is None else next(out) for t in (dq, dk, q_weight, k_weight))
+    return gq, gk, None, None, None, None, gqw, gkw, None, None
+
+
+register_autograd("xdit_amd::axes_rope", _axes_rope_grad, setup_context=_axes_rope_setup)
+
+
+@custom_op("xdit_amd::fp8_block_quant", mutates_args=(), device_types="cuda")
+def fp8_block_quant(x: Tensor, block_rows: int) -> Tuple[Tensor, Tensor]:
+    return block_ops.fp8_block_quant(x, block_rows)
+
+
+@register_fake("xdit_amd::fp8_block_quant")
+def _fp8_block_quant_fake(x, block_rows):
+    y = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    M, kb = x.shape[-2], (x.shape[-1] + 127) // 128
+    if block_rows != 1:
+        return y, x.new_empty(((M + 127) // 128, kb), dtype=torch.float32)
+    if x.ndim == 3:
+        return y, x.new_empty((kb, x.shape[0], M), dtype=torch.float32).permute(1, 2, 0)
+    return y, x.new_empty((kb, M), dtype=torch.float32).t()
+
+
+@custom_op("xdit_amd::fp8_block_matmul", mutates_args=(), device_types="cuda")
+def fp8_block_matmul(x: Tensor, x_scale: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor], out_dtype: torch.dtype,
+                     exact_sums: Optional[bool]) -> Tensor:
+    return block_ops.fp8_block_matmul(x, x_scale, w, w_scale, bias, out_dtype, exact_sums=exact_sums)
+
+
+@register_fake("xdit_amd::fp8_block_matmul")
+def _fp8_block_matmul_fake(x, x_scale, w, w_scale, bias, out_dtype, exact_sums):
+    return x.new_empty((*x.shape[:-1], w.shape[0]), dtype=out_dtype)
+
+
+@custom_op("xdit_amd::fp8_linear", mutates_args=(), device_types="cuda")
+def fp8_linear(x: Tensor, w: Tensor, w_scale: Tensor, w_t: Optional[Tensor], w_t_scale: Optional[Tensor], bias: Optional[Tensor]) -> Tensor:
+    """x w^T + bias of a 16- or 32-bit x, quantised here, and a frozen block-scaled weight; the gradient to x is the
+    same product of dy with the transposed weight (w_t, w_t_scale)."""
+    x8, xs = block_ops.fp8_block_quant(_rows16(x))
+    return block_ops.fp8_block_matmul(x8, xs, w, w_scale, bias, x.dtype)
+
+
+@register_fake("xdit_amd::fp8_linear")
+def _fp8_linear_fake(x, w, w_scale, w_t, w_t_scale, bias):
+    return x.new_empty((*x.shape[:-1], w.shape[0]))
+
+
+def _fp8_linear_setup(ctx, inputs, output):
+    ctx.save_for_backward(inputs[3], inputs[4])
+
+
+def _fp8_linear_grad(ctx, dy):
+    w_t, w_t_scale = ctx.saved_tensors
+    if w_t is None:
+        raise RuntimeError("the gradient of an fp8 projection needs its transposed weight")
+    return torch.ops.xdit_amd.fp8_linear(dy, w_t, w_t_scale, None, None, None), None, None, None, None, None
+
+
+register_autograd("xdit_amd::fp8_linear", _fp8_linear_grad, setup_context=_fp8_linear_setup)
