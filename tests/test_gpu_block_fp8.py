@@ -211,3 +211,24 @@ def test_refusals(gpu):
         f(*q(torch.zeros(2, 24, device=gpu)), *q(torch.zeros(8, 24, device=gpu), block_rows=128))
     with pytest.raises(RuntimeError):
         q(src.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,K,dtype", [(1, 14801, 1416, torch.bfloat16), (3, 5003, 1416, torch.float16), (1, 161003, 104, torch.float32), (2, 53, 260008, torch.bfloat16)])
+def test_quantiser_of_many_blocks(gpu, B, S, K, dtype):
+    """Large tensors, rows that are not next to each other, against the plain form and against the same rows a few at a time."""
+    g = torch.Generator(device=gpu).manual_seed(S)
+    wide = torch.randn(B, S, K + 24, generator=g, device=gpu).to(dtype)
+    wide[:, 7] = 0
+    x = wide[:, :, 16:16 + K]
+    y, s = block_ops.fp8_block_quant(x)
+    assert y.is_contiguous() and s.shape == (B, S, -(-K // 128))
+    for b in range(B):
+        for r0 in (0, S // 2, S - 19):
+            part = x[b, r0:r0 + 19]
+            ry, rs = quant_plain(part.cpu(), 1)
+            py, ps = block_ops.fp8_block_quant(part)
+            assert torch.equal(s[b, r0:r0 + 19].cpu(), rs) and torch.equal(y[b, r0:r0 + 19].cpu().view(torch.uint8), ry.view(torch.uint8))
+            assert torch.equal(s[b, r0:r0 + 19], ps) and torch.equal(y[b, r0:r0 + 19].view(torch.uint8), py.view(torch.uint8))
+    back = y.float() * s.repeat_interleave(128, -1)[..., :K]
+    assert bool(((back - x.float()).abs() <= x.float().abs() / 16 + s.repeat_interleave(128, -1)[..., :K] * 2.0 ** -9).all())
