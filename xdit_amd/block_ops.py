@@ -158,7 +158,7 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
     n = n_scale = stats = None
     if fp8:
         n = x.new_empty((B, S, C), dtype=torch.float8_e4m3fn)
-        n_scale = x.new_empty(((C + 127) // 128, B, S), dtype=torch.float32)
+        n_scale = x.new_empty_strided((B, S, (C + 127) // 128), (S, 1, B * S), dtype=torch.float32)
     elif norm is not None:
         n = _new_like(x)
     if return_stats:
@@ -174,7 +174,7 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
         if rc != 0:
             _lib.check(rc)
     if fp8:
-        n = (n, n_scale.permute(1, 2, 0))
+        n = (n, n_scale)
     return (h, n, stats) if return_stats else (h, n)
 
 
@@ -452,16 +452,19 @@ def fp8_block_quant(x, block_rows=1):
 
     a = _plan(key, build)
     y = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
-    scale = x.new_empty((kb, B, S) if block_rows == 1 else ((S + 127) // 128, kb), dtype=torch.float32)
+    if block_rows != 1:
+        scale = x.new_empty(((S + 127) // 128, kb), dtype=torch.float32)
+    elif x.ndim == 3:
+        scale = x.new_empty_strided((B, S, kb), (S, 1, B * S), dtype=torch.float32)
+    else:
+        scale = x.new_empty_strided((S, kb), (1, S), dtype=torch.float32)
     if B * S * K:
         a.x, a.y, a.scale, a.stream = x.data_ptr(), y.data_ptr(), scale.data_ptr(), _stream(device)
         with _on_device(device):
             rc = _lib.lib().xdit_fp8_block_quant(ctypes.byref(a))
         if rc != 0:
             _lib.check(rc)
-    if block_rows != 1:
-        return y, scale
-    return y, (scale.permute(1, 2, 0) if x.ndim == 3 else scale.view(kb, S).t())
+    return y, scale
 
 
 def fp8_block_matmul(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, out=None, exact_sums=None):
