@@ -218,3 +218,11 @@ def test_registered_ops_announce_shapes():
     assert ws.shape == (3, 2)
     assert o.fp8_block_matmul(m(2, 5, 136, dtype=torch.float8_e4m3fn), m(2, 5, 2), w, ws, None, torch.float32, None).shape == (2, 5, 300)
     assert o.fp8_linear(x, w, ws, None, None, None).shape == (2, 5, 300)
+
+
+def test_plans_with_rows_behind_whole_rounds():
+    """The workspace tells the parts of K of the rows that are a product of their own: fewer rows than the whole product's."""
+    need = _lib.lib().xdit_fp8_block_matmul_workspace_bytes
+    for cus, M, N, K, exact, rows in ((3, 485, 206, 1456, 1, 101), (2, 578, 132, 2736, 0, 66)):
+        n = need(ctypes.byref(matmul_args(cu_count=cus, M=M, N=N, K=K, exact_sums=exact, x_stride=K, w_stride=K, out_stride=N)))
+        assert n > 0 and n % (rows * N * 4) == 0 and n < M * N * 4 * 2

@@ -232,3 +232,22 @@ def test_quantiser_of_many_blocks(gpu, B, S, K, dtype):
             assert torch.equal(s[b, r0:r0 + 19], ps) and torch.equal(y[b, r0:r0 + 19].view(torch.uint8), py.view(torch.uint8))
     back = y.float() * s.repeat_interleave(128, -1)[..., :K]
     assert bool(((back - x.float()).abs() <= x.float().abs() / 16 + s.repeat_interleave(128, -1)[..., :K] * 2.0 ** -9).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cus,M,N,K", [(5, 1300, 520, 640), (7, 2000, 520, 656), (12, 1900, 700, 1280), (20, 1500, 1100, 1920), (24, 3300, 700, 1024), (3, 777, 264, 512), (3, 485, 206, 1456), (2, 578, 132, 2736)])
+def test_product_of_rows_beyond_whole_rounds(gpu, cus, M, N, K, monkeypatch):
+    """Rows behind the last full round of large tiles may be a product of their own, in the last two cases with K in parts: results, offsets of every
+    operand, padded outputs."""
+    monkeypatch.setitem(ops.TUNING, "cu_count", cus)
+    x, xs, w, ws, bias = operands(gpu, M, N, K)
+    sp = torch.full((M, 2 * xs.shape[1]), float("nan"), device=gpu)[:, ::2]
+    sp.copy_(xs)
+    for exact in (True, False):
+        y = block_ops.fp8_block_matmul(x, xs, w, ws, bias=bias, exact_sums=exact)
+        check(y, x, xs, w, ws, bias, exact)
+        wide = torch.full((M + 2, N + 24), 7.0, dtype=torch.bfloat16, device=gpu)
+        block_ops.fp8_block_matmul(x, sp, w, ws, bias=bias, exact_sums=exact, out=wide[1:-1, 8:8 + N])
+        assert torch.equal(wide[1:-1, 8:8 + N], y)
+        wide[1:-1, 8:8 + N] = 7
+        assert bool((wide == 7).all())
