@@ -114,15 +114,15 @@ __device__ __forceinline__ void turn(const AxesRopeParams& p, int b, int s, int 
 // One wavefront per token and head group: `lpr` lanes per row, 64 / lpr heads at a time.  32760 tokens of 40 + 40 heads of 128: 264 us, 5.1 TB/s.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void axes_rope_kernel(const AxesRopeParams p) {
-  const int64_t tok = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (tok >= (int64_t)p.B * p.S) return;  // whole wavefronts leave together
+  const unsigned tok = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // uniform, as everything of the token
+  if (tok >= (unsigned)p.B * (unsigned)p.S) return;
   const int lane = threadIdx.x & 63;
   const int c = lane & (p.lpr - 1), slot = lane / p.lpr, slots = 64 / p.lpr;
   const bool live = c * 8 < p.D;
   const int cc = live ? c : 0;
   const bool apart = SPLIT && 4 * cc < p.P;
   const int ca = apart ? 4 * cc : 8 * cc, cb = apart ? p.P + 4 * cc : 8 * cc + 4;
-  const int b = (int)(tok / p.S), s = (int)(tok - (int64_t)b * p.S);
+  const int b = (int)(tok / (unsigned)p.S), s = (int)(tok - (unsigned)b * (unsigned)p.S);
   float cs[4], sn[4];
   turn<sizeof(T) == 4>(p, b, s, cc, 1.f, cs, sn);
   const int g0 = blockIdx.y * p.heads_per_wave, g1 = g0 + p.heads_per_wave;
@@ -155,40 +155,40 @@ __global__ __launch_bounds__(256) void axes_rope_kernel(const AxesRopeParams p) 
 }
 
 // Backward: a workgroup's wavefronts go over the tokens (token group, token group + groups, ...), four at a time, and
-// keep the sums of d x^ of their lanes' columns.  8500 tokens of 24 + 24 heads of 64, fp16, split halves: 38 us, 4.1 TB/s.
+// keep the sums of d x^ of their lanes' columns.  8500 tokens of 24 + 24 heads of 64, fp16, split halves: 37 us, 4.2 TB/s.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256, 4) void axes_rope_bwd_kernel(const AxesRopeParams p) {
   __shared__ float part[4][2][512];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & (p.lpr - 1), slot = lane / p.lpr, slots = 64 / p.lpr;
   const bool live = c * 8 < p.D;
   const int cc = live ? c : 0;
   const bool apart = SPLIT && 4 * cc < p.P;
   const int ca = apart ? 4 * cc : 8 * cc, cb = apart ? p.P + 4 * cc : 8 * cc + 4;
-  const int g0 = blockIdx.y * p.heads_per_wave, g1 = g0 + p.heads_per_wave;
+  const int g0 = blockIdx.y * p.heads_per_wave, g1 = g0 + p.heads_per_wave, first = p.t[0].H;
+  const int begin[2] = {min(g0, first), max(0, g0 - first)}, end[2] = {min(first, g1), p.tensors == 2 ? min(p.t[1].H, g1 - first) : 0};   // heads of q and k
   float sum[2][8] = {};
-  for (int64_t tok = (int64_t)blockIdx.x * 4 + wave; tok < (int64_t)p.B * p.S; tok += (int64_t)p.token_groups * 4) {
-    const int b = (int)(tok / p.S), s = (int)(tok - (int64_t)b * p.S);
+  for (int64_t tok = (int64_t)blockIdx.x * 4 + wave; tok < (int64_t)p.B * p.S; tok += (int64_t)p.token_groups * 4) {   // uniform
+    const int b = (int)((unsigned)tok / (unsigned)p.S), s = (int)((unsigned)tok - (unsigned)b * (unsigned)p.S);
+    RowPart<T, SPLIT> next_d, next_x;   // the heads after these, k's first too, are on their way while these are worked on
+    auto request = [&](const RopeTensor& q, int h0, int h_end) __attribute__((always_inline)) {
+      const int h = min(h0 + slot, h_end - 1);
+      next_d.load(q.dy, b * q.ds_b + h * q.ds_h + s * q.ds_s, ca, cb);
+      if (p.norm) next_x.load(q.x, b * q.xs_b + h * q.xs_h + s * q.xs_s, ca, cb);
+    };
+    if (begin[0] < end[0]) request(p.t[0], begin[0], end[0]);
+    else request(p.t[1], begin[1], end[1]);
     float cs[4], sn[4];
     turn<sizeof(T) == 4>(p, b, s, cc, -1.f, cs, sn);
-    int base = 0;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-      if (t >= p.tensors) break;
+      if (begin[t] >= end[t]) continue;
       const RopeTensor& q = p.t[t];
-      const int h_begin = max(0, g0 - base), h_end = min(q.H, g1 - base);
-      base += q.H;
+      const int h_begin = begin[t], h_end = end[t];
       float w[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) w[i] = 1.f;
-      if (q.weight != nullptr && h_begin < h_end) load_gain<T, SPLIT>(q.weight, p.weight_wide, ca, cb, w);
-      RowPart<T, SPLIT> next_d, next_x;   // the heads after these are on their way while these are worked on
-      auto request = [&](int h0) {
-        const int h = min(h0 + slot, h_end - 1);
-        next_d.load(q.dy, b * q.ds_b + h * q.ds_h + s * q.ds_s, ca, cb);
-        if (p.norm) next_x.load(q.x, b * q.xs_b + h * q.xs_h + s * q.xs_s, ca, cb);
-      };
-      if (h_begin < h_end) request(h_begin);
+      if (q.weight != nullptr) load_gain<T, SPLIT>(q.weight, p.weight_wide, ca, cb, w);
       for (int h0 = h_begin; h0 < h_end; h0 += slots) {
         const int h = h0 + slot;
         const bool there = live && h < h_end;
@@ -196,7 +196,8 @@ __global__ __launch_bounds__(256, 4) void axes_rope_bwd_kernel(const AxesRopePar
         float d[8], x[8];
         next_d.get(d);
         if (p.norm) next_x.get(x);
-        if (h0 + slots < h_end) request(h0 + slots);
+        if (h0 + slots < h_end) request(q, h0 + slots, h_end);
+        else if (t == 0 && begin[1] < end[1]) request(p.t[1], begin[1], end[1]);
         rotate<SPLIT>(d, cs, sn);
         if (p.norm) {
           float ss = 0.f, dot = 0.f;
@@ -234,22 +235,24 @@ __global__ __launch_bounds__(256, 4) void axes_rope_bwd_kernel(const AxesRopePar
   }
 }
 
-// The workgroups' sums in a fixed order, 64 runs of every 64th and then the runs; 4 columns per workgroup.
+// The workgroups' sums in a fixed order, 256 runs of every 256th and then the runs; 4 columns per workgroup.
 template <typename T>
-__global__ __launch_bounds__(256) void axes_rope_bwd_finish_kernel(const AxesRopeParams p) {
-  __shared__ float part[64][5];
+__global__ __launch_bounds__(1024) void axes_rope_bwd_finish_kernel(const AxesRopeParams p) {
+  __shared__ float part[256][5];
   const int t = blockIdx.y;
   const RopeTensor& q = p.t[t];
   if (q.dweight == nullptr) return;
   const int run = threadIdx.x >> 2;
   const int n = p.head_groups * p.token_groups;
   float s = 0.f;
-#pragma unroll 8
-  for (int i = run; i < n; i += 64) s += p.partial[((int64_t)i * 2 + t) * p.D + blockIdx.x * 4 + (threadIdx.x & 3)];
+#pragma unroll 4
+  for (int i = run; i < n; i += 256) s += p.partial[((int64_t)i * 2 + t) * p.D + blockIdx.x * 4 + (threadIdx.x & 3)];
   part[run][threadIdx.x & 3] = s;
   __syncthreads();
-  s = wave_sum(part[threadIdx.x & 63][threadIdx.x >> 6]);   // a wavefront adds the runs of a column
-  if ((threadIdx.x & 63) != 0) return;
+  if (threadIdx.x >= 256) return;
+  const int lane = threadIdx.x & 63, of = threadIdx.x >> 6;   // a wavefront adds the runs of a column
+  s = wave_sum((part[lane][of] + part[lane + 64][of]) + (part[lane + 128][of] + part[lane + 192][of]));
+  if (lane != 0) return;
   const int col = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (p.weight_wide) ((float*)q.dweight)[col] = s;
   else ((T*)q.dweight)[col] = (T)s;
@@ -269,7 +272,7 @@ static hipError_t run(const AxesRopeParams& p, bool backward, hipStream_t stream
   else hipLaunchKernelGGL((axes_rope_bwd_kernel<T, false>), grid, block, 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.sums) return e;
-  hipLaunchKernelGGL((axes_rope_bwd_finish_kernel<T>), dim3((unsigned)(p.D / 4), (unsigned)p.tensors), block, 0, stream, p);
+  hipLaunchKernelGGL((axes_rope_bwd_finish_kernel<T>), dim3((unsigned)(p.D / 4), (unsigned)p.tensors), dim3(1024), 0, stream, p);
   return hipGetLastError();
 }
 
