@@ -80,12 +80,12 @@ __device__ __forceinline__ void row_stats(const float (&v)[R][8], bool layer, bo
   }
 }
 
-// Eight columns of a row of n as T or as part of an fp8 block: 16 lanes, a DPP row, hold its 128 columns.
+// Eight columns of a row of n as T or as part of an fp8 block, whose scale is returned: 16 lanes, a DPP row, hold its 128 columns.
 template <typename T>
-__device__ __forceinline__ void put_row8(const GatedNormParams& p, float (&n)[8], void* to, int col, int64_t row, bool live, int lane) {
+__device__ __forceinline__ float put_row8(const GatedNormParams& p, float (&n)[8], void* to, bool live) {
   if (!p.fp8) {
     if (live) store8<T>(to, 0, n);
-    return;
+    return 0.f;
   }
   // n has no bits of its own to keep (it is not stored): a product with the reciprocal, within two units of the quotient, in place
   // of the division (which with its scale took 40 % of the time: VALU instructions)
@@ -95,13 +95,11 @@ __device__ __forceinline__ void put_row8(const GatedNormParams& p, float (&n)[8]
   const float inv = __builtin_amdgcn_rcpf(scale);
 #pragma unroll
   for (int i = 0; i < 8; i++) n[i] *= inv;
-  if (live) {
-    *(i32x2*)to = to_fp8(n);
-    if ((lane & 15) == 0) p.n_scale[(int64_t)(col >> 7) * p.rows + row] = scale;
-  }
+  if (live) *(i32x2*)to = to_fp8(n);
+  return scale;
 }
 
-// TOKEN: modulation has a row per token and is fetched with it.  32760 x 5120 bf16 with y to fp8: 254 us, 4.6 TB/s; without y 141 us.
+// TOKEN: modulation has a row per token and is fetched with it.  32760 x 5120 bf16 with y to fp8: 250 us, 4.7 TB/s; without y 141 us.
 template <typename T, bool TOKEN>
 __global__ __launch_bounds__(1024, TOKEN ? 4 : 6) void gated_norm_kernel(const GatedNormParams p) {
   constexpr int R = 1;   // rows at a time
@@ -153,6 +151,7 @@ __global__ __launch_bounds__(1024, TOKEN ? 4 : 6) void gated_norm_kernel(const G
     fold_gate(0);
     fold_scale(0);
   }
+  float kept = 0.f;
   for (int s = s0, turn = 0; s < s1; s += R, turn ^= 1) {
     float h[R][8], v[R][8];
     float ym[R], yr[R], m[R], rs[R];
@@ -197,7 +196,12 @@ __global__ __launch_bounds__(1024, TOKEN ? 4 : 6) void gated_norm_kernel(const G
 #pragma unroll
       for (int i = 0; i < 8; i++) n[i] = __builtin_fmaf((h[r][i] - m[r]) * rs[r], sc[i], sh[i]);
       const int64_t at = b * p.ns.b + (s + r) * p.ns.s + col;
-      put_row8<T>(p, n, p.fp8 ? (void*)((unsigned char*)p.n + at) : (void*)((T*)p.n + at), col, row, live, lane);
+      const float scale = put_row8<T>(p, n, p.fp8 ? (void*)((unsigned char*)p.n + at) : (void*)((T*)p.n + at), live);
+      if (p.fp8) {   // a block's 16 lanes keep the scales of 16 rows and store them side by side (one at a time they cost 42 MB of partial lines there)
+        const int k = (s + r - s0) & 15, mine = lane & 15;
+        if (k == mine) kept = scale;
+        if ((k == 15 || s + r + 1 == s1) && mine <= k && (int)(threadIdx.x & ~15u) < chunks) p.n_scale[(int64_t)(threadIdx.x >> 4) * p.rows + row - k + mine] = kept;
+      }
     }
   }
 }
@@ -342,7 +346,9 @@ __global__ __launch_bounds__(256, N >= 6 ? 3 : 4) void gated_norm_wave_kernel(co
       vec8(1, k, sh);
 #pragma unroll
       for (int i = 0; i < 8; i++) n[i] = __builtin_fmaf((h[k][i] - m) * rs, sc[i], sh[i]);
-      put_row8<T>(p, n, nrow + col(k) * (p.fp8 ? 1u : (unsigned)sizeof(T)), col(k), row, k < N - 1 || last, lane);
+      const bool in = k < N - 1 || last;
+      const float scale = put_row8<T>(p, n, nrow + col(k) * (p.fp8 ? 1u : (unsigned)sizeof(T)), in);
+      if (p.fp8 && in && (lane & 15) == 0) p.n_scale[(int64_t)(col(k) >> 7) * p.rows + row] = scale;
       __builtin_amdgcn_sched_barrier(0);
     }
   }
