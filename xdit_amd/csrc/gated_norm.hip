@@ -206,7 +206,7 @@ __global__ __launch_bounds__(1024, TOKEN ? 4 : 6) void gated_norm_kernel(const G
   }
 }
 
-// Many rows: a wavefront to a row, 64 N chunks of 8 columns; the three parameter vectors of the batch entry lie in LDS, as
+// Many rows: a wavefront to a row of more than 64 (N - 1) and up to 64 N chunks of 8 columns; the three parameter vectors of the batch entry lie in LDS, as
 // halves of chunks so that a lane's 16-byte reads are consecutive.  Nothing is exchanged between wavefronts, so twelve to
 // thirty-two of them on a compute unit keep 150 KB of rows on their way.
 template <typename T, int N>
@@ -383,6 +383,7 @@ static hipError_t run(GatedNormParams p, hipStream_t stream) {
     if (waves <= 2) return launch_wave<T, 2>(p, stream);
     if (waves <= 3) return launch_wave<T, 3>(p, stream);
     if (waves <= 4) return launch_wave<T, 4>(p, stream);
+    if (waves <= 5) return launch_wave<T, 5>(p, stream);
     return launch_wave<T, 6>(p, stream);
   }
   const int per_simd = (waves + 3) / 4;   // of the six wavefronts (with modulation per token four) that fit a SIMD by registers
