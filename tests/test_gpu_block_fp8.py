@@ -251,3 +251,13 @@ def test_product_of_rows_beyond_whole_rounds(gpu, cus, M, N, K, monkeypatch):
         assert torch.equal(wide[1:-1, 8:8 + N], y)
         wide[1:-1, 8:8 + N] = 7
         assert bool((wide == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cus,M,N,K", [(12, 1900, 700, 1296), (2, 300, 520, 1936), (1, 500, 300, 144), (20, 1500, 1101, 1904)])
+def test_large_tiles_with_a_ragged_last_block(gpu, cus, M, N, K, monkeypatch):
+    monkeypatch.setitem(ops.TUNING, "cu_count", cus)
+    x, xs, w, ws, bias = operands(gpu, M, N, K)
+    for exact in (True, False):
+        for dtype in (torch.bfloat16, torch.float32):
+            check(block_ops.fp8_block_matmul(x, xs, w, ws, bias=bias, out_dtype=dtype, exact_sums=exact), x, xs, w, ws, bias, exact)

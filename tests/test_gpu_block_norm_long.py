@@ -64,3 +64,20 @@ def test_fp8_output_of_many_rows(gpu, dtype, B, S, C, y):
     full = O.spread(sc.double().reshape(B * S, -1), 1, B * S, C).view(B, S, C)
     err = (q.double() * full - rn).abs()
     assert bool((err <= 2.0 ** -4 * rn.abs() * 1.001 + 2.0 ** -10 * full + 2 * F32 * size).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,S,C,per_token", [(2, 2100, 1536, False), (1, 3001, 2056, False), (1, 1301, 5128, True), (3, 901, 520, True), (1, 5003, 8, False)])
+def test_gradients_of_many_rows(gpu, dtype, B, S, C, per_token):
+    """The chain of a column sum: rows of a part over its teams, teams, runs of parts, runs: far below a sixteenth of the rows and 80."""
+    k = problem(gpu, B, S, C, dtype, "wide", per_token)
+    opt = dict(norm="layer", y_norm="rms", residual_scale=0.7)
+    h, _, st = block_ops.gated_norm(return_stats=True, **opt, **k)
+    k.pop("x")
+    dh, dn = (torch.randn(h.shape, generator=torch.Generator(device=gpu).manual_seed(s), device=gpu).to(dtype) for s in (1, 2))
+    ref, big = O.gated_norm_backward(dh, dn, h, st, **opt, **k)
+    got = block_ops.gated_norm_backward(dh, dn, h, st, **opt, **k)
+    assert set(got) == set(ref)
+    chain = (B * S / 16 + 80) * 2.0 ** -24
+    for name in got:
+        close(got[name], ref[name], big[name], F32 if name in ("dx", "dy") else chain + F32)
