@@ -1,0 +1,68 @@
+"""Host-side logic of the operators around the attention call on the CPU: no kernels run, device calls are stubbed."""
+import contextlib
+import ctypes
+
+import pytest
+import torch
+
+from xdit_amd import block_ops, ops
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """`block_ops` on CPU tensors -> a list of the workspace that each C call was given; `calls.capturing` is what the stream says."""
+    class Calls(list):
+        capturing = False
+
+    seen = Calls()
+
+    class Lib:
+        def __getattr__(self, name):
+            if name.endswith("workspace_bytes"):
+                return lambda a: 4096
+
+            def call(a):
+                seen.append(ctypes.cast(a, ctypes.POINTER(type(a._obj))).contents.workspace)
+                return 0
+            return call
+
+    monkeypatch.setattr(block_ops, "_check", lambda *a: None)
+    monkeypatch.setattr(block_ops, "_stream", lambda device: 7)
+    monkeypatch.setattr(block_ops, "_on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(block_ops, "_capturing", lambda device: seen.capturing, raising=False)
+    monkeypatch.setattr(block_ops._lib, "lib", Lib)
+    monkeypatch.setattr(block_ops, "_SCRATCH", {})
+    monkeypatch.setattr(ops._TLS, "plans", {}, raising=False)
+    return seen
+
+
+def norm_backward():
+    h = torch.zeros(1, 4, 64)
+    block_ops.gated_norm_backward(h, h, h, torch.zeros(1, 4, 4), scale=torch.zeros(1, 64))
+
+
+def rope_backward():
+    d = torch.zeros(1, 2, 4, 64)
+    block_ops.axes_rope_backward(d, None, torch.zeros(4, 1), torch.zeros(32), (32,), q=d, norm=True, q_weight=torch.zeros(64))
+
+
+def product():
+    x = torch.zeros(4, 256).to(torch.float8_e4m3fn)
+    block_ops.fp8_block_matmul(x, torch.zeros(4, 2), x, torch.zeros(1, 2))
+
+
+@pytest.mark.parametrize("call", [norm_backward, rope_backward, product])
+def test_a_captured_call_has_scratch_of_its_own(calls, call):
+    """A graph keeps the scratch's address and may run beside other graphs and eager calls: it holds neither what the eager
+    calls of its stream share nor, through that, what another graph holds."""
+    calls.capturing = True
+    call()
+    assert calls[-1] and block_ops._SCRATCH == {}
+    calls.capturing = False
+    call()
+    call()
+    (buf,) = block_ops._SCRATCH.values()
+    assert calls[-1] == calls[-2] == buf.data_ptr()
+    calls.capturing = True
+    call()
+    assert calls[-1] != buf.data_ptr() and list(block_ops._SCRATCH.values())[0] is buf

@@ -207,3 +207,59 @@ def test_block_gradients(gpu):
     want = torch.autograd.grad(part(x), (x, m.q_gain, m.k_gain))
     for a, b in zip(torch.autograd.grad(torch.compile(part, backend="aot_eager", fullgraph=True)(x), (x, m.q_gain, m.k_gain)), want):
         assert torch.equal(a, b)
+
+
+def test_graphs_of_one_stream_replayed_side_by_side(gpu, monkeypatch):
+    """Two graphs captured on the same stream hold different scratch, and replays of them on two streams, beside eager calls on the
+    stream of the capture, give the eager bits."""
+    g = torch.Generator(device=gpu).manual_seed(3)
+    rn = lambda *s: torch.randn(*s, generator=g, device=gpu)  # noqa: E731
+    w, ws = block_ops.fp8_block_quant(rn(640, 4096) / 64, 128)
+    h, dn, y = (rn(1, 3000, 640).bfloat16() for _ in range(3))
+    scale, gate = rn(1, 640), rn(1, 640)
+    st = block_ops.gated_norm(h, scale=scale, return_stats=True)[2]
+    q, d, gain = rn(1, 5, 700, 128).bfloat16(), rn(1, 5, 700, 128).bfloat16(), rn(128)
+    inv, pairs = block_ops.rope_frequencies((44, 42, 42), device=gpu)
+    pos = torch.arange(2100, device=gpu).view(700, 3)
+
+    def work(x):
+        y8 = block_ops.fp8_block_matmul(*block_ops.fp8_block_quant(x), w, ws)
+        n = block_ops.gated_norm_backward(None, dn * x[0, 0], h, st, y=y, gate=gate, scale=scale)
+        r = block_ops.axes_rope_backward(d * x[0, 0], None, pos, inv, pairs, q=q, norm=True, q_weight=gain)
+        return (y8, *(n[k] for k in sorted(n)), r[0], r[2])
+
+    taken = []
+    plain = block_ops._scratch
+    monkeypatch.setattr(block_ops, "_scratch", lambda *a: taken.append(plain(*a)) or taken[-1])
+    side, s1, s2 = (torch.cuda.Stream() for _ in range(3))
+    xs = [rn(8, 4096).bfloat16() for _ in range(3)]
+    want = [work(x) for x in xs]
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        work(xs[2])
+    torch.cuda.synchronize()
+    graphs, outs, held = [torch.cuda.CUDAGraph() for _ in range(2)], [], []
+    for graph, x in zip(graphs, xs):
+        del taken[:]
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(work(x))
+        held.append({t.data_ptr() for t in taken})
+    del taken[:]
+    with torch.cuda.stream(side):
+        work(xs[2])
+    held.append({t.data_ptr() for t in taken})
+    assert all(held) and not held[0] & held[1] and not held[2] & (held[0] | held[1])
+    for _ in range(5):
+        for o in (*outs[0], *outs[1]):
+            o.zero_()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            with torch.cuda.stream(s1):
+                graphs[0].replay()
+            with torch.cuda.stream(s2):
+                graphs[1].replay()
+            with torch.cuda.stream(side):
+                eager = work(xs[2])
+        torch.cuda.synchronize()
+        for got, ref in zip((*outs, eager), want):
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))

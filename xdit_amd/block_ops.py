@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import TUNING, _PLANS_MAX, _RETIRED, _TLS, _code, _on_device, _sig, _stream, _stream_lock
+from .ops import TUNING, _PLANS_MAX, _RETIRED, _TLS, _capturing, _code, _on_device, _sig, _stream, _stream_lock
 
 _ROWNORM = {None: _lib.ROWNORM_NONE, "rms": _lib.ROWNORM_RMS, "layer": _lib.ROWNORM_LAYER}
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -19,14 +19,17 @@ _SCRATCH = {}
 
 
 def _scratch(device, stream, nbytes):
-    """Scratch of the calls of one (device, stream), which are ordered; taken under the stream's lock.  One that a call
-    has outgrown stays allocated: a graph captured on the stream may hold its address."""
+    """Scratch of a call, to be held until it has launched; taken under the stream's lock.  The eager calls of one (device,
+    stream) are ordered and share a buffer; one that a call has outgrown stays allocated.  A captured call has a buffer of
+    its own from the graph's memory pool, which its later calls may take over in the graph's order."""
+    if _capturing(device):
+        return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
     buf = _SCRATCH.get((device, stream))
     if buf is None or buf.numel() < nbytes:
         if buf is not None:
             _RETIRED.append(buf)
         buf = _SCRATCH[(device, stream)] = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
-    return buf.data_ptr()
+    return buf
 
 
 def _plan(key, build):
@@ -258,7 +261,8 @@ def gated_norm_backward(dh, dn, h, stats, y=None, gate=None, scale=None, shift=N
     a.stream = stream = _stream(device)
     with _stream_lock(device, stream), _on_device(device):
         if need:
-            a.workspace, a.workspace_bytes = _scratch(device, stream, need), need
+            scratch = _scratch(device, stream, need)
+            a.workspace, a.workspace_bytes = scratch.data_ptr(), need
         rc = _lib.lib().xdit_gated_norm_backward(ctypes.byref(a))
     if rc != 0:
         _lib.check(rc)
@@ -419,7 +423,8 @@ def axes_rope_backward(dq, dk, positions, inv_freq, pairs, q=None, k=None, norm=
     a.stream = stream = _stream(device)
     with _stream_lock(device, stream), _on_device(device):
         if need:
-            a.workspace, a.workspace_bytes = _scratch(device, stream, need), need
+            scratch = _scratch(device, stream, need)
+            a.workspace, a.workspace_bytes = scratch.data_ptr(), need
         rc = _lib.lib().xdit_axes_rope_backward(ctypes.byref(a))
     if rc != 0:
         _lib.check(rc)
@@ -529,7 +534,9 @@ def fp8_block_matmul(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16
     a.x, a.x_scale, a.w, a.w_scale, a.bias, a.out = x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), _ptr(bias), y.data_ptr()
     a.stream = stream = _stream(device)
     with _stream_lock(device, stream), _on_device(device):
-        a.workspace, a.workspace_bytes = (_scratch(device, stream, need), need) if need else (None, 0)
+        if need:
+            scratch = _scratch(device, stream, need)
+            a.workspace, a.workspace_bytes = scratch.data_ptr(), need
         rc = _lib.lib().xdit_fp8_block_matmul(ctypes.byref(a))
     if rc != 0:
         _lib.check(rc)

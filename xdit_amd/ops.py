@@ -45,6 +45,12 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
 
 
+def _capturing(device):
+    """Whether the current stream is being captured into a graph.  A captured call needs scratch of its own: the graph keeps the
+    address and may be replayed on any stream, beside other graphs and eager calls."""
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class _on_device:
     """`with torch.cuda.device(device)` only when the device is not the current one already."""
     __slots__ = ("ctx",)
