@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define XDIT_ATTN_ABI_VERSION 9
+#define XDIT_ATTN_ABI_VERSION 10
 
 typedef enum {
   XDIT_OK = 0,
@@ -620,6 +620,13 @@ typedef struct {
 
 int64_t xdit_fp8_block_matmul_workspace_bytes(const xdit_block_matmul_args* args);
 int xdit_fp8_block_matmul(const xdit_block_matmul_args* args);
+
+/*
+ * Number of the capture that `stream` is under, 0 if it is under none.  A captured call keeps the address of its workspace,
+ * and its graph may be replayed on any stream: give the calls of one capture a workspace that no eager call and no other
+ * capture is given, with `workspace_preserved` 0 on the first of them.
+ */
+uint64_t xdit_stream_capture_id(void* stream);
 
 /* Message of the last error on the calling thread ("" if none). Never NULL. */
 const char* xdit_attn_last_error(void);

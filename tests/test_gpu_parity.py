@@ -1879,3 +1879,50 @@ def test_fp32_error_over_many_keys_stays_at_one_rounding_per_tile(gpu, monkeypat
     ro, rl = torch.softmax(s, -1) @ v.double(), torch.logsumexp(s, -1)
     assert (o.cpu().double() - ro).norm() / ro.norm() <= 2.0 ** -24 * 500 ** 0.5
     assert (l.cpu().double() - rl).abs().max() <= 1e-5
+
+
+def test_graphs_of_one_stream_do_not_share_scratch(gpu, force_rows, monkeypatch):
+    """Two graphs captured on one stream, each with balanced attention calls and a quantiser call.  The second is replayed before
+    the first has ever run, then both at once on two streams beside eager calls on the capture's stream: always the eager bits."""
+    force_rows(384)
+    monkeypatch.setitem(ops.TUNING, "streamed", 0)   # bit equality: the fixed work geometry on both sides
+    a, b = _claimed_ranges_problem(gpu, 7), _claimed_ranges_problem(gpu, 8)
+
+    def work(q, k, v):
+        (o, l), (o2, _) = ops.attn_fwd(q, k, v), ops.attn_fwd(q, v, k)
+        y, d = ops.fp8_quant(q, per_tensor=True)
+        return o, l, o2, y.view(torch.uint8), d
+
+    assert ops.launch_plan(a[0], a[1])["ranges"] > 0
+    want = [work(*a), work(*b)]
+    side, s1, s2 = (torch.cuda.Stream() for _ in range(3))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        work(*a)
+    torch.cuda.synchronize()
+    graphs, outs, ids = [torch.cuda.CUDAGraph() for _ in range(2)], [], []
+    for graph, x in zip(graphs, (a, b)):
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(work(*x))
+            ids.append(ops._capture_id(gpu, side.cuda_stream))
+    assert None not in ids and 0 not in ids and ids[0] != ids[1] and ops._capture_id(gpu, side.cuda_stream) is None
+    key = (gpu, side.cuda_stream)
+    assert ops._CAPTURED[key][0] == ids[1] and ops._CAPTURED[key][1][0].data_ptr() != ops._WORKSPACE[key][0].data_ptr()
+    for i in (1, 0):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs[i], want[i]))
+    for _ in range(3):
+        for o in (*outs[0], *outs[1]):
+            o.zero_()
+        torch.cuda.synchronize()
+        for _ in range(2):
+            with torch.cuda.stream(s1):
+                graphs[0].replay()
+            with torch.cuda.stream(s2):
+                graphs[1].replay()
+            with torch.cuda.stream(side):
+                eager = work(*a)
+        torch.cuda.synchronize()
+        for got, ref in zip((*outs, eager), (*want, want[0])):
+            assert all(torch.equal(x, y) for x, y in zip(got, ref))

@@ -320,3 +320,43 @@ def test_the_quantisers_quotient_lies_on_the_divisions_side_of_every_fp8_roundin
                     assert ((y > m) - (y < m)) == ((quotient > m) - (quotient < m)), (x, s)
                     seen += 1
     assert seen > 200, seen
+
+
+def test_captured_calls_share_scratch_with_nothing_outside_their_capture(monkeypatch):
+    """A graph keeps the addresses of its calls' scratch and may be replayed before, beside or without any other graph and eager
+    call.  The attention calls of one capture share a workspace, which the first of them clears; the quantiser's have their own
+    (device calls stubbed, tensors on the CPU)."""
+    seen, capture = [], [None]
+
+    class Lib:
+        def xdit_attn_fwd(self, a):
+            seen.append((a._obj.workspace, a._obj.workspace_preserved))
+            return 0
+
+        def xdit_fp8_quant_batch(self, arr, n):
+            seen.append(arr[0].scratch)
+            return 0
+
+        xdit_attn_workspace_bytes = staticmethod(lambda a: 4096)
+
+    monkeypatch.setattr(ops, "_check4", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream", lambda device: 7)
+    monkeypatch.setattr(ops, "_on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(ops, "_capturing", lambda device: capture[0] is not None, raising=False)
+    monkeypatch.setattr(ops, "_capture_id", lambda device, stream: capture[0], raising=False)
+    monkeypatch.setattr(ops._lib, "lib", Lib)
+    for pool in ("_QUANT_SCRATCH", "_WORKSPACE", "_CAPTURED"):
+        monkeypatch.setattr(ops, pool, {}, raising=False)
+    x = torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16)
+    order = (None, None, 1, 1, None, 2, 2, None)
+    held = []
+    for capture[0] in order:
+        ops.attn_fwd(x, x, x)
+        held.append([e[0] for e in ops._WORKSPACE.values()] + [e[0] for _, e in getattr(ops, "_CAPTURED", {}).values()])   # no address comes back
+    eager, first, second = seen[0][0], seen[2][0], seen[5][0]
+    assert len({eager, first, second}) == 3
+    assert seen == [(eager, 0), (eager, 1), (first, 0), (first, 1), (eager, 1), (second, 0), (second, 1), (eager, 1)]
+    for capture[0] in order:
+        ops.fp8_quant(x)
+        (buf,) = ops._QUANT_SCRATCH.values()
+        assert (seen[-1] == buf.data_ptr()) == (capture[0] is None)

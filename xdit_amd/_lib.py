@@ -9,7 +9,7 @@ import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libxdit_amd_attn.so")
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 XDIT_OK = 0
 XDIT_ERR_INVALID_ARG = -1
@@ -259,7 +259,7 @@ EXPORTS = ("xdit_attn_fwd", "xdit_attn_fwd_two_queries", "xdit_attn_fwd_noalloc"
            "xdit_gated_norm", "xdit_gated_norm_backward", "xdit_gated_norm_backward_workspace_bytes",
            "xdit_axes_rope", "xdit_axes_rope_backward", "xdit_axes_rope_backward_workspace_bytes",
            "xdit_fp8_block_quant", "xdit_fp8_block_matmul", "xdit_fp8_block_matmul_workspace_bytes",
-           "xdit_attn_last_error", "xdit_attn_abi_version")
+           "xdit_stream_capture_id", "xdit_attn_last_error", "xdit_attn_abi_version")
 
 _lib = None
 _lock = threading.Lock()
@@ -312,6 +312,8 @@ def lib():
                                    ("xdit_fp8_block_matmul_workspace_bytes", BlockMatmulArgs, ctypes.c_int64)):
             f = getattr(L, name)
             f.argtypes, f.restype = [ctypes.POINTER(args)], result
+        L.xdit_stream_capture_id.argtypes = [ctypes.c_void_p]
+        L.xdit_stream_capture_id.restype = ctypes.c_uint64
         L.xdit_attn_last_error.argtypes = []
         L.xdit_attn_last_error.restype = ctypes.c_char_p
         L.xdit_attn_abi_version.argtypes = []

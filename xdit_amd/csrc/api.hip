@@ -327,6 +327,13 @@ int api_fail(int code, const char* fmt, ...) {
 
 extern "C" {
 
+uint64_t xdit_stream_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess || status != hipStreamCaptureStatusActive) return 0;
+  return id;
+}
+
 const char* xdit_attn_last_error(void) { return g_err; }
 
 int xdit_attn_abi_version(void) { return XDIT_ATTN_ABI_VERSION; }

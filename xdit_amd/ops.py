@@ -51,6 +51,11 @@ def _capturing(device):
     return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
 
+def _capture_id(device, stream):
+    """What tells the capture that `stream`, the current one, is under from every other capture; None if it is under none."""
+    return _lib.lib().xdit_stream_capture_id(stream) if _capturing(device) else None
+
+
 class _on_device:
     """`with torch.cuda.device(device)` only when the device is not the current one already."""
     __slots__ = ("ctx",)
@@ -69,6 +74,7 @@ class _on_device:
 
 
 _WORKSPACE = {}
+_CAPTURED = {}
 _RETIRED = []
 _STREAM_LOCKS = {}
 
@@ -86,8 +92,17 @@ def _workspace(device, stream, nbytes):
     Calls on one stream are ordered, so one buffer per (device, stream) is reused from call to
     call; nothing else ever writes it, which is what `workspace_preserved` tells the library once
     a call on the buffer has returned without error (the caller sets entry[1] then).  A buffer that has become too small is kept alive rather than freed, so
-    that its address cannot come back as a new buffer with foreign contents."""
+    that its address cannot come back as a new buffer with foreign contents.
+    The calls of one capture on the stream share a buffer from the graph's memory pool: the first of them clears its counters in
+    every replay, and neither eager calls nor other graphs ever write it."""
     key = (device, stream)
+    capture = _capture_id(device, stream)
+    if capture is not None:
+        known, entry = _CAPTURED.get(key, (None, None))
+        if known != capture or entry[0].numel() < nbytes:
+            entry = [torch.empty(int(nbytes), dtype=torch.uint8, device=device), 0]
+            _CAPTURED[key] = (capture, entry)
+        return entry
     entry = _WORKSPACE.get(key)
     if entry is None or entry[0].numel() < nbytes:
         if entry is not None:
@@ -483,12 +498,15 @@ def fp8_quant_batch(jobs, joined=()):
                 a.x2, a.y2 = x2.data_ptr(), y2.data_ptr()
             out.append((y, y2, descale))
     with _stream_lock(device, stream), _on_device(device):
-        buf = _QUANT_SCRATCH.get((device, stream))
-        if buf is None or buf.numel() < sum(need):
-            if buf is not None:
-                _RETIRED.append(buf)   # a graph captured on this stream may hold its address
+        if _capturing(device):
             buf = torch.empty(sum(need), dtype=torch.uint8, device=device)
-            _QUANT_SCRATCH[(device, stream)] = buf
+        else:
+            buf = _QUANT_SCRATCH.get((device, stream))
+            if buf is None or buf.numel() < sum(need):
+                if buf is not None:
+                    _RETIRED.append(buf)
+                buf = torch.empty(sum(need), dtype=torch.uint8, device=device)
+                _QUANT_SCRATCH[(device, stream)] = buf
         scratch = buf.data_ptr()
         for a, size in zip(arr, need):
             a.scratch, a.scratch_bytes = scratch, size
