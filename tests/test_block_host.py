@@ -66,3 +66,14 @@ def test_a_captured_call_has_scratch_of_its_own(calls, call):
     calls.capturing = True
     call()
     assert calls[-1] != buf.data_ptr() and list(block_ops._SCRATCH.values())[0] is buf
+
+
+@pytest.mark.parametrize("norm,C", [(None, 64), ("layer", 0)])
+def test_statistics_of_a_call_without_a_launch(calls, norm, C):
+    """Mean 0 and reciprocal deviation 1 for norms that are absent, also where nothing is left to compute."""
+    poison = [torch.full((3, 5, 4), 7.0) for _ in range(50)]
+    del poison
+    x = torch.zeros(3, 5, C)
+    h, n, stats = block_ops.gated_norm(x, norm=norm, return_stats=True)
+    assert calls == [] and h is x and (n is None) == (norm is None)
+    assert torch.equal(stats, torch.tensor([0.0, 1.0, 0.0, 1.0]).expand(3, 5, 4))

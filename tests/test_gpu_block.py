@@ -263,3 +263,13 @@ def test_graphs_of_one_stream_replayed_side_by_side(gpu, monkeypatch):
         torch.cuda.synchronize()
         for got, ref in zip((*outs, eager), want):
             assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_norm_of_nothing_has_the_statistics_of_absent_norms(gpu):
+    x = torch.randn(2, 5, 64, device=gpu).bfloat16()
+    torch.full((2, 5, 4), 7.0, device=gpu)
+    want = torch.tensor([0.0, 1.0, 0.0, 1.0], device=gpu).expand(2, 5, 4)
+    assert torch.equal(block_ops.gated_norm(x, norm=None, return_stats=True)[2], want)
+    torch.full((2, 5, 4), 7.0, device=gpu)
+    assert torch.equal(torch.ops.xdit_amd.gated_norm(x, *(None,) * 7, "none", 1e-6, "none", 1e-6, 1.0)[2], want)
+    assert torch.equal(block_ops.gated_norm(x, y=x, norm=None, return_stats=True)[2], want)

@@ -176,6 +176,8 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
             rc = _lib.lib().xdit_gated_norm(ctypes.byref(a))
         if rc != 0:
             _lib.check(rc)
+    elif return_stats:   # nothing to compute: the statistics of norms that are absent
+        stats.zero_()[..., 1::2] = 1
     if fp8:
         n = (n, n_scale)
     return (h, n, stats) if return_stats else (h, n)
