@@ -4,8 +4,9 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from xdit_amd import block_ops, ops
+from xdit_amd import block, block_ops, ops
 
 
 @pytest.fixture
@@ -77,3 +78,22 @@ def test_statistics_of_a_call_without_a_launch(calls, norm, C):
     h, n, stats = block_ops.gated_norm(x, norm=norm, return_stats=True)
     assert calls == [] and h is x and (n is None) == (norm is None)
     assert torch.equal(stats, torch.tensor([0.0, 1.0, 0.0, 1.0]).expand(3, 5, 4))
+
+
+def test_tangents_are_refused():
+    """A forward-mode dual tensor wants no reverse gradient, so the kernels would read its values and drop its tangent."""
+    x, w, q = torch.randn(1, 4, 64), torch.ones(64), torch.randn(1, 2, 4, 64)
+    freq, pairs = block.rope_frequencies((64,))
+    linear = block.Fp8Linear.__new__(block.Fp8Linear)
+    torch.nn.Module.__init__(linear)
+    pos = torch.zeros(4, 1)
+    with forward_ad.dual_level():
+        d = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: block.gated_norm(d(x)), lambda: block.gated_norm(x, weight=d(w)), lambda: block.axes_rope(d(q), None, pos, freq, pairs),
+                     lambda: block.axes_rope(q, q, pos, freq, pairs, norm=True, k_weight=d(w)), lambda: linear(d(x))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="no CPU path"):   # no tangent: as ever
+            block.gated_norm(x)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: block.gated_norm(t)[1], (x,), (x,))

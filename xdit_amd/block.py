@@ -1,9 +1,11 @@
 """Module-level forms of the operators around the attention call of a DiT block, differentiable and traceable.
 
 The functions take what `xdit_amd.block_ops` takes.  Where a gradient is wanted, or under `torch.compile`, they go through the
-registered ops of `xdit_amd.custom_ops`; otherwise straight to the kernels.
+registered ops of `xdit_amd.custom_ops`; otherwise straight to the kernels.  Gradients are those of reverse mode: tangents of
+forward-mode differentiation are refused.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import block_ops
 from . import custom_ops  # noqa: F401  (registers torch.ops.xdit_amd.*)
@@ -12,6 +14,8 @@ rope_frequencies = block_ops.rope_frequencies
 
 
 def _registered(*tensors):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode differentiation is not supported: the tangent would be lost")
     return torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
