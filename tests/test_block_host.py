@@ -97,3 +97,14 @@ def test_tangents_are_refused():
             block.gated_norm(x)
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda t: block.gated_norm(t)[1], (x,), (x,))
+
+
+def test_a_gradient_that_starts_anywhere_is_copied():
+    from xdit_amd import custom_ops
+    flat = torch.arange(3 * 64 + 8, dtype=torch.bfloat16)
+    for at in range(8):
+        t = flat[at:at + 3 * 64].view(1, 3, 64)
+        r = custom_ops._rows16(t)
+        assert r.data_ptr() % 16 == 0 and r.is_contiguous() and torch.equal(r, t)
+        assert (r is t) == (t.data_ptr() % 16 == 0)
+    assert custom_ops._rows16(torch.ones(()).expand(1, 3, 64)).is_contiguous() and custom_ops._rows16(None) is None

@@ -273,3 +273,21 @@ def test_norm_of_nothing_has_the_statistics_of_absent_norms(gpu):
     torch.full((2, 5, 4), 7.0, device=gpu)
     assert torch.equal(torch.ops.xdit_amd.gated_norm(x, *(None,) * 7, "none", 1e-6, "none", 1e-6, 1.0)[2], want)
     assert torch.equal(block_ops.gated_norm(x, y=x, norm=None, return_stats=True)[2], want)
+
+
+def test_gradients_that_start_anywhere(gpu):
+    """The gradient of a result that went into a concatenation is a part of that one's, at any element: the same bits as one by itself."""
+    g = torch.Generator(device=gpu).manual_seed(9)
+    rn = lambda *s: torch.randn(*s, generator=g, device=gpu)  # noqa: E731
+    x = rn(1, 6, 128).bfloat16().requires_grad_()
+    q = rn(1, 2, 6, 128).bfloat16().requires_grad_()
+    pad, r = torch.zeros(3, device=gpu, dtype=torch.bfloat16), rn(6 * 128 * 2).bfloat16()
+    freq, pairs = block.rope_frequencies((44, 42, 42), device=gpu)
+    linear = block.Fp8Linear((rn(256, 128) / 11).bfloat16(), backward=True)
+    pos = torch.arange(18, device=gpu).view(6, 3)
+    for t, f in ((x, lambda: block.gated_norm(x, norm="rms")[1]), (q, lambda: block.axes_rope(q, None, pos, freq, pairs, norm=True)[0]), (x, lambda: linear(x))):
+        y = f().flatten()
+        (want,) = torch.autograd.grad(y, t, r[:y.numel()])
+        cat = torch.cat([pad, f().flatten()])
+        (got,) = torch.autograd.grad(cat, t, torch.cat([pad, r[:y.numel()]]))
+        assert torch.equal(got, want)
