@@ -1,6 +1,5 @@
 """Host-side logic of the operators around the attention call on the CPU: no kernels run, device calls are stubbed."""
 import contextlib
-import ctypes
 
 import pytest
 import torch
@@ -23,7 +22,7 @@ def calls(monkeypatch):
                 return lambda a: 4096
 
             def call(a):
-                seen.append(ctypes.cast(a, ctypes.POINTER(type(a._obj))).contents.workspace)
+                seen.append(getattr(a._obj, "workspace", None))
                 return 0
             return call
 
@@ -108,3 +107,17 @@ def test_a_gradient_that_starts_anywhere_is_copied():
         assert r.data_ptr() % 16 == 0 and r.is_contiguous() and torch.equal(r, t)
         assert (r is t) == (t.data_ptr() % 16 == 0)
     assert custom_ops._rows16(torch.ones(()).expand(1, 3, 64)).is_contiguous() and custom_ops._rows16(None) is None
+
+
+def test_projection_takes_any_rows_without_gradients_too(calls):
+    """What a call with gradients takes (the registered op copies rows that are not dense and aligned) one without them takes as well."""
+    linear = block.Fp8Linear(torch.zeros(32, 64))
+    seen = []
+    plain, block_ops.fp8_block_quant = block_ops.fp8_block_quant, lambda x, *a: seen.append(x) or plain(x, *a)
+    try:
+        for x in (torch.zeros(2, 64, 6).transpose(1, 2), torch.zeros(2 * 64 + 1)[1:].view(2, 64), torch.zeros(4, 66)[:, :64], torch.zeros(4, 64)):
+            assert linear(x).shape == (*x.shape[:-1], 32)
+            assert seen[-1].stride(-1) == 1 and seen[-1].stride(-2) % 4 == 0 and seen[-1].data_ptr() % 16 == 0
+        assert seen[-1] is x
+    finally:
+        block_ops.fp8_block_quant = plain

@@ -291,3 +291,13 @@ def test_gradients_that_start_anywhere(gpu):
         cat = torch.cat([pad, f().flatten()])
         (got,) = torch.autograd.grad(cat, t, torch.cat([pad, r[:y.numel()]]))
         assert torch.equal(got, want)
+
+
+def test_projection_of_strided_and_unaligned_activations(gpu):
+    g = torch.Generator(device=gpu).manual_seed(10)
+    linear = block.Fp8Linear(torch.randn(200, 128, generator=g, device=gpu) / 11)
+    x = torch.randn(2, 128, 7, generator=g, device=gpu).bfloat16().transpose(1, 2)
+    flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=gpu)
+    flat[1:] = x.contiguous().flatten()
+    want = linear(x.contiguous())
+    assert torch.equal(linear(x), want) and torch.equal(linear(flat[1:].view(2, 7, 128)), want) and torch.equal(linear(x.clone().requires_grad_()), want)

@@ -8,7 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import block_ops
-from . import custom_ops  # noqa: F401  (registers torch.ops.xdit_amd.*)
+from . import custom_ops  # registers torch.ops.xdit_amd.*
 
 rope_frequencies = block_ops.rope_frequencies
 
@@ -56,7 +56,7 @@ def axes_rope(q, k, positions, inv_freq, pairs, norm=False, q_weight=None, k_wei
 class Fp8Linear(torch.nn.Module):
     """A projection with a frozen weight in fp8 and a scale per 128 x 128 block.
 
-    forward(x): x (M, K) or (B, S, K) in 16 or 32 bits, or the (values, scales) pair of `fp8_block_quant` or of `gated_norm(fp8=True)`
+    forward(x): x (M, K) or (B, S, K) in 16 or 32 bits (copied first where its rows are not 16-byte aligned and dense), or the (values, scales) pair of `fp8_block_quant` or of `gated_norm(fp8=True)`
     -> x w^T + bias in x's dtype (for a pair in that of the weight it was made from).  `backward=True` also lays out the transposed
     weight, whose blocks keep their bytes, for the gradient to x; in_features has to be a multiple of 16, out_features too then."""
 
@@ -95,5 +95,5 @@ class Fp8Linear(torch.nn.Module):
             return block_ops.fp8_block_matmul(x8, scale, self.weight, self.weight_scale, self.bias, self.dtype)
         if _registered(x):
             return torch.ops.xdit_amd.fp8_linear(x, self.weight, self.weight_scale, self.weight_t, self.weight_t_scale, self.bias)
-        x8, scale = block_ops.fp8_block_quant(x)
+        x8, scale = block_ops.fp8_block_quant(custom_ops._rows16(x))
         return block_ops.fp8_block_matmul(x8, scale, self.weight, self.weight_scale, self.bias, x.dtype)

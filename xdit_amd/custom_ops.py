@@ -192,9 +192,9 @@ def _or_none(kind: str):
 
 
 def _rows16(t):
-    """A gradient as the kernels take it: autograd may pass one that was expanded from a scalar, or a part of a larger
+    """A tensor as the kernels take it: autograd may pass a gradient that was expanded from a scalar, or a part of a larger
     one that starts anywhere (a copy: `contiguous` would return the part itself)."""
-    if t is None or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1])):
+    if t is None or (t.data_ptr() % 16 == 0 and (t.is_contiguous() or (t.stride(-1) == 1 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1])))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
