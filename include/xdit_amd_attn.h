@@ -420,6 +420,7 @@ int xdit_qk_prologue_batch(const xdit_prologue_args* jobs, int32_t count);
  *     n = (rms(h) | layer(h)) * weight + bias, times (1 + scale), plus shift   (norm)
  * with layer(h) = (h - mean) / sqrt(var + eps) and rms(h) = h / sqrt(mean(h^2) + eps) over C.  What is NULL is
  * left out.  Everything is computed in fp32 from the inputs; h and n are rounded once, n from the unrounded h.
+ * A row whose mean square is beyond fp32 (elements of some 2^63 and more) has an infinite deviation: its norm is zero.
  * `fp8 != 0`: n is written as e4m3 bytes with one fp32 scale per block of 128 columns of a row, as
  * xdit_fp8_block_quant would quantise the unrounded n; n_scale[kb * B*S + b*S + s] holds the scale of columns
  * [128 kb, 128 kb + 128).  `stats` (optional) receives (mean, 1/deviation) of h and of y, four floats a row

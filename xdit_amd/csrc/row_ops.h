@@ -102,9 +102,11 @@ __device__ __forceinline__ unsigned absmax8(const float (&v)[8]) {
   for (int i = 1; i < 8; i++) m = __builtin_elementwise_maximum(m, __builtin_fabsf(v[i]));
   return __float_as_uint(m) & 0x7fffffffu;
 }
-// 1 / sqrt(x) within a unit: the hardware's estimate and one Newton step; numbers too small for that by division.
+// 1 / sqrt(x) within a unit: the hardware's estimate and one Newton step; numbers too small for that by division, and
+// infinity (the step would make its zero a NaN), which one comparison of the bits finds with them.
 __device__ __forceinline__ float inv_sqrt(float x) {
-  if (x < 0x1p-100f) return 1.0f / sqrtf(x);
+  constexpr unsigned kLow = 0x0d800000u, kInf = 0x7f800000u;   // 2^-100, infinity
+  if (__float_as_uint(x) - kLow >= kInf - kLow) return 1.0f / sqrtf(x);
   const float r = __builtin_amdgcn_rsqf(x);
   return r * __builtin_fmaf(-0.5f * x * r, r, 1.5f);
 }
