@@ -226,3 +226,20 @@ def test_plans_with_rows_behind_whole_rounds():
     for cus, M, N, K, exact, rows in ((3, 485, 206, 1456, 1, 101), (2, 578, 132, 2736, 0, 66)):
         n = need(ctypes.byref(matmul_args(cu_count=cus, M=M, N=N, K=K, exact_sums=exact, x_stride=K, w_stride=K, out_stride=N)))
         assert n > 0 and n % (rows * N * 4) == 0 and n < M * N * 4 * 2
+
+
+def test_outputs_whose_rows_overlap_across_axes():
+    """Strides that clear a row by themselves but meet between two axes: two rows at one place would be written in any order."""
+    L, R, T = _lib.lib(), _lib.RowStrides, _lib.Strides
+    for kw in (dict(h_stride=R(64, 64)), dict(n_stride=R(128, 64)), dict(h_stride=R(64 * 4, 64)), dict(h_stride=R(96, 64)), dict(h_stride=R(72, 64))):
+        refused(L.xdit_gated_norm, norm_args(**kw), BAD, "overlap")
+    refused(L.xdit_gated_norm_backward, norm_backward_args(dx_stride=R(64, 64)), BAD, "overlap")
+    refused(L.xdit_fp8_block_quant, quant_args(B=2, y_stride=R(136, 136), x_stride=R(6 * 136, 136)), BAD, "overlap")
+    for st in (T(18 * 64, 64, 64), T(18 * 64, 128, 64), T(64, 64, 64), T(18 * 64, 64, 128), T(18 * 64, 64 * 5, 64)):
+        refused(L.xdit_axes_rope, rope_args(t=dict(y_stride=st)), BAD, "overlap")
+    refused(L.xdit_axes_rope, rope_args(B=2, t=dict(y_stride=T(64, 6 * 64, 64))), BAD, "overlap")
+    # what does not meet gets as far as the next refusal: any order of the axes, rows with space between them
+    for st in (R(320, 64), R(64, 128), R(72, 144), R(1 << 60, 64), R(5 * 72, 72)):
+        refused(L.xdit_gated_norm, norm_args(h_stride=st, weight=P + 4), BAD, "weight is not")
+    for st in (T(0, 6 * 64, 64), T(0, 64, 3 * 64), T(0, 72, 72 * 3), T(0, 72 * 6, 72)):
+        refused(L.xdit_axes_rope, rope_args(t=dict(y_stride=st, weight=P + 4)), BAD, "weight is not")

@@ -2,6 +2,7 @@
 // Nothing here allocates device memory or synchronises; every launch goes to the caller's stream.
 #include "../../include/xdit_amd_attn.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -17,6 +18,20 @@ bool multiple_of(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t
 bool float_dtype(int d) { return d == XDIT_DTYPE_BF16 || d == XDIT_DTYPE_FP16 || d == XDIT_DTYPE_FP32; }
 int size_of(int d) { return d == XDIT_DTYPE_FP32 ? 4 : 2; }
 
+// Whether no two rows of `C` elements share one: going from the smallest stride up, each has to step over all that those below it reach.
+struct Axis { int64_t n, stride; };
+template <int N>
+bool rows_apart(int64_t C, Axis (&axes)[N]) {
+  std::sort(axes, axes + N, [](const Axis& a, const Axis& b) { return a.stride < b.stride; });
+  __int128 reach = C;
+  for (const Axis& a : axes) {
+    if (a.n <= 1) continue;
+    if (a.stride < reach) return false;
+    reach += (__int128)a.stride * (a.n - 1);
+  }
+  return true;
+}
+
 // A (B, S, C) tensor whose rows are read or written 8 elements at a time.  `written`: rows must not overlap.
 int check_rows(const char* name, const void* p, const xdit_row_strides& st, int esize, int64_t B, int64_t S, int64_t C, bool written) {
   if (p == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "%s is NULL", name);
@@ -26,7 +41,8 @@ int check_rows(const char* name, const void* p, const xdit_row_strides& st, int 
   if ((B > 1 && st.b % m) || (S > 1 && st.s % m))
     return api_fail(XDIT_ERR_INVALID_ARG, "%s: strides (%lld,%lld) must be multiples of %lld elements", name, (long long)st.b, (long long)st.s, (long long)m);
   if (st.b < 0 || st.s < 0) return api_fail(XDIT_ERR_INVALID_ARG, "%s: negative stride", name);
-  if (written && ((S > 1 && st.s < C) || (B > 1 && st.b < C)))
+  Axis axes[] = {{B, st.b}, {S, st.s}};
+  if (written && !rows_apart(C, axes))
     return api_fail(XDIT_ERR_INVALID_ARG, "%s: strides (%lld,%lld) make its rows of %lld overlap", name, (long long)st.b, (long long)st.s, (long long)C);
   return 0;
 }
@@ -223,6 +239,9 @@ static int fill_axes_rope(const xdit_axes_rope_args* a, xdit::AxesRopeParams& p,
       if (!r.used) continue;
       const xdit_row_strides bs = {r.st->b, r.st->s}, bh = {r.st->b, r.st->h};
       if ((rc = check_rows(r.name, r.ptr, bs, es, a->B, a->S, a->D, r.written)) || (rc = check_rows(r.name, r.ptr, bh, es, a->B, t.H, a->D, r.written))) return rc;
+      Axis axes[] = {{a->B, r.st->b}, {t.H, r.st->h}, {a->S, r.st->s}};
+      if (r.written && !rows_apart(a->D, axes))
+        return api_fail(XDIT_ERR_INVALID_ARG, "%s: strides (%lld,%lld,%lld) make its rows of %d overlap", r.name, (long long)r.st->b, (long long)r.st->h, (long long)r.st->s, a->D);
     }
     if (t.weight != nullptr && !p.norm) return api_fail(XDIT_ERR_INVALID_ARG, "a weight needs the norm");
     if ((rc = check_vector("weight", t.weight))) return rc;
