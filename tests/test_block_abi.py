@@ -243,3 +243,12 @@ def test_outputs_whose_rows_overlap_across_axes():
         refused(L.xdit_gated_norm, norm_args(h_stride=st, weight=P + 4), BAD, "weight is not")
     for st in (T(0, 6 * 64, 64), T(0, 64, 3 * 64), T(0, 72, 72 * 3), T(0, 72 * 6, 72)):
         refused(L.xdit_axes_rope, rope_args(t=dict(y_stride=st, weight=P + 4)), BAD, "weight is not")
+
+
+def test_the_row_stride_of_a_single_row_is_not_looked_at():
+    L = _lib.lib()
+    for stride in (1 << 24, 1 << 40, 5, -16, 0):
+        for kw in (dict(M=1, x_stride=stride), dict(N=1, w_stride=stride)):
+            refused(L.xdit_fp8_block_matmul, matmul_args(bias=P + 2, **kw), BAD, "bias")
+    refused(L.xdit_fp8_block_matmul, matmul_args(x_stride=1 << 24), BAD, "2^24")
+    refused(L.xdit_fp8_block_matmul, matmul_args(w_stride=1 << 24), BAD, "2^24")

@@ -261,3 +261,16 @@ def test_large_tiles_with_a_ragged_last_block(gpu, cus, M, N, K, monkeypatch):
     for exact in (True, False):
         for dtype in (torch.bfloat16, torch.float32):
             check(block_ops.fp8_block_matmul(x, xs, w, ws, bias=bias, out_dtype=dtype, exact_sums=exact), x, xs, w, ws, bias, exact)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stride", [1 << 24, 1 << 33, 16])
+def test_a_single_row_of_any_stride(gpu, stride):
+    """One row of x, one of w: the stride to the next row does not matter."""
+    x, xs, w, ws, bias = operands(gpu, 1, 130, 400)
+    far = torch.as_strided(x, (1, 400), (stride, 1))
+    assert far.stride(0) == stride
+    assert torch.equal(block_ops.fp8_block_matmul(far, xs, w, ws, bias=bias), block_ops.fp8_block_matmul(x, xs, w, ws, bias=bias))
+    x, xs, w, ws, bias = operands(gpu, 70, 1, 400)
+    far = torch.as_strided(w, (1, 400), (stride, 1))
+    assert torch.equal(block_ops.fp8_block_matmul(x, xs, far, ws, bias=bias), block_ops.fp8_block_matmul(x, xs, w, ws, bias=bias))

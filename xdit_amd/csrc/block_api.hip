@@ -335,7 +335,7 @@ static int fill_block_matmul(const xdit_block_matmul_args* a, xdit::BlockMatmulP
   if (!multiple_of(a->x, 16) || !multiple_of(a->w, 16)) return api_fail(XDIT_ERR_INVALID_ARG, "x and w must be 16-byte aligned");
   if ((a->M > 1 && (a->x_stride % 16 || a->x_stride < a->K)) || (a->N > 1 && (a->w_stride % 16 || a->w_stride < a->K)))
     return api_fail(XDIT_ERR_INVALID_ARG, "rows of x and w must be multiples of 16 bytes apart, at least K = %lld", (long long)a->K);
-  if (a->x_stride >= (1 << 24) || a->w_stride >= (1 << 24)) return api_fail(XDIT_ERR_INVALID_ARG, "row strides of 2^24 bytes or more are not supported");
+  if ((a->M > 1 && a->x_stride >= (1 << 24)) || (a->N > 1 && a->w_stride >= (1 << 24))) return api_fail(XDIT_ERR_INVALID_ARG, "row strides of 2^24 bytes or more are not supported");
   if (!multiple_of(a->out, size_of(a->out_dtype)) || (a->M > 1 && a->out_stride < a->N))
     return api_fail(XDIT_ERR_INVALID_ARG, "out is not aligned to its elements or its rows overlap");
   if (a->x_scale_stride_m < 0 || a->x_scale_stride_k < 0 || a->w_scale_stride_n < 0 || a->w_scale_stride_k < 0)
