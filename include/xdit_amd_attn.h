@@ -516,7 +516,7 @@ int xdit_gated_norm_backward(const xdit_gated_norm_backward_args* args);
  * with the pair's elements 2p and 2p + 1 (XDIT_ROPE_INTERLEAVED) or p and p + P (XDIT_ROPE_SPLIT_HALF); columns from 2P on
  * are not rotated.  norm != 0: x is first divided by sqrt(mean(x^2) + eps) over head_dim and multiplied by `weight`.
  * Angles are reduced in fp64, everything else is fp32, the result is rounded once.  No tables: a token's sines and cosines
- * are computed once for all of its heads.  head_dim: a multiple of 8 up to 512; P a multiple of 4.
+ * are computed once for all of its heads.  head_dim: a multiple of 8 up to 512; P a multiple of 4 (0: the norm alone).
  * Replaces: the position embedding modules that build (cos, sin) tables and the rotation of the processors
  * (transformer_flux.py:146-147, transformer_hunyuan_video.py:60-83, transformer_wan.py:108-120).
  *

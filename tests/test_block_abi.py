@@ -252,3 +252,10 @@ def test_the_row_stride_of_a_single_row_is_not_looked_at():
             refused(L.xdit_fp8_block_matmul, matmul_args(bias=P + 2, **kw), BAD, "bias")
     refused(L.xdit_fp8_block_matmul, matmul_args(x_stride=1 << 24), BAD, "2^24")
     refused(L.xdit_fp8_block_matmul, matmul_args(w_stride=1 << 24), BAD, "2^24")
+
+
+def test_no_rotated_pairs_need_no_frequencies():
+    L = _lib.lib()
+    none = dict(pairs=PAIRS(0, 0), positions=None, inv_freq=None)
+    refused(L.xdit_axes_rope_backward, rope_args(t=dict(dweight=P), **none), BAD, "workspace")   # past every check of what is read
+    refused(L.xdit_axes_rope_backward, rope_args(t=dict(dweight=P), **{**none, "pairs": PAIRS(0, 4)}), BAD, "positions")

@@ -161,3 +161,20 @@ def test_refusals(gpu):
         f(q, k, p, *block_ops.rope_frequencies((2, 4, 4), device=gpu))
     with pytest.raises(RuntimeError):
         f(q.cpu(), k.cpu(), p.cpu(), inv.cpu(), pairs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_no_rotated_pairs_leave_the_norm(gpu, dtype):
+    q, k, p, _, _, qw, kw = problem(gpu, 2, 9, 3, 2, 72, (0, 36, 36), dtype, "bshd")
+    inv, pairs = block_ops.rope_frequencies((0, 0, 0), device=gpu)
+    opt = dict(norm=True, q_weight=qw, k_weight=kw, eps=1e-5)
+    y, z = block_ops.axes_rope(q, k, p, inv, pairs, **opt)
+    for x, w, got in ((q, qw, y), (k, kw, z)):
+        ref = O.axes_rope(x, w, p, inv, pairs, True, 1e-5, "interleaved")
+        close(got, ref, ref.abs().amax(-1, keepdim=True))
+    got = block_ops.axes_rope_backward(y, z, p, inv, pairs, q=q, k=k, **opt)
+    for x, w, d, dx in ((q, qw, y, got[0]), (k, kw, z, got[1])):
+        rdx, _, sx, _ = O.axes_rope_backward(d, x, w, p, inv, pairs, True, 1e-5, "interleaved")
+        close(dx, rdx, sx)
+    assert torch.equal(block_ops.axes_rope(q, None, p, inv, pairs)[0], q)

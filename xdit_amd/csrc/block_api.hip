@@ -247,7 +247,7 @@ static int fill_axes_rope(const xdit_axes_rope_args* a, xdit::AxesRopeParams& p,
     if ((rc = check_vector("weight", t.weight))) return rc;
     if (o.dweight != nullptr && t.weight == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "dweight needs weight");
   }
-  if (pointers) {
+  if (pointers && P > 0) {   // without a rotated pair neither is read
     if (a->positions == nullptr || !multiple_of(a->positions, a->pos_bits == 64 ? 8 : 4)) return api_fail(XDIT_ERR_INVALID_ARG, "positions is NULL or not aligned to its elements");
     if (a->inv_freq == nullptr || !multiple_of(a->inv_freq, a->freq_bits / 8)) return api_fail(XDIT_ERR_INVALID_ARG, "inv_freq is NULL or not aligned to its elements");
     if (a->pos_stride_b < 0 || a->pos_stride_s < 0) return api_fail(XDIT_ERR_INVALID_ARG, "positions: negative stride");
