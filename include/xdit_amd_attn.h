@@ -421,8 +421,10 @@ int xdit_qk_prologue_batch(const xdit_prologue_args* jobs, int32_t count);
  * with layer(h) = (h - mean) / sqrt(var + eps) and rms(h) = h / sqrt(mean(h^2) + eps) over C.  What is NULL is
  * left out.  Everything is computed in fp32 from the inputs; h and n are rounded once, n from the unrounded h.
  * A row whose mean square is beyond fp32 (elements of some 2^63 and more) has an infinite deviation: its norm is zero.
- * `fp8 != 0`: n is written as e4m3 bytes with one fp32 scale per block of 128 columns of a row, as
- * xdit_fp8_block_quant would quantise the unrounded n; n_scale[kb * B*S + b*S + s] holds the scale of columns
+ * `fp8 != 0`: n is written as e4m3 bytes with one fp32 scale per block of 128 columns of a row, quantised from the unrounded n
+ * as by xdit_fp8_block_quant but with products by reciprocals for its divisions: a scale may differ from that call's by 3 * 2^-24 of
+ * itself, and a value whose quotient is within 7 * 2^-24 of the middle of two e4m3 numbers may become the other one.  What
+ * xdit_fp8_block_matmul takes where C is a multiple of 16.  n_scale[kb * B*S + b*S + s] holds the scale of columns
  * [128 kb, 128 kb + 128).  `stats` (optional) receives (mean, 1/deviation) of h and of y, four floats a row
  * (0 and 1 for a norm that is absent; an RMS norm's mean is 0): what the backward call reads.
  * gate, scale and shift are (B, 1 or S, C): s stride 0 for one row per batch entry.  C: a multiple of 8, at most 8192.

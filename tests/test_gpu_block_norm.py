@@ -233,3 +233,21 @@ def test_refusals(gpu):
 def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError):
         block_ops.gated_norm(torch.zeros(1, 2, 64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,C", [(40, 1160), (1500, 640), (1100, 2304), (9, 8192)])
+def test_fp8_output_beside_the_quantiser(gpu, S, C):
+    """fp32 n is the unrounded one, so the quantiser's result from it can be had.  Scales: a product with 1 / 448 against a division, two roundings
+    against one, 3 * 2^-24.  Values: the hardware's reciprocal (a unit, 2^-23) and a product against a division, and the scale's difference: 7 * 2^-24;
+    only quotients that close to the middle of two e4m3 numbers may differ, by one step."""
+    k = problem(gpu, 2, S, C, torch.float32)
+    n = block_ops.gated_norm(**k)[1]
+    q, s = block_ops.gated_norm(fp8=True, **k)[1]
+    rq, rs = block_ops.fp8_block_quant(n)
+    assert bool(((s.double() - rs.double()).abs() <= 3 * 2.0 ** -24 * 1.001 * rs.double()).all())
+    other = q.view(torch.uint8) != rq.view(torch.uint8)
+    a, b = q.double()[other], rq.double()[other]
+    quotient = (n.double() / rs.double().repeat_interleave(128, -1)[..., :C])[other]
+    assert bool(((a - b).abs() <= a.abs().maximum(b.abs()) / 8 + 2.0 ** -9 * 1.001).all())
+    assert bool((((a + b) / 2 - quotient).abs() <= 8 * 2.0 ** -24 * quotient.abs()).all())

@@ -114,7 +114,8 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
     x, y: (B, S, C), bf16 / fp16 / fp32, C a multiple of 8 up to 8192.  gate, scale, shift: (B, C), (B, 1, C) or one row per
     token (B, S, C); weight, bias, y_weight: (C,); each in x's dtype or fp32, or None.  `norm` None leaves out n (returned as
     None).  All arithmetic is fp32, h and n are rounded once.  `fp8`: n is a pair (e4m3 tensor, scales (B, S, ceil(C / 128))
-    fp32), what `fp8_block_quant` makes of the unrounded n.  `return_stats` appends the (B, S, 4) fp32 statistics that
+    fp32) quantised from the unrounded n, as by `fp8_block_quant` up to fp32 roundings of scale and quotient; `fp8_block_matmul` takes it where C is
+    a multiple of 16.  `return_stats` appends the (B, S, 4) fp32 statistics that
     `gated_norm_backward` takes.  `out_h` receives h (it may be x: the residual stream is then updated in place)."""
     try:
         B, S, C = x.shape
