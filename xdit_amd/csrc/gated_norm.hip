@@ -103,7 +103,7 @@ __device__ __forceinline__ float put_row8(const GatedNormParams& p, float (&n)[8
 // TOKEN: modulation has a row per token and is fetched with it.  32760 x 5120 bf16 with y to fp8: 250 us, 4.7 TB/s; without y 141 us.
 template <typename T, bool TOKEN>
 __global__ __launch_bounds__(1024, TOKEN ? 4 : 6) void gated_norm_kernel(const GatedNormParams p) {
-  constexpr int R = 1;   // rows at a time
+  constexpr int R = 1;   // rows at a time; written for one row without the arrays, the 16-bit kernel spills 22 registers
   __shared__ Posted post[2][4];   // by turns: [y sums, y squares, h sums, h squares]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int chunks = p.C >> 3, waves = (int)blockDim.x >> 6;

@@ -1,5 +1,5 @@
 // Pieces of the row-wise kernels (norms, rotations, block quantiser): 8-element loads and stores, sums over a
-// wavefront and over a workgroup, the scale and cast of a 1 x 128 fp8 block.
+// wavefront, the scale and cast of a 1 x 128 fp8 block.
 #pragma once
 #include "common.h"
 #include "fp8_cast.h"
@@ -65,28 +65,6 @@ __device__ __forceinline__ unsigned row16_max(unsigned x) {
   x = max(x, dpp_bits<0x4E>(x));
   x = max(x, dpp_bits<0x141>(x));
   return max(x, dpp_bits<0x140>(x));
-}
-
-// Sums of K values over the NW wavefronts of a workgroup, to every thread, with one barrier.  `part` holds K * NW floats;
-// two consecutive calls must be given different arrays (the first's readers may still be at it).
-template <int K, int NW>
-__device__ __forceinline__ void block_sums(float (&x)[K], float* part) {
-#pragma unroll
-  for (int k = 0; k < K; k++) x[k] = wave_sum(x[k]);
-  if constexpr (NW > 1) {
-    if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-      for (int k = 0; k < K; k++) part[k * NW + (threadIdx.x >> 6)] = x[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-      float s = part[k * NW];
-#pragma unroll
-      for (int w = 1; w < NW; w++) s += part[k * NW + w];
-      x[k] = s;
-    }
-  }
 }
 
 // Scale of an fp8 block from the bits of its abs-max: absmax / 448, at least the smallest normal number, 1 for a block
