@@ -259,3 +259,10 @@ def test_no_rotated_pairs_need_no_frequencies():
     none = dict(pairs=PAIRS(0, 0), positions=None, inv_freq=None)
     refused(L.xdit_axes_rope_backward, rope_args(t=dict(dweight=P), **none), BAD, "workspace")   # past every check of what is read
     refused(L.xdit_axes_rope_backward, rope_args(t=dict(dweight=P), **{**none, "pairs": PAIRS(0, 4)}), BAD, "positions")
+
+
+def test_scales_off_their_alignment():
+    L = _lib.lib()
+    refused(L.xdit_gated_norm, norm_args(fp8=1, n_scale=P + 2), BAD, "n_scale")
+    for name in ("x_scale", "w_scale"):
+        refused(L.xdit_fp8_block_matmul, matmul_args(**{name: P + 2, "bias": P + 2}), BAD, "x_scale and w_scale")

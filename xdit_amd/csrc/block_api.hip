@@ -93,7 +93,7 @@ int xdit_gated_norm(const xdit_gated_norm_args* a) {
   } else if ((rc = check_rows("n", a->n, a->n_stride, a->fp8 ? 1 : es, B, S, C, true))) {
     return rc;
   }
-  if (a->fp8 && a->n_scale == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "n_scale is NULL");
+  if (a->fp8 && (a->n_scale == nullptr || !multiple_of(a->n_scale, 4))) return api_fail(XDIT_ERR_INVALID_ARG, "n_scale is NULL or not 4-byte aligned");
   if ((a->norm != XDIT_ROWNORM_NONE && !(a->eps >= 0.f && std::isfinite(a->eps))) || (a->y_norm != XDIT_ROWNORM_NONE && !(a->y_eps >= 0.f && std::isfinite(a->y_eps))))
     return api_fail(XDIT_ERR_INVALID_ARG, "eps must be finite and >= 0");
   if (a->gate != nullptr && (rc = check_rows("gate", a->gate, a->gate_stride, ms, B, S, C, false))) return rc;
@@ -332,6 +332,7 @@ static int fill_block_matmul(const xdit_block_matmul_args* a, xdit::BlockMatmulP
   if (!pointers) return 0;
   if (a->x == nullptr || a->w == nullptr || a->x_scale == nullptr || a->w_scale == nullptr || a->out == nullptr)
     return api_fail(XDIT_ERR_INVALID_ARG, "x, x_scale, w, w_scale or out is NULL");
+  if (!multiple_of(a->x_scale, 4) || !multiple_of(a->w_scale, 4)) return api_fail(XDIT_ERR_INVALID_ARG, "x_scale and w_scale must be 4-byte aligned");
   if (!multiple_of(a->x, 16) || !multiple_of(a->w, 16)) return api_fail(XDIT_ERR_INVALID_ARG, "x and w must be 16-byte aligned");
   if ((a->M > 1 && (a->x_stride % 16 || a->x_stride < a->K)) || (a->N > 1 && (a->w_stride % 16 || a->w_stride < a->K)))
     return api_fail(XDIT_ERR_INVALID_ARG, "rows of x and w must be multiples of 16 bytes apart, at least K = %lld", (long long)a->K);
