@@ -32,7 +32,8 @@ def calls(monkeypatch):
     monkeypatch.setattr(block_ops, "_capturing", lambda device: seen.capturing, raising=False)
     monkeypatch.setattr(block_ops._lib, "lib", Lib)
     monkeypatch.setattr(block_ops, "_SCRATCH", {})
-    monkeypatch.setattr(ops._TLS, "plans", {}, raising=False)
+    for store in ("plans", "block_plans"):
+        monkeypatch.setattr(ops._TLS, store, {}, raising=False)
     return seen
 
 
@@ -121,3 +122,13 @@ def test_projection_takes_any_rows_without_gradients_too(calls):
         assert seen[-1] is x
     finally:
         block_ops.fp8_block_quant = plain
+
+
+def test_attention_keeps_its_plans_beside_many_block_calls(calls, monkeypatch):
+    """Blocks of many sequence lengths do not use up the store of attention's argument structs."""
+    monkeypatch.setattr(ops, "_PLANS_MAX", 8)
+    monkeypatch.setattr(block_ops, "_PLANS_MAX", 8)
+    ops._TLS.plans["attention"] = "kept"
+    for S in range(1, 30):
+        block_ops.gated_norm(torch.zeros(1, S, 64))
+    assert ops._TLS.plans["attention"] == "kept" and 0 < len(ops._TLS.block_plans) <= 8

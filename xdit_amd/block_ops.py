@@ -33,7 +33,9 @@ def _scratch(device, stream, nbytes):
 
 
 def _plan(key, build):
-    plans = _TLS.__dict__.setdefault("plans", {})
+    """The argument struct of a call signature on this thread, from a store of its own: a block makes ten signatures a sequence length, and
+    attention's plans go all at once when theirs is full."""
+    plans = _TLS.__dict__.setdefault("block_plans", {})
     plan = plans.get(key)
     if plan is None:
         plan = build()
