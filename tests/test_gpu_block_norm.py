@@ -251,3 +251,22 @@ def test_fp8_output_beside_the_quantiser(gpu, S, C):
     quotient = (n.double() / rs.double().repeat_interleave(128, -1)[..., :C])[other]
     assert bool(((a - b).abs() <= a.abs().maximum(b.abs()) / 8 + 2.0 ** -9 * 1.001).all())
     assert bool((((a + b) / 2 - quotient).abs() <= 8 * 2.0 ** -24 * quotient.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,S,C,per_token", [(1, 600, 3080, False), (2, 301, 4096, False), (1, 601, 4088, True), (300, 1, 136, False), (150, 3, 1032, True), (2100, 1, 64, False)])
+def test_gradients_of_two_teams_and_of_many_batch_entries(gpu, dtype, B, S, C, per_token):
+    """Rows that fill a workgroup's LDS with two teams' sums, and entries of one to three tokens.  A column sum adds at most 16 rows of a team, 16 teams, its
+    entry's parts in 64 runs and, for what the entries share, B totals."""
+    k = problem(gpu, B, S, C, dtype, "wide", per_token)
+    opt = dict(norm="layer", y_norm="rms", residual_scale=0.7)
+    h, n, st = block_ops.gated_norm(return_stats=True, **opt, **k)
+    rh, rn, _, size = O.gated_norm(**opt, **k)
+    close(n, rn, size)
+    k.pop("x")
+    dh, dn = (torch.randn(h.shape, generator=torch.Generator(device=gpu).manual_seed(s), device=gpu).to(dtype) for s in (1, 2))
+    ref, big = O.gated_norm_backward(dh, dn, h, st, **opt, **k)
+    got = block_ops.gated_norm_backward(dh, dn, h, st, **opt, **k)
+    for name in got:
+        close(got[name], ref[name], big[name], F32 if name in ("dx", "dy") else (16 + 16 + 10 + B) * 2.0 ** -24 + F32)
