@@ -132,3 +132,24 @@ def test_attention_keeps_its_plans_beside_many_block_calls(calls, monkeypatch):
     for S in range(1, 30):
         block_ops.gated_norm(torch.zeros(1, S, 64))
     assert ops._TLS.plans["attention"] == "kept" and 0 < len(ops._TLS.block_plans) <= 8
+
+
+def test_numbers_are_taken_by_value(calls, monkeypatch):
+    """Scalars given as tensors that change in place: each call is made with what they hold then."""
+    seen = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return (lambda a: 4096) if name.endswith("workspace_bytes") else lambda a: seen.append((round(getattr(a._obj, "eps", 0), 3), round(getattr(a._obj, "residual_scale", 0), 3))) or 0
+
+    monkeypatch.setattr(block_ops._lib, "lib", Lib)
+    x, q, pos, freq = torch.zeros(1, 4, 64), torch.zeros(1, 2, 4, 64), torch.zeros(4, 1), torch.zeros(32)
+    eps, scale = torch.tensor(0.25), torch.tensor(0.5)
+    for call, want in ((lambda: block_ops.gated_norm(x, y=x, eps=eps, residual_scale=scale), (1, 1)), (lambda: block_ops.gated_norm_backward(x, x, x, torch.zeros(1, 4, 4), y=x, residual_scale=scale), (0, 1)),
+                       (lambda: block_ops.axes_rope(q, None, pos, freq, (32,), norm=True, eps=eps), (1, 0)), (lambda: block_ops.axes_rope_backward(q, None, pos, freq, (32,), q=q, norm=True, eps=eps), (1, 0))):
+        for _ in range(2):
+            call()
+            eps += 1
+            scale += 2
+            call()
+            assert seen[-1] == (want[0] * round(float(eps), 3), want[1] * round(float(scale), 3)) and (seen[-2] != seen[-1])

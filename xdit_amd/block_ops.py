@@ -124,6 +124,7 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
     except (AttributeError, TypeError, ValueError):
         raise ValueError("hidden states must be a 3-D tensor (B, S, C)") from None
     device, dtype = x.device, x.dtype
+    eps, y_eps, residual_scale = float(eps), float(y_eps), float(residual_scale)   # values: a tensor would be known by its identity
     key = ("gnorm", _sig(x), _sig(y), _sig(gate), _sig(scale), _sig(shift), _sig(weight), _sig(bias), _sig(y_weight), _sig(out_h), norm, y_norm, fp8,
            eps, y_eps, residual_scale)
 
@@ -136,7 +137,7 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
         a.weight_dtype = _code(_shared("weight, bias and y_weight", (weight, bias, y_weight), dtype))
         a.norm, a.y_norm, a.fp8 = _norm_code("norm", norm), _norm_code("y_norm", y_norm), 1 if fp8 else 0
         a.B, a.S, a.C = B, S, C
-        a.eps, a.y_eps, a.residual_scale = float(eps), float(y_eps), float(residual_scale)
+        a.eps, a.y_eps, a.residual_scale = eps, y_eps, residual_scale
         a.x_stride = _rows(x)
         if y is not None:
             _check("y", y, x.shape, (dtype,), device)
@@ -194,6 +195,7 @@ def gated_norm_backward(dh, dn, h, stats, y=None, gate=None, scale=None, shift=N
     expand it); scale and shift must agree on having a row per token.  Sums over rows are fp32, in a fixed order."""
     B, S, C = _hidden(h)
     device, dtype = h.device, h.dtype
+    residual_scale = float(residual_scale)
     key = ("gnorm_bwd", _sig(dh), _sig(dn), _sig(h), _sig(stats), _sig(y), _sig(gate), _sig(scale), _sig(shift), _sig(weight), _sig(bias), _sig(y_weight),
            norm, y_norm, residual_scale)
 
@@ -208,7 +210,7 @@ def gated_norm_backward(dh, dn, h, stats, y=None, gate=None, scale=None, shift=N
         a.mod_dtype, a.weight_dtype = _code(mod), _code(wt)
         a.norm, a.y_norm = _norm_code("norm", norm), _norm_code("y_norm", y_norm)
         a.B, a.S, a.C = B, S, C
-        a.residual_scale = float(residual_scale)
+        a.residual_scale = residual_scale
         _check("stats", stats, (B, S, 4), (torch.float32,), device)
         if not stats.is_contiguous():
             raise ValueError("stats must be contiguous")
@@ -305,7 +307,7 @@ def _rope_args(first, tensors, positions, inv_freq, pairs, norm, eps, rope):
         raise ValueError("between 1 and %d axes are supported" % _lib.ROPE_MAX_AXES)
     a = _lib.AxesRopeArgs()
     a.struct_size = ctypes.sizeof(a)
-    a.dtype, a.rope, a.norm, a.eps = _code(dtype), _ROPE[rope], 1 if norm else 0, float(eps)
+    a.dtype, a.rope, a.norm, a.eps = _code(dtype), _ROPE[rope], 1 if norm else 0, eps
     a.weight_dtype = _code(_shared("q_weight and k_weight", [t[4] for t in tensors], dtype))
     _check("positions", positions, None, tuple(_POS_BITS), device)
     A = len(pairs)
@@ -318,7 +320,7 @@ def _rope_args(first, tensors, positions, inv_freq, pairs, norm, eps, rope):
     a.B, a.S, a.D = B, S, D
     a.tensors, a.axes = len(tensors), A
     for i, n in enumerate(pairs):
-        a.pairs[i] = int(n)
+        a.pairs[i] = n
     for i, (name, x, dy, y, weight) in enumerate(tensors):
         t = a.t[i]
         t.H = (x if x is not None else dy).shape[1]
@@ -348,7 +350,7 @@ def axes_rope(q, k, positions, inv_freq, pairs, norm=False, q_weight=None, k_wei
     Angles are reduced in fp64, the rest is fp32, the result is rounded once."""
     if not isinstance(q, torch.Tensor) or q.ndim != 4:
         raise ValueError("q must be a 4-D tensor (B, H, S, D)")
-    device, dtype, pairs = q.device, q.dtype, tuple(pairs)
+    device, dtype, pairs, eps = q.device, q.dtype, tuple(map(int, pairs)), float(eps)
     B, H, S, D = q.shape
     key = ("arope", _sig(q), _sig(k), _sig(positions), _sig(inv_freq), pairs, norm, _sig(q_weight), _sig(k_weight), eps, rope, _sig(out_q), _sig(out_k))
 
@@ -388,7 +390,7 @@ def axes_rope_backward(dq, dk, positions, inv_freq, pairs, q=None, k=None, norm=
     gradients are summed in fp32 in a fixed order."""
     if not isinstance(dq, torch.Tensor) or dq.ndim != 4:
         raise ValueError("dq must be a 4-D tensor (B, H, S, D)")
-    device, dtype, pairs = dq.device, dq.dtype, tuple(pairs)
+    device, dtype, pairs, eps = dq.device, dq.dtype, tuple(map(int, pairs)), float(eps)
     B, H, S, D = dq.shape
     if not norm:
         q = k = None
