@@ -153,3 +153,14 @@ def test_numbers_are_taken_by_value(calls, monkeypatch):
             scale += 2
             call()
             assert seen[-1] == (want[0] * round(float(eps), 3), want[1] * round(float(scale), 3)) and (seen[-2] != seen[-1])
+
+
+def test_gradients_to_positions_and_frequencies_are_refused():
+    q, pos = torch.zeros(1, 2, 4, 64), torch.zeros(4, 1)
+    freq, pairs = block.rope_frequencies((64,))
+    for p, f in ((pos.clone().requires_grad_(), freq), (pos, freq.clone().requires_grad_())):
+        for x in (q, q.clone().requires_grad_()):
+            with pytest.raises(ValueError, match="no gradient"):
+                block.axes_rope(x, None, p, f, pairs)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):   # nothing wants it: as ever
+            block.axes_rope(q, None, p, f, pairs)
