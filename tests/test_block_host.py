@@ -164,3 +164,12 @@ def test_gradients_to_positions_and_frequencies_are_refused():
                 block.axes_rope(x, None, p, f, pairs)
         with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):   # nothing wants it: as ever
             block.axes_rope(q, None, p, f, pairs)
+
+
+def test_tangents_of_positions_and_frequencies_are_refused():
+    q, pos = torch.zeros(1, 2, 4, 64), torch.zeros(4, 1)
+    freq, pairs = block.rope_frequencies((64,))
+    with forward_ad.dual_level():
+        for p, f in ((forward_ad.make_dual(pos, torch.ones_like(pos)), freq), (pos, forward_ad.make_dual(freq, torch.ones_like(freq)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                block.axes_rope(q, None, p, f, pairs)

@@ -47,7 +47,7 @@ def gated_norm(x, y=None, gate=None, scale=None, shift=None, weight=None, bias=N
 
 def axes_rope(q, k, positions, inv_freq, pairs, norm=False, q_weight=None, k_weight=None, eps=1e-6, rope="interleaved"):
     """`block_ops.axes_rope` -> (q, k), differentiable in q, k and the gains; positions and frequencies that want a gradient are refused."""
-    registered = _registered(q, k, q_weight, k_weight)
+    registered = _registered(q, k, positions, inv_freq, q_weight, k_weight)
     if (positions.requires_grad or inv_freq.requires_grad) and torch.is_grad_enabled():
         raise ValueError("positions and inv_freq have no gradient here: detach them")
     if not registered:
