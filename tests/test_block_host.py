@@ -29,7 +29,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(block_ops, "_check", lambda *a: None)
     monkeypatch.setattr(block_ops, "_stream", lambda device: 7)
     monkeypatch.setattr(block_ops, "_on_device", lambda device: contextlib.nullcontext())
-    monkeypatch.setattr(block_ops, "_capturing", lambda device: seen.capturing, raising=False)
+    monkeypatch.setattr(block_ops, "_capturing", lambda device, stream: seen.capturing, raising=False)
     monkeypatch.setattr(block_ops._lib, "lib", Lib)
     monkeypatch.setattr(block_ops, "_SCRATCH", {})
     for store in ("plans", "block_plans"):

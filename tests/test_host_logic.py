@@ -342,7 +342,7 @@ def test_captured_calls_share_scratch_with_nothing_outside_their_capture(monkeyp
     monkeypatch.setattr(ops, "_check4", lambda *a: None)
     monkeypatch.setattr(ops, "_stream", lambda device: 7)
     monkeypatch.setattr(ops, "_on_device", lambda device: contextlib.nullcontext())
-    monkeypatch.setattr(ops, "_capturing", lambda device: capture[0] is not None, raising=False)
+    monkeypatch.setattr(ops, "_capturing", lambda device, stream: capture[0] is not None, raising=False)
     monkeypatch.setattr(ops, "_capture_id", lambda device, stream: capture[0], raising=False)
     monkeypatch.setattr(ops._lib, "lib", Lib)
     for pool in ("_QUANT_SCRATCH", "_WORKSPACE", "_CAPTURED"):

@@ -22,7 +22,7 @@ def _scratch(device, stream, nbytes):
     """Scratch of a call, to be held until it has launched; taken under the stream's lock.  The eager calls of one (device,
     stream) are ordered and share a buffer; one that a call has outgrown stays allocated.  A captured call has a buffer of
     its own from the graph's memory pool, which its later calls may take over in the graph's order."""
-    if _capturing(device):
+    if _capturing(device, stream):
         return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
     buf = _SCRATCH.get((device, stream))
     if buf is None or buf.numel() < nbytes:

@@ -45,15 +45,15 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
 
 
-def _capturing(device):
-    """Whether the current stream is being captured into a graph.  A captured call needs scratch of its own: the graph keeps the
-    address and may be replayed on any stream, beside other graphs and eager calls."""
-    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+def _capturing(device, stream):
+    """Whether `stream`, the current one, is being captured into a graph (the default stream, 0, never is).  A captured call needs
+    scratch of its own: the graph keeps the address and may be replayed on any stream, beside other graphs and eager calls."""
+    return stream != 0 and device.type == "cuda" and torch._C._cuda_isCurrentStreamCapturing()
 
 
 def _capture_id(device, stream):
     """What tells the capture that `stream`, the current one, is under from every other capture; None if it is under none."""
-    return _lib.lib().xdit_stream_capture_id(stream) if _capturing(device) else None
+    return _lib.lib().xdit_stream_capture_id(stream) if _capturing(device, stream) else None
 
 
 class _on_device:
@@ -498,7 +498,7 @@ def fp8_quant_batch(jobs, joined=()):
                 a.x2, a.y2 = x2.data_ptr(), y2.data_ptr()
             out.append((y, y2, descale))
     with _stream_lock(device, stream), _on_device(device):
-        if _capturing(device):
+        if _capturing(device, stream):
             buf = torch.empty(sum(need), dtype=torch.uint8, device=device)
         else:
             buf = _QUANT_SCRATCH.get((device, stream))
