@@ -595,7 +595,8 @@ int xdit_fp8_block_quant(const xdit_block_quant_args* args);
  * multiple of 16, rows 16-byte aligned.  The scaled sums of the blocks are held in fp32 and the result is rounded once to
  * out_dtype.  Within a block, exact_sums != 0: products are exact and summed in fp32 (the operands are widened to fp16 on their
  * way into the matrix cores); 0: the fp8 matrix instructions, twice as fast, which add eight consecutive k at a time and cut
- * every product of those at 2^-13 of the largest one's binade.  `workspace` (optional, xdit_fp8_block_matmul_workspace_bytes, 16-byte
+ * every product of those at 2^-13 of the largest one's binade (an error of 1.4e-5 to 3.3e-5 of the result's size: beside a rounding to
+ * bf16 nothing, beside one to fp16 0.2 to 1.2 % more).  `workspace` (optional, xdit_fp8_block_matmul_workspace_bytes, 16-byte
  * aligned, private to the stream until the call's kernels finish) lets a product of few rows cut K over the chip; without it
  * K is not cut.  Results are reproducible bit for bit for the same arguments and workspace.
  */

@@ -488,7 +488,8 @@ def fp8_block_matmul(x, x_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16
     ceil(K / 128)) (`fp8_block_quant` of both; scales may have any strides); K a multiple of 16; bias (N,) in out_dtype or fp32.
     The blocks' sums are held in fp32 and the result is rounded once; the same call gives the same bits.  `exact_sums` True:
     products are exact and summed in fp32; False: the fp8 matrix instructions, twice as fast, which add eight consecutive k at a
-    time with every product cut at 2^-13 of the largest one's binade; None: exact for fp32 results, where that shows."""
+    time with every product cut at 2^-13 of the largest one's binade (1.4e-5 to 3.3e-5 of the result's size: nothing beside a rounding to bf16, 0.2 to
+    1.2 % more error beside one to fp16); None: exact for fp32 results, where that shows."""
     for name, t in (("x", x), ("x_scale", x_scale), ("w", w), ("w_scale", w_scale)):
         if not isinstance(t, torch.Tensor):
             raise ValueError("%s must be a tensor" % name)

@@ -111,7 +111,8 @@ __device__ __forceinline__ void turn(const AxesRopeParams& p, int b, int s, int 
   }
 }
 
-// One wavefront per token and head group: `lpr` lanes per row, 64 / lpr heads at a time.  32760 tokens of 40 + 40 heads of 128: 264 us, 5.1 TB/s.
+// One wavefront per token and head group: `lpr` lanes per row, 64 / lpr heads at a time.  32760 tokens of 40 + 40 heads of 128: 264 us, 5.1 TB/s
+// (fp32, a call, 549 us, 4.9 TB/s).
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256) void axes_rope_kernel(const AxesRopeParams p) {
   const unsigned tok = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // uniform, as everything of the token
@@ -155,7 +156,8 @@ __global__ __launch_bounds__(256) void axes_rope_kernel(const AxesRopeParams p) 
 }
 
 // Backward: a workgroup's wavefronts go over the tokens (token group, token group + groups, ...), four at a time, and
-// keep the sums of d x^ of their lanes' columns.  8500 tokens of 24 + 24 heads of 64, fp16, split halves: 37 us, 4.2 TB/s.
+// keep the sums of d x^ of their lanes' columns.  8500 tokens of 24 + 24 heads of 64, fp16, split halves: 37 us, 4.2 TB/s;
+// 32760 of 40 + 40 of 128 in fp32, a call, 792 us, 5.1 TB/s (of the fp32 forms split halves spill 4 registers).
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(256, 4) void axes_rope_bwd_kernel(const AxesRopeParams p) {
   __shared__ float part[4][2][512];

@@ -100,7 +100,9 @@ __device__ __forceinline__ float put_row8(const GatedNormParams& p, float (&n)[8
   return scale;
 }
 
-// TOKEN: modulation has a row per token and is fetched with it.  32760 x 5120 bf16 with y to fp8: 250 us, 4.7 TB/s; without y 141 us.
+// 32760 x 5120 bf16 with y to fp8: 252 us, 4.7 TB/s; without y 141 us.  TOKEN: modulation has a row per token and is fetched when it is
+// needed, nothing ahead: the same call to bf16 601 us, 3.9 TB/s.  The bound of six wavefronts a SIMD is that of 16-bit rows; fp32 rows spill 22
+// registers under it (32760 x 5120: 637 us, 4.2 TB/s).
 template <typename T, bool TOKEN>
 __global__ __launch_bounds__(1024, TOKEN ? 4 : 6) void gated_norm_kernel(const GatedNormParams p) {
   constexpr int R = 1;   // rows at a time; written for one row without the arrays, the 16-bit kernel spills 22 registers
@@ -413,7 +415,8 @@ __device__ __forceinline__ void two_sums(float& a, float& b, int waves, int wave
 
 // A workgroup runs over the rows of one part of one batch entry, as many at a time as it has teams of wavefronts (short rows
 // leave room for several); a thread keeps the sums of its eight columns, and the teams' sums are added in LDS at the end.
-// 8500 x 1536 fp16: 35 us, 4.5 TB/s (one team to a workgroup 44); 32760 x 5120 bf16 with the sums 442 us, 4.6 TB/s.
+// 8500 x 1536 fp16: 35 us, 4.5 TB/s (one team to a workgroup 44); 32760 x 5120 bf16 with the sums, a call, 458 us, 4.4 TB/s.
+// The other forms spill: fp32 rows 5 registers (811 us, 5.0 TB/s), modulation per token 9, in fp32 36 (bf16 976 us, 3.8 TB/s).
 template <typename T, bool TOKEN>
 __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwdParams p) {
   __shared__ Posted posts[kMaxWaves][2][2];
@@ -437,7 +440,7 @@ __global__ __launch_bounds__(1024) void gated_norm_bwd_kernel(const GatedNormBwd
     }
     if (has_y) ry = load_raw8<T>(p.y, b * p.ys.b + s * p.ys.s + col);
   };
-  constexpr bool AHEAD = sizeof(T) == 2 && !TOKEN;   // the next row is requested ahead where the registers allow it
+  constexpr bool AHEAD = sizeof(T) == 2 && !TOKEN;   // the next row is requested ahead where the registers allow it (the other forms spill as it is)
   if constexpr (AHEAD) load(min(s0 + team, s1 - 1));
   float scw[8], gyw[8], sa[8] = {}, sf[8] = {}, sg[8] = {};   // (1 + scale) w, alpha gate w_y, column sums
   auto fill = [](float (&v)[8], float c) {
@@ -587,7 +590,7 @@ __device__ __forceinline__ void put_param(void* p, int64_t i, bool wide, float v
 }
 
 // The parts' sums, added in a fixed order (64 runs of every 64th part, then the runs), and from them the parameters'
-// gradients; 16 columns per workgroup.
+// gradients; 16 columns per workgroup, one batch entry after the other: 2 entries of 1536 columns 7 us, 1024 entries 1.7 ms.
 template <typename T>
 __global__ __launch_bounds__(1024) void gated_norm_bwd_finish_kernel(const GatedNormBwdParams p) {
   constexpr int RUNS = 64;
