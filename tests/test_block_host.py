@@ -173,3 +173,16 @@ def test_tangents_of_positions_and_frequencies_are_refused():
         for p, f in ((forward_ad.make_dual(pos, torch.ones_like(pos)), freq), (pos, forward_ad.make_dual(freq, torch.ones_like(freq)))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 block.axes_rope(q, None, p, f, pairs)
+
+
+def test_projection_of_a_weight_that_starts_anywhere(calls):
+    """A weight may be a part of a flat buffer: a contiguous one off a 16-byte boundary is copied, as one that is not dense is."""
+    seen = []
+    plain, block_ops.fp8_block_quant = block_ops.fp8_block_quant, lambda x, *a: seen.append(x) or plain(x, *a)
+    try:
+        flat = torch.arange(32 * 64 + 8, dtype=torch.float32)
+        for w in (flat[:32 * 64].view(32, 64), flat[1:1 + 32 * 64].view(32, 64), flat[:32 * 64].view(64, 32).t(), torch.zeros(32, 66)[:, 1:65]):
+            block.Fp8Linear(w)
+            assert seen[-1].data_ptr() % 16 == 0 and seen[-1].stride(-1) == 1 and torch.equal(seen[-1], w)
+    finally:
+        block_ops.fp8_block_quant = plain

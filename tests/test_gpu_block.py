@@ -301,3 +301,13 @@ def test_projection_of_strided_and_unaligned_activations(gpu):
     flat[1:] = x.contiguous().flatten()
     want = linear(x.contiguous())
     assert torch.equal(linear(x), want) and torch.equal(linear(flat[1:].view(2, 7, 128)), want) and torch.equal(linear(x.clone().requires_grad_()), want)
+
+
+def test_projection_of_a_weight_in_a_flat_buffer(gpu):
+    g = torch.Generator(device=gpu).manual_seed(12)
+    flat = (torch.randn(96 * 128 + 8, generator=g, device=gpu) / 11).bfloat16()
+    x = torch.randn(5, 128, generator=g, device=gpu).bfloat16()
+    for at in (1, 4, 8):
+        w = flat[at:at + 96 * 128].view(96, 128)
+        assert torch.equal(block.Fp8Linear(w)(x), block.Fp8Linear(w.clone())(x))
+        assert torch.equal(block.Fp8Linear(w.t().contiguous().t())(x), block.Fp8Linear(w.clone())(x))

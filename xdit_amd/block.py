@@ -71,7 +71,7 @@ class Fp8Linear(torch.nn.Module):
         if self.in_features % 16 or (backward and self.out_features % 16):
             raise ValueError("in_features (for the gradient out_features too) must be a multiple of 16")
         self.dtype = weight.dtype
-        w, scale = block_ops.fp8_block_quant(weight.detach().contiguous(), 128)
+        w, scale = block_ops.fp8_block_quant(custom_ops._rows16(weight.detach()), 128)
         self.register_buffer("weight", w)
         self.register_buffer("weight_scale", scale)
         self.register_buffer("weight_t", w.t().contiguous() if backward else None)
