@@ -186,3 +186,11 @@ def test_projection_of_a_weight_that_starts_anywhere(calls):
             assert seen[-1].data_ptr() % 16 == 0 and seen[-1].stride(-1) == 1 and torch.equal(seen[-1], w)
     finally:
         block_ops.fp8_block_quant = plain
+
+
+def test_projection_keeps_its_own_bias(calls):
+    """Weight and bias are frozen as they were given, an fp32 bias as well as one that is converted; one that is not dense is laid out."""
+    for b in (torch.ones(32), torch.ones(32, dtype=torch.bfloat16), torch.ones(64)[::2]):
+        linear = block.Fp8Linear(torch.zeros(32, 64), b)
+        b += 1
+        assert torch.equal(linear.bias, torch.ones(32)) and linear.bias.is_contiguous()

@@ -76,7 +76,7 @@ class Fp8Linear(torch.nn.Module):
         self.register_buffer("weight_scale", scale)
         self.register_buffer("weight_t", w.t().contiguous() if backward else None)
         self.register_buffer("weight_t_scale", scale.t().contiguous() if backward else None)
-        self.register_buffer("bias", None if bias is None else bias.detach().float())   # any result's dtype takes it
+        self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32, copy=True).contiguous())   # its own, and any result's dtype takes it
 
     @classmethod
     def from_linear(cls, linear, backward=False):
