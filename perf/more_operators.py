@@ -3,7 +3,7 @@ a model's gradients with their clipping.
 
 A case is a dict of plain values; `op` says which entry point it goes through:
 
-  attn_bwd    ops.attn_bwd: gradients of q, k, v (and of the joint text keys and values) from those of the
+  attn_bwd    grad_ops.attn_bwd: gradients of q, k, v (and of the joint text keys and values) from those of the
               output, with what the forward pass has left behind (output and log-sum-exp)
   grad_norm   grad_ops.grad_norm of a list of gradients
   clip        grad_ops.clip_grads into a second list (the optimizer's own gradients)
@@ -187,9 +187,9 @@ def _clip_plain(s):
 
 def run(s):
     if own:
-        from xdit_amd import grad_ops, ops
+        from xdit_amd import grad_ops
         if s.op == "attn_bwd":
-            return ops.attn_bwd(s.dout, s.q, s.k, s.v, s.out, s.lse, softmax_scale=s.scale, k2=s.k2, v2=s.v2)
+            return grad_ops.attn_bwd(s.dout, s.q, s.k, s.v, s.out, s.lse, softmax_scale=s.scale, k2=s.k2, v2=s.v2)
         if s.op == "grad_norm":
             return grad_ops.grad_norm(s.grads)
         return grad_ops.clip_grads(s.grads, s.max_norm, out=s.out), s.main
