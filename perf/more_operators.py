@@ -72,11 +72,11 @@ def draw(rng):
         B, H = rng.choice([1, 1, 2, 3]), rng.randint(1, 40)
         most = 8e11 if dtype == "fp32" else 5e12   # operations
         Sq = _log_int(rng, 1, min(32760, math.sqrt(most / (10 * B * H * D)) * rng.choice([1, 1, 4])))
-        room = max(1.0, most / (10 * B * H * D * Sq))
+        room = max(2.0, most / (10 * B * H * D * Sq))   # over one key the gradients of queries and keys are zeros
         kind = rng.choice(["self", "joint", "cross"])
         if kind == "cross":
-            return _attn(B, H, Sq, _log_int(rng, 1, min(1024, room)), D, 0, dtype, rng.choice(["bshd", "bhsd"]))
-        keys = max(1, min(Sq, int(room)))
+            return _attn(B, H, Sq, _log_int(rng, 2, min(1024, room)), D, 0, dtype, rng.choice(["bshd", "bhsd"]))
+        keys = max(2, min(Sq, int(room)))
         text = min(keys - 1, _log_int(rng, 16, 512)) if kind == "joint" else 0
         return _attn(B, H, Sq, keys - text, D, text, dtype, rng.choice(["bshd", "bhsd"]))
     D = rng.choice([40, 64, 72, 128])
