@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define XDIT_ATTN_ABI_VERSION 10
+#define XDIT_ATTN_ABI_VERSION 11
 
 typedef enum {
   XDIT_OK = 0,
@@ -410,6 +410,98 @@ int xdit_qk_prologue(const xdit_prologue_args* args);
  * kernels).  All jobs share dtype and stream; XDIT_NORM_TOKEN jobs cannot be batched.
  */
 int xdit_qk_prologue_batch(const xdit_prologue_args* jobs, int32_t count);
+
+/* ---- training ------------------------------------------------------------------------------------ */
+
+/*
+ * Backward pass of xdit_attn_fwd: gradients of q, k, v (and of the second segment k2, v2) from those of its results.
+ *     P_ij = exp(softmax_scale q_i.k_j - lse_i)          delta_i = dout_i.out_i - dlse_i
+ *     dv_j = sum_i P_ij dout_i                            dS_ij = P_ij (dout_i.v_j - delta_i)
+ *     dk_j = softmax_scale sum_i dS_ij q_i                dq_i = softmax_scale sum_j dS_ij k_j
+ * `out` and `lse` are what the forward call gave for the same q, k, v and scale; `dlse` (may be NULL: zeros) is the gradient of lse.
+ * With the out, lse and dout of a whole ring it gives one chunk's dk and dv, and that chunk's share of dq.  A row whose lse is
+ * -infinity attended nothing: it gives and gets no gradient.
+ * bf16, fp16 or fp32, head_dim a multiple of 8 up to 128.  P and dS are rounded to dtype for the products (fp16: scaled by powers of
+ * two, that of dS by the size of dout, so that small ones keep their bits), everything else is fp32, each gradient is rounded
+ * once.  The same call gives the same bits.  dq, or dk and dv (then dk2 and dv2 too where Sk2 > 0), may be NULL: not computed.
+ * Gradients must not overlap each other or an input.
+ */
+typedef struct {
+  uint32_t struct_size;        /* = sizeof(xdit_attn_bwd_args) */
+  int32_t dtype;               /* of every tensor but lse and dlse: bf16, fp16 or fp32 */
+  int32_t B, H, D;
+  int32_t cu_count;            /* 0 = plan the launch for the compute units of the current device; > 0 = for that many */
+  int64_t Sq, Sk, Sk2;
+  float softmax_scale;         /* > 0 */
+  int32_t reserved0;           /* must be 0 */
+  const void* dout;            /* (B,H,Sq,D) */
+  const void* q;
+  const void* k;               /* (B,H,Sk,D) */
+  const void* v;
+  const void* k2;              /* (B,H,Sk2,D); may be NULL when Sk2 == 0 */
+  const void* v2;
+  const void* out;             /* (B,H,Sq,D) */
+  const float* lse;            /* (B,H,Sq), any strides, as dlse */
+  const float* dlse;           /* (B,H,Sq); may be NULL */
+  void* dq;
+  void* dk;
+  void* dv;
+  void* dk2;
+  void* dv2;
+  xdit_strides dout_stride, q_stride, k_stride, v_stride, k2_stride, v2_stride, out_stride;
+  xdit_strides dq_stride, dk_stride, dv_stride, dk2_stride, dv2_stride;
+  xdit_strides lse_stride, dlse_stride;
+  void* workspace;             /* 16-byte aligned, of the size below, private to the call until its kernels finish */
+  int64_t workspace_bytes;
+  void* stream;
+} xdit_attn_bwd_args;
+
+int xdit_attn_bwd(const xdit_attn_bwd_args* args);
+int64_t xdit_attn_bwd_workspace_bytes(const xdit_attn_bwd_args* args);  /* which gradients are asked for counts, no pointer is followed */
+
+/*
+ * Norm of a list of gradients, as if they were one vector: the largest size of an element, the sum of sizes or the root of
+ * the sum of squares.  Sums are in 64 bits, in a fixed order; the result is rounded to fp32.  An element that is not a number makes the norm one.
+ * The tables are HOST arrays of `count` entries; they are read before the call returns.
+ */
+enum xdit_grad_norm_kind { XDIT_GRADNORM_MAX = 0, XDIT_GRADNORM_L1 = 1, XDIT_GRADNORM_L2 = 2 };
+
+typedef struct {
+  uint32_t struct_size;        /* = sizeof(xdit_grad_norm_args) */
+  int32_t kind;                /* xdit_grad_norm_kind */
+  int64_t count;               /* 0: the norm is 0 */
+  const void* const* data;     /* device pointers, aligned to their elements; contiguous tensors */
+  const int64_t* numel;        /* 0 is allowed */
+  const int32_t* dtype;        /* xdit_dtype: bf16, fp16 or fp32, any mixture */
+  float* norm;                 /* device: one fp32 */
+  void* workspace;             /* 8-byte aligned, of the size below, private to the call until its kernels finish */
+  int64_t workspace_bytes;
+  void* stream;
+} xdit_grad_norm_args;
+
+int xdit_grad_norm(const xdit_grad_norm_args* args);
+int64_t xdit_grad_norm_workspace_bytes(const xdit_grad_norm_args* args);  /* from count and numel */
+
+/*
+ * Clipping by a norm that is in device memory (of these gradients, or of those of every rank):
+ *     dst = src * min(1, max_norm / (norm + 1e-6))
+ * in fp32, rounded once.  dst may be src itself; otherwise no dst may overlap another dst or a src.  Where the factor is 1 a dst
+ * that is its src is left as it is.  The tables are HOST arrays, read before the call returns.
+ */
+typedef struct {
+  uint32_t struct_size;        /* = sizeof(xdit_clip_grads_args) */
+  float max_norm;              /* finite, >= 0 */
+  int64_t count;
+  const void* const* src;
+  void* const* dst;
+  const int64_t* numel;
+  const int32_t* src_dtype;    /* bf16, fp16 or fp32 */
+  const int32_t* dst_dtype;
+  const float* norm;           /* device: one fp32 */
+  void* stream;
+} xdit_clip_grads_args;
+
+int xdit_clip_grads(const xdit_clip_grads_args* args);
 
 /* ---- around the attention call: the rest of a DiT block ------------------------------------------ */
 

@@ -9,7 +9,7 @@ import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libxdit_amd_attn.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 XDIT_OK = 0
 XDIT_ERR_INVALID_ARG = -1
@@ -250,6 +250,29 @@ class BlockMatmulArgs(ctypes.Structure):
                 + [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
 
 
+class AttnBwdArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", ctypes.c_uint32)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "B", "H", "D", "cu_count")]
+                + [(n, ctypes.c_int64) for n in ("Sq", "Sk", "Sk2")]
+                + [("softmax_scale", ctypes.c_float), ("reserved0", ctypes.c_int32)]
+                + [(n, ctypes.c_void_p) for n in ("dout", "q", "k", "v", "k2", "v2", "out", "lse", "dlse", "dq", "dk", "dv", "dk2", "dv2")]
+                + [(n + "_stride", Strides) for n in ("dout", "q", "k", "v", "k2", "v2", "out", "dq", "dk", "dv", "dk2", "dv2", "lse", "dlse")]
+                + [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
+
+
+class GradNormArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", ctypes.c_uint32), ("kind", ctypes.c_int32), ("count", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("data", "numel", "dtype", "norm", "workspace")]
+                + [("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
+
+
+class ClipGradsArgs(ctypes.Structure):
+    _fields_ = ([("struct_size", ctypes.c_uint32), ("max_norm", ctypes.c_float), ("count", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("src", "dst", "numel", "src_dtype", "dst_dtype", "norm", "stream")])
+
+
+GRADNORM_MAX, GRADNORM_L1, GRADNORM_L2 = 0, 1, 2
+
 ROWNORM_NONE, ROWNORM_RMS, ROWNORM_LAYER = 0, 1, 2
 
 NORM_NONE, NORM_HEAD, NORM_TOKEN = 0, 1, 2
@@ -259,6 +282,7 @@ EXPORTS = ("xdit_attn_fwd", "xdit_attn_fwd_two_queries", "xdit_attn_fwd_noalloc"
            "xdit_gated_norm", "xdit_gated_norm_backward", "xdit_gated_norm_backward_workspace_bytes",
            "xdit_axes_rope", "xdit_axes_rope_backward", "xdit_axes_rope_backward_workspace_bytes",
            "xdit_fp8_block_quant", "xdit_fp8_block_matmul", "xdit_fp8_block_matmul_workspace_bytes",
+           "xdit_attn_bwd", "xdit_attn_bwd_workspace_bytes", "xdit_grad_norm", "xdit_grad_norm_workspace_bytes", "xdit_clip_grads",
            "xdit_stream_capture_id", "xdit_attn_last_error", "xdit_attn_abi_version")
 
 _lib = None
@@ -309,7 +333,12 @@ def lib():
                                    ("xdit_axes_rope_backward_workspace_bytes", AxesRopeArgs, ctypes.c_int64),
                                    ("xdit_fp8_block_quant", BlockQuantArgs, ctypes.c_int),
                                    ("xdit_fp8_block_matmul", BlockMatmulArgs, ctypes.c_int),
-                                   ("xdit_fp8_block_matmul_workspace_bytes", BlockMatmulArgs, ctypes.c_int64)):
+                                   ("xdit_fp8_block_matmul_workspace_bytes", BlockMatmulArgs, ctypes.c_int64),
+                                   ("xdit_attn_bwd", AttnBwdArgs, ctypes.c_int),
+                                   ("xdit_attn_bwd_workspace_bytes", AttnBwdArgs, ctypes.c_int64),
+                                   ("xdit_grad_norm", GradNormArgs, ctypes.c_int),
+                                   ("xdit_grad_norm_workspace_bytes", GradNormArgs, ctypes.c_int64),
+                                   ("xdit_clip_grads", ClipGradsArgs, ctypes.c_int)):
             f = getattr(L, name)
             f.argtypes, f.restype = [ctypes.POINTER(args)], result
         L.xdit_stream_capture_id.argtypes = [ctypes.c_void_p]

@@ -12,7 +12,7 @@ from enum import Enum
 
 import torch
 
-from . import custom_ops  # noqa: F401  (registers torch.ops.xdit_amd.*)
+from . import custom_ops  # registers torch.ops.xdit_amd.*
 from . import ops
 
 ATTENTION_FUNCTION_REGISTRY = {}
@@ -65,13 +65,14 @@ def _split_joint(key, value, joint_kv):
 @register_attention_function(AttentionBackendType.MI355)
 def _mi355_attn_call(query, key, value, dropout_p, is_causal, attention_kwargs=None, joint_kv=None):
     """bf16 / fp16 / fp32 attention; softmax scale is D**-0.5 as on the reference's AITER path
-    (attention_backend.py:790).  Returns (out BHSD in query's dtype, lse (B,H,S) fp32)."""
+    (attention_backend.py:790).  Returns (out BHSD in query's dtype, lse (B,H,S) fp32), differentiable in every tensor."""
     _check_call(dropout_p, is_causal, attention_kwargs)
     k1, v1, k2, v2 = _split_joint(key, value, joint_kv)
     scale = query.shape[-1] ** -0.5
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or custom_ops.attn_grad_wanted(query, k1, v1, k2, v2):
         # under torch.compile the call goes through the registered custom ops (fake
-        # implementations describe the outputs, so tracing does not break the graph)
+        # implementations describe the outputs, so tracing does not break the graph), and where a
+        # gradient is wanted (they have one)
         if k2 is None:
             return torch.ops.xdit_amd.attn_fwd(query, k1, v1, scale)
         return torch.ops.xdit_amd.attn_fwd_joint(query, k1, v1, k2, v2, scale)
@@ -91,11 +92,13 @@ def _kernel_reads_rows(t):
 def joint_queries_call(func, query, joint_query, joint_strategy, key, value, dropout_p, is_causal, attention_kwargs, joint_kv):
     """One call of the registered function `func` on the image queries and the joint queries in the order
     torch.cat would give them, without that copy; None where this does not apply (another function than
-    the adapters of this module, tensors that cannot be read in place, tracing).  Joint attention of 24
+    the adapters of this module, tensors that cannot be read in place, tracing, a gradient to be left behind).  Joint attention of 24
     heads of 4096 + 512 rows (bf16): the copy was 24 of 262 us."""
     if torch.compiler.is_compiling() or joint_strategy not in ("front", "rear") or joint_kv[0] is None or joint_kv[1] is None:
         return None
     if not (_kernel_reads_rows(query) and _kernel_reads_rows(joint_query)):
+        return None
+    if func is _mi355_attn_call and custom_ops.attn_grad_wanted(query, joint_query, key, value, *joint_kv[:2]):
         return None
     if (joint_query.dtype != query.dtype or joint_query.device != query.device or joint_query.shape[:2] != query.shape[:2]
             or joint_query.shape[3] != query.shape[3]):

@@ -315,6 +315,8 @@ namespace xdit {
 
 void api_clear_error() { g_err[0] = 0; }
 
+int api_check_tensor(const char* name, const void* p, const xdit_strides& st, int esize, int D) { return check_tensor(name, p, st, esize, D); }
+
 int api_fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);

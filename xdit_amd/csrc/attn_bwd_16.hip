@@ -1,0 +1,358 @@
+// Backward pass of the non-causal attention forward for 16-bit tensors on gfx950.
+//
+//   P_ij = exp(scale q_i.k_j - lse_i)      delta_i = dout_i.out_i - dlse_i
+//   dV_j = sum_i P_ij dout_i               dS_ij = P_ij (dout_i.v_j - delta_i)
+//   dK_j = scale sum_i dS_ij q_i           dQ_i = scale sum_j dS_ij k_j
+//
+// P is recomputed from the forward's log-sum-exp, so nothing of size Sq x Sk is ever in memory.
+//
+// Work decomposition: three launches.  bwd_stats_kernel writes lse / ln 2 and -delta of every row.  Then two roles of one kernel:
+//   keys     a workgroup owns 32 NW keys, wavefront w keys [32w, 32w+32); it streams the queries: dK and dV (four products)
+//   queries  a workgroup owns 32 NW queries; it streams the keys: dQ (three products)
+// Seven products instead of the five of a single pass: that one adds every workgroup's share of dQ up in memory, by
+// atomics (whose order changes the result) or through Sk / 256 fp32 copies of dQ, which cost as much time as the two products more.
+//
+// MFMA orientation (v_mfma_f32_32x32x16; A is 32x16, B is 16x32, lane l holds row/column l%32 and contraction elements
+// 8*(l/32)..+7; the result puts column l%32 and rows 8*(i/4) + 4*(l/32) + i%4, i = 0..15, in lane l).  X, Y: the streamed tensors
+// (keys role: q, dout; queries role: k, v); F, G: the owned rows (k, v; q, dout), in registers for the whole kernel:
+//   S  = X F^T, dP = Y G^T   A = rows of X, Y from LDS, B = F^T, G^T: a lane owns ONE row of F, and P, dS of it in its accumulators
+//   dV^T += Y^T P (keys role), dF^T += X^T dS   A = X^T, Y^T read transposed from LDS; B = P, dS: the accumulators, converted, are the operand
+// P and dS are rounded to the tensors' type for their products; all sums are fp32.
+#include "attn_bwd_rows.h"
+#include "attn_split.h"
+#include "attn_tiles.h"
+
+namespace xdit {
+namespace {
+
+constexpr int kTileRows = 64;   // streamed rows per LDS tile
+
+// LDS layout of a streamed tile: 64 rows, filled by 1 KiB pieces (a direct load writes lane i at 16 i), pieces 16 bytes more apart.
+// It is read in two ways: 16 consecutive rows at one 16-byte column (contraction over head_dim) and 4 consecutive rows at 64 bytes of
+// columns (transposed).  Rows r sit 16 * (4 (r % 4) + (r / 4) % 4) bytes apart modulo 256, which spreads either over all banks.
+template <int D> struct BwdGeom {
+  static constexpr int ROW_BYTES = 2 * D;
+  static constexpr int NG = kTileRows * ROW_BYTES / 1024;   // pieces
+  static constexpr int PITCH = 1024 + 16;
+  static constexpr int TENSOR_BYTES = NG * PITCH;
+  static constexpr int STAT_BYTES = 2 * kTileRows * 4;
+  static constexpr int BUF_BYTES = 2 * TENSOR_BYTES + STAT_BYTES;
+  static constexpr int LANES_PER_ROW = ROW_BYTES / 16;
+  static __device__ __forceinline__ int piece(int r) { return D == 128 ? 4 * (r & 3) + ((r >> 2) & 3) : 4 * (r & 1) + ((r >> 2) & 3); }
+  static __device__ __forceinline__ int slot(int r) { return D == 128 ? r >> 4 : ((r >> 1) & 1) + 2 * (r >> 4); }
+  static __device__ __forceinline__ int row(int g, int s) {
+    return D == 128 ? ((g >> 2) & 3) + 4 * (g & 3) + 16 * s : (g >> 2) + 2 * (s & 1) + 4 * (g & 3) + 16 * (s >> 1);
+  }
+  static constexpr int STEP32 = (D == 128 ? 2 : 4) * ROW_BYTES;  // +32 rows
+  static constexpr int STEP16 = STEP32 / 2;                      // +16 rows
+  static constexpr int STEP8 = 2 * PITCH;                        // +8 rows where bit 3 of the row is clear
+};
+
+__device__ __forceinline__ void load_lds_4(const void* base, unsigned off, unsigned lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, %2"
+      :
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base)
+      : "memory", "m0");
+}
+
+// fp16's numbers end at 2^-24, and P and dS are small.  P is computed times 2^13 (it stays below 2^14), which is free: the exponent gets it.  dS is computed
+// times 2^m, m between 0 and 13 so that 2^m times the largest |dout| of the (batch, head) is below 16 (dS, about
+// 16 sqrt(D) |v| P, is far below 65504 then).  The gradients are multiplied by 2^-13 and 2^-m at the end.
+constexpr int kFp16Exponent = 13;
+__device__ __forceinline__ int fp16_exponent(const AttnBwdParams& p, int bh) {
+  __shared__ float tops[8];
+  float top = 0.f;
+  const int blocks = p.sq_pad / kBwdStatRows;
+  for (int i = threadIdx.x; i < blocks; i += blockDim.x) top = fmaxf(top, p.amax[(int64_t)bh * blocks + i]);
+  for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  for (int i = 0; i < (int)blockDim.x >> 6; i++) top = fmaxf(top, tops[i]);
+  const int e = 130 - (int)(__float_as_uint(top) >> 23);   // 3 - floor(log2 top)
+  return __builtin_amdgcn_readfirstlane(e < 0 ? 0 : e > kFp16Exponent ? kFp16Exponent : e);
+}
+
+constexpr int kAhead = 4;  // LDS fragment reads in flight
+
+// acc = X_half F^T (contraction over head_dim, KSTEPS steps of 16), acc's initial values given.
+template <typename T, int KSTEPS, int OFF>
+__device__ __forceinline__ void rows_product(f32x16& acc, const typename Mfma16<T>::vec8 (&f)[KSTEPS], unsigned addr) {
+  typename Mfma16<T>::vec8 x[KSTEPS];
+  static_for<(kAhead < KSTEPS ? kAhead : KSTEPS)>([&](auto I) { constexpr int i = I; lds_read_b128<OFF + 32 * i>(x[i], addr); });
+  static_for<KSTEPS>([&](auto I) {
+    constexpr int i = I;
+    constexpr int younger = (i + kAhead <= KSTEPS ? kAhead : KSTEPS - i) - 1;
+    lds_wait<younger>(x[i]);
+    acc = Mfma16<T>::mma(x[i], f[i], acc);
+    if constexpr (i + kAhead < KSTEPS) lds_read_b128<OFF + 32 * (i + kAhead)>(x[i + kAhead], addr);
+  });
+}
+
+// acc[db] += X_half^T B, contraction over the half's 32 rows; B: two steps of 16.
+template <typename T, int D, int DBLOCKS, int OFF>
+__device__ __forceinline__ void columns_product(f32x16 (&acc)[DBLOCKS], const typename Mfma16<T>::vec8 (&pf)[2], unsigned addr) {
+  typedef typename Mfma16<T>::vec8 vec8;
+  typedef BwdGeom<D> G;
+  constexpr int NM = 2 * DBLOCKS;
+  constexpr int PD = kAhead / 2 < NM ? kAhead / 2 : NM;   // products whose two reads are in flight
+  typedef __attribute__((ext_vector_type(8))) short s16x8;
+  s16x4 v0[NM], v1[NM];
+  static_for<PD>([&](auto I) {
+    constexpr int i = I;
+    constexpr int off = OFF + (i / DBLOCKS) * G::STEP16 + (i % DBLOCKS) * 64;
+    lds_read_tr16_b64<off>(v0[i], addr);
+    lds_read_tr16_b64<off + G::STEP8>(v1[i], addr);
+  });
+  static_for<NM>([&](auto I) {
+    constexpr int i = I;
+    constexpr int younger = 2 * ((i + PD <= NM ? PD : NM - i) - 1);
+    lds_wait2<younger>(v0[i], v1[i]);
+    const s16x8 vv = __builtin_shufflevector(v0[i], v1[i], 0, 1, 2, 3, 4, 5, 6, 7);
+    acc[i % DBLOCKS] = Mfma16<T>::mma(__builtin_bit_cast(vec8, vv), pf[i / DBLOCKS], acc[i % DBLOCKS]);
+    if constexpr (i + PD < NM) {
+      constexpr int n = i + PD;
+      constexpr int off = OFF + (n / DBLOCKS) * G::STEP16 + (n % DBLOCKS) * 64;
+      lds_read_tr16_b64<off>(v0[n], addr);
+      lds_read_tr16_b64<off + G::STEP8>(v1[n], addr);
+    }
+  });
+}
+
+// A workgroup's part of one role.  D: the head_dim of the LDS geometry, DC (a multiple of 32) the computed one; columns between the
+// tensors' head_dim and DC are zeros in F and G and in the LDS tiles.
+template <typename T, int D, int DC, int NW, bool KEYS>
+__global__ __launch_bounds__(64 * NW, 2) void attn_bwd_16_kernel(const AttnBwdParams p) {
+  typedef typename Mfma16<T>::vec8 vec8;
+  typedef typename Mfma16<T>::vec2 vec2;
+  typedef __attribute__((ext_vector_type(4))) T vec4;
+  typedef BwdGeom<D> G;
+  constexpr int KSTEPS = DC / 16, DBLOCKS = DC / 32, ROWS = 32 * NW;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+
+  // Workgroup i runs on XCD i % 8: an XCD takes a contiguous range, whose tiles of one (batch, head) stream the same rows through one L2.
+  const BwdRole& R = KEYS ? p.keys : p.queries;
+  const int units = p.B * p.H * R.tiles * R.parts;
+  const int per_xcd = (units + 7) / 8;
+  const int unit = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+  if (unit >= units) return;
+  const int part = unit % R.parts;
+  const int bt = unit / R.parts;
+  const int bh = bt / R.tiles;
+  int tile = bt - bh * R.tiles;
+  const int b = bh / p.H, h = bh - b * p.H;
+  const int first = part * R.len;
+  const int last = first + R.len < R.steps ? first + R.len : R.steps;
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+
+  // ---- owned rows ----
+  const bool second = KEYS && tile >= p.tiles1;
+  if (second) tile -= p.tiles1;
+  const BwdTensor& F = KEYS ? (second ? p.k2 : p.k) : p.q;
+  const BwdTensor& Gt = KEYS ? (second ? p.v2 : p.v) : p.dout;
+  const int own_rows = KEYS ? (second ? p.Sk2 : p.Sk) : p.Sq;
+  const int own0 = tile * ROWS + wave * 32;
+  const int own = own0 + l32;
+  vec8 f[KSTEPS], g[KSTEPS];
+  {
+    const int r = own < own_rows ? own : own_rows - 1;
+    const T* fp = (const T*)F.p + b * F.b + h * F.h + (int64_t)r * F.s + hh * 8;
+    const T* gp = (const T*)Gt.p + b * Gt.b + h * Gt.h + (int64_t)r * Gt.s + hh * 8;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ks++) {
+      if (ks * 16 + hh * 8 < p.D) {
+        f[ks] = *(const vec8*)(fp + ks * 16);
+        g[ks] = *(const vec8*)(gp + ks * 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[ks][e] = g[ks][e] = (T)0.f;
+      }
+    }
+  }
+  const float c = p.scale * kLog2e;
+  const float* stats = p.stats + (int64_t)bh * 2 * p.sq_pad;
+  constexpr bool FP16 = __is_same(T, _Float16);
+  const int m = FP16 ? fp16_exponent(p, bh) : 0;
+  const float shift = !FP16 ? 0.f : KEYS ? (float)kFp16Exponent : (float)m;   // of P
+  const float p_to_ds = FP16 && KEYS ? __builtin_ldexpf(1.f, m - kFp16Exponent) : 1.f;
+  float own_lse = 0.f, own_nd = 0.f;
+  if constexpr (!KEYS) {
+    if (own < p.sq_pad) { own_lse = stats[own] - shift; own_nd = stats[p.sq_pad + own]; }
+  }
+
+  // ---- tile loads ----
+  const unsigned lds_base = (unsigned)(uintptr_t)(XDIT_LDS unsigned char*)smem;
+  const bool ld_on = (lane % G::LANES_PER_ROW) * 8 < p.D;
+  auto issue = [&](int t, unsigned bo) {
+    const bool s2 = !KEYS && t >= p.step1;
+    const BwdTensor& X = KEYS ? p.q : s2 ? p.k2 : p.k;
+    const BwdTensor& Y = KEYS ? p.dout : s2 ? p.v2 : p.v;
+    const int rows = KEYS ? p.Sq : s2 ? p.Sk2 : p.Sk;
+    const int row0 = (s2 ? t - p.step1 : t) * kTileRows;
+    const int left = rows - row0 < kTileRows ? rows - row0 : kTileRows;
+    const T* xb = (const T*)X.p + b * X.b + h * X.h + (int64_t)row0 * X.s;
+    const T* yb = (const T*)Y.p + b * Y.b + h * Y.h + (int64_t)row0 * Y.s;
+    const unsigned xs = (unsigned)X.s * 2, ys = (unsigned)Y.s * 2;
+    if (ld_on) {
+      for (int gidx = wave; gidx < G::NG; gidx += NW) {
+        int r = G::row(gidx, lane / G::LANES_PER_ROW);
+        r = r < left ? r : left - 1;   // rows past the end re-read the last one
+        const unsigned col = (lane % G::LANES_PER_ROW) * 16;
+        load_lds_16(xb, __umul24((unsigned)r, xs) + col, lds_base + bo + gidx * G::PITCH);
+        load_lds_16(yb, __umul24((unsigned)r, ys) + col, lds_base + bo + G::TENSOR_BYTES + gidx * G::PITCH);
+      }
+    }
+    if (KEYS && wave < 2)
+      load_lds_4(stats + wave * p.sq_pad + row0, lane * 4, lds_base + bo + 2 * G::TENSOR_BYTES + wave * kTileRows * 4);
+  };
+  // Columns that the tensors do not have: zeros, once.
+  if (DC > p.D) {
+    typedef __attribute__((ext_vector_type(4))) int i32x4;
+    const i32x4 zero = {0, 0, 0, 0};
+    const int c0 = p.D / 8, n = DC / 8 - c0;
+    for (int i = threadIdx.x; i < 4 * kTileRows * n; i += 64 * NW) {
+      const int which = i / (kTileRows * n), j = i % (kTileRows * n), r = j % kTileRows, ch = c0 + j / kTileRows;
+      *(XDIT_LDS i32x4*)((XDIT_LDS unsigned char*)smem + (which >> 1) * G::BUF_BYTES + (which & 1) * G::TENSOR_BYTES + G::piece(r) * G::PITCH + G::slot(r) * G::ROW_BYTES + ch * 16) = zero;
+    }
+  }
+
+  const unsigned row_addr = lds_base + G::piece(l32) * G::PITCH + G::slot(l32) * G::ROW_BYTES + hh * 16;
+  const int tr_row = 4 * hh + ((lane & 15) >> 2);
+  const unsigned col_addr = lds_base + G::piece(tr_row) * G::PITCH + G::slot(tr_row) * G::ROW_BYTES + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+
+  f32x16 acc_f[DBLOCKS], acc_g[KEYS ? DBLOCKS : 1];
+#pragma unroll
+  for (int db = 0; db < DBLOCKS; db++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      acc_f[db][e] = 0.f;
+      if (KEYS) acc_g[KEYS ? db : 0][e] = 0.f;
+    }
+#pragma unroll
+  for (int ks = 0; ks < KSTEPS; ks++) asm volatile("" : "+v"(f[ks]), "+v"(g[ks]));
+
+  issue(first, 0);
+  for (int t = first; t < last; t++) {
+    const unsigned bo = ((t - first) & 1) * G::BUF_BYTES;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t + 1 < last) issue(t + 1, G::BUF_BYTES - bo);
+    int left = kTileRows;   // keys of the tile that exist
+    if (!KEYS) {
+      const int l = t >= p.step1 ? p.Sk2 - (t - p.step1) * kTileRows : p.Sk - t * kTileRows;
+      left = l < kTileRows ? l : kTileRows;
+    }
+#pragma unroll 1
+    for (int hb = 0; hb < 2; hb++) {   // 32 streamed rows at a time
+      const unsigned ra = row_addr + bo + hb * G::STEP32, ca = col_addr + bo + hb * G::STEP32;
+      f32x16 s, dp;
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = 0.f;
+      rows_product<T, KSTEPS, 0>(s, f, ra);
+      __builtin_amdgcn_sched_barrier(0);
+      const XDIT_LDS f32x4* st = (const XDIT_LDS f32x4*)((XDIT_LDS unsigned char*)smem + bo + 2 * G::TENSOR_BYTES + hb * 128 + hh * 16);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        f32x4 x = {own_nd, own_nd, own_nd, own_nd};
+        if (KEYS) x = st[kTileRows / 4 + 2 * i];
+#pragma unroll
+        for (int e = 0; e < 4; e++) dp[4 * i + e] = x[e];
+      }
+      rows_product<T, KSTEPS, G::TENSOR_BYTES>(dp, g, ra);
+      __builtin_amdgcn_sched_barrier(0);
+      vec8 pf[2], df[2];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        f32x4 x = {own_lse, own_lse, own_lse, own_lse};
+        if (KEYS) x = st[2 * i];
+        if (KEYS && FP16) x -= shift;
+        f32x4 pr, ds;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          pr[e] = fast_exp2(__builtin_fmaf(s[4 * i + e], c, -x[e]));
+          if (!KEYS && left < kTileRows && 32 * hb + 8 * i + 4 * hh + e >= left) pr[e] = 0.f;
+          ds[e] = (FP16 && KEYS ? pr[e] * p_to_ds : pr[e]) * dp[4 * i + e];
+        }
+        const vec4 a = __builtin_convertvector(pr, vec4), d = __builtin_convertvector(ds, vec4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          pf[i >> 1][4 * (i & 1) + e] = a[e];
+          df[i >> 1][4 * (i & 1) + e] = d[e];
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (KEYS) columns_product<T, D, DBLOCKS, G::TENSOR_BYTES>(acc_g, pf, ca);
+      columns_product<T, D, DBLOCKS, 0>(acc_f, df, ca);
+    }
+  }
+
+  // ---- results ----
+#pragma unroll
+  for (int which = 0; which < (KEYS ? 2 : 1); which++) {   // 0: gradient of F, 1: of G
+    const float w = which ? __builtin_ldexpf(1.f, FP16 ? -kFp16Exponent : 0) : __builtin_ldexpf(p.scale, -m);
+    const BwdTensor& O = KEYS ? (which ? (second ? p.dv2 : p.dv) : (second ? p.dk2 : p.dk)) : p.dq;
+    T* orow = (T*)O.p + b * O.b + h * O.h + (int64_t)own * O.s;
+    float* prow = R.partial + (((int64_t)bt * R.parts + part) * (KEYS ? 2 : 1) + which) * ROWS * DC + (int64_t)(wave * 32 + l32) * DC;
+#pragma unroll
+    for (int db = 0; db < DBLOCKS; db++)
+#pragma unroll
+      for (int a = 0; a < 4; a++) {
+        const int col = 32 * db + 8 * a + 4 * hh;
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = (which ? acc_g[KEYS ? db : 0] : acc_f[db])[4 * a + e] * w;
+        if (R.parts > 1) *(f32x4*)(prow + col) = x;
+        else if (own < own_rows && col < p.D) *(vec4*)(orow + col) = __builtin_convertvector(x, vec4);
+      }
+  }
+}
+
+template <typename T, int D, int DC, int NW, bool KEYS>
+hipError_t launch_role(const AttnBwdParams& p, hipStream_t stream) {
+  const BwdRole& R = KEYS ? p.keys : p.queries;
+  static std::atomic<bool> lds_ready[kMaxDevices];
+  constexpr int lds = 2 * BwdGeom<D>::BUF_BYTES;
+  const int slot = current_device_slot();
+  if (!lds_ready[slot].load(std::memory_order_relaxed)) {
+    hipError_t e = hipFuncSetAttribute((const void*)attn_bwd_16_kernel<T, D, DC, NW, KEYS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+    lds_ready[slot].store(true, std::memory_order_relaxed);
+  }
+  const int units = p.B * p.H * R.tiles * R.parts;
+  hipLaunchKernelGGL((attn_bwd_16_kernel<T, D, DC, NW, KEYS>), dim3((unsigned)(units + 7) / 8 * 8), dim3(64 * NW), lds, stream, p);
+  if (R.parts > 1)
+    hipLaunchKernelGGL((bwd_fold_kernel<T, DC, KEYS>), dim3((unsigned)(p.B * p.H * R.tiles) * (32 * NW * (DC / 4) / 256), KEYS ? 2 : 1), dim3(256), 0, stream, p, 32 * NW);
+  return hipGetLastError();
+}
+
+template <typename T, int D, int DC, int NW>
+hipError_t launch_roles(const AttnBwdParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL((bwd_stats_kernel<T>), dim3((unsigned)(p.B * p.H) * (p.sq_pad / kBwdStatRows)), dim3(256), 0, stream, p);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && p.dk.p != nullptr) e = launch_role<T, D, DC, NW, true>(p, stream);
+  if (e == hipSuccess && p.dq.p != nullptr) e = launch_role<T, D, DC, NW, false>(p, stream);
+  return e;
+}
+
+template <typename T>
+hipError_t launch_typed(const AttnBwdParams& p, int waves, hipStream_t stream) {
+  if (waves == 8) {
+    if (p.D <= 32) return launch_roles<T, 64, 32, 8>(p, stream);
+    if (p.D <= 64) return launch_roles<T, 64, 64, 8>(p, stream);
+    if (p.D <= 96) return launch_roles<T, 128, 96, 8>(p, stream);
+    return launch_roles<T, 128, 128, 8>(p, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_attn_bwd_16(const AttnBwdParams& p, int dtype_is_fp16, int waves, hipStream_t stream) {
+  return dtype_is_fp16 ? launch_typed<_Float16>(p, waves, stream) : launch_typed<__bf16>(p, waves, stream);
+}
+
+}  // namespace xdit

@@ -2,7 +2,6 @@
 // Nothing here allocates device memory or synchronises; every launch goes to the caller's stream.
 #include "../../include/xdit_amd_attn.h"
 
-#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -12,25 +11,13 @@
 namespace {
 
 using xdit::api_fail;
+using xdit::Axis;
+using xdit::rows_apart;
 
 bool multiple_of(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 bool float_dtype(int d) { return d == XDIT_DTYPE_BF16 || d == XDIT_DTYPE_FP16 || d == XDIT_DTYPE_FP32; }
 int size_of(int d) { return d == XDIT_DTYPE_FP32 ? 4 : 2; }
-
-// Whether no two rows of `C` elements share one: going from the smallest stride up, each has to step over all that those below it reach.
-struct Axis { int64_t n, stride; };
-template <int N>
-bool rows_apart(int64_t C, Axis (&axes)[N]) {
-  std::sort(axes, axes + N, [](const Axis& a, const Axis& b) { return a.stride < b.stride; });
-  __int128 reach = C;
-  for (const Axis& a : axes) {
-    if (a.n <= 1) continue;
-    if (a.stride < reach) return false;
-    reach += (__int128)a.stride * (a.n - 1);
-  }
-  return true;
-}
 
 // A (B, S, C) tensor whose rows are read or written 8 elements at a time.  `written`: rows must not overlap.
 int check_rows(const char* name, const void* p, const xdit_row_strides& st, int esize, int64_t B, int64_t S, int64_t C, bool written) {

@@ -1,0 +1,177 @@
+// The norm of a list of gradients, and their clipping:  norm = (sum |g|^p)^(1/p) or max |g|,  g <- g min(1, max_norm / (norm + 1e-6)).
+//
+// Memory decides both: every element is read once for the norm, read and written once for the clipping.  A workgroup takes a chunk of
+// one tensor and finds it by comparing its number with all first chunks at once (they are kernel arguments).  Sums are in 64
+// bits from the first square on (a square of a bf16 or fp32 gradient can leave fp32's range, and 1e9 of them its precision); the conversion
+// to it and the multiply-add take about half of the time that a compute unit waits for the element.  Partial sums are added by one workgroup, in a fixed order.
+#include "grad_norm.h"
+#include "launchers.h"
+#include "row_ops.h"
+
+namespace xdit {
+namespace {
+
+// Which tensor a chunk belongs to: the number of first chunks at or below it, less one.
+template <int N>
+__device__ __forceinline__ int tensor_of(const GradTable<N>& t, unsigned chunk) {
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < (N + 63) / 64; i++) {
+    const int at = i * 64 + (threadIdx.x & 63);
+    n += __popcll(__builtin_amdgcn_ballot_w64(at < N && t.first[at < N ? at : N - 1] <= chunk));
+  }
+  return __builtin_amdgcn_readfirstlane(n - 1);
+}
+
+// Element indices count from the 16-byte boundary at or below a tensor's start (`lead` elements before it), so that groups of eight
+// are aligned wherever a tensor starts; groups that its ends cut are read element by element.
+template <typename T> __device__ __forceinline__ int lead_of(const void* p) { return (int)((uintptr_t)p & 15) / (int)sizeof(T); }
+
+template <int KIND>
+__device__ __forceinline__ double norm_join(double a, double b) { return KIND == 0 ? (b > a || b != b ? b : a) : a + b; }
+template <int KIND>
+__device__ __forceinline__ double norm_add(double acc, float x) {
+  const double v = (double)__builtin_fabsf(x);
+  return KIND == 2 ? __builtin_fma(v, v, acc) : norm_join<KIND>(acc, v);
+}
+// Joins the workgroup's values, in a fixed order; the result is thread 0's.
+template <int KIND, int WAVES>
+__device__ __forceinline__ double workgroup_join(double v) {
+  __shared__ double parts[WAVES];
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v = norm_join<KIND>(v, __shfl_xor(v, m));
+  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int i = 1; i < WAVES; i++) v = norm_join<KIND>(v, parts[i]);
+  return v;
+}
+
+template <typename T, int KIND>
+__global__ __launch_bounds__(256) void grad_norm_kernel(const NormParams p) {
+  const int which = tensor_of(p.t, blockIdx.x);
+  const T* src = (const T*)p.t.src[which];
+  const int lead = lead_of<T>(src);
+  const int64_t begin = (int64_t)(blockIdx.x - p.t.first[which]) * p.chunk;
+  const int64_t end = p.t.numel[which] + lead;   // of the tensor
+  const T* base = src - lead;
+  const int64_t last = begin + p.chunk < end ? begin + p.chunk : end;
+  double acc[4] = {0., 0., 0., 0.};
+  int64_t i = begin + threadIdx.x * 8;
+  // four groups asked for at a time
+  for (; i + 3 * 2048 + 8 <= last && i >= lead; i += 4 * 2048) {
+    Raw8<T> x[4];
+#pragma unroll
+    for (int n = 0; n < 4; n++) x[n] = load_raw8<T>(base, i + n * 2048);
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) acc[n] = norm_add<KIND>(acc[n], x[n][e]);
+  }
+  for (; i < last; i += 2048) {
+    if (i >= lead && i + 8 <= last) {
+      const Raw8<T> x = load_raw8<T>(base, i);
+#pragma unroll
+      for (int e = 0; e < 8; e++) acc[0] = norm_add<KIND>(acc[0], x[e]);
+    } else {
+      for (int64_t j = i; j < i + 8; j++)
+        if (j >= lead && j < last) acc[0] = norm_add<KIND>(acc[0], (float)base[j]);
+    }
+  }
+  const double v = workgroup_join<KIND, 4>(norm_join<KIND>(norm_join<KIND>(acc[0], acc[1]), norm_join<KIND>(acc[2], acc[3])));
+  if (threadIdx.x == 0) p.partial[blockIdx.x] = v;
+}
+
+template <int KIND>
+__global__ __launch_bounds__(1024) void grad_norm_total_kernel(const double* partial, int64_t n, float* norm) {
+  double v = 0.;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) v = norm_join<KIND>(v, partial[i]);
+  v = workgroup_join<KIND, 16>(v);
+  if (threadIdx.x == 0) *norm = (float)(KIND == 2 ? __builtin_sqrt(v) : v);
+}
+
+template <typename S, typename D>
+__global__ __launch_bounds__(256) void grad_clip_kernel(const ClipParams p) {
+  float factor = p.max_norm / (*p.norm + 1e-6f);
+  if (factor > 1.f) factor = 1.f;   // a norm that is not a number stays one
+  const int which = tensor_of(p.t, blockIdx.x);
+  const S* src = (const S*)p.t.src[which];
+  D* dst = (D*)p.dst[which];
+  if (factor == 1.f && (const void*)src == (const void*)dst) return;   // nothing to clip
+  const int64_t numel = p.t.numel[which];
+  const int64_t begin = (int64_t)(blockIdx.x - p.t.first[which]) * p.chunk;
+  const int lead = lead_of<S>(src);
+  if (lead == lead_of<D>(dst)) {
+    const S* sb = src - lead;
+    D* db = dst - lead;
+    const int64_t end = numel + lead;
+    const int64_t last = begin + p.chunk < end ? begin + p.chunk : end;
+    int64_t i = begin + threadIdx.x * 8;
+    for (; i + 3 * 2048 + 8 <= last && i >= lead; i += 4 * 2048) {
+      Raw8<S> x[4];
+#pragma unroll
+      for (int n = 0; n < 4; n++) x[n] = load_raw8<S>(sb, i + n * 2048);
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = x[n][e] * factor;
+        store8<D>(db, i + n * 2048, v);
+      }
+    }
+    for (; i < last; i += 2048) {
+      if (i >= lead && i + 8 <= last) {
+        const Raw8<S> x = load_raw8<S>(sb, i);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = x[e] * factor;
+        store8<D>(db, i, v);
+      } else {
+        for (int64_t j = i; j < i + 8; j++)
+          if (j >= lead && j < last) db[j] = (D)((float)sb[j] * factor);
+      }
+    }
+  } else {   // source and destination differ in where their 16-byte groups start: element by element
+    const int64_t last = begin + p.chunk < numel ? begin + p.chunk : numel;
+    for (int64_t i = begin + threadIdx.x; i < last; i += 256) dst[i] = (D)((float)src[i] * factor);
+  }
+}
+
+template <typename T>
+void norm_typed(const NormParams& p, unsigned workgroups, hipStream_t stream) {
+  if (p.kind == 0) hipLaunchKernelGGL((grad_norm_kernel<T, 0>), dim3(workgroups), dim3(256), 0, stream, p);
+  else if (p.kind == 1) hipLaunchKernelGGL((grad_norm_kernel<T, 1>), dim3(workgroups), dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((grad_norm_kernel<T, 2>), dim3(workgroups), dim3(256), 0, stream, p);
+}
+
+template <typename S>
+void clip_typed(const ClipParams& p, int dst_dtype, unsigned workgroups, hipStream_t stream) {
+  if (dst_dtype == 0) hipLaunchKernelGGL((grad_clip_kernel<S, __bf16>), dim3(workgroups), dim3(256), 0, stream, p);
+  else if (dst_dtype == 1) hipLaunchKernelGGL((grad_clip_kernel<S, _Float16>), dim3(workgroups), dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((grad_clip_kernel<S, float>), dim3(workgroups), dim3(256), 0, stream, p);
+}
+
+}  // namespace
+
+hipError_t launch_grad_norm(const NormParams& p, int dtype, unsigned workgroups, hipStream_t stream) {
+  if (dtype == 0) norm_typed<__bf16>(p, workgroups, stream);
+  else if (dtype == 1) norm_typed<_Float16>(p, workgroups, stream);
+  else norm_typed<float>(p, workgroups, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_grad_norm_total(const double* partial, int64_t n, int kind, float* norm, hipStream_t stream) {
+  if (kind == 0) hipLaunchKernelGGL((grad_norm_total_kernel<0>), dim3(1), dim3(1024), 0, stream, partial, n, norm);
+  else if (kind == 1) hipLaunchKernelGGL((grad_norm_total_kernel<1>), dim3(1), dim3(1024), 0, stream, partial, n, norm);
+  else hipLaunchKernelGGL((grad_norm_total_kernel<2>), dim3(1), dim3(1024), 0, stream, partial, n, norm);
+  return hipGetLastError();
+}
+
+hipError_t launch_grad_clip(const ClipParams& p, int src_dtype, int dst_dtype, unsigned workgroups, hipStream_t stream) {
+  if (src_dtype == 0) clip_typed<__bf16>(p, dst_dtype, workgroups, stream);
+  else if (src_dtype == 1) clip_typed<_Float16>(p, dst_dtype, workgroups, stream);
+  else clip_typed<float>(p, dst_dtype, workgroups, stream);
+  return hipGetLastError();
+}
+
+}  // namespace xdit

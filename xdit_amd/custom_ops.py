@@ -20,6 +20,9 @@ The reference wraps a vendor kernel the same way (xfuser/core/distributed/attent
     xdit_amd::norm_rope       (x, weight, cos, sin, eps, norm, rope,
                                rope_row0, rope_rows)                        -> y (BHSD-contiguous)
 
+    xdit_amd::attn_bwd        (dout, q, k, v, k2?, v2?, out, lse, dlse?, softmax_scale, need_q,
+                               need_kv)             -> list of gradients of attn_fwd or attn_fwd_joint
+
 and the operators around the attention call (`xdit_amd.block_ops`), with their gradients:
 
     xdit_amd::gated_norm      (x, y?, gate?, scale?, shift?, weight?, bias?, y_weight?, norm, eps,
@@ -43,7 +46,7 @@ from typing import List, Optional, Tuple
 import torch
 from torch.library import custom_op, register_autograd, register_fake
 
-from . import block_ops, ops
+from . import block_ops, grad_ops, ops
 
 Tensor = torch.Tensor
 
@@ -73,6 +76,88 @@ def attn_fwd_joint(query: Tensor, key: Tensor, value: Tensor, key2: Tensor, valu
 @register_fake("xdit_amd::attn_fwd_joint")
 def _attn_fwd_joint_fake(query, key, value, key2, value2, softmax_scale):
     return _fake_out_lse(query, query.dtype)
+
+
+def _attn_rows(t):
+    """A tensor whose rows attention's kernels read in place; a copy of any other (autograd may pass an expanded or transposed gradient)."""
+    es, (sb, sh, ss, sd) = t.element_size(), t.stride()
+    if (sd == 1 and ss >= t.shape[3] and ss * es < 1 << 24 and sb * es % 16 == 0 and sh * es % 16 == 0 and ss * es % 16 == 0
+            and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+@custom_op("xdit_amd::attn_bwd", mutates_args=(), device_types="cuda")
+def attn_bwd(dout: Tensor, query: Tensor, key: Tensor, value: Tensor, key2: Optional[Tensor], value2: Optional[Tensor], out: Tensor, lse: Tensor,
+             dlse: Optional[Tensor], softmax_scale: float, need_q: bool, need_kv: bool) -> List[Tensor]:
+    """`grad_ops.attn_bwd`: those of dq, dk, dv, dk2 and dv2 that there are."""
+    r = grad_ops.attn_bwd(_attn_rows(dout), query, key, value, _attn_rows(out), lse, softmax_scale, key2, value2, dlse, need_q=need_q, need_kv=need_kv)
+    return [t for t in r if t is not None]
+
+
+@register_fake("xdit_amd::attn_bwd")
+def _attn_bwd_fake(dout, query, key, value, key2, value2, out, lse, dlse, softmax_scale, need_q, need_kv):
+    return [t.new_empty(t.shape) for t, need in ((query, need_q), (key, need_kv), (value, need_kv), (key2, need_kv), (value2, need_kv))
+            if t is not None and need]
+
+
+def _attn_grads(needs, dout, dlse, query, key, value, key2, value2, out, lse, softmax_scale):
+    """Gradients of query, key, value, key2 and value2 as far as `needs` (one truth value each) asks; None for the others."""
+    need_q, need_kv = bool(needs[0]), any(needs[1:])
+    if (dout is None and dlse is None) or not (need_q or need_kv):
+        return (None,) * 5
+    if dout is None:
+        dout = torch.zeros_like(out)
+    r = iter(torch.ops.xdit_amd.attn_bwd(dout, query, key, value, key2, value2, out, lse, dlse, softmax_scale, need_q, need_kv))
+    there = (need_q, need_kv, need_kv, need_kv and key2 is not None, need_kv and key2 is not None)
+    return tuple(next(r) if t else None for t in there)
+
+
+def _attn_fwd_setup(ctx, inputs, output):
+    *tensors, ctx.scale = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(*tensors, *output)
+
+
+def _attn_fwd_grad(ctx, dout, dlse):
+    q, k, v, out, lse = ctx.saved_tensors
+    return (*_attn_grads(ctx.needs_input_grad[:3], dout, dlse, q, k, v, None, None, out, lse, ctx.scale)[:3], None)
+
+
+def _attn_fwd_joint_grad(ctx, dout, dlse):
+    return (*_attn_grads(ctx.needs_input_grad[:5], dout, dlse, *ctx.saved_tensors, ctx.scale), None)
+
+
+register_autograd("xdit_amd::attn_fwd", _attn_fwd_grad, setup_context=_attn_fwd_setup)
+register_autograd("xdit_amd::attn_fwd_joint", _attn_fwd_joint_grad, setup_context=_attn_fwd_setup)
+
+
+def attn_grad_wanted(*tensors):
+    """Whether an attention call on these tensors has to leave a graph behind (of the types that have a backward pass; fp8 has none)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad and t.dtype in (torch.bfloat16, torch.float16, torch.float32) for t in tensors)
+
+
+class RingAttention(torch.autograd.Function):
+    """Attention over all of key, value [, key2, value2] that `call()` computes in its own steps -> (out, lse); the gradient is one backward
+    call over the whole key range, from the merged output and log-sum-exp.  `bshd`: query, key, value and out are BSHD, lse is (B, H, Sq) either way."""
+
+    @staticmethod
+    def forward(ctx, call, scale, bshd, query, key, value, key2, value2):
+        out, lse = call()
+        ctx.scale, ctx.bshd = scale, bshd
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(query, key, value, key2, value2, out, lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlse):
+        def t(x):
+            return x.transpose(1, 2) if ctx.bshd and x is not None else x
+
+        q, k, v, k2, v2, out, lse = ctx.saved_tensors
+        grads = _attn_grads(ctx.needs_input_grad[3:], t(dout), dlse, t(q), t(k), t(v), t(k2), t(v2), t(out), lse, ctx.scale)
+        return (None, None, None, *map(t, grads))
 
 
 @custom_op("xdit_amd::attn_fwd_fp8", mutates_args=(), device_types="cuda")

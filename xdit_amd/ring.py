@@ -16,7 +16,7 @@ import math
 
 import torch
 
-from . import ops
+from . import custom_ops, ops
 
 
 class LocalRing:
@@ -51,10 +51,14 @@ def flash_attn_forward(q, k, v, dropout_p=0.0, softmax_scale=None, causal=False,
                        softcap=0.0, alibi_slopes=None, return_softmax=False, q_descale=None,
                        k_descale=None, v_descale=None, joint_k=None, joint_v=None, out_dtype=None):
     """Attention forward on BSHD tensors -> (block_out (B,Sq,H,D), block_lse (B,H,Sq) fp32).
-    `joint_k`/`joint_v` (BSHD) are a second KV segment appended after `k`/`v`."""
+    `joint_k`/`joint_v` (BSHD) are a second KV segment appended after `k`/`v`.  Differentiable in 16 and 32 bits."""
     _check_kernel_options(dropout_p, causal, window_size, softcap, alibi_slopes)
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(q.size(-1))
+    if custom_ops.attn_grad_wanted(q, k, v, joint_k, joint_v):
+        return custom_ops.RingAttention.apply(
+            lambda: flash_attn_forward(q, k, v, softmax_scale=softmax_scale, joint_k=joint_k, joint_v=joint_v, out_dtype=out_dtype),
+            softmax_scale, True, q, k, v, joint_k, joint_v)
     t = lambda x: None if x is None else x.transpose(1, 2)  # BSHD -> logical BHSD view, no copy
     B, Sq, H, D = q.shape
     if out_dtype is None:
@@ -95,7 +99,13 @@ def xdit_ring_flash_attn_forward(process_group, q, k, v, softmax_scale, dropout_
     process_group None        -> one step over all of k, v (the reference's single-GPU case).
     process_group LocalRing(P) -> k, v hold the FULL key/value sequence; they are split into P
                                  chunks visited in the order the ring would deliver them.
-    Returns (out in q's dtype (bf16 for fp8 inputs), lse (B,H,Sq) fp32)."""
+    Returns (out in q's dtype (bf16 for fp8 inputs), lse (B,H,Sq) fp32), differentiable in 16 and 32 bits."""
+    if custom_ops.attn_grad_wanted(q, k, v, joint_tensor_key, joint_tensor_value):
+        return custom_ops.RingAttention.apply(
+            lambda: xdit_ring_flash_attn_forward(process_group, q, k, v, softmax_scale, dropout_p, causal, window_size, alibi_slopes, deterministic,
+                                                 attn_type, attn_processor, attn_layer, joint_tensor_key, joint_tensor_value, joint_strategy,
+                                                 q_descale, k_descale, v_descale),
+            softmax_scale, True, q, k, v, joint_tensor_key, joint_tensor_value)
     is_joint = False
     if joint_tensor_key is not None and joint_tensor_value is not None:
         supported_joint_strategy = ["front", "rear"]
@@ -170,8 +180,8 @@ def xdit_ring_flash_attn_func(q, k, v, dropout_p=0.0, softmax_scale=None, causal
                               attn_type=None, attn_processor=None, attn_layer=None, joint_tensor_key=None,
                               joint_tensor_value=None, joint_strategy="none", q_descale=None, k_descale=None,
                               v_descale=None):
-    """Forward-only counterpart of xdit_ring_flash_attn_func / xFuserRingFlashAttnFunc.forward
-    (ring_flash_attn.py:153-210, :248-312): default scale 1/sqrt(D), `alibi_slopes` must be None,
+    """Counterpart of xdit_ring_flash_attn_func / xFuserRingFlashAttnFunc
+    (ring_flash_attn.py:153-210, :248-312), whose gradient is one backward call over the whole ring: default scale 1/sqrt(D), `alibi_slopes` must be None,
     returns `out` or `(out, lse, None)` when `return_attn_probs`."""
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)

@@ -11,7 +11,7 @@ import functools
 
 import torch
 
-from . import ops
+from . import custom_ops, ops
 from . import attention_backend as AB
 from .attention_backend import ATTENTION_FUNCTION_REGISTRY, AttentionBackendType
 
@@ -122,7 +122,8 @@ class SDPAMerger:
 def ring_attn(attention_function, query, key, value, dropout_p=0.0, is_causal=False,
               joint_attn_kwargs=None, attention_kwargs=None, ring_chunks=1, order=None):
     """The ring schedule of usp.py:46-74 on one device.  K/V are split into `ring_chunks`
-    contiguous chunks; `order` defaults to what rank 0 sees: [0, P-1, P-2, ..., 1]."""
+    contiguous chunks; `order` defaults to what rank 0 sees: [0, P-1, P-2, ..., 1].  On the 16- and 32-bit
+    backend the result is differentiable (outside torch.compile), joint tensors included."""
     P = ring_chunks
     if key.shape[2] % P != 0:
         raise ValueError(f"key length {key.shape[2]} is not divisible by ring_chunks={P}")
@@ -138,27 +139,39 @@ def ring_attn(attention_function, query, key, value, dropout_p=0.0, is_causal=Fa
         # bits as the call + merge below); the joint keys/values join on the step the decorator
         # would pick
         AB._check_call(dropout_p, is_causal, attention_kwargs)
-        acc_out = torch.empty(query.shape, dtype=torch.float32, device=query.device)
-        acc_lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device)
-        final = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        for i, c in enumerate(order):
-            joint_kv = None
-            if joint_attn_kwargs is not None:
-                strategy = joint_attn_kwargs.get("joint_strategy", None)
-                step = joint_attn_kwargs.get("step", 0)
-                if (strategy == "front" and step == 0) or (strategy == "rear" and step == joint_attn_kwargs.get("total_steps", 1) - 1):
-                    joint_kv = (joint_attn_kwargs.get("joint_key", None), joint_attn_kwargs.get("joint_value", None), strategy)
-                joint_attn_kwargs["step"] = step + 1
-            k1, v1, k2, v2 = AB._split_joint(k_chunks[c], v_chunks[c], joint_kv)
-            last = i == P - 1
-            if torch.compiler.is_compiling():   # the same call as a registered custom op (traceable)
-                torch.ops.xdit_amd.attn_fwd_accumulate(query, k1, v1, k2, v2, acc_out, acc_lse, final if last else None,
-                                                       i == 0, last, query.shape[-1] ** -0.5)
-            else:
-                ops.attn_fwd_accumulate(query, k1, v1, acc_out, acc_lse, first=i == 0,
-                                        final_out=final if last else None, discard_acc_out=last,
-                                        softmax_scale=query.shape[-1] ** -0.5, k2=k2, v2=v2)
-        return final
+        scale = query.shape[-1] ** -0.5
+
+        def steps():
+            acc_out = torch.empty(query.shape, dtype=torch.float32, device=query.device)
+            acc_lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device)
+            final = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+            for i, c in enumerate(order):
+                joint_kv = None
+                if joint_attn_kwargs is not None:
+                    strategy = joint_attn_kwargs.get("joint_strategy", None)
+                    step = joint_attn_kwargs.get("step", 0)
+                    if (strategy == "front" and step == 0) or (strategy == "rear" and step == joint_attn_kwargs.get("total_steps", 1) - 1):
+                        joint_kv = (joint_attn_kwargs.get("joint_key", None), joint_attn_kwargs.get("joint_value", None), strategy)
+                    joint_attn_kwargs["step"] = step + 1
+                k1, v1, k2, v2 = AB._split_joint(k_chunks[c], v_chunks[c], joint_kv)
+                last = i == P - 1
+                if torch.compiler.is_compiling():   # the same call as a registered custom op (traceable)
+                    torch.ops.xdit_amd.attn_fwd_accumulate(query, k1, v1, k2, v2, acc_out, acc_lse, final if last else None,
+                                                           i == 0, last, scale)
+                else:
+                    ops.attn_fwd_accumulate(query, k1, v1, acc_out, acc_lse, first=i == 0,
+                                            final_out=final if last else None, discard_acc_out=last,
+                                            softmax_scale=scale, k2=k2, v2=v2)
+            return final, acc_lse
+
+        joint = (None, None) if joint_attn_kwargs is None else (joint_attn_kwargs.get("joint_key", None), joint_attn_kwargs.get("joint_value", None))
+        if not torch.compiler.is_compiling() and custom_ops.attn_grad_wanted(query, key, value, *joint):
+            return custom_ops.RingAttention.apply(steps, scale, False, query, key, value, *joint)[0]
+        return steps()[0]
+    if P == 1 and ours and custom_ops.attn_grad_wanted(query, key, value):
+        # one block: the merge is the identity, and the call itself has the gradient
+        return attention_function(query, key, value, dropout_p=dropout_p, is_causal=is_causal,
+                                  joint_attn_kwargs=joint_attn_kwargs, attention_kwargs=attention_kwargs)[0]
     merger = SDPAMerger()
     for i, c in enumerate(order):
         out, lse = attention_function(query, k_chunks[c], v_chunks[c], dropout_p=dropout_p, is_causal=is_causal,
