@@ -146,7 +146,9 @@ def test_some_of_the_gradients(gpu, need_q, need_kv, dtype):
     t = inputs(gpu, 1, 2, 300, 200, 64, 50, dtype)
     every, some = call(*t), call(*t, need_q=need_q, need_kv=need_kv)
     assert [x is not None for x in some] == [need_q] + 4 * [need_kv]
-    assert all(torch.equal(a, b) for a, b in zip(every, some) if b is not None)
+    (want, far) = bounds(*t)   # the launches are cut up differently: each within its own bounds
+    for got in (every, some):
+        close(*zip(*((g, w, f) for g, w, f in zip(got, want, far) if g is not None)))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])

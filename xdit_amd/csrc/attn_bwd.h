@@ -12,11 +12,15 @@ struct BwdTensor {  // a logical (B, H, S, D) tensor with a unit stride over D
   int64_t b, h, s;
 };
 
-// The work of one role (see attn_bwd_16.hip): every (batch, head) has `tiles` row tiles, whose streamed range of
-// `steps` tiles is cut into `parts` parts of `len` tiles.
+// The work of one role (see attn_bwd_16.hip).  Every (batch, head) has `tiles` row tiles that stream `steps` tiles each.  An XCD takes
+// `per_xcd` consecutive tiles of all (batch, head)s: the first `whole` of them are one unit each, the ranges of the others are cut into
+// `parts` units of `len` steps, whose fp32 results a launch of its own adds up.
 struct BwdRole {
-  int tiles, steps, parts, len;
-  float* partial;  // parts > 1: [(bh, tile)][part][tensor][row][column] in fp32, folded by a launch of its own
+  int tiles, steps;
+  int total;            // tiles of all (batch, head)s; 0: the role's gradients are not asked for
+  int per_xcd, whole, parts, len;
+  int units;            // per XCD
+  float* partial;       // [XCD][tile behind `whole`][part][tensor][row][column]
 };
 
 struct AttnBwdParams {
@@ -38,8 +42,29 @@ struct AttnBwdParams {
 };
 
 constexpr int kBwdStatRows = 64;  // rows of a workgroup of the statistics kernel
+constexpr int kBwdWaves = 4;      // wavefronts of a workgroup, 32 owned rows each
+constexpr int kBwdRows = 32 * kBwdWaves;
 
-hipError_t launch_attn_bwd_16(const AttnBwdParams& p, int dtype_is_fp16, int waves, hipStream_t stream);
+// A unit's tile (of all), part and slot of its partial result; false for the units that an XCD's last tiles do not have.
+struct BwdUnit {
+  int tile, part;
+  int64_t slot;   // < 0: a whole tile
+};
+__device__ __forceinline__ bool bwd_unit(const BwdRole& r, int xcd, int n, BwdUnit& u) {
+  int t = n;
+  u.part = 0;
+  u.slot = -1;
+  if (n >= r.whole) {
+    const int i = (n - r.whole) / r.parts;
+    t = r.whole + i;
+    u.part = n - r.whole - i * r.parts;
+    if (r.parts > 1) u.slot = ((int64_t)xcd * (r.per_xcd - r.whole) + i) * r.parts + u.part;
+  }
+  u.tile = xcd * r.per_xcd + t;
+  return u.tile < r.total;
+}
+
+hipError_t launch_attn_bwd_16(const AttnBwdParams& p, int dtype_is_fp16, hipStream_t stream);
 hipError_t launch_attn_bwd_f32(const AttnBwdParams& p, hipStream_t stream);
 
 }  // namespace xdit

@@ -6,11 +6,15 @@
 //
 // P is recomputed from the forward's log-sum-exp, so nothing of size Sq x Sk is ever in memory.
 //
-// Work decomposition: three launches.  bwd_stats_kernel writes lse / ln 2 and -delta of every row.  Then two roles of one kernel:
-//   keys     a workgroup owns 32 NW keys, wavefront w keys [32w, 32w+32); it streams the queries: dK and dV (four products)
-//   queries  a workgroup owns 32 NW queries; it streams the keys: dQ (three products)
+// Work decomposition: bwd_stats_kernel writes lse / ln 2 and -delta of every row, then one launch has the units of two roles:
+//   keys     a workgroup owns 128 keys, wavefront w keys [32w, 32w+32); it streams the queries: dK and dV (four products)
+//   queries  a workgroup owns 128 queries; it streams the keys: dQ (three products)
 // Seven products instead of the five of a single pass: that one adds every workgroup's share of dQ up in memory, by
-// atomics (whose order changes the result) or through Sk / 256 fp32 copies of dQ, which cost as much time as the two products more.
+// atomics (whose order changes the result) or through Sk / 128 fp32 copies of dQ, which cost as much time as the two products more.
+// The longer units, those of the keys, start first; the last units may be parts of tiles, which even out the end of the launch
+// and let few tiles fill the chip (BwdRole; the parts are added up by bwd_fold_kernel).
+// Workgroups have four wavefronts, two of them share a compute unit (three at head_dim 64): with eight wavefronts in step 5 heads of 32760 tokens took
+// 3939 us in the queries role, with four 3596, 24 heads of 4250 x 2 at head_dim 64 1010 and 877 us in both.
 //
 // MFMA orientation (v_mfma_f32_32x32x16; A is 32x16, B is 16x32, lane l holds row/column l%32 and contraction elements
 // 8*(l/32)..+7; the result puts column l%32 and rows 8*(i/4) + 4*(l/32) + i%4, i = 0..15, in lane l).  X, Y: the streamed tensors
@@ -77,6 +81,10 @@ __device__ __forceinline__ int fp16_exponent(const AttnBwdParams& p, int bh) {
 
 constexpr int kAhead = 4;  // LDS fragment reads in flight
 
+// Staging block of a wavefront for its results: 32 rows of 64 columns, rows 8 bytes apart from a multiple of 128.
+constexpr int kBwdStagePitch = 64 * 2 + 8;
+constexpr int kBwdStageBytes = 32 * kBwdStagePitch;
+
 // acc = X_half F^T (contraction over head_dim, KSTEPS steps of 16), acc's initial values given.
 template <typename T, int KSTEPS, int OFF>
 __device__ __forceinline__ void rows_product(f32x16& acc, const typename Mfma16<T>::vec8 (&f)[KSTEPS], unsigned addr) {
@@ -121,30 +129,23 @@ __device__ __forceinline__ void columns_product(f32x16 (&acc)[DBLOCKS], const ty
   });
 }
 
-// A workgroup's part of one role.  D: the head_dim of the LDS geometry, DC (a multiple of 32) the computed one; columns between the
+// One unit of a role.  D: the head_dim of the LDS geometry, DC (a multiple of 32) the computed one; columns between the
 // tensors' head_dim and DC are zeros in F and G and in the LDS tiles.
-template <typename T, int D, int DC, int NW, bool KEYS>
-__global__ __launch_bounds__(64 * NW, 2) void attn_bwd_16_kernel(const AttnBwdParams p) {
+template <typename T, int D, int DC, bool KEYS>
+__device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n, unsigned char* smem) {
   typedef typename Mfma16<T>::vec8 vec8;
-  typedef typename Mfma16<T>::vec2 vec2;
   typedef __attribute__((ext_vector_type(4))) T vec4;
   typedef BwdGeom<D> G;
-  constexpr int KSTEPS = DC / 16, DBLOCKS = DC / 32, ROWS = 32 * NW;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  constexpr int NW = kBwdWaves, KSTEPS = DC / 16, DBLOCKS = DC / 32, ROWS = kBwdRows;
 
-  // Workgroup i runs on XCD i % 8: an XCD takes a contiguous range, whose tiles of one (batch, head) stream the same rows through one L2.
   const BwdRole& R = KEYS ? p.keys : p.queries;
-  const int units = p.B * p.H * R.tiles * R.parts;
-  const int per_xcd = (units + 7) / 8;
-  const int unit = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
-  if (unit >= units) return;
-  const int part = unit % R.parts;
-  const int bt = unit / R.parts;
-  const int bh = bt / R.tiles;
-  int tile = bt - bh * R.tiles;
+  BwdUnit unit;
+  if (!bwd_unit(R, xcd, n, unit)) return;
+  const int bh = unit.tile / R.tiles;
+  int tile = unit.tile - bh * R.tiles;
   const int b = bh / p.H, h = bh - b * p.H;
-  const int first = part * R.len;
-  const int last = first + R.len < R.steps ? first + R.len : R.steps;
+  const int first = unit.slot < 0 ? 0 : unit.part * R.len;
+  const int last = unit.slot < 0 || first + R.len > R.steps ? R.steps : first + R.len;
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
@@ -265,16 +266,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_16_kernel(const AttnBwdPa
       rows_product<T, KSTEPS, G::TENSOR_BYTES>(dp, g, ra);
       __builtin_amdgcn_sched_barrier(0);
       vec8 pf[2], df[2];
+      if constexpr (!KEYS) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = fast_exp2(__builtin_fmaf(s[e], c, -own_lse));
+        if (left < kTileRows) {   // only a segment's last tile: keys behind its end
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (32 * hb + 8 * (e >> 2) + 4 * hh + (e & 3) >= left) s[e] = 0.f;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        f32x4 x = {own_lse, own_lse, own_lse, own_lse};
-        if (KEYS) x = st[2 * i];
-        if (KEYS && FP16) x -= shift;
         f32x4 pr, ds;
+        if constexpr (KEYS) {
+          f32x4 x = st[2 * i];
+          if (FP16) x -= shift;
+#pragma unroll
+          for (int e = 0; e < 4; e++) pr[e] = fast_exp2(__builtin_fmaf(s[4 * i + e], c, -x[e]));
+        }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          pr[e] = fast_exp2(__builtin_fmaf(s[4 * i + e], c, -x[e]));
-          if (!KEYS && left < kTileRows && 32 * hb + 8 * i + 4 * hh + e >= left) pr[e] = 0.f;
+          if (!KEYS) pr[e] = s[4 * i + e];
           ds[e] = (FP16 && KEYS ? pr[e] * p_to_ds : pr[e]) * dp[4 * i + e];
         }
         const vec4 a = __builtin_convertvector(pr, vec4), d = __builtin_convertvector(ds, vec4);
@@ -291,68 +303,94 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_16_kernel(const AttnBwdPa
   }
 
   // ---- results ----
+  if (unit.slot < 0) __syncthreads();   // the staging blocks lie over the tiles
 #pragma unroll
   for (int which = 0; which < (KEYS ? 2 : 1); which++) {   // 0: gradient of F, 1: of G
     const float w = which ? __builtin_ldexpf(1.f, FP16 ? -kFp16Exponent : 0) : __builtin_ldexpf(p.scale, -m);
-    const BwdTensor& O = KEYS ? (which ? (second ? p.dv2 : p.dv) : (second ? p.dk2 : p.dk)) : p.dq;
-    T* orow = (T*)O.p + b * O.b + h * O.h + (int64_t)own * O.s;
-    float* prow = R.partial + (((int64_t)bt * R.parts + part) * (KEYS ? 2 : 1) + which) * ROWS * DC + (int64_t)(wave * 32 + l32) * DC;
+    if (unit.slot >= 0) {
+      float* prow = R.partial + ((unit.slot * (KEYS ? 2 : 1) + which) * ROWS + wave * 32 + l32) * DC + 4 * hh;
 #pragma unroll
-    for (int db = 0; db < DBLOCKS; db++)
+      for (int db = 0; db < DBLOCKS; db++)
 #pragma unroll
-      for (int a = 0; a < 4; a++) {
-        const int col = 32 * db + 8 * a + 4 * hh;
-        f32x4 x;
+        for (int a = 0; a < 4; a++) {
+          f32x4 x;
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = (which ? acc_g[KEYS ? db : 0] : acc_f[db])[4 * a + e] * w;
-        if (R.parts > 1) *(f32x4*)(prow + col) = x;
-        else if (own < own_rows && col < p.D) *(vec4*)(orow + col) = __builtin_convertvector(x, vec4);
+          for (int e = 0; e < 4; e++) x[e] = (which ? acc_g[KEYS ? db : 0] : acc_f[db])[4 * a + e] * w;
+          *(f32x4*)(prow + 32 * db + 8 * a) = x;
+        }
+    } else {
+      // Through LDS, 64 columns at a time, so that a store covers whole 128-byte lines of 8 rows.
+      const BwdTensor& O = KEYS ? (which ? (second ? p.dv2 : p.dv) : (second ? p.dk2 : p.dk)) : p.dq;
+      T* orow = (T*)O.p + b * O.b + h * O.h + (int64_t)own0 * O.s;
+      XDIT_LDS unsigned char* stage = (XDIT_LDS unsigned char*)smem + wave * kBwdStageBytes;
+      const int rows_live = own_rows - own0;   // may be <= 0 or above 32
+#pragma unroll
+      for (int half = 0; half < (DBLOCKS + 1) / 2; half++) {
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+          const int db = 2 * half + d;
+          if (db < DBLOCKS) {
+#pragma unroll
+            for (int a = 0; a < 4; a++) {
+              f32x4 x;
+#pragma unroll
+              for (int e = 0; e < 4; e++) x[e] = (which ? acc_g[KEYS ? db : 0] : acc_f[db])[4 * a + e] * w;
+              *(XDIT_LDS vec4*)(stage + l32 * kBwdStagePitch + (32 * d + 8 * a + 4 * hh) * 2) = __builtin_convertvector(x, vec4);
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int row = (lane >> 3) + 8 * r, col = 64 * half + (lane & 7) * 8;
+          const vec8 x = *(const XDIT_LDS vec8*)(stage + row * kBwdStagePitch + (lane & 7) * 16);
+          if (row < rows_live && col < p.D) *(vec8*)(orow + row * O.s + col) = x;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
       }
+    }
   }
 }
 
-template <typename T, int D, int DC, int NW, bool KEYS>
-hipError_t launch_role(const AttnBwdParams& p, hipStream_t stream) {
-  const BwdRole& R = KEYS ? p.keys : p.queries;
+// Workgroup i runs on XCD i % 8: an XCD takes consecutive tiles, so that those of one (batch, head) stream the same rows through one L2.
+template <typename T, int D, int DC>
+__global__ __launch_bounds__(64 * kBwdWaves, D == 64 ? 3 : 2) void attn_bwd_16_kernel(const AttnBwdParams p) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int xcd = blockIdx.x % 8, n = blockIdx.x / 8;
+  if (n < p.keys.units) bwd_role<T, D, DC, true>(p, xcd, n, smem);
+  else bwd_role<T, D, DC, false>(p, xcd, n - p.keys.units, smem);
+}
+
+template <typename T, int D, int DC>
+hipError_t launch_kernels(const AttnBwdParams& p, hipStream_t stream) {
   static std::atomic<bool> lds_ready[kMaxDevices];
   constexpr int lds = 2 * BwdGeom<D>::BUF_BYTES;
+  static_assert(lds >= kBwdWaves * kBwdStageBytes, "staging blocks");
   const int slot = current_device_slot();
-  if (!lds_ready[slot].load(std::memory_order_relaxed)) {
-    hipError_t e = hipFuncSetAttribute((const void*)attn_bwd_16_kernel<T, D, DC, NW, KEYS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (!lds_ready[slot].load(std::memory_order_relaxed)) {  // > 64 KiB of dynamic LDS must be enabled once per kernel and device
+    hipError_t e = hipFuncSetAttribute((const void*)attn_bwd_16_kernel<T, D, DC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     lds_ready[slot].store(true, std::memory_order_relaxed);
   }
-  const int units = p.B * p.H * R.tiles * R.parts;
-  hipLaunchKernelGGL((attn_bwd_16_kernel<T, D, DC, NW, KEYS>), dim3((unsigned)(units + 7) / 8 * 8), dim3(64 * NW), lds, stream, p);
-  if (R.parts > 1)
-    hipLaunchKernelGGL((bwd_fold_kernel<T, DC, KEYS>), dim3((unsigned)(p.B * p.H * R.tiles) * (32 * NW * (DC / 4) / 256), KEYS ? 2 : 1), dim3(256), 0, stream, p, 32 * NW);
-  return hipGetLastError();
-}
-
-template <typename T, int D, int DC, int NW>
-hipError_t launch_roles(const AttnBwdParams& p, hipStream_t stream) {
   hipLaunchKernelGGL((bwd_stats_kernel<T>), dim3((unsigned)(p.B * p.H) * (p.sq_pad / kBwdStatRows)), dim3(256), 0, stream, p);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && p.dk.p != nullptr) e = launch_role<T, D, DC, NW, true>(p, stream);
-  if (e == hipSuccess && p.dq.p != nullptr) e = launch_role<T, D, DC, NW, false>(p, stream);
-  return e;
+  hipLaunchKernelGGL((attn_bwd_16_kernel<T, D, DC>), dim3(8u * (unsigned)(p.keys.units + p.queries.units)), dim3(64 * kBwdWaves), lds, stream, p);
+  return launch_bwd_fold<T, DC>(p, stream);
 }
 
 template <typename T>
-hipError_t launch_typed(const AttnBwdParams& p, int waves, hipStream_t stream) {
-  if (waves == 8) {
-    if (p.D <= 32) return launch_roles<T, 64, 32, 8>(p, stream);
-    if (p.D <= 64) return launch_roles<T, 64, 64, 8>(p, stream);
-    if (p.D <= 96) return launch_roles<T, 128, 96, 8>(p, stream);
-    return launch_roles<T, 128, 128, 8>(p, stream);
-  }
-  return hipErrorInvalidValue;
+hipError_t launch_typed(const AttnBwdParams& p, hipStream_t stream) {
+  if (p.D <= 32) return launch_kernels<T, 64, 32>(p, stream);
+  if (p.D <= 64) return launch_kernels<T, 64, 64>(p, stream);
+  if (p.D <= 96) return launch_kernels<T, 128, 96>(p, stream);
+  return launch_kernels<T, 128, 128>(p, stream);
 }
 
 }  // namespace
 
-hipError_t launch_attn_bwd_16(const AttnBwdParams& p, int dtype_is_fp16, int waves, hipStream_t stream) {
-  return dtype_is_fp16 ? launch_typed<_Float16>(p, waves, stream) : launch_typed<__bf16>(p, waves, stream);
+hipError_t launch_attn_bwd_16(const AttnBwdParams& p, int dtype_is_fp16, hipStream_t stream) {
+  return dtype_is_fp16 ? launch_typed<_Float16>(p, stream) : launch_typed<__bf16>(p, stream);
 }
 
 }  // namespace xdit

@@ -14,7 +14,6 @@
 namespace xdit {
 namespace {
 
-constexpr int kWaves32 = 4;
 constexpr int kRows32 = 32;   // streamed rows per LDS tile
 
 // KG: groups of 8 columns that hold the tensors' head_dim; DB: blocks of 32 columns of the gradients.
@@ -24,24 +23,19 @@ template <int KG, int DB>
 constexpr int buf_f32() { return 2 * kRows32 * pitch_f32<KG, DB>() + 2 * kRows32; }
 
 template <int KG, int DB, bool KEYS>
-__global__ __launch_bounds__(64 * kWaves32, 1) void attn_bwd_f32_kernel(const AttnBwdParams p) {
-  constexpr int ROWS = 32 * kWaves32, PITCH = pitch_f32<KG, DB>(), BUF = buf_f32<KG, DB>(), THREADS = 64 * kWaves32;
+__device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, int n, float* lds32) {
+  constexpr int ROWS = kBwdRows, PITCH = pitch_f32<KG, DB>(), BUF = buf_f32<KG, DB>(), THREADS = 64 * kBwdWaves;
   constexpr int CHUNKS = kRows32 * KG * 2;                      // 16-byte pieces of a tensor's tile
   constexpr int LOADS = (CHUNKS + THREADS - 1) / THREADS;
-  extern __shared__ __attribute__((aligned(16))) float lds32[];
 
   const BwdRole& R = KEYS ? p.keys : p.queries;
-  const int units = p.B * p.H * R.tiles * R.parts;
-  const int per_xcd = (units + 7) / 8;
-  const int unit = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;   // as in the 16-bit kernel
-  if (unit >= units) return;
-  const int part = unit % R.parts;
-  const int bt = unit / R.parts;
-  const int bh = bt / R.tiles;
-  int tile = bt - bh * R.tiles;
+  BwdUnit unit;
+  if (!bwd_unit(R, xcd, n, unit)) return;
+  const int bh = unit.tile / R.tiles;
+  int tile = unit.tile - bh * R.tiles;
   const int b = bh / p.H, h = bh - b * p.H;
-  const int first = part * R.len;
-  const int last = first + R.len < R.steps ? first + R.len : R.steps;
+  const int first = unit.slot < 0 ? 0 : unit.part * R.len;
+  const int last = unit.slot < 0 || first + R.len > R.steps ? R.steps : first + R.len;
 
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
   const bool second = KEYS && tile >= p.tiles1;
@@ -176,7 +170,7 @@ __global__ __launch_bounds__(64 * kWaves32, 1) void attn_bwd_f32_kernel(const At
     const float w = which ? 1.f : p.scale;
     const BwdTensor& O = KEYS ? (which ? (second ? p.dv2 : p.dv) : (second ? p.dk2 : p.dk)) : p.dq;
     float* orow = (float*)O.p + b * O.b + h * O.h + (int64_t)own * O.s;
-    float* prow = R.partial + (((int64_t)bt * R.parts + part) * (KEYS ? 2 : 1) + which) * ROWS * 32 * DB + (int64_t)(wave * 32 + l32) * 32 * DB;
+    float* prow = R.partial + ((unit.slot * (KEYS ? 2 : 1) + which) * ROWS + wave * 32 + l32) * 32 * DB;
 #pragma unroll
     for (int db = 0; db < DB; db++)
 #pragma unroll
@@ -185,48 +179,44 @@ __global__ __launch_bounds__(64 * kWaves32, 1) void attn_bwd_f32_kernel(const At
         f32x4 x;
 #pragma unroll
         for (int e = 0; e < 4; e++) x[e] = (which ? acc_g[KEYS ? db : 0] : acc_f[db])[4 * a + e] * w;
-        if (R.parts > 1) *(f32x4*)(prow + col) = x;
+        if (unit.slot >= 0) *(f32x4*)(prow + col) = x;
         else if (own < own_rows && col < p.D) *(f32x4*)(orow + col) = x;
       }
   }
 }
 
-template <int KG, int DB, bool KEYS>
-hipError_t launch_role(const AttnBwdParams& p, hipStream_t stream) {
-  const BwdRole& R = KEYS ? p.keys : p.queries;
+template <int KG, int DB>
+__global__ __launch_bounds__(64 * kBwdWaves, 1) void attn_bwd_f32_kernel(const AttnBwdParams p) {
+  extern __shared__ __attribute__((aligned(16))) float lds32[];
+  const int xcd = blockIdx.x % 8, n = blockIdx.x / 8;   // as in the 16-bit kernel
+  if (n < p.keys.units) bwd_role_f32<KG, DB, true>(p, xcd, n, lds32);
+  else bwd_role_f32<KG, DB, false>(p, xcd, n - p.keys.units, lds32);
+}
+
+template <int KG, int DB>
+hipError_t launch_kernels(const AttnBwdParams& p, hipStream_t stream) {
   static std::atomic<bool> lds_ready[kMaxDevices];
   constexpr int lds = 2 * buf_f32<KG, DB>() * 4;
   const int slot = current_device_slot();
   if (!lds_ready[slot].load(std::memory_order_relaxed)) {
-    hipError_t e = hipFuncSetAttribute((const void*)attn_bwd_f32_kernel<KG, DB, KEYS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipError_t e = hipFuncSetAttribute((const void*)attn_bwd_f32_kernel<KG, DB>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     lds_ready[slot].store(true, std::memory_order_relaxed);
   }
-  const int units = p.B * p.H * R.tiles * R.parts;
-  hipLaunchKernelGGL((attn_bwd_f32_kernel<KG, DB, KEYS>), dim3((unsigned)(units + 7) / 8 * 8), dim3(64 * kWaves32), lds, stream, p);
-  if (R.parts > 1)
-    hipLaunchKernelGGL((bwd_fold_kernel<float, 32 * DB, KEYS>), dim3((unsigned)(p.B * p.H * R.tiles) * (32 * kWaves32 * 8 * DB / 256), KEYS ? 2 : 1), dim3(256), 0, stream, p, 32 * kWaves32);
-  return hipGetLastError();
-}
-
-template <int KG, int DB>
-hipError_t launch_roles(const AttnBwdParams& p, hipStream_t stream) {
   hipLaunchKernelGGL((bwd_stats_kernel<float>), dim3((unsigned)(p.B * p.H) * (p.sq_pad / kBwdStatRows)), dim3(256), 0, stream, p);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && p.dk.p != nullptr) e = launch_role<KG, DB, true>(p, stream);
-  if (e == hipSuccess && p.dq.p != nullptr) e = launch_role<KG, DB, false>(p, stream);
-  return e;
+  hipLaunchKernelGGL((attn_bwd_f32_kernel<KG, DB>), dim3(8u * (unsigned)(p.keys.units + p.queries.units)), dim3(64 * kBwdWaves), lds, stream, p);
+  return launch_bwd_fold<float, 32 * DB>(p, stream);
 }
 
 }  // namespace
 
 // head_dims up to 80 of the 96-column form contract over 80 columns (72 is a model's own).
 hipError_t launch_attn_bwd_f32(const AttnBwdParams& p, hipStream_t stream) {
-  if (p.D <= 32) return launch_roles<4, 1>(p, stream);
-  if (p.D <= 64) return launch_roles<8, 2>(p, stream);
-  if (p.D <= 80) return launch_roles<10, 3>(p, stream);
-  if (p.D <= 96) return launch_roles<12, 3>(p, stream);
-  return launch_roles<16, 4>(p, stream);
+  if (p.D <= 32) return launch_kernels<4, 1>(p, stream);
+  if (p.D <= 64) return launch_kernels<8, 2>(p, stream);
+  if (p.D <= 80) return launch_kernels<10, 3>(p, stream);
+  if (p.D <= 96) return launch_kernels<12, 3>(p, stream);
+  return launch_kernels<16, 4>(p, stream);
 }
 
 }  // namespace xdit

@@ -52,30 +52,44 @@ __global__ __launch_bounds__(256) void bwd_stats_kernel(const AttnBwdParams p) {
   }
 }
 
-// Adds the parts of every row up, in their order, and rounds.
-template <typename T, int DC, bool KEYS>
-__global__ __launch_bounds__(256) void bwd_fold_kernel(const AttnBwdParams p, int rows_per_tile) {
+// Adds the parts of every row of the tiles that were cut up, in their order, and rounds.  Blocks of the keys role first, dk and dv of a tile
+// side by side, then those of the queries role.
+template <typename T, int DC>
+__global__ __launch_bounds__(256) void bwd_fold_kernel(const AttnBwdParams p) {
   typedef __attribute__((ext_vector_type(4))) T vec4;
-  const BwdRole& R = KEYS ? p.keys : p.queries;
-  const int per_tile = (rows_per_tile * (DC / 4) + 255) / 256;
-  const int bt = blockIdx.x / per_tile;
+  constexpr int BLOCKS = kBwdRows * (DC / 4) / 256;   // of a tile's gradient
+  int n = blockIdx.x / BLOCKS;
+  const int i = (blockIdx.x - n * BLOCKS) * 256 + threadIdx.x;
+  const int row = i / (DC / 4), col = (i % (DC / 4)) * 4;
+  const int from_keys = p.keys.parts > 1 ? 8 * (p.keys.per_xcd - p.keys.whole) * 2 : 0;
+  const bool keys = n < from_keys;
+  const BwdRole& R = keys ? p.keys : p.queries;
+  const int tensors = keys ? 2 : 1;
+  if (!keys) n -= from_keys;
+  const int which = n % tensors, cut = n / tensors;
+  const int xcd = cut / (R.per_xcd - R.whole), t = cut - xcd * (R.per_xcd - R.whole);
+  const int bt = xcd * R.per_xcd + R.whole + t;
+  if (bt >= R.total) return;
   const int bh = bt / R.tiles;
   int tile = bt - bh * R.tiles;
   const int b = bh / p.H, h = bh - b * p.H;
-  const int which = blockIdx.y;
-  const int i = (blockIdx.x - bt * per_tile) * 256 + threadIdx.x;
-  const int row = i / (DC / 4), col = (i % (DC / 4)) * 4;
-  const bool second = KEYS && tile >= p.tiles1;
+  const bool second = keys && tile >= p.tiles1;
   if (second) tile -= p.tiles1;
-  const int rows = KEYS ? (second ? p.Sk2 : p.Sk) : p.Sq;
-  const int own = tile * rows_per_tile + row;
-  if (row >= rows_per_tile || own >= rows || col >= p.D) return;
-  const int tensors = KEYS ? 2 : 1;
-  const float* src = R.partial + ((int64_t)bt * R.parts * tensors + which) * rows_per_tile * DC + (int64_t)row * DC + col;
+  const int rows = keys ? (second ? p.Sk2 : p.Sk) : p.Sq;
+  const int own = tile * kBwdRows + row;
+  if (own >= rows || col >= p.D) return;
+  const float* src = R.partial + ((int64_t)cut * R.parts * tensors + which) * kBwdRows * DC + (int64_t)row * DC + col;
   f32x4 x = *(const f32x4*)src;
-  for (int n = 1; n < R.parts; n++) x += *(const f32x4*)(src + (int64_t)n * tensors * rows_per_tile * DC);
-  const BwdTensor& O = KEYS ? (which ? (second ? p.dv2 : p.dv) : (second ? p.dk2 : p.dk)) : p.dq;
+  for (int k = 1; k < R.parts; k++) x += *(const f32x4*)(src + (int64_t)k * tensors * kBwdRows * DC);
+  const BwdTensor& O = keys ? (which ? (second ? p.dv2 : p.dv) : (second ? p.dk2 : p.dk)) : p.dq;
   *(vec4*)((T*)O.p + b * O.b + h * O.h + (int64_t)own * O.s + col) = __builtin_convertvector(x, vec4);
+}
+
+template <typename T, int DC>
+hipError_t launch_bwd_fold(const AttnBwdParams& p, hipStream_t stream) {
+  const int tiles = (p.keys.parts > 1 ? 8 * (p.keys.per_xcd - p.keys.whole) * 2 : 0) + (p.queries.parts > 1 ? 8 * (p.queries.per_xcd - p.queries.whole) : 0);
+  if (tiles) hipLaunchKernelGGL((bwd_fold_kernel<T, DC>), dim3((unsigned)tiles * (kBwdRows * (DC / 4) / 256)), dim3(256), 0, stream, p);
+  return hipGetLastError();
 }
 
 }  // namespace

@@ -18,49 +18,121 @@ using xdit::api_fail;
 
 int64_t align256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
-// Cuts the streamed steps of every row tile into parts so that the units fill the compute units.  A unit costs its steps and about
-// two more (operands, first tile, results); a call in parts also writes and reads fp32 partial results, `fold` steps' time a unit for a
-// compute unit, and has one launch more.  The cheapest number of parts, at most four units per compute unit.
-void plan_role(xdit::BwdRole& r, int64_t bh, int cus, double fold) {
-  const int64_t base = bh * r.tiles;
-  double best = -1;
-  for (int parts = 1; parts <= r.steps && parts <= 64 && (parts == 1 || base * parts <= 4 * (int64_t)cus); parts++) {
-    const int len = (r.steps + parts - 1) / parts;
-    const int n = (r.steps + len - 1) / len;
-    if (n != parts) continue;
-    const double rounds = (double)((base * n + cus - 1) / cus);
-    const double cost = rounds * (len + 2.0) + (n > 1 ? rounds * fold + 1.0 : 0.0);
-    if (best < 0 || cost < best) { best = cost; r.parts = n; r.len = len; }
+// A compute unit's workgroups over time: how many of an XCD's places become free when.  Units are dealt out in the order of the launch,
+// each to the place that is free first, as the hardware does it.
+struct Places {
+  struct Group { double time; int64_t n; } g[8];
+  int used;
+  explicit Places(int64_t places) : used(1) { g[0] = {0.0, places}; }
+  void run(int64_t units, double each) {
+    int64_t all = 0;
+    for (int i = 0; i < used; i++) all += g[i].n;
+    if (units > 4 * all) {   // whole rounds shift every place alike
+      const int64_t rounds = (units - 3 * all) / all;
+      for (int i = 0; i < used; i++) g[i].time += rounds * each;
+      units -= rounds * all;
+    }
+    while (units > 0) {
+      const Group first = g[0];   // kept in order of time
+      const int64_t n = first.n < units ? first.n : units;
+      units -= n;
+      if (n < first.n) g[0].n -= n;
+      else std::copy(g + 1, g + used--, g);
+      int at = 0;
+      while (at < used && g[at].time < first.time + each) at++;
+      if (at < used && g[at].time < first.time + each + 1e-9) { g[at].n += n; continue; }
+      if (used == 8) { g[7].n += n; continue; }   // (an estimate: the latest of them takes it)
+      std::copy_backward(g + at, g + used, g + used + 1);
+      g[at] = {first.time + each, n};
+      used++;
+    }
   }
+  double end() const { return g[used - 1].time; }
+};
+
+// Microseconds of a launch's roles, from the time of a step (64 streamed rows; fp32: 32) of a unit beside others, measured at D 128 / 64 / fp32, plus two steps for
+// its operands and results; partial results are written and read at 4 TB/s, by a launch that takes 4 us.
+struct StepCost { double keys, queries; };
+
+double launch_us(const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t places, const StepCost& c, double part_us) {
+  Places p(places);
+  double us = 0.0;
+  const struct { const xdit::BwdRole& r; double step; double tensors; } roles[2] = {{k, c.keys, 2.0}, {q, c.queries, 1.0}};
+  for (const auto& role : roles) {
+    const xdit::BwdRole& r = role.r;
+    if (r.total == 0) continue;
+    if (r.whole) p.run(r.whole, (r.steps + 2) * role.step);
+    if (r.per_xcd > r.whole) p.run((int64_t)(r.per_xcd - r.whole) * r.parts, (r.len + 2) * role.step);
+    if (r.parts > 1) us += 8.0 * (r.per_xcd - r.whole) * r.parts * role.tensors * part_us;
+  }
+  return p.end() + us + (k.parts > 1 || q.parts > 1 ? 4.0 : 0.0);
+}
+
+void set_parts(xdit::BwdRole& r, int whole, int parts) {
+  r.whole = whole < r.per_xcd ? whole : r.per_xcd;
+  r.len = (r.steps + parts - 1) / parts;
+  r.parts = r.whole == r.per_xcd ? 1 : (r.steps + r.len - 1) / r.len;
+  if (r.parts == 1) { r.whole = r.per_xcd; r.len = r.steps; }
+  r.units = r.total ? r.whole + (r.per_xcd - r.whole) * r.parts : 0;
+}
+
+// Which tiles of a role are cut into parts, and into how many: of none, all, and the last `n` of every XCD's tiles the way with the shortest estimate of the
+// launch.  `last`: the role's units are the last of the launch.
+void plan_role(xdit::BwdRole& r, const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t places, const StepCost& c, double part_us, bool last) {
+  static const int kParts[] = {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  set_parts(r, r.per_xcd, 1);
+  double best = launch_us(k, q, places, c, part_us);
+  int best_whole = r.per_xcd, best_parts = 1;
+  for (int parts : kParts) {
+    if (parts > r.steps) break;
+    for (int64_t cut = r.per_xcd, round = 0; cut > 0 && round < 4; round++) {
+      if (cut * parts <= 4 * places) {
+        set_parts(r, r.per_xcd - (int)cut, parts);
+        const double us = launch_us(k, q, places, c, part_us);
+        if (us < best * 0.99) { best = us; best_whole = r.per_xcd - (int)cut; best_parts = parts; }
+      }
+      if (!last) break;
+      cut = round == 0 ? std::min<int64_t>(cut - 1, places) : cut / 2;
+    }
+  }
+  set_parts(r, best_whole, best_parts);
 }
 
 struct BwdPlan {
-  int waves;
-  int64_t stats, amax, partial;   // bytes
+  int64_t stats, amax, keys, queries;   // bytes
+  int64_t need() const { return stats + amax + keys + queries; }
 };
 
 BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   BwdPlan plan;
   const bool f32 = a->dtype == XDIT_DTYPE_FP32;
-  plan.waves = f32 ? 4 : 8;
-  const int rows = 32 * plan.waves, step = f32 ? 32 : 64;
+  const int rows = xdit::kBwdRows, step = f32 ? 32 : 64;
   const int dc = (a->D + 31) / 32 * 32;
   const int64_t bh = (int64_t)a->B * a->H;
-  const int cus = xdit::resident_cus(a->cu_count);
+  const int per_cu = f32 ? 1 : a->D <= 64 ? 3 : 2;   // workgroups on a compute unit
+  const int64_t places = (int64_t)((xdit::resident_cus(a->cu_count) + 7) / 8) * per_cu;
   p.tiles1 = (int)((a->Sk + rows - 1) / rows);
   p.keys.tiles = p.tiles1 + (int)((a->Sk2 + rows - 1) / rows);
   p.keys.steps = (int)((a->Sq + step - 1) / step);
   p.queries.tiles = (int)((a->Sq + rows - 1) / rows);
   p.step1 = (int)((a->Sk + step - 1) / step);
   p.queries.steps = p.step1 + (int)((a->Sk2 + step - 1) / step);
-  plan_role(p.keys, bh, cus, 4.0);
-  plan_role(p.queries, bh, cus, 2.0);
+  p.keys.total = a->dk != nullptr ? (int)(bh * p.keys.tiles) : 0;
+  p.queries.total = a->dq != nullptr ? (int)(bh * p.queries.tiles) : 0;
+  for (xdit::BwdRole* r : {&p.keys, &p.queries}) {
+    r->per_xcd = (r->total + 7) / 8;
+    set_parts(*r, r->per_xcd, 1);
+  }
+  const StepCost cost = f32 ? StepCost{3.5, 2.8} : a->D <= 64 ? StepCost{2.46, 1.9} : StepCost{3.3, 2.5};
+  const double part_us = 2.0 * rows * dc * 4 / 4e6;
+  plan_role(p.keys, p.keys, p.queries, places, cost, part_us, p.queries.total == 0);
+  plan_role(p.queries, p.keys, p.queries, places, cost, part_us, true);
   p.sq_pad = (int)((a->Sq + xdit::kBwdStatRows - 1) / xdit::kBwdStatRows * xdit::kBwdStatRows);
   plan.stats = align256(bh * 2 * p.sq_pad * 4);
   plan.amax = a->dtype == XDIT_DTYPE_FP16 ? align256(bh * (p.sq_pad / xdit::kBwdStatRows) * 4) : 0;
-  const int64_t pk = a->dk != nullptr && p.keys.parts > 1 ? bh * p.keys.tiles * p.keys.parts * 2 * rows * dc * 4 : 0;
-  const int64_t pq = a->dq != nullptr && p.queries.parts > 1 ? bh * p.queries.tiles * p.queries.parts * rows * dc * 4 : 0;
-  plan.partial = pk > pq ? pk : pq;   // the roles run one after the other
+  auto partial = [&](const xdit::BwdRole& r, int tensors) { return r.parts > 1 ? 8 * (int64_t)(r.per_xcd - r.whole) * r.parts * tensors * rows * dc * 4 : 0; };
+  plan.keys = partial(p.keys, 2);
+  plan.queries = partial(p.queries, 1);
   return plan;
 }
 
@@ -264,7 +336,7 @@ int64_t xdit_attn_bwd_workspace_bytes(const xdit_attn_bwd_args* a) {
   xdit::AttnBwdParams p;
   std::memset(&p, 0, sizeof(p));
   const BwdPlan plan = plan_bwd(a, p);
-  return plan.stats + plan.amax + plan.partial;
+  return plan.need();
 }
 
 int xdit_attn_bwd(const xdit_attn_bwd_args* a) {
@@ -299,7 +371,7 @@ int xdit_attn_bwd(const xdit_attn_bwd_args* a) {
   xdit::AttnBwdParams p;
   std::memset(&p, 0, sizeof(p));
   const BwdPlan plan = plan_bwd(a, p);
-  const int64_t need = plan.stats + plan.amax + plan.partial;
+  const int64_t need = plan.need();
   if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) || a->workspace_bytes < need)
     return api_fail(XDIT_ERR_INVALID_ARG, "workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
   p.q = tensor(a->q, a->q_stride);
@@ -326,10 +398,11 @@ int xdit_attn_bwd(const xdit_attn_bwd_args* a) {
   unsigned char* ws = (unsigned char*)a->workspace;
   p.stats = (float*)ws;
   if (plan.amax) p.amax = (float*)(ws + plan.stats);
-  p.keys.partial = p.queries.partial = (float*)(ws + plan.stats + plan.amax);
+  p.keys.partial = (float*)(ws + plan.stats + plan.amax);
+  p.queries.partial = (float*)(ws + plan.stats + plan.amax + plan.keys);
   hipStream_t stream = (hipStream_t)a->stream;
   const hipError_t e = a->dtype == XDIT_DTYPE_FP32 ? xdit::launch_attn_bwd_f32(p, stream)
-                                                   : xdit::launch_attn_bwd_16(p, a->dtype == XDIT_DTYPE_FP16, plan.waves, stream);
+                                                   : xdit::launch_attn_bwd_16(p, a->dtype == XDIT_DTYPE_FP16, stream);
   if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "attention backward launch failed: %s", hipGetErrorString(e));
   return XDIT_OK;
 }
