@@ -483,7 +483,7 @@ int xdit_grad_norm(const xdit_grad_norm_args* args);
 int64_t xdit_grad_norm_workspace_bytes(const xdit_grad_norm_args* args);  /* from count and numel */
 
 /*
- * Clipping by a norm that is in device memory (of these gradients, or of those of every rank):
+ * Clipping by the gradients' own norm, or by one that is in device memory (e.g. of those of every rank):
  *     dst = src * min(1, max_norm / (norm + 1e-6))
  * in fp32, rounded once.  dst may be src itself; otherwise no dst may overlap another dst or a src.  Where the factor is 1 a dst
  * that is its src is left as it is.  The tables are HOST arrays, read before the call returns.
@@ -497,7 +497,12 @@ typedef struct {
   const int64_t* numel;
   const int32_t* src_dtype;    /* bf16, fp16 or fp32 */
   const int32_t* dst_dtype;
-  const float* norm;           /* device: one fp32 */
+  const float* norm;           /* device: one fp32; NULL: the norm of src, as xdit_grad_norm computes it */
+  float* norm_out;             /* device: one fp32, receives the norm where `norm` is NULL */
+  int32_t kind;                /* xdit_grad_norm_kind of that norm */
+  int32_t reserved0;
+  void* workspace;             /* for that norm, of the size that xdit_grad_norm_workspace_bytes gives for src */
+  int64_t workspace_bytes;
   void* stream;
 } xdit_clip_grads_args;
 

@@ -152,7 +152,9 @@ def test_results_that_overlap(src, dst, dtypes):
 
 @pytest.mark.parametrize("kw,needle", [(dict(struct_size=4), "struct_size"), (dict(count=-1), "count"), (dict(max_norm=-1.0), "max_norm"),
                                        (dict(max_norm=float("nan")), "max_norm"), (dict(max_norm=float("inf")), "max_norm"), (dict(norm=None), "norm"),
-                                       (dict(src=None), "table"), (dict(dst=None), "table"), (dict(dst_dtype=None), "table")])
+                                       (dict(norm=P + 2), "norm"), (dict(norm=None, norm_out=P + 2), "norm"), (dict(norm=None, norm_out=P, kind=3), "unknown norm"),
+                                       (dict(norm=None, norm_out=P, kind=2), "workspace"), (dict(norm=None, norm_out=P, kind=2, workspace=P + 4, workspace_bytes=64), "workspace"),
+                                       (dict(norm=None, norm_out=P, kind=2, workspace=P, workspace_bytes=4), "workspace"), (dict(src=None), "table"), (dict(dst=None), "table"), (dict(dst_dtype=None), "table")])
 def test_clip_refusals(kw, needle):
     t = Table([(P, 10)])
     refused(_lib.lib().xdit_clip_grads, clip_args(t, t, **kw), BAD, needle)

@@ -268,7 +268,9 @@ class GradNormArgs(ctypes.Structure):
 
 class ClipGradsArgs(ctypes.Structure):
     _fields_ = ([("struct_size", ctypes.c_uint32), ("max_norm", ctypes.c_float), ("count", ctypes.c_int64)]
-                + [(n, ctypes.c_void_p) for n in ("src", "dst", "numel", "src_dtype", "dst_dtype", "norm", "stream")])
+                + [(n, ctypes.c_void_p) for n in ("src", "dst", "numel", "src_dtype", "dst_dtype", "norm", "norm_out")]
+                + [("kind", ctypes.c_int32), ("reserved0", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+                   ("stream", ctypes.c_void_p)])
 
 
 GRADNORM_MAX, GRADNORM_L1, GRADNORM_L2 = 0, 1, 2

@@ -233,10 +233,11 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
       acc_f[db][e] = 0.f;
       if (KEYS) acc_g[KEYS ? db : 0][e] = 0.f;
     }
+  issue(first, 0);
+  // The compiler accounts for the loads of the owned rows here: any wait for them inside the loop would be one for the tile loads too.
 #pragma unroll
   for (int ks = 0; ks < KSTEPS; ks++) asm volatile("" : "+v"(f[ks]), "+v"(g[ks]));
 
-  issue(first, 0);
   for (int t = first; t < last; t++) {
     const unsigned bo = ((t - first) & 1) * G::BUF_BYTES;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

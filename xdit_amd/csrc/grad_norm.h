@@ -22,12 +22,17 @@ struct NormParams {
   double* partial;     // one per workgroup, from this launch's first on
 };
 
+constexpr int kClipPartials = 1024;  // partial sums that the workgroups of a clipping launch add up by themselves
+
 struct ClipParams {
   GradTable<kClipTensors> t;
   void* dst[kClipTensors];
   int chunk;
   float max_norm;
-  const float* norm;
+  const float* norm;      // given, or written by an earlier launch; nullptr: of `partial`
+  const double* partial;  // at most kClipPartials partial sums
+  int partials, kind;
+  float* norm_out;        // receives the norm of `partial` (nullptr: another launch writes it)
 };
 
 hipError_t launch_grad_norm(const NormParams& p, int dtype, unsigned workgroups, hipStream_t stream);

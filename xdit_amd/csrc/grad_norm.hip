@@ -82,17 +82,42 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const NormParams p) {
   if (threadIdx.x == 0) p.partial[blockIdx.x] = v;
 }
 
+// The norm of n partial values, for thread 0 of 256; in the same order wherever it is called.
 template <int KIND>
-__global__ __launch_bounds__(1024) void grad_norm_total_kernel(const double* partial, int64_t n, float* norm) {
+__device__ __forceinline__ float norm_of(const double* partial, int64_t n) {
   double v = 0.;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) v = norm_join<KIND>(v, partial[i]);
-  v = workgroup_join<KIND, 16>(v);
-  if (threadIdx.x == 0) *norm = (float)(KIND == 2 ? __builtin_sqrt(v) : v);
+  for (int64_t i = threadIdx.x; i < n; i += 256) v = norm_join<KIND>(v, partial[i]);
+  v = workgroup_join<KIND, 4>(v);
+  return (float)(KIND == 2 ? __builtin_sqrt(v) : v);
+}
+__device__ __forceinline__ float norm_of(const double* partial, int64_t n, int kind) {
+  return kind == 0 ? norm_of<0>(partial, n) : kind == 1 ? norm_of<1>(partial, n) : norm_of<2>(partial, n);
 }
 
+__global__ __launch_bounds__(256) void grad_norm_total_kernel(const double* partial, int64_t n, int kind, float* norm) {
+  const float v = norm_of(partial, n, kind);
+  if (threadIdx.x == 0) *norm = v;
+}
+
+// A list of few chunks saves the launch between the norm and this one: every workgroup adds the partial sums up (84 tensors of a model's
+// gains: 23.8 us a call with a launch of its own for the sum and a C call of its own for the norm, 17.3 with neither).  Taking the chunks from the last to
+// the first, so that what the norm read last might still be in the memory-side cache, changed nothing (1097 us for 2 GB).
 template <typename S, typename D>
 __global__ __launch_bounds__(256) void grad_clip_kernel(const ClipParams p) {
-  float factor = p.max_norm / (*p.norm + 1e-6f);
+  float norm;
+  if (p.norm != nullptr) {
+    norm = *p.norm;
+  } else {
+    __shared__ float total;
+    const float v = norm_of(p.partial, p.partials, p.kind);
+    if (threadIdx.x == 0) {
+      total = v;
+      if (p.norm_out != nullptr && blockIdx.x == 0) *p.norm_out = v;
+    }
+    __syncthreads();
+    norm = total;
+  }
+  float factor = p.max_norm / (norm + 1e-6f);
   if (factor > 1.f) factor = 1.f;   // a norm that is not a number stays one
   const int which = tensor_of(p.t, blockIdx.x);
   const S* src = (const S*)p.t.src[which];
@@ -161,9 +186,7 @@ hipError_t launch_grad_norm(const NormParams& p, int dtype, unsigned workgroups,
 }
 
 hipError_t launch_grad_norm_total(const double* partial, int64_t n, int kind, float* norm, hipStream_t stream) {
-  if (kind == 0) hipLaunchKernelGGL((grad_norm_total_kernel<0>), dim3(1), dim3(1024), 0, stream, partial, n, norm);
-  else if (kind == 1) hipLaunchKernelGGL((grad_norm_total_kernel<1>), dim3(1), dim3(1024), 0, stream, partial, n, norm);
-  else hipLaunchKernelGGL((grad_norm_total_kernel<2>), dim3(1), dim3(1024), 0, stream, partial, n, norm);
+  hipLaunchKernelGGL(grad_norm_total_kernel, dim3(1), dim3(256), 0, stream, partial, n, kind, norm);
   return hipGetLastError();
 }
 

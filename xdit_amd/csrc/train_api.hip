@@ -5,6 +5,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <cstdio>
+#include <cstdlib>
 #include <vector>
 
 #include "api_error.h"
@@ -50,20 +52,26 @@ struct Places {
   double end() const { return g[used - 1].time; }
 };
 
-// Microseconds of a launch's roles, from the time of a step (64 streamed rows; fp32: 32) of a unit beside others, measured at D 128 / 64 / fp32, plus two steps for
-// its operands and results; partial results are written and read at 4 TB/s, by a launch that takes 4 us.
-struct StepCost { double keys, queries; };
+// Microseconds that a launch takes.  A unit's step (64 streamed rows; fp32: 32) takes `shared` beside the others that a compute unit holds and `alone`
+// where no compute unit has more than one; `fixed` are its operands, first tile and results.  Partial results are read back at 5 TB/s by a launch of 4 us
+// (they are written while other units compute).
+struct StepCost {
+  double alone[2], shared[2];   // keys, queries
+  double fixed[2];
+  double part;                  // of a tensor's partial tile
+};
 
-double launch_us(const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t places, const StepCost& c, double part_us) {
-  Places p(places);
+double launch_us(const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t cus, int per_cu, const StepCost& c) {
+  const bool alone = k.units + q.units <= cus;
+  Places p(cus * per_cu);
   double us = 0.0;
-  const struct { const xdit::BwdRole& r; double step; double tensors; } roles[2] = {{k, c.keys, 2.0}, {q, c.queries, 1.0}};
-  for (const auto& role : roles) {
-    const xdit::BwdRole& r = role.r;
+  for (int i = 0; i < 2; i++) {
+    const xdit::BwdRole& r = i ? q : k;
+    const double step = (alone ? c.alone : c.shared)[i];
     if (r.total == 0) continue;
-    if (r.whole) p.run(r.whole, (r.steps + 2) * role.step);
-    if (r.per_xcd > r.whole) p.run((int64_t)(r.per_xcd - r.whole) * r.parts, (r.len + 2) * role.step);
-    if (r.parts > 1) us += 8.0 * (r.per_xcd - r.whole) * r.parts * role.tensors * part_us;
+    if (r.whole) p.run(r.whole, r.steps * step + c.fixed[i]);
+    if (r.per_xcd > r.whole) p.run((int64_t)(r.per_xcd - r.whole) * r.parts, r.len * step + c.fixed[i]);
+    if (r.parts > 1) us += 8.0 * (r.per_xcd - r.whole) * r.parts * (2 - i) * c.part;
   }
   return p.end() + us + (k.parts > 1 || q.parts > 1 ? 4.0 : 0.0);
 }
@@ -76,26 +84,46 @@ void set_parts(xdit::BwdRole& r, int whole, int parts) {
   r.units = r.total ? r.whole + (r.per_xcd - r.whole) * r.parts : 0;
 }
 
-// Which tiles of a role are cut into parts, and into how many: of none, all, and the last `n` of every XCD's tiles the way with the shortest estimate of the
-// launch.  `last`: the role's units are the last of the launch.
-void plan_role(xdit::BwdRole& r, const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t places, const StepCost& c, double part_us, bool last) {
-  static const int kParts[] = {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
-  set_parts(r, r.per_xcd, 1);
-  double best = launch_us(k, q, places, c, part_us);
-  int best_whole = r.per_xcd, best_parts = 1;
+constexpr int kParts[] = {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+
+// Which tiles of a role are cut into parts, and into how many: all of them, or (`last`: the role's units are the last of the launch) the last ones of
+// every XCD's tiles; kept where the estimate of the launch gets shorter by it.
+void plan_role(xdit::BwdRole& r, const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t cus, int per_cu, const StepCost& c, bool last) {
+  if (r.total == 0) return;
+  xdit::BwdRole best = r;
+  double best_us = launch_us(k, q, cus, per_cu, c);
   for (int parts : kParts) {
     if (parts > r.steps) break;
-    for (int64_t cut = r.per_xcd, round = 0; cut > 0 && round < 4; round++) {
-      if (cut * parts <= 4 * places) {
+    int64_t cut = r.per_xcd;
+    for (int round = 0; cut > 0 && round < (last ? 4 : 1); round++) {
+      if (cut * parts <= 4 * cus * per_cu) {
         set_parts(r, r.per_xcd - (int)cut, parts);
-        const double us = launch_us(k, q, places, c, part_us);
-        if (us < best * 0.99) { best = us; best_whole = r.per_xcd - (int)cut; best_parts = parts; }
+        const double us = launch_us(k, q, cus, per_cu, c);
+        if (us < best_us * 0.99) { best_us = us; best = r; }
       }
-      if (!last) break;
-      cut = round == 0 ? std::min<int64_t>(cut - 1, places) : cut / 2;
+      cut = round == 0 ? std::min<int64_t>(cut - 1, cus * per_cu) : cut / 2;
     }
   }
-  set_parts(r, best_whole, best_parts);
+  r = best;
+}
+
+void plan_roles(xdit::AttnBwdParams& p, int64_t cus, int per_cu, const StepCost& c) {
+  xdit::BwdRole &k = p.keys, &q = p.queries;
+  if (k.total && q.total && k.units + q.units <= cus * per_cu) {   // few tiles: the roles run side by side, so that both have to be cut for either to matter
+    double best_us = launch_us(k, q, cus, per_cu, c);
+    xdit::BwdRole best_k = k, best_q = q;
+    for (int parts : kParts) {
+      if (parts > k.steps && parts > q.steps) break;
+      set_parts(k, 0, std::min(parts, k.steps));
+      set_parts(q, 0, std::min(parts, q.steps));
+      const double us = launch_us(k, q, cus, per_cu, c);
+      if (us < best_us * 0.99) { best_us = us; best_k = k; best_q = q; }
+    }
+    k = best_k;
+    q = best_q;
+  }
+  plan_role(k, k, q, cus, per_cu, c, q.total == 0);
+  plan_role(q, k, q, cus, per_cu, c, true);
 }
 
 struct BwdPlan {
@@ -110,7 +138,7 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   const int dc = (a->D + 31) / 32 * 32;
   const int64_t bh = (int64_t)a->B * a->H;
   const int per_cu = f32 ? 1 : a->D <= 64 ? 3 : 2;   // workgroups on a compute unit
-  const int64_t places = (int64_t)((xdit::resident_cus(a->cu_count) + 7) / 8) * per_cu;
+  const int64_t cus = (xdit::resident_cus(a->cu_count) + 7) / 8;   // of an XCD
   p.tiles1 = (int)((a->Sk + rows - 1) / rows);
   p.keys.tiles = p.tiles1 + (int)((a->Sk2 + rows - 1) / rows);
   p.keys.steps = (int)((a->Sq + step - 1) / step);
@@ -123,10 +151,13 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
     r->per_xcd = (r->total + 7) / 8;
     set_parts(*r, r->per_xcd, 1);
   }
-  const StepCost cost = f32 ? StepCost{3.5, 2.8} : a->D <= 64 ? StepCost{2.46, 1.9} : StepCost{3.3, 2.5};
-  const double part_us = 2.0 * rows * dc * 4 / 4e6;
-  plan_role(p.keys, p.keys, p.queries, places, cost, part_us, p.queries.total == 0);
-  plan_role(p.queries, p.keys, p.queries, places, cost, part_us, true);
+  // measured: 8 and 16 heads of 16384 rows on 4096 and of 4096 on 16384, 3 of 1536 on 1536
+  StepCost cost = f32 ? StepCost{{3.5, 2.8}, {3.5, 2.8}, {8.0, 6.0}, 0.0} : a->D <= 64 ? StepCost{{1.42, 1.2}, {2.99, 2.35}, {6.0, 5.0}, 0.0}
+                                                                              : StepCost{{2.07, 1.77}, {3.56, 2.8}, {7.0, 5.5}, 0.0};
+  cost.part = rows * dc * 4 / 5e6;
+  plan_roles(p, cus, per_cu, cost);
+  if (getenv("XK")) { int w, n; sscanf(getenv("XK"), "%d,%d", &w, &n); set_parts(p.keys, w, n); }
+  if (getenv("XQ")) { int w, n; sscanf(getenv("XQ"), "%d,%d", &w, &n); set_parts(p.queries, w, n); }
   p.sq_pad = (int)((a->Sq + xdit::kBwdStatRows - 1) / xdit::kBwdStatRows * xdit::kBwdStatRows);
   plan.stats = align256(bh * 2 * p.sq_pad * 4);
   plan.amax = a->dtype == XDIT_DTYPE_FP16 ? align256(bh * (p.sq_pad / xdit::kBwdStatRows) * 4) : 0;
@@ -206,6 +237,52 @@ int64_t chunk_elements(int64_t count, const int64_t* numel) {
 }
 int64_t chunks_of(int64_t numel, int64_t chunk) { return numel == 0 ? 0 : (numel + 7 + chunk - 1) / chunk; }   // up to 7 elements before its aligned start
 
+// The launches that leave a partial value of every chunk; their count, or a negative status.
+int64_t launch_partials(int64_t count, const void* const* data, const int64_t* numel, const int32_t* dtypes, int kind, double* partial, hipStream_t stream) {
+  const int64_t chunk = chunk_elements(count, numel);
+  const double* const start = partial;
+  xdit::NormParams p;
+  p.chunk = (int)chunk;
+  p.kind = kind;
+  for (int dtype = XDIT_DTYPE_BF16; dtype <= XDIT_DTYPE_FP32; dtype++) {   // a launch holds tensors of one dtype
+    int n = 0;
+    int64_t chunks = 0;
+    for (int64_t i = 0; i <= count; i++) {
+      const bool takes = i < count && dtypes[i] == dtype && numel[i] != 0;
+      const int64_t more = takes ? chunks_of(numel[i], chunk) : 0;
+      if (n && (i == count || (takes && (n == xdit::kNormTensors || chunks + more > (1 << 30))))) {
+        std::fill(p.t.first + n, p.t.first + xdit::kNormTensors, 0xffffffffu);
+        p.partial = partial;
+        const hipError_t e = xdit::launch_grad_norm(p, dtype, (unsigned)chunks, stream);
+        if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "gradient norm launch failed: %s", hipGetErrorString(e));
+        partial += chunks;
+        n = 0;
+        chunks = 0;
+      }
+      if (takes) {
+        p.t.first[n] = (uint32_t)chunks;
+        p.t.numel[n] = numel[i];
+        p.t.src[n++] = data[i];
+        chunks += more;
+      }
+    }
+  }
+  return partial - start;
+}
+
+int64_t partials_of(int64_t count, const int64_t* numel) {
+  const int64_t chunk = chunk_elements(count, numel);
+  int64_t n = 0;
+  for (int64_t i = 0; i < count; i++) n += chunks_of(numel[i], chunk);
+  return n;
+}
+
+int check_partials(int64_t n, const void* workspace, int64_t bytes) {
+  if (n && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7u) || bytes < n * (int64_t)sizeof(double)))
+    return api_fail(XDIT_ERR_INVALID_ARG, "workspace must be 8-byte aligned and hold %lld bytes", (long long)(n * sizeof(double)));
+  return 0;
+}
+
 // Whether no destination overlaps another one, or a source other than itself.
 bool destinations_apart(const xdit_clip_grads_args* a) {
   struct Span { uintptr_t begin, end; int64_t i; };
@@ -233,51 +310,19 @@ extern "C" {
 int64_t xdit_grad_norm_workspace_bytes(const xdit_grad_norm_args* a) {
   xdit::api_clear_error();
   if (int rc = check_norm_list(a)) return rc;
-  const int64_t chunk = chunk_elements(a->count, a->numel);
-  int64_t n = 0;
-  for (int64_t i = 0; i < a->count; i++) n += chunks_of(a->numel[i], chunk);
-  return n * (int64_t)sizeof(double);
+  return partials_of(a->count, a->numel) * (int64_t)sizeof(double);
 }
 
 int xdit_grad_norm(const xdit_grad_norm_args* a) {
   xdit::api_clear_error();
   if (int rc = check_norm_list(a)) return rc;
   if (a->norm == nullptr || reinterpret_cast<uintptr_t>(a->norm) & 3u) return api_fail(XDIT_ERR_INVALID_ARG, "norm is NULL or not 4-byte aligned");
-  const int64_t chunk = chunk_elements(a->count, a->numel);
-  int64_t need = 0;
-  for (int64_t i = 0; i < a->count; i++) need += chunks_of(a->numel[i], chunk);
-  if (need && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 7u) || a->workspace_bytes < need * (int64_t)sizeof(double)))
-    return api_fail(XDIT_ERR_INVALID_ARG, "workspace must be 8-byte aligned and hold %lld bytes", (long long)(need * sizeof(double)));
+  if (int rc = check_partials(partials_of(a->count, a->numel), a->workspace, a->workspace_bytes)) return rc;
   hipStream_t stream = (hipStream_t)a->stream;
-  hipError_t e = hipSuccess;
-  double* partial = (double*)a->workspace;
-  xdit::NormParams p;
-  p.chunk = (int)chunk;
-  p.kind = a->kind;
-  for (int dtype = XDIT_DTYPE_BF16; dtype <= XDIT_DTYPE_FP32; dtype++) {   // a launch holds tensors of one dtype
-    int n = 0;
-    int64_t chunks = 0;
-    for (int64_t i = 0; i <= a->count; i++) {
-      const bool takes = i < a->count && a->dtype[i] == dtype && a->numel[i] != 0;
-      const int64_t more = takes ? chunks_of(a->numel[i], chunk) : 0;
-      if (n && (i == a->count || (takes && (n == xdit::kNormTensors || chunks + more > (1 << 30))))) {
-        std::fill(p.t.first + n, p.t.first + xdit::kNormTensors, 0xffffffffu);
-        p.partial = partial;
-        if ((e = xdit::launch_grad_norm(p, dtype, (unsigned)chunks, stream)) != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "gradient norm launch failed: %s", hipGetErrorString(e));
-        partial += chunks;
-        n = 0;
-        chunks = 0;
-      }
-      if (takes) {
-        p.t.first[n] = (uint32_t)chunks;
-        p.t.numel[n] = a->numel[i];
-        p.t.src[n++] = a->data[i];
-        chunks += more;
-      }
-    }
-  }
-  if ((e = xdit::launch_grad_norm_total((const double*)a->workspace, need, a->kind, a->norm, stream)) != hipSuccess)
-    return api_fail(XDIT_ERR_LAUNCH, "gradient norm launch failed: %s", hipGetErrorString(e));
+  const int64_t n = launch_partials(a->count, a->data, a->numel, a->dtype, a->kind, (double*)a->workspace, stream);
+  if (n < 0) return (int)n;
+  const hipError_t e = xdit::launch_grad_norm_total((const double*)a->workspace, n, a->kind, a->norm, stream);
+  if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "gradient norm launch failed: %s", hipGetErrorString(e));
   return XDIT_OK;
 }
 
@@ -288,11 +333,15 @@ int xdit_clip_grads(const xdit_clip_grads_args* a) {
     return api_fail(XDIT_ERR_INVALID_ARG, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(xdit_clip_grads_args));
   if (a->count < 0 || a->count > (1 << 24)) return api_fail(XDIT_ERR_INVALID_ARG, "count %lld must lie between 0 and 2^24", (long long)a->count);
   if (!(a->max_norm >= 0.f) || !std::isfinite(a->max_norm)) return api_fail(XDIT_ERR_INVALID_ARG, "max_norm must be finite and >= 0");
-  if (a->norm == nullptr || reinterpret_cast<uintptr_t>(a->norm) & 3u) return api_fail(XDIT_ERR_INVALID_ARG, "norm is NULL or not 4-byte aligned");
-  if (a->count == 0) return XDIT_OK;
+  const bool given = a->norm != nullptr;
+  if (given ? reinterpret_cast<uintptr_t>(a->norm) & 3u : a->norm_out == nullptr || reinterpret_cast<uintptr_t>(a->norm_out) & 3u)
+    return api_fail(XDIT_ERR_INVALID_ARG, "norm and norm_out are NULL, or one is not 4-byte aligned");
+  if (!given && (a->kind < XDIT_GRADNORM_MAX || a->kind > XDIT_GRADNORM_L2)) return api_fail(XDIT_ERR_INVALID_ARG, "unknown norm %d", a->kind);
   int rc;
-  if ((rc = check_list("gradient", a->count, const_cast<void* const*>(a->src), a->numel, a->src_dtype))) return rc;
-  if ((rc = check_list("result", a->count, a->dst, a->numel, a->dst_dtype))) return rc;
+  if (a->count) {
+    if ((rc = check_list("gradient", a->count, const_cast<void* const*>(a->src), a->numel, a->src_dtype))) return rc;
+    if ((rc = check_list("result", a->count, a->dst, a->numel, a->dst_dtype))) return rc;
+  }
   try {
     if (!destinations_apart(a)) return api_fail(XDIT_ERR_INVALID_ARG, "a result overlaps another one, or a gradient other than its own");
   } catch (const std::bad_alloc&) {
@@ -304,6 +353,24 @@ int xdit_clip_grads(const xdit_clip_grads_args* a) {
   p.chunk = (int)chunk;
   p.max_norm = a->max_norm;
   p.norm = a->norm;
+  p.partial = nullptr;
+  p.norm_out = nullptr;
+  p.partials = 0;
+  p.kind = a->kind;
+  if (!given) {
+    if ((rc = check_partials(partials_of(a->count, a->numel), a->workspace, a->workspace_bytes))) return rc;
+    const int64_t n = launch_partials(a->count, a->src, a->numel, a->src_dtype, a->kind, (double*)a->workspace, stream);
+    if (n < 0) return (int)n;
+    if (n == 0 || n > xdit::kClipPartials) {
+      const hipError_t e = xdit::launch_grad_norm_total((const double*)a->workspace, n, a->kind, a->norm_out, stream);
+      if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "gradient norm launch failed: %s", hipGetErrorString(e));
+      p.norm = a->norm_out;
+    } else {
+      p.partial = (const double*)a->workspace;
+      p.partials = (int)n;
+      p.norm_out = a->norm_out;   // of the first launch
+    }
+  }
   for (int pair = 0; pair < 9; pair++) {   // a launch holds tensors of one dtype and results of one
     const int sd = pair / 3, dd = pair % 3;
     int n = 0;
@@ -315,6 +382,7 @@ int xdit_clip_grads(const xdit_clip_grads_args* a) {
         std::fill(p.t.first + n, p.t.first + xdit::kClipTensors, 0xffffffffu);
         const hipError_t e = xdit::launch_grad_clip(p, sd, dd, (unsigned)chunks, stream);
         if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "clipping launch failed: %s", hipGetErrorString(e));
+        p.norm_out = nullptr;
         n = 0;
         chunks = 0;
       }

@@ -178,28 +178,29 @@ def _kind(norm_type):
         raise ValueError("norm_type must be 2, 1 or inf") from None
 
 
-def _norm(g, kind):
-    a = _lib.GradNormArgs()
-    a.struct_size = ctypes.sizeof(a)
-    a.kind, a.count = kind, g.count
-    a.data, a.numel, a.dtype = ctypes.addressof(g.ptr), ctypes.addressof(g.numel), ctypes.addressof(g.dtype)
-    norm = torch.empty((), dtype=torch.float32, device=g.device)
-    a.norm = norm.data_ptr()
-    L = _lib.lib()
+def _norm_need(g):
+    """Workspace bytes of the norm of a list."""
     if g.need is None:
-        need = L.xdit_grad_norm_workspace_bytes(ctypes.byref(a))
+        a = _lib.GradNormArgs()
+        a.struct_size = ctypes.sizeof(a)
+        a.kind, a.count = _lib.GRADNORM_L2, g.count
+        a.data, a.numel, a.dtype = ctypes.addressof(g.ptr), ctypes.addressof(g.numel), ctypes.addressof(g.dtype)
+        need = _lib.lib().xdit_grad_norm_workspace_bytes(ctypes.byref(a))
         if need < 0:
             _lib.check(need)
         g.need = need
-    a.stream = stream = _stream(g.device)
-    with _stream_lock(g.device, stream), _on_device(g.device):
-        if g.need:
-            scratch = _scratch(g.device, stream, g.need)
-            a.workspace, a.workspace_bytes = scratch.data_ptr(), g.need
-        rc = L.xdit_grad_norm(ctypes.byref(a))
+    return g.need
+
+
+def _launch(entry, a, device, need):
+    a.stream = stream = _stream(device)
+    with _stream_lock(device, stream), _on_device(device):
+        if need:
+            scratch = _scratch(device, stream, need)
+            a.workspace, a.workspace_bytes = scratch.data_ptr(), need
+        rc = entry(ctypes.byref(a))
     if rc != 0:
         _lib.check(rc)
-    return norm
 
 
 def grad_norm(grads, norm_type=2.0):
@@ -208,7 +209,12 @@ def grad_norm(grads, norm_type=2.0):
     grads: contiguous bf16, fp16 or fp32 tensors (any mixture, any sizes) of one device, or a `GradList` of them.  norm_type: 2, 1 or inf.  Sums are in
     64 bits, in a fixed order.  Of gradients that are sharded over ranks the norms can be joined before `clip_grads`."""
     kind = _kind(norm_type)
-    return _norm(_listed(grads), kind)
+    g = _listed(grads)
+    norm = torch.empty((), dtype=torch.float32, device=g.device)
+    a = _lib.GradNormArgs(ctypes.sizeof(_lib.GradNormArgs), kind, g.count, ctypes.addressof(g.ptr), ctypes.addressof(g.numel), ctypes.addressof(g.dtype),
+                          norm.data_ptr())
+    _launch(_lib.lib().xdit_grad_norm, a, g.device, _norm_need(g))
+    return norm
 
 
 def clip_grads(grads, max_norm, norm=None, norm_type=2.0, out=None):
@@ -222,19 +228,14 @@ def clip_grads(grads, max_norm, norm=None, norm_type=2.0, out=None):
     o = g if out is None else _listed(out)
     if o is not g and (o.sizes != g.sizes or o.device != g.device):
         raise ValueError("out must be %d tensors of the gradients' sizes on %s" % (g.count, g.device))
-    max_norm = float(max_norm)
+    need = 0
     if norm is None:
-        norm = _norm(g, kind)
+        need, result = _norm_need(g), torch.empty((), dtype=torch.float32, device=g.device)
     elif not isinstance(norm, torch.Tensor) or norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != g.device:
         raise ValueError("norm must be an fp32 tensor of one element on %s" % g.device)
-    a = _lib.ClipGradsArgs()
-    a.struct_size = ctypes.sizeof(a)
-    a.max_norm, a.count = max_norm, g.count
-    a.src, a.dst, a.numel = ctypes.addressof(g.ptr), ctypes.addressof(o.ptr), ctypes.addressof(g.numel)
-    a.src_dtype, a.dst_dtype = ctypes.addressof(g.dtype), ctypes.addressof(o.dtype)
-    a.norm, a.stream = norm.data_ptr(), _stream(g.device)
-    with _on_device(g.device):
-        rc = _lib.lib().xdit_clip_grads(ctypes.byref(a))
-    if rc != 0:
-        _lib.check(rc)
-    return norm
+    else:
+        result = norm
+    a = _lib.ClipGradsArgs(ctypes.sizeof(_lib.ClipGradsArgs), float(max_norm), g.count, ctypes.addressof(g.ptr), ctypes.addressof(o.ptr),
+                           ctypes.addressof(g.numel), ctypes.addressof(g.dtype), ctypes.addressof(o.dtype), _ptr(norm), result.data_ptr(), kind)
+    _launch(_lib.lib().xdit_clip_grads, a, g.device, need)
+    return result
