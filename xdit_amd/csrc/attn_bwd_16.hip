@@ -52,16 +52,6 @@ template <int D> struct BwdGeom {
   static constexpr int STEP8 = 2 * PITCH;                        // +8 rows where bit 3 of the row is clear
 };
 
-__device__ __forceinline__ void load_lds_4(const void* base, unsigned off, unsigned lds) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dword %1, %2"
-      :
-      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base)
-      : "memory", "m0");
-}
-
 // fp16's numbers end at 2^-24, and P and dS are small.  P is computed times 2^13 (it stays below 2^14), which is free: the exponent gets it.  dS is computed
 // times 2^m, m between 0 and 13 so that 2^m times the largest |dout| of the (batch, head) is below 16 (dS, about
 // 16 sqrt(D) |v| P, is far below 65504 then).  The gradients are multiplied by 2^-13 and 2^-m at the end.

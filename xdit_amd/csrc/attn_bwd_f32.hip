@@ -6,27 +6,34 @@
 // time; contraction over streamed rows takes rows 8*(i/4) + 4*(l/32) + i%4 in step i, which is where accumulator register i of P or dS
 // has them.
 //
-// The instruction takes 64 clocks, so one wavefront per SIMD (four of 32 owned rows, whose operands and accumulators then have
-// 512 registers) keeps the matrix pipe fed; it bounds the kernel.
+// The instruction takes 64 clocks, which bounds the kernel; two workgroups of four wavefronts on a compute unit keep the matrix pipe fed (one at head_dims above 96, whose
+// operands and accumulators take more than 256 registers).
 #include "attn_bwd_rows.h"
 #include "attn_split.h"
+#include "attn_tiles.h"
 
 namespace xdit {
 namespace {
 
 constexpr int kRows32 = 32;   // streamed rows per LDS tile
 
-// KG: groups of 8 columns that hold the tensors' head_dim; DB: blocks of 32 columns of the gradients.
-template <int KG, int DB>
-constexpr int pitch_f32() { return (32 * DB > 8 * KG ? 32 * DB : 8 * KG) + 4; }   // floats; 16 bytes more: rows on other banks
-template <int KG, int DB>
-constexpr int buf_f32() { return 2 * kRows32 * pitch_f32<KG, DB>() + 2 * kRows32; }
+// LDS layout of a streamed tile, filled by 1 KiB pieces (a direct load writes lane i at 16 i) that lie 16 bytes more apart: rows that are read together (one
+// 16-byte column of 16 consecutive rows) sit in different pieces, on other banks.  KG: groups of 8 columns that hold the
+// tensors' head_dim; DB: blocks of 32 columns of the gradients.
+template <int KG, int DB> struct Geom32 {
+  static constexpr int ROW_BYTES = KG <= 8 && DB <= 2 ? 256 : 512;
+  static constexpr int NG = kRows32 * ROW_BYTES / 1024;
+  static constexpr int PITCH = 1024 + 16;
+  static constexpr int TENSOR_BYTES = NG * PITCH;
+  static constexpr int BUF_BYTES = 2 * TENSOR_BYTES + 2 * kRows32 * 4;
+  static constexpr int LANES_PER_ROW = ROW_BYTES / 16;
+  static __device__ __forceinline__ int at(int r) { return r % NG * PITCH + r / NG * ROW_BYTES; }   // byte offset of a row
+};
 
 template <int KG, int DB, bool KEYS>
-__device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, int n, float* lds32) {
-  constexpr int ROWS = kBwdRows, PITCH = pitch_f32<KG, DB>(), BUF = buf_f32<KG, DB>(), THREADS = 64 * kBwdWaves;
-  constexpr int CHUNKS = kRows32 * KG * 2;                      // 16-byte pieces of a tensor's tile
-  constexpr int LOADS = (CHUNKS + THREADS - 1) / THREADS;
+__device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, int n, unsigned char* smem) {
+  typedef Geom32<KG, DB> G;
+  constexpr int ROWS = kBwdRows;
 
   const BwdRole& R = KEYS ? p.keys : p.queries;
   BwdUnit unit;
@@ -37,7 +44,7 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
   const int first = unit.slot < 0 ? 0 : unit.part * R.len;
   const int last = unit.slot < 0 || first + R.len > R.steps ? R.steps : first + R.len;
 
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
   const bool second = KEYS && tile >= p.tiles1;
   if (second) tile -= p.tiles1;
   const BwdTensor& F = KEYS ? (second ? p.k2 : p.k) : p.q;
@@ -65,43 +72,42 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
   if (!KEYS && own < p.sq_pad) { own_lse = stats[own]; own_nd = stats[p.sq_pad + own]; }
 
   // Columns of the LDS tiles that the tensors do not have (never written by the loads): zeros.
-  for (int i = threadIdx.x; i < 2 * BUF; i += THREADS) lds32[i] = 0.f;
-  __syncthreads();
+  XDIT_LDS unsigned char* const tiles = (XDIT_LDS unsigned char*)smem;
+  constexpr int WIDE = (8 * KG > 32 * DB ? 8 * KG : 32 * DB) / 4;   // 16-byte columns that are read
+  if (4 * WIDE > p.D) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const int c0 = p.D / 4, n0 = WIDE - c0;
+    for (int i = threadIdx.x; i < 4 * kRows32 * n0; i += 64 * kBwdWaves) {
+      const int which = i / (kRows32 * n0), j = i % (kRows32 * n0);
+      *(XDIT_LDS f32x4*)(tiles + (which >> 1) * G::BUF_BYTES + (which & 1) * G::TENSOR_BYTES + G::at(j % kRows32) + (c0 + j / kRows32) * 16) = zero;
+    }
+  }
 
-  f32x4 rx[LOADS], ry[LOADS];
-  float rs = 0.f;
-  auto fetch = [&](int t) {
+  const unsigned lds_base = (unsigned)(uintptr_t)tiles;
+  const bool ld_on = (lane % G::LANES_PER_ROW) * 4 < p.D;
+  auto issue = [&](int t, unsigned bo) {
     const bool s2 = !KEYS && t >= p.step1;
     const BwdTensor& X = KEYS ? p.q : s2 ? p.k2 : p.k;
     const BwdTensor& Y = KEYS ? p.dout : s2 ? p.v2 : p.v;
     const int rows = KEYS ? p.Sq : s2 ? p.Sk2 : p.Sk;
     const int row0 = (s2 ? t - p.step1 : t) * kRows32;
-    const float* xb = (const float*)X.p + b * X.b + h * X.h;
-    const float* yb = (const float*)Y.p + b * Y.b + h * Y.h;
+    const int left = rows - row0 < kRows32 ? rows - row0 : kRows32;
+    const float* xb = (const float*)X.p + b * X.b + h * X.h + (int64_t)row0 * X.s;
+    const float* yb = (const float*)Y.p + b * Y.b + h * Y.h + (int64_t)row0 * Y.s;
+    const unsigned xs = (unsigned)X.s * 4, ys = (unsigned)Y.s * 4;
+    if (ld_on) {
 #pragma unroll
-    for (int n = 0; n < LOADS; n++) {
-      const int i = threadIdx.x + n * THREADS;
-      int r = row0 + i / (2 * KG);
-      const int col = i % (2 * KG) * 4;
-      if (i < CHUNKS && col < p.D) {
-        r = r < rows ? r : rows - 1;   // rows past the end re-read the last one
-        rx[n] = *(const f32x4*)(xb + (int64_t)r * X.s + col);
-        ry[n] = *(const f32x4*)(yb + (int64_t)r * Y.s + col);
+      for (int i = 0; i < G::NG / kBwdWaves; i++) {
+        const int piece = wave + i * kBwdWaves;
+        int r = piece + lane / G::LANES_PER_ROW * G::NG;
+        r = r < left ? r : left - 1;   // rows past the end re-read the last one
+        const unsigned col = (lane % G::LANES_PER_ROW) * 16;
+        load_lds_16(xb, __umul24((unsigned)r, xs) + col, lds_base + bo + piece * G::PITCH);
+        load_lds_16(yb, __umul24((unsigned)r, ys) + col, lds_base + bo + G::TENSOR_BYTES + piece * G::PITCH);
       }
     }
-    if (KEYS && threadIdx.x < 2 * kRows32) rs = stats[(threadIdx.x / kRows32) * (int64_t)p.sq_pad + row0 + threadIdx.x % kRows32];
-  };
-  auto put = [&](float* buf) {
-#pragma unroll
-    for (int n = 0; n < LOADS; n++) {
-      const int i = threadIdx.x + n * THREADS;
-      const int r = i / (2 * KG), col = i % (2 * KG) * 4;
-      if (i < CHUNKS && col < p.D) {
-        *(f32x4*)(buf + r * PITCH + col) = rx[n];
-        *(f32x4*)(buf + (kRows32 + r) * PITCH + col) = ry[n];
-      }
-    }
-    if (KEYS && threadIdx.x < 2 * kRows32) buf[2 * kRows32 * PITCH + threadIdx.x] = rs;
+    if (KEYS && wave == 0)   // 32 of lse / ln 2, then 32 of -delta
+      load_lds_4(stats + row0, ((lane >> 5) * p.sq_pad + l32) * 4u, lds_base + bo + 2 * G::TENSOR_BYTES);
   };
 
   f32x16 acc_f[DB], acc_g[KEYS ? DB : 1];
@@ -113,30 +119,34 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
       if (KEYS) acc_g[KEYS ? db : 0][e] = 0.f;
     }
 
-  fetch(first);
-  put(lds32);
+  issue(first, 0);
+  // The compiler accounts for the loads of the owned rows here: any wait for them inside the loop would be one for the tile loads too.
+#pragma unroll
+  for (int j = 0; j < KG; j++) asm volatile("" : "+v"(f[j]), "+v"(g[j]));
+
   for (int t = first; t < last; t++) {
-    float* buf = lds32 + ((t - first) & 1) * BUF;
+    const unsigned bo = ((t - first) & 1) * G::BUF_BYTES;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (t + 1 < last) fetch(t + 1);
+    if (t + 1 < last) issue(t + 1, G::BUF_BYTES - bo);
     int left = kRows32;
     if (!KEYS) {
       const int l = t >= p.step1 ? p.Sk2 - (t - p.step1) * kRows32 : p.Sk - t * kRows32;
       left = l < kRows32 ? l : kRows32;
     }
+    const XDIT_LDS unsigned char* const buf = tiles + bo;
+    const XDIT_LDS float* const st = (const XDIT_LDS float*)(buf + 2 * G::TENSOR_BYTES);
     f32x16 s, dp;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        s[4 * i + e] = 0.f;
-        dp[4 * i + e] = KEYS ? buf[2 * kRows32 * PITCH + kRows32 + 8 * i + 4 * hh + e] : own_nd;
-      }
-    const float* xr = buf + l32 * PITCH + 4 * hh;
+    for (int i = 0; i < 16; i++) {
+      s[i] = 0.f;
+      dp[i] = KEYS ? st[kRows32 + 8 * (i >> 2) + 4 * hh + (i & 3)] : own_nd;
+    }
+    const XDIT_LDS unsigned char* const xr = buf + G::at(l32) + 16 * hh;
 #pragma unroll
     for (int j = 0; j < KG; j++) {
-      const f32x4 x = *(const f32x4*)(xr + 8 * j);
-      const f32x4 y = *(const f32x4*)(xr + kRows32 * PITCH + 8 * j);
+      const f32x4 x = *(const XDIT_LDS f32x4*)(xr + 32 * j);
+      const f32x4 y = *(const XDIT_LDS f32x4*)(xr + G::TENSOR_BYTES + 32 * j);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], f[j][e], s, 0, 0, 0);
@@ -147,22 +157,26 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const int r = 8 * (i >> 2) + 4 * hh + (i & 3);
-      const float l = KEYS ? buf[2 * kRows32 * PITCH + r] : own_lse;
+      const float l = KEYS ? st[r] : own_lse;
       pr[i] = fast_exp2(__builtin_fmaf(s[i], c, -l));
-      if (!KEYS && r >= left) pr[i] = 0.f;
-      ds[i] = pr[i] * dp[i];
     }
-    const float* xc = buf + 4 * hh * PITCH + l32;
+    if (!KEYS && left < kRows32) {   // only a segment's last tile: keys behind its end
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (8 * (i >> 2) + 4 * hh + (i & 3) >= left) pr[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) ds[i] = pr[i] * dp[i];
+    const XDIT_LDS unsigned char* const columns = buf + 4 * hh * G::PITCH + 4 * l32;   // row 4 hh, column l32
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-      const int r = 8 * (i >> 2) + (i & 3);
+      const XDIT_LDS float* const xc = (const XDIT_LDS float*)(columns + G::at(8 * (i >> 2) + (i & 3)));
 #pragma unroll
       for (int db = 0; db < DB; db++) {
-        if constexpr (KEYS) acc_g[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(xc[(kRows32 + r) * PITCH + 32 * db], pr[i], acc_g[db], 0, 0, 0);
-        acc_f[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(xc[r * PITCH + 32 * db], ds[i], acc_f[db], 0, 0, 0);
+        if constexpr (KEYS) acc_g[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(xc[G::TENSOR_BYTES / 4 + 32 * db], pr[i], acc_g[db], 0, 0, 0);
+        acc_f[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(xc[32 * db], ds[i], acc_f[db], 0, 0, 0);
       }
     }
-    if (t + 1 < last) put(lds32 + ((t + 1 - first) & 1) * BUF);   // the buffer of the tile before this one
   }
 
 #pragma unroll
@@ -186,8 +200,8 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
 }
 
 template <int KG, int DB>
-__global__ __launch_bounds__(64 * kBwdWaves, 1) void attn_bwd_f32_kernel(const AttnBwdParams p) {
-  extern __shared__ __attribute__((aligned(16))) float lds32[];
+__global__ __launch_bounds__(64 * kBwdWaves, DB <= 3 ? 2 : 1) void attn_bwd_f32_kernel(const AttnBwdParams p) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds32[];
   const int xcd = blockIdx.x % 8, n = blockIdx.x / 8;   // as in the 16-bit kernel
   if (n < p.keys.units) bwd_role_f32<KG, DB, true>(p, xcd, n, lds32);
   else bwd_role_f32<KG, DB, false>(p, xcd, n - p.keys.units, lds32);
@@ -196,7 +210,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 1) void attn_bwd_f32_kernel(const A
 template <int KG, int DB>
 hipError_t launch_kernels(const AttnBwdParams& p, hipStream_t stream) {
   static std::atomic<bool> lds_ready[kMaxDevices];
-  constexpr int lds = 2 * buf_f32<KG, DB>() * 4;
+  constexpr int lds = 2 * Geom32<KG, DB>::BUF_BYTES;
   const int slot = current_device_slot();
   if (!lds_ready[slot].load(std::memory_order_relaxed)) {
     hipError_t e = hipFuncSetAttribute((const void*)attn_bwd_f32_kernel<KG, DB>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);

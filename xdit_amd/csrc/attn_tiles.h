@@ -62,6 +62,17 @@ __device__ __forceinline__ void load_lds_16(const void* base, unsigned off, unsi
       : "memory", "m0");
 }
 
+// The same of 4 bytes per lane.
+__device__ __forceinline__ void load_lds_4(const void* base, unsigned off, unsigned lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, %2"
+      :
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base)
+      : "memory", "m0");
+}
+
 // Compile-time loop: f(std::integral_constant<int, I>) for I = 0..N-1.
 template <typename F, int... I>
 __device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
