@@ -177,28 +177,55 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
 
   // ---- tile loads ----
   const unsigned lds_base = (unsigned)(uintptr_t)(XDIT_LDS unsigned char*)smem;
+  // Wavefront w loads pieces w, w + 4, ...: piece w + 4 i holds the rows i + ld_row of its lanes.
   const bool ld_on = (lane % G::LANES_PER_ROW) * 8 < p.D;
-  auto issue = [&](int t, unsigned bo) {
+  // (Lane numbers are asked for again where they are needed: two registers more through the loop would spill at head_dim 128.)
+  auto ld_row = [&] { return G::row(wave, lane_now() / G::LANES_PER_ROW); };
+  auto ld_col = [&] { return (unsigned)(lane_now() % G::LANES_PER_ROW) * 16; };
+  const unsigned char* ld_x;   // first rows of the tile to be loaded next
+  const unsigned char* ld_y;
+  const float* ld_stats = stats;
+  unsigned ld_xs, ld_ys, ld_vx, ld_vy;   // row strides, the lane's offsets in bytes
+  int ld_left;                 // rows of the segment from that tile on
+  auto aim = [&](int t) {
     const bool s2 = !KEYS && t >= p.step1;
     const BwdTensor& X = KEYS ? p.q : s2 ? p.k2 : p.k;
     const BwdTensor& Y = KEYS ? p.dout : s2 ? p.v2 : p.v;
-    const int rows = KEYS ? p.Sq : s2 ? p.Sk2 : p.Sk;
     const int row0 = (s2 ? t - p.step1 : t) * kTileRows;
-    const int left = rows - row0 < kTileRows ? rows - row0 : kTileRows;
-    const T* xb = (const T*)X.p + b * X.b + h * X.h + (int64_t)row0 * X.s;
-    const T* yb = (const T*)Y.p + b * Y.b + h * Y.h + (int64_t)row0 * Y.s;
-    const unsigned xs = (unsigned)X.s * 2, ys = (unsigned)Y.s * 2;
+    ld_left = (KEYS ? p.Sq : s2 ? p.Sk2 : p.Sk) - row0;
+    ld_xs = (unsigned)X.s * 2;
+    ld_ys = (unsigned)Y.s * 2;
+    ld_x = (const unsigned char*)((const T*)X.p + b * X.b + h * X.h + (int64_t)row0 * X.s);
+    ld_y = (const unsigned char*)((const T*)Y.p + b * Y.b + h * Y.h + (int64_t)row0 * Y.s);
+    if (KEYS) ld_stats = stats + row0;
+    ld_vx = __umul24((unsigned)ld_row(), ld_xs) + ld_col();
+    ld_vy = __umul24((unsigned)ld_row(), ld_ys) + ld_col();
+  };
+  // Loads that tile and moves on to the one behind it.
+  auto issue = [&](unsigned bo) {
     if (ld_on) {
-      for (int gidx = wave; gidx < G::NG; gidx += NW) {
-        int r = G::row(gidx, lane / G::LANES_PER_ROW);
-        r = r < left ? r : left - 1;   // rows past the end re-read the last one
-        const unsigned col = (lane % G::LANES_PER_ROW) * 16;
-        load_lds_16(xb, __umul24((unsigned)r, xs) + col, lds_base + bo + gidx * G::PITCH);
-        load_lds_16(yb, __umul24((unsigned)r, ys) + col, lds_base + bo + G::TENSOR_BYTES + gidx * G::PITCH);
+      const unsigned dst = lds_base + bo + wave * G::PITCH;
+      if (ld_left >= kTileRows) {
+#pragma unroll
+        for (int i = 0; i < G::NG / NW; i++) {
+          load_lds_16(ld_x + (uint64_t)i * ld_xs, ld_vx, dst + i * NW * G::PITCH);
+          load_lds_16(ld_y + (uint64_t)i * ld_ys, ld_vy, dst + G::TENSOR_BYTES + i * NW * G::PITCH);
+        }
+      } else {   // a segment's last tile: rows past its end re-read the last one
+#pragma unroll
+        for (int i = 0; i < G::NG / NW; i++) {
+          int r = ld_row() + i;
+          r = r < ld_left ? r : ld_left - 1;
+          load_lds_16(ld_x, __umul24((unsigned)r, ld_xs) + ld_col(), dst + i * NW * G::PITCH);
+          load_lds_16(ld_y, __umul24((unsigned)r, ld_ys) + ld_col(), dst + G::TENSOR_BYTES + i * NW * G::PITCH);
+        }
       }
     }
-    if (KEYS && wave < 2)
-      load_lds_4(stats + wave * p.sq_pad + row0, lane * 4, lds_base + bo + 2 * G::TENSOR_BYTES + wave * kTileRows * 4);
+    if (KEYS && wave < 2) load_lds_4(ld_stats + wave * p.sq_pad, lane_now() * 4, lds_base + bo + 2 * G::TENSOR_BYTES + wave * kTileRows * 4);
+    ld_x += (uint64_t)ld_xs * kTileRows;
+    ld_y += (uint64_t)ld_ys * kTileRows;
+    ld_left -= kTileRows;
+    if (KEYS) ld_stats += kTileRows;
   };
   // Columns that the tensors do not have: zeros, once.
   if (DC > p.D) {
@@ -223,7 +250,8 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
       acc_f[db][e] = 0.f;
       if (KEYS) acc_g[KEYS ? db : 0][e] = 0.f;
     }
-  issue(first, 0);
+  aim(first);
+  issue(0);
   // The compiler accounts for the loads of the owned rows here: any wait for them inside the loop would be one for the tile loads too.
 #pragma unroll
   for (int ks = 0; ks < KSTEPS; ks++) asm volatile("" : "+v"(f[ks]), "+v"(g[ks]));
@@ -232,11 +260,10 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
     const unsigned bo = ((t - first) & 1) * G::BUF_BYTES;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (t + 1 < last) issue(t + 1, G::BUF_BYTES - bo);
-    int left = kTileRows;   // keys of the tile that exist
-    if (!KEYS) {
-      const int l = t >= p.step1 ? p.Sk2 - (t - p.step1) * kTileRows : p.Sk - t * kTileRows;
-      left = l < kTileRows ? l : kTileRows;
+    const int left = ld_left + kTileRows;   // rows of the segment from this tile on
+    if (t + 1 < last) {
+      if (!KEYS && t + 1 == p.step1) aim(t + 1);   // the second segment's first tile
+      issue(G::BUF_BYTES - bo);
     }
 #pragma unroll 1
     for (int hb = 0; hb < 2; hb++) {   // 32 streamed rows at a time
