@@ -75,49 +75,60 @@ constexpr int kAhead = 4;  // LDS fragment reads in flight
 constexpr int kBwdStagePitch = 64 * 2 + 8;
 constexpr int kBwdStageBytes = 32 * kBwdStagePitch;
 
-// acc = X_half F^T (contraction over head_dim, KSTEPS steps of 16), acc's initial values given.
-template <typename T, int KSTEPS, int OFF>
-__device__ __forceinline__ void rows_product(f32x16& acc, const typename Mfma16<T>::vec8 (&f)[KSTEPS], unsigned addr) {
-  typename Mfma16<T>::vec8 x[KSTEPS];
-  static_for<(kAhead < KSTEPS ? kAhead : KSTEPS)>([&](auto I) { constexpr int i = I; lds_read_b128<OFF + 32 * i>(x[i], addr); });
-  static_for<KSTEPS>([&](auto I) {
+// S += X_half F^T, then dP += Y_half G^T (contraction over head_dim, KSTEPS steps of 16 each): one sequence of fragment reads, so that
+// the second product does not wait for its first ones.  Y lies Y_OFF bytes behind X.
+template <typename T, int KSTEPS, int Y_OFF>
+__device__ __forceinline__ void rows_products(f32x16& s, f32x16& dp, const typename Mfma16<T>::vec8 (&f)[KSTEPS], const typename Mfma16<T>::vec8 (&g)[KSTEPS], unsigned addr) {
+  constexpr int N = 2 * KSTEPS;
+  typename Mfma16<T>::vec8 x[N];
+  auto read = [&](auto I) {
     constexpr int i = I;
-    constexpr int younger = (i + kAhead <= KSTEPS ? kAhead : KSTEPS - i) - 1;
+    lds_read_b128<(i < KSTEPS ? 32 * i : Y_OFF + 32 * (i - KSTEPS))>(x[i], addr);
+  };
+  static_for<kAhead>([&](auto I) { read(I); });
+  static_for<N>([&](auto I) {
+    constexpr int i = I;
+    constexpr int younger = (i + kAhead <= N ? kAhead : N - i) - 1;
     lds_wait<younger>(x[i]);
-    acc = Mfma16<T>::mma(x[i], f[i], acc);
-    if constexpr (i + kAhead < KSTEPS) lds_read_b128<OFF + 32 * (i + kAhead)>(x[i + kAhead], addr);
+    if constexpr (i < KSTEPS) s = Mfma16<T>::mma(x[i], f[i], s);
+    else dp = Mfma16<T>::mma(x[i], g[i - KSTEPS], dp);
+    if constexpr (i + kAhead < N) read(std::integral_constant<int, i + kAhead>{});
   });
 }
 
-// acc[db] += X_half^T B, contraction over the half's 32 rows; B: two steps of 16.
-template <typename T, int D, int DBLOCKS, int OFF>
-__device__ __forceinline__ void columns_product(f32x16 (&acc)[DBLOCKS], const typename Mfma16<T>::vec8 (&pf)[2], unsigned addr) {
+// Transposed products over the half's 32 rows, a sequence of fragment reads again: G_PRODUCTS: acc_g[db] += Y_half^T P, then acc_f[db] += X_half^T dS (pf, df:
+// two steps of 16 rows).  The first reads are started by `start`, ahead of the arithmetic that makes P and dS.
+template <typename T, int D, int DBLOCKS, bool G_PRODUCTS, int Y_OFF>
+struct ColumnsProducts {
   typedef typename Mfma16<T>::vec8 vec8;
   typedef BwdGeom<D> G;
-  constexpr int NM = 2 * DBLOCKS;
-  constexpr int PD = kAhead / 2 < NM ? kAhead / 2 : NM;   // products whose two reads are in flight
   typedef __attribute__((ext_vector_type(8))) short s16x8;
-  s16x4 v0[NM], v1[NM];
-  static_for<PD>([&](auto I) {
-    constexpr int i = I;
-    constexpr int off = OFF + (i / DBLOCKS) * G::STEP16 + (i % DBLOCKS) * 64;
+  static constexpr int NM = 2 * DBLOCKS, N = G_PRODUCTS ? 2 * NM : NM;
+  static constexpr int PD = kAhead / 2 < N ? kAhead / 2 : N;   // products whose two reads are in flight
+  s16x4 v0[N], v1[N];
+  template <int i> __device__ __forceinline__ void read(unsigned addr) {
+    constexpr int j = G_PRODUCTS && i >= NM ? i - NM : i;
+    constexpr int off = (G_PRODUCTS && i < NM ? Y_OFF : 0) + (j / DBLOCKS) * G::STEP16 + (j % DBLOCKS) * 64;
     lds_read_tr16_b64<off>(v0[i], addr);
     lds_read_tr16_b64<off + G::STEP8>(v1[i], addr);
-  });
-  static_for<NM>([&](auto I) {
-    constexpr int i = I;
-    constexpr int younger = 2 * ((i + PD <= NM ? PD : NM - i) - 1);
-    lds_wait2<younger>(v0[i], v1[i]);
-    const s16x8 vv = __builtin_shufflevector(v0[i], v1[i], 0, 1, 2, 3, 4, 5, 6, 7);
-    acc[i % DBLOCKS] = Mfma16<T>::mma(__builtin_bit_cast(vec8, vv), pf[i / DBLOCKS], acc[i % DBLOCKS]);
-    if constexpr (i + PD < NM) {
-      constexpr int n = i + PD;
-      constexpr int off = OFF + (n / DBLOCKS) * G::STEP16 + (n % DBLOCKS) * 64;
-      lds_read_tr16_b64<off>(v0[n], addr);
-      lds_read_tr16_b64<off + G::STEP8>(v1[n], addr);
-    }
-  });
-}
+  }
+  __device__ __forceinline__ void start(unsigned addr) {
+    static_for<PD>([&](auto I) { this->template read<decltype(I)::value>(addr); });
+  }
+  template <int NG>
+  __device__ __forceinline__ void run(f32x16 (&acc_g)[NG], f32x16 (&acc_f)[DBLOCKS], const vec8 (&pf)[2], const vec8 (&df)[2], unsigned addr) {
+    static_for<N>([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      constexpr int younger = 2 * ((i + PD <= N ? PD : N - i) - 1);
+      lds_wait2<younger>(v0[i], v1[i]);
+      const s16x8 vv = __builtin_shufflevector(v0[i], v1[i], 0, 1, 2, 3, 4, 5, 6, 7);
+      constexpr int j = G_PRODUCTS && i >= NM ? i - NM : i;
+      if constexpr (G_PRODUCTS && i < NM) acc_g[j % DBLOCKS] = Mfma16<T>::mma(__builtin_bit_cast(vec8, vv), pf[j / DBLOCKS], acc_g[j % DBLOCKS]);
+      else acc_f[j % DBLOCKS] = Mfma16<T>::mma(__builtin_bit_cast(vec8, vv), df[j / DBLOCKS], acc_f[j % DBLOCKS]);
+      if constexpr (i + PD < N) this->template read<i + PD>(addr);
+    });
+  }
+};
 
 // One unit of a role.  D: the head_dim of the LDS geometry, DC (a multiple of 32) the computed one; columns between the
 // tensors' head_dim and DC are zeros in F and G and in the LDS tiles.
@@ -269,20 +280,21 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
     for (int hb = 0; hb < 2; hb++) {   // 32 streamed rows at a time
       const unsigned ra = row_addr + bo + hb * G::STEP32, ca = col_addr + bo + hb * G::STEP32;
       f32x16 s, dp;
-#pragma unroll
-      for (int e = 0; e < 16; e++) s[e] = 0.f;
-      rows_product<T, KSTEPS, 0>(s, f, ra);
-      __builtin_amdgcn_sched_barrier(0);
       const XDIT_LDS f32x4* st = (const XDIT_LDS f32x4*)((XDIT_LDS unsigned char*)smem + bo + 2 * G::TENSOR_BYTES + hb * 128 + hh * 16);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         f32x4 x = {own_nd, own_nd, own_nd, own_nd};
         if (KEYS) x = st[kTileRows / 4 + 2 * i];
 #pragma unroll
-        for (int e = 0; e < 4; e++) dp[4 * i + e] = x[e];
+        for (int e = 0; e < 4; e++) {
+          s[4 * i + e] = 0.f;
+          dp[4 * i + e] = x[e];
+        }
       }
-      rows_product<T, KSTEPS, G::TENSOR_BYTES>(dp, g, ra);
+      rows_products<T, KSTEPS, G::TENSOR_BYTES>(s, dp, f, g, ra);
       __builtin_amdgcn_sched_barrier(0);
+      ColumnsProducts<T, D, DBLOCKS, KEYS, G::TENSOR_BYTES> columns;
+      columns.start(ca);
       vec8 pf[2], df[2];
       if constexpr (!KEYS) {
 #pragma unroll
@@ -315,8 +327,7 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (KEYS) columns_product<T, D, DBLOCKS, G::TENSOR_BYTES>(acc_g, pf, ca);
-      columns_product<T, D, DBLOCKS, 0>(acc_f, df, ca);
+      columns.run(acc_g, acc_f, pf, df, ca);
     }
   }
 
