@@ -11,8 +11,8 @@
     (h, n)  = gated_norm(h, Fp8Linear(o), gate, scale, shift)
     h       = gated_norm(h, Fp8Linear(gelu(Fp8Linear(n))), gate)
 
-Forward runs every step on the library's kernels but the activation function.  Training runs the same norms, rotation and projections forward and
-backward; attention has no backward kernel here and is PyTorch's then, in float32.  Weights are random and frozen.
+Every step runs on the library's kernels but the activation function, forward and backward; a training step clips the gradients of what it
+trains (the modulation and the gains) to a common norm.  Weights are random and frozen.
 """
 import argparse
 import os
@@ -21,7 +21,7 @@ import sys
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-from xdit_amd import block, ops  # noqa: E402
+from xdit_amd import block, grad_ops, ops, usp  # noqa: E402
 
 F = torch.nn.functional
 
@@ -65,7 +65,7 @@ class DiTBlock(torch.nn.Module):
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
         q, k = block.axes_rope(q, k, positions, self.freq, self.pairs, norm=True, q_weight=self.q_gain, k_weight=self.k_gain)
         if train:
-            o = F.scaled_dot_product_attention(q.float(), k.float(), v.float()).to(x.dtype).transpose(1, 2).reshape(B, S, C)
+            o = usp.attention(q, k, v).transpose(1, 2).reshape(B, S, C)
         else:
             o = torch.empty_like(x, memory_format=torch.contiguous_format)
             ops.attn_fwd(q, k, v, out=o.view(B, S, self.heads, self.head_dim).transpose(1, 2), return_lse=False)
@@ -131,6 +131,26 @@ def check_gradients(m, x, modulation, positions, seed=2):
     return {n: distance(a, b) for n, a, b in zip(("x", "modulation", "q_gain", "k_gain"), got, want)}
 
 
+def training_step(m, x, modulation, positions, r, max_norm=1.0):
+    """Gradients of sum(block(x) * r) to the modulation and the gains, clipped to a common norm -> (gradients, their norm before that)."""
+    leaves = [modulation, m.q_gain, m.k_gain]
+    grads = [g.contiguous() for g in torch.autograd.grad(m(x, modulation, positions), leaves, r)]
+    return grads, grad_ops.clip_grads(grads, max_norm)
+
+
+def timed(fn, n=10):
+    """Milliseconds of a call among others."""
+    for _ in range(3):
+        fn()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    for _ in range(n):
+        fn()
+    end.record()
+    end.synchronize()
+    return start.elapsed_time(end) / n
+
+
 def main():
     p = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     p.add_argument("--grid", type=int, nargs=3, default=(1, 64, 64), help="frames, rows and columns of the latent")
@@ -138,26 +158,25 @@ def main():
     p.add_argument("--head-dim", type=int, default=128)
     p.add_argument("--mlp", type=int, default=8192)
     p.add_argument("--batch", type=int, default=1)
-    p.add_argument("--train", action="store_true", help="check the gradients instead of timing the forward pass")
+    p.add_argument("--train", action="store_true", help="check the gradients and time a training step instead of the forward pass")
     p.add_argument("--no-check", action="store_true")
     a = p.parse_args()
     m = DiTBlock(a.heads, a.head_dim, a.mlp, train=a.train)
     data = inputs(a.grid, a.heads, a.head_dim, a.batch)
+    size = "%d tokens, %d heads of %d, MLP %d" % (data[0].shape[1], a.heads, a.head_dim, a.mlp)
     if a.train:
-        print("gradients, relative distance to float32:", {n: round(d, 4) for n, d in check_gradients(m, *data).items()})
+        if not a.no_check:
+            print("gradients, relative distance to float32:", {n: round(d, 4) for n, d in check_gradients(m, *data).items()})
+        x, modulation, positions = data
+        modulation.requires_grad_()
+        r = torch.randn_like(x)
+        print("norm of the gradients: %.3f" % float(training_step(m, x, modulation, positions, r)[1]))
+        print("%s: %.3f ms a training step" % (size, timed(lambda: training_step(m, x, modulation, positions, r))))
         return
     if not a.no_check:
         print("output, relative distance to float32: %.4f" % check(m, *data))
     with torch.no_grad():
-        for _ in range(3):
-            m(*data)
-        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        start.record()
-        for _ in range(10):
-            m(*data)
-        end.record()
-        end.synchronize()
-    print("%d tokens, %d heads of %d, MLP %d: %.3f ms a block" % (data[0].shape[1], a.heads, a.head_dim, a.mlp, start.elapsed_time(end) / 10))
+        print("%s: %.3f ms a block" % (size, timed(lambda: m(*data))))
 
 
 if __name__ == "__main__":
