@@ -33,7 +33,7 @@ struct AttnBwdParams {
   int B, H, Sq, Sk, Sk2, D;
   float scale;
   int sq_pad;         // Sq rounded up to whole tiles
-  float* stats;       // workspace: per (batch, head) lse / ln 2 of every row, then -delta of every row, sq_pad of each
+  float* stats;       // workspace: per (batch, head) lse / ln 2 of every row (fp16: less kFp16Exponent), then -delta of every row, sq_pad of each
   float* amax;        // workspace, fp16: largest |dout| of every block of kBwdStatRows rows of a (batch, head)
   int tiles1;         // row tiles of the first segment of keys
   int step1;          // streamed tiles of the first segment of keys
@@ -41,6 +41,8 @@ struct AttnBwdParams {
   BwdRole queries;    // row tiles of queries, keys streamed: dq
 };
 
+// fp16's numbers end at 2^-24, and P and dS are small: P is computed times 2^13 (it stays below 2^14) where it is rounded (attn_bwd_16.hip).
+constexpr int kFp16Exponent = 13;
 constexpr int kBwdStatRows = 64;  // rows of a workgroup of the statistics kernel
 constexpr int kBwdWaves = 4;      // wavefronts of a workgroup, 32 owned rows each
 constexpr int kBwdRows = 32 * kBwdWaves;

@@ -52,10 +52,9 @@ template <int D> struct BwdGeom {
   static constexpr int STEP8 = 2 * PITCH;                        // +8 rows where bit 3 of the row is clear
 };
 
-// fp16's numbers end at 2^-24, and P and dS are small.  P is computed times 2^13 (it stays below 2^14), which is free: the exponent gets it.  dS is computed
-// times 2^m, m between 0 and 13 so that 2^m times the largest |dout| of the (batch, head) is below 16 (dS, about
-// 16 sqrt(D) |v| P, is far below 65504 then).  The gradients are multiplied by 2^-13 and 2^-m at the end.
-constexpr int kFp16Exponent = 13;
+// fp16: P is computed times 2^13 in the keys role, which is free: the exponent gets it.  dS is computed times 2^m, m between 0 and 13 so that 2^m
+// times the largest |dout| of the (batch, head) is below 16 (dS, about 16 sqrt(D) |v| P, is far below 65504 then).  The gradients are multiplied by 2^-13
+// and 2^-m at the end.
 __device__ __forceinline__ int fp16_exponent(const AttnBwdParams& p, int bh) {
   __shared__ float tops[8];
   float top = 0.f;
@@ -179,11 +178,10 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
   const float* stats = p.stats + (int64_t)bh * 2 * p.sq_pad;
   constexpr bool FP16 = __is_same(T, _Float16);
   const int m = FP16 ? fp16_exponent(p, bh) : 0;
-  const float shift = !FP16 ? 0.f : KEYS ? (float)kFp16Exponent : (float)m;   // of P
   const float p_to_ds = FP16 && KEYS ? __builtin_ldexpf(1.f, m - kFp16Exponent) : 1.f;
   float own_lse = 0.f, own_nd = 0.f;
   if constexpr (!KEYS) {
-    if (own < p.sq_pad) { own_lse = stats[own] - shift; own_nd = stats[p.sq_pad + own]; }
+    if (own < p.sq_pad) { own_lse = stats[own] + (FP16 ? (float)(kFp16Exponent - m) : 0.f); own_nd = stats[p.sq_pad + own]; }
   }
 
   // ---- tile loads ----
@@ -310,7 +308,6 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
         f32x4 pr, ds;
         if constexpr (KEYS) {
           f32x4 x = st[2 * i];
-          if (FP16) x -= shift;
 #pragma unroll
           for (int e = 0; e < 4; e++) pr[e] = fast_exp2(__builtin_fmaf(s[4 * i + e], c, -x[e]));
         }

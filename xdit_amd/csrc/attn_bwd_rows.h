@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256) void bwd_stats_kernel(const AttnBwdParams p) {
       if (row < p.Sq) {
         const float l = p.lse[b * p.ls_b + h * p.ls_h + row * p.ls_s];
         if (l != -INFINITY) {
-          lse2 = l * kLog2e;
+          lse2 = l * kLog2e - (__is_same(T, _Float16) ? (float)kFp16Exponent : 0.f);
           nd = (p.dlse != nullptr ? p.dlse[b * p.dl_b + h * p.dl_h + row * p.dl_s] : 0.f) - dot;
         }
       }
