@@ -400,7 +400,7 @@ hipError_t launch_kernels(const AttnBwdParams& p, hipStream_t stream) {
     if (e != hipSuccess) return e;
     lds_ready[slot].store(true, std::memory_order_relaxed);
   }
-  hipLaunchKernelGGL((bwd_stats_kernel<T>), dim3((unsigned)(p.B * p.H) * (p.sq_pad / kBwdStatRows)), dim3(256), 0, stream, p);
+  launch_bwd_stats<T>(p, stream);
   hipLaunchKernelGGL((attn_bwd_16_kernel<T, D, DC>), dim3(8u * (unsigned)(p.keys.units + p.queries.units)), dim3(64 * kBwdWaves), lds, stream, p);
   return launch_bwd_fold<T, DC>(p, stream);
 }

@@ -8,39 +8,54 @@ namespace {
 
 // lse / ln 2 and -delta of every row; rows up to the padded count get (infinity, 0), whose probabilities are zeros.  A row whose
 // log-sum-exp is -infinity attended nothing: the same.  fp16: also the largest |dout| of the block's rows.
-template <typename T>
+// Reading out and dout bounds it: all loads of a thread are asked for at once, `out`, which nothing reads again, past the caches' replacement order, and where the heads of
+// a token lie side by side, blocks that run together take all heads of their tokens (40 heads of 32760 x 128, BSHD: 139 us with two
+// loads at a time and head by head, 126 so).  LPR: lanes per row, 8 columns each.
+template <typename T, int LPR>
 __global__ __launch_bounds__(256) void bwd_stats_kernel(const AttnBwdParams p) {
-  const int lpr = p.D > 64 ? 16 : 8;   // lanes per row, 8 columns each
-  const int blocks = p.sq_pad / kBwdStatRows;
-  const int bh = blockIdx.x / blocks, block = blockIdx.x - bh * blocks;
+  constexpr int STEP = 256 / LPR, PASSES = kBwdStatRows / STEP;
+  const int blocks = p.sq_pad / kBwdStatRows, heads = p.B * p.H;
+  const bool by_token = p.dout.h < p.dout.s;
+  const int bh = by_token ? blockIdx.x % heads : blockIdx.x / blocks;
+  const int block = by_token ? blockIdx.x / heads : blockIdx.x - bh * blocks;
   const int b = bh / p.H, h = bh - b * p.H;
-  const int sub = threadIdx.x & (lpr - 1);
-  float top = 0.f;
-  for (int r = threadIdx.x / lpr; r < kBwdStatRows; r += 256 / lpr) {
-    const int row = block * kBwdStatRows + r;
-    float dot = 0.f;
-    if (row < p.Sq && sub * 8 < p.D) {
-      const Raw8<T> o = load_raw8<T>(p.out.p, b * p.out.b + h * p.out.h + (int64_t)row * p.out.s + sub * 8);
-      const Raw8<T> g = load_raw8<T>(p.dout.p, b * p.dout.b + h * p.dout.h + (int64_t)row * p.dout.s + sub * 8);
+  const int sub = threadIdx.x & (LPR - 1);
+  const int row0 = block * kBwdStatRows + threadIdx.x / LPR;
+  const T* const op = (const T*)p.out.p + b * p.out.b + h * p.out.h + sub * 8;
+  const T* const gp = (const T*)p.dout.p + b * p.dout.b + h * p.dout.h + sub * 8;
+  Raw8<T> o[PASSES], g[PASSES];
+  float lse[PASSES], dlse[PASSES];
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        dot = __builtin_fmaf(o[e], g[e], dot);
-        top = fmaxf(top, __builtin_fabsf(g[e]));
-      }
+  for (int i = 0; i < PASSES; i++) {
+    int row = row0 + i * STEP;
+    row = row < p.Sq ? row : p.Sq - 1;
+    if (sub * 8 < p.D) {
+#pragma unroll
+      for (int n = 0; n < Raw8<T>::N; n++) o[i].x[n] = __builtin_nontemporal_load((const typename Raw8<T>::vec*)(op + (int64_t)row * p.out.s) + n);
+      g[i] = load_raw8<T>(gp, (int64_t)row * p.dout.s);
+    } else {
+#pragma unroll
+      for (int n = 0; n < Raw8<T>::N; n++) o[i].x[n] = g[i].x[n] = (typename Raw8<T>::vec)(T)0.f;
     }
-    for (int m = 1; m < lpr; m <<= 1) dot += __shfl_xor(dot, m);
+    lse[i] = p.lse[b * p.ls_b + h * p.ls_h + row * p.ls_s];
+    dlse[i] = p.dlse != nullptr ? p.dlse[b * p.dl_b + h * p.dl_h + row * p.dl_s] : 0.f;
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < PASSES; i++) {
+    const int row = row0 + i * STEP;
+    float dot = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      dot = __builtin_fmaf(o[i][e], g[i][e], dot);
+      top = fmaxf(top, __builtin_fabsf(g[i][e]));
+    }
+    for (int m = 1; m < LPR; m <<= 1) dot += __shfl_xor(dot, m);
     if (sub == 0) {
-      float lse2 = INFINITY, nd = 0.f;
-      if (row < p.Sq) {
-        const float l = p.lse[b * p.ls_b + h * p.ls_h + row * p.ls_s];
-        if (l != -INFINITY) {
-          lse2 = l * kLog2e - (__is_same(T, _Float16) ? (float)kFp16Exponent : 0.f);
-          nd = (p.dlse != nullptr ? p.dlse[b * p.dl_b + h * p.dl_h + row * p.dl_s] : 0.f) - dot;
-        }
-      }
+      const bool live = row < p.Sq && lse[i] != -INFINITY;
       float* st = p.stats + (int64_t)bh * 2 * p.sq_pad + row;
-      st[0] = lse2;
-      st[p.sq_pad] = nd;
+      st[0] = live ? lse[i] * kLog2e - (__is_same(T, _Float16) ? (float)kFp16Exponent : 0.f) : INFINITY;
+      st[p.sq_pad] = live ? dlse[i] - dot : 0.f;
     }
   }
   if (p.amax != nullptr) {
@@ -50,6 +65,13 @@ __global__ __launch_bounds__(256) void bwd_stats_kernel(const AttnBwdParams p) {
     __syncthreads();
     if (threadIdx.x == 0) p.amax[(int64_t)bh * blocks + block] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   }
+}
+
+template <typename T>
+void launch_bwd_stats(const AttnBwdParams& p, hipStream_t stream) {
+  const dim3 grid((unsigned)(p.B * p.H) * (p.sq_pad / kBwdStatRows));
+  if (p.D > 64) hipLaunchKernelGGL((bwd_stats_kernel<T, 16>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((bwd_stats_kernel<T, 8>), grid, dim3(256), 0, stream, p);
 }
 
 // Adds the parts of every row of the tiles that were cut up, in their order, and rounds.  Blocks of the keys role first, dk and dv of a tile
