@@ -33,7 +33,7 @@ def bwd_args(**kw):
                   lse_stride=_lib.Strides(H * Sq, Sq, 1), workspace=P, workspace_bytes=1 << 40)
     for names, S in ((("q", "dout", "out", "dq"), Sq), (("k", "v", "dk", "dv"), Sk), (("k2", "v2", "dk2", "dv2"), Sk2)):
         for n in names:
-            values[n], values[n + "_stride"] = P, _lib.Strides(H * S * D, S * D, D)
+            values[n], values[n + "_stride"] = P * (2 + len(values)), _lib.Strides(H * S * D, S * D, D)
     values["lse"] = P
     for k, v in {**values, **kw}.items():
         setattr(a, k, v)
@@ -60,6 +60,7 @@ S = _lib.Strides
   + [(dict([(n + "_stride", S(0, 64, 60))]), BAD, n) for n in ("q", "v", "out", "dq", "dk")]
   + [(dict([(n + "_stride", S(6400, 0, 64))]), BAD, "overlap") for n in ("dq", "dk", "dv", "dk2", "dv2")]
   + [(dict(q_stride=S(0, 0, 1 << 23)), BAD, "too large"), (dict(k_stride=S(-8, 0, 64)), BAD, "negative"), (dict(lse=P + 2), BAD, "4-byte"),
+     (dict(dq=P), BAD, "place of an input"), (dict(dk=P * 100, dv=P * 100), BAD, "one place"), (dict(dk2=P * 100, q=P * 100), BAD, "place of an input"),
      (dict(lse_stride=S(0, -1, 1)), BAD, "negative"), (dict(dlse=P, dlse_stride=S(0, 0, -1)), BAD, "negative"), (dict(workspace=None), BAD, "workspace"),
      (dict(workspace_bytes=16), BAD, "workspace"), (dict(workspace=P + 4), BAD, "workspace")])
 def test_attention_backward_refusals(kw, code, needle):

@@ -201,6 +201,20 @@ int check_grad(const char* name, const void* p, const xdit_strides& st, int es, 
   return 0;
 }
 
+// A gradient in the place of an input, or two in one place: other workgroups still read what a workgroup writes.
+int check_places(const xdit_attn_bwd_args* a) {
+  const void* in[] = {a->dout, a->q, a->k, a->v, a->out, a->lse, a->dlse, a->Sk2 > 0 ? a->k2 : nullptr, a->Sk2 > 0 ? a->v2 : nullptr};
+  const void* out[] = {a->dq, a->dk, a->dv, a->Sk2 > 0 ? a->dk2 : nullptr, a->Sk2 > 0 ? a->dv2 : nullptr};
+  for (int i = 0; i < 5; i++) {
+    if (out[i] == nullptr) continue;
+    for (const void* p : in)
+      if (p == out[i]) return api_fail(XDIT_ERR_INVALID_ARG, "a gradient lies in the place of an input");
+    for (int j = 0; j < i; j++)
+      if (out[j] == out[i]) return api_fail(XDIT_ERR_INVALID_ARG, "two gradients lie in one place");
+  }
+  return 0;
+}
+
 xdit::BwdTensor tensor(const void* p, const xdit_strides& st) { return {const_cast<void*>(p), st.b, st.h, st.s}; }
 
 // ---- norm and clipping of a list of gradients ----
@@ -432,6 +446,7 @@ int xdit_attn_bwd(const xdit_attn_bwd_args* a) {
     }
   }
   if (a->lse == nullptr) return api_fail(XDIT_ERR_INVALID_ARG, "lse is NULL");
+  if ((rc = check_places(a))) return rc;
   if (reinterpret_cast<uintptr_t>(a->lse) & 3u || reinterpret_cast<uintptr_t>(a->dlse) & 3u)
     return api_fail(XDIT_ERR_INVALID_ARG, "lse and dlse must be 4-byte aligned");
   if (a->lse_stride.b < 0 || a->lse_stride.h < 0 || a->lse_stride.s < 0 || a->dlse_stride.b < 0 || a->dlse_stride.h < 0 || a->dlse_stride.s < 0)
