@@ -44,6 +44,7 @@ fp32.  The ops are registered for GPU tensors only: there is no CPU implementati
 from typing import List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.library import custom_op, register_autograd, register_fake
 
 from . import block_ops, grad_ops, ops
@@ -133,7 +134,10 @@ register_autograd("xdit_amd::attn_fwd_joint", _attn_fwd_joint_grad, setup_contex
 
 
 def attn_grad_wanted(*tensors):
-    """Whether an attention call on these tensors has to leave a graph behind (of the types that have a backward pass; fp8 has none)."""
+    """Whether an attention call on these tensors has to leave a graph behind (of the types that have a backward pass; fp8 has none).  Gradients are those
+    of reverse mode: tangents of forward-mode differentiation are refused."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode differentiation is not supported: the tangent would be lost")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad and t.dtype in (torch.bfloat16, torch.float16, torch.float32) for t in tensors)
 
 

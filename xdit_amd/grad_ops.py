@@ -89,7 +89,7 @@ def attn_bwd(dout, q, k, v, out, lse, softmax_scale=None, k2=None, v2=None, dlse
             need = 0 if empty else _lib.lib().xdit_attn_bwd_workspace_bytes(ctypes.byref(a))
         if need < 0:
             _lib.check(need)
-        return a, wanted, need, empty
+        return a, wanted, 1 << (need - 1).bit_length(), empty   # a power of two: what calls of growing sizes leave allocated stays below the last one's
 
     a, wanted, need, empty = _plan(key, build)
     given = {"dq": dq, "dk": dk, "dv": dv, "dk2": dk2, "dv2": dv2}
