@@ -130,7 +130,13 @@ def test_lists_of_gradients(monkeypatch):
     b.data = torch.zeros(30)
     second = grad_ops._listed(g)
     assert second is not first and second.sizes == [6, 30] and second.ptr[1] == b.data_ptr()
-    b.data = torch.zeros(5, 6).t()
+    whole = b.data
+    b.data = whole[:20]   # at the same address
+    third = grad_ops._listed(g)
+    assert third is not second and third.sizes == [6, 20] and list(third.numel) == [6, 20]
+    b.data = whole[:20].bfloat16()
+    assert list(grad_ops._listed(g).dtype) == [2, 0]
+    b.data = whole.view(5, 6).t()
     with pytest.raises(ValueError, match="contiguous"):
         grad_ops._listed(g)
     for kind, code in ((2, 2), (1, 1), (float("inf"), 0), (2.0, 2)):
