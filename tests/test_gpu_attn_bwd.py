@@ -329,6 +329,82 @@ def test_gradient_of_joint_attention_and_of_the_ring(gpu, strategy, chunks, dtyp
     close((got[3],), (dq[1],), (fq[1],))
 
 
+def ring_call(**joint):
+    """The ring over four chunks, with joint keys as `joint` says -> a function of (q, k, v, joint key, joint value)."""
+    def f(q, k, v, k2, v2, order=None, chunks=4):
+        kw = dict(joint_key=k2, joint_value=v2, **joint) if joint else None
+        return usp.ring_attn(usp._get_attention_function(), q, k, v, joint_attn_kwargs=kw, ring_chunks=chunks, order=order)
+    return f
+
+
+def test_no_gradient_of_a_ring_is_lost(gpu):
+    """Whichever one tensor asks for a gradient."""
+    ts = [rand(gpu, i, 1, 2, 32, 64, dtype=torch.bfloat16) for i in range(5)]
+    for chunks in (1, 4):
+        for i in range(5):
+            one = [t.clone().requires_grad_(j == i) for j, t in enumerate(ts)]
+            o = ring_call(joint_strategy="front", total_steps=chunks)(*one, chunks=chunks)
+            (g,) = torch.autograd.grad(o.square().sum(), one[i:i + 1])
+            assert bool(g.any())
+
+
+@pytest.mark.parametrize("joint", [dict(joint_strategy="front", step=1), dict(joint_strategy="rear", total_steps=9), dict(joint_strategy="none")])
+def test_joint_keys_that_no_step_takes(gpu, joint):
+    q, k, v, k2, v2, dout, _, _ = inputs(gpu, 1, 2, 60, 80, 64, 20)
+    ls = leaves(q, k, v, k2, v2)
+    got = torch.autograd.grad(ring_call(**joint)(*ls), ls, dout, allow_unused=True)
+    want = torch.autograd.grad(ring_call()(*ls), ls[:3], dout)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[3] is None and got[4] is None
+
+
+def test_ring_that_takes_a_chunk_twice(gpu):
+    q, k, v, _, _, dout, _, _ = inputs(gpu, 1, 2, 60, 80, 64)
+    ls = leaves(q, k, v)
+    order = [0, 2, 2, 1]
+    o = ring_call()(*ls, None, None, order=order)
+    dq, dk, dv = torch.autograd.grad(o, ls, dout)
+    kk, vv = (torch.cat([t.chunk(4, 2)[c] for c in order], 2) for t in (k, v))
+    lse = ops.attn_fwd(q, kk, vv)[1]
+    (wq, wk, wv), (fq, fk, fv) = bounds(q, kk, vv, None, None, dout, o.detach(), lse)
+    close((dq,), (wq,), (fq,))
+    for got, w, f in ((dk, wk, fk), (dv, wv, fv)):
+        w, f = w.chunk(4, 2), f.chunk(4, 2)
+        both = w[1] + w[2]
+        close((got,), (torch.cat((w[0], w[3], both, torch.zeros_like(both)), 2),),
+              (torch.cat((f[0], f[3], f[1] + f[2] + 2.0 ** -8 * both.abs(), torch.zeros_like(both)), 2),))   # and their sum's own rounding
+    with pytest.raises(ValueError, match="order"):
+        ring_call()(*ls, None, None, order=[0, 1, 2])
+
+
+@pytest.mark.parametrize("joint", [{}, dict(joint_strategy="rear", total_steps=4)])
+def test_compiled_ring_has_the_eager_gradient(gpu, joint):
+    q, k, v, k2, v2, dout, _, _ = inputs(gpu, 1, 2, 60, 80, 64, 20)
+    ls = leaves(q, k, v, *((k2, v2) if joint else ()))
+    rest = () if joint else (None, None)
+    eager = ring_call(**joint)(*ls, *rest)
+    traced = torch.compile(ring_call(**joint), backend="aot_eager", fullgraph=True)(*ls, *rest)
+    assert torch.equal(eager, traced)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(traced, ls, dout), torch.autograd.grad(eager, ls, dout)))
+
+
+@pytest.mark.parametrize("call", [ring.flash_attn_forward, lambda q, k, v: ring.xdit_ring_flash_attn_func(q, k, v, group=ring.LocalRing(2), return_attn_probs=True)[:2]])
+def test_compiled_ring_on_bshd_tensors(gpu, call):
+    ls = leaves(*(rand(gpu, i, 1, 64, 2, 32, dtype=torch.bfloat16) for i in range(3)))
+    dout, dlse = rand(gpu, 3, 1, 64, 2, 32, dtype=torch.bfloat16), rand(gpu, 4, 1, 2, 64)
+    eager, traced = call(*ls), torch.compile(call, backend="aot_eager")(*ls)
+    assert all(torch.equal(a, b) for a, b in zip(eager, traced))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(traced, ls, (dout, dlse)), torch.autograd.grad(eager, ls, (dout, dlse))))
+
+
+def test_second_gradients_are_refused(gpu):
+    q, k, v, _, _, dout, _, _ = inputs(gpu, 1, 2, 20, 30, 64)
+    for call in (usp.attention, lambda *t: ring_call()(*t[:1], *(x[:, :, :28] for x in t[1:]), None, None)):
+        ls = leaves(q, k, v)
+        (dq,) = torch.autograd.grad(call(*ls), ls[:1], dout, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(dq.sum(), ls[1:2])
+
+
 @pytest.mark.parametrize("world", [1, 2])
 @pytest.mark.parametrize("joint", [False, True])
 def test_gradient_of_the_ring_on_bshd_tensors(gpu, world, joint):

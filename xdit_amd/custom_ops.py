@@ -22,6 +22,7 @@ The reference wraps a vendor kernel the same way (xfuser/core/distributed/attent
 
     xdit_amd::attn_bwd        (dout, q, k, v, k2?, v2?, out, lse, dlse?, softmax_scale, need_q,
                                need_kv)             -> list of gradients of attn_fwd or attn_fwd_joint
+    xdit_amd::attn_result     (out, lse, q, k, v, k2?, v2?, softmax_scale)    -> (out, lse), differentiable in q .. v2
 
 and the operators around the attention call (`xdit_amd.block_ops`), with their gradients:
 
@@ -162,6 +163,41 @@ class RingAttention(torch.autograd.Function):
         q, k, v, k2, v2, out, lse = ctx.saved_tensors
         grads = _attn_grads(ctx.needs_input_grad[3:], t(dout), dlse, t(q), t(k), t(v), t(k2), t(v2), t(out), lse, ctx.scale)
         return (None, None, None, *map(t, grads))
+
+
+@custom_op("xdit_amd::attn_result", mutates_args=(), device_types="cuda")
+def attn_result(out: Tensor, lse: Tensor, query: Tensor, key: Tensor, value: Tensor, key2: Optional[Tensor], value2: Optional[Tensor],
+                softmax_scale: float) -> Tuple[Tensor, Tensor]:
+    """Copies of the out and lse that several calls made of attention over all of key, value [, key2, value2]: with its gradient, in a traced graph."""
+    return out.clone(), lse.clone()
+
+
+@register_fake("xdit_amd::attn_result")
+def _attn_result_fake(out, lse, query, key, value, key2, value2, softmax_scale):
+    return torch.empty_like(out), torch.empty_like(lse)
+
+
+def _attn_result_setup(ctx, inputs, output):
+    _attn_fwd_setup(ctx, inputs[2:], output)
+
+
+def _attn_result_grad(ctx, dout, dlse):
+    return (None, None, *_attn_grads(ctx.needs_input_grad[2:7], dout, dlse, *ctx.saved_tensors, ctx.scale), None)
+
+
+register_autograd("xdit_amd::attn_result", _attn_result_grad, setup_context=_attn_result_setup)
+
+
+def attn_in_steps(call, scale, bshd, *tensors):
+    """`RingAttention` of query, key, value, key2, value2, in traced code by the registered operator."""
+    if not torch.compiler.is_compiling():
+        return RingAttention.apply(call, scale, bshd, *tensors)
+    with torch.no_grad():
+        out, lse = call()
+    if not bshd:
+        return torch.ops.xdit_amd.attn_result(out, lse, *tensors, scale)
+    out, lse = torch.ops.xdit_amd.attn_result(out.transpose(1, 2), lse, *(None if t is None else t.transpose(1, 2) for t in tensors), scale)
+    return out.transpose(1, 2), lse
 
 
 @custom_op("xdit_amd::attn_fwd_fp8", mutates_args=(), device_types="cuda")

@@ -56,8 +56,9 @@ def flash_attn_forward(q, k, v, dropout_p=0.0, softmax_scale=None, causal=False,
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(q.size(-1))
     if custom_ops.attn_grad_wanted(q, k, v, joint_k, joint_v):
-        return custom_ops.RingAttention.apply(
-            lambda: flash_attn_forward(q, k, v, softmax_scale=softmax_scale, joint_k=joint_k, joint_v=joint_v, out_dtype=out_dtype),
+        return custom_ops.attn_in_steps(
+            lambda: flash_attn_forward(q, k, v, softmax_scale=softmax_scale, q_descale=q_descale, k_descale=k_descale, v_descale=v_descale,
+                                       joint_k=joint_k, joint_v=joint_v, out_dtype=out_dtype),
             softmax_scale, True, q, k, v, joint_k, joint_v)
     t = lambda x: None if x is None else x.transpose(1, 2)  # BSHD -> logical BHSD view, no copy
     B, Sq, H, D = q.shape
@@ -101,7 +102,7 @@ def xdit_ring_flash_attn_forward(process_group, q, k, v, softmax_scale, dropout_
                                  chunks visited in the order the ring would deliver them.
     Returns (out in q's dtype (bf16 for fp8 inputs), lse (B,H,Sq) fp32), differentiable in 16 and 32 bits."""
     if custom_ops.attn_grad_wanted(q, k, v, joint_tensor_key, joint_tensor_value):
-        return custom_ops.RingAttention.apply(
+        return custom_ops.attn_in_steps(
             lambda: xdit_ring_flash_attn_forward(process_group, q, k, v, softmax_scale, dropout_p, causal, window_size, alibi_slopes, deterministic,
                                                  attn_type, attn_processor, attn_layer, joint_tensor_key, joint_tensor_value, joint_strategy,
                                                  q_descale, k_descale, v_descale),

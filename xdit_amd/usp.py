@@ -123,7 +123,7 @@ def ring_attn(attention_function, query, key, value, dropout_p=0.0, is_causal=Fa
               joint_attn_kwargs=None, attention_kwargs=None, ring_chunks=1, order=None):
     """The ring schedule of usp.py:46-74 on one device.  K/V are split into `ring_chunks`
     contiguous chunks; `order` defaults to what rank 0 sees: [0, P-1, P-2, ..., 1].  On the 16- and 32-bit
-    backend the result is differentiable (outside torch.compile), joint tensors included."""
+    backend the result is differentiable, joint tensors included."""
     P = ring_chunks
     if key.shape[2] % P != 0:
         raise ValueError(f"key length {key.shape[2]} is not divisible by ring_chunks={P}")
@@ -134,50 +134,62 @@ def ring_attn(attention_function, query, key, value, dropout_p=0.0, is_causal=Fa
     mi355 = ATTENTION_FUNCTION_REGISTRY.get(AttentionBackendType.MI355)
     decorated = _DECORATED.get(AttentionBackendType.MI355)
     ours = attention_function is mi355 or (decorated is not None and decorated[0] is mi355 and attention_function is decorated[1])
-    if P > 1 and ops.fused_ring_step_supported(query) and ours:
-        # every step is one launch: the kernel folds its block into the accumulator itself (same
-        # bits as the call + merge below); the joint keys/values join on the step the decorator
-        # would pick
-        AB._check_call(dropout_p, is_causal, attention_kwargs)
-        scale = query.shape[-1] ** -0.5
-
-        def steps():
-            acc_out = torch.empty(query.shape, dtype=torch.float32, device=query.device)
-            acc_lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device)
-            final = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-            for i, c in enumerate(order):
-                joint_kv = None
-                if joint_attn_kwargs is not None:
-                    strategy = joint_attn_kwargs.get("joint_strategy", None)
-                    step = joint_attn_kwargs.get("step", 0)
-                    if (strategy == "front" and step == 0) or (strategy == "rear" and step == joint_attn_kwargs.get("total_steps", 1) - 1):
-                        joint_kv = (joint_attn_kwargs.get("joint_key", None), joint_attn_kwargs.get("joint_value", None), strategy)
-                    joint_attn_kwargs["step"] = step + 1
-                k1, v1, k2, v2 = AB._split_joint(k_chunks[c], v_chunks[c], joint_kv)
-                last = i == P - 1
-                if torch.compiler.is_compiling():   # the same call as a registered custom op (traceable)
-                    torch.ops.xdit_amd.attn_fwd_accumulate(query, k1, v1, k2, v2, acc_out, acc_lse, final if last else None,
-                                                           i == 0, last, scale)
-                else:
-                    ops.attn_fwd_accumulate(query, k1, v1, acc_out, acc_lse, first=i == 0,
-                                            final_out=final if last else None, discard_acc_out=last,
-                                            softmax_scale=scale, k2=k2, v2=v2)
-            return final, acc_lse
-
-        joint = (None, None) if joint_attn_kwargs is None else (joint_attn_kwargs.get("joint_key", None), joint_attn_kwargs.get("joint_value", None))
-        if not torch.compiler.is_compiling() and custom_ops.attn_grad_wanted(query, key, value, *joint):
-            return custom_ops.RingAttention.apply(steps, scale, False, query, key, value, *joint)[0]
-        return steps()[0]
-    if P == 1 and ours and custom_ops.attn_grad_wanted(query, key, value):
+    joint = joint_attn_kwargs or {}
+    grad = ours and custom_ops.attn_grad_wanted(query, key, value, joint.get("joint_key", None), joint.get("joint_value", None))
+    if grad and P == 1:
         # one block: the merge is the identity, and the call itself has the gradient
         return attention_function(query, key, value, dropout_p=dropout_p, is_causal=is_causal,
                                   joint_attn_kwargs=joint_attn_kwargs, attention_kwargs=attention_kwargs)[0]
-    merger = SDPAMerger()
-    for i, c in enumerate(order):
-        out, lse = attention_function(query, k_chunks[c], v_chunks[c], dropout_p=dropout_p, is_causal=is_causal,
-                                      joint_attn_kwargs=joint_attn_kwargs, attention_kwargs=attention_kwargs)
-        merger.step(out, lse, final_step=(i == P - 1))
-    return merger.results()[0]
+    scale = query.shape[-1] ** -0.5
+
+    def merged():
+        merger = SDPAMerger()
+        for i, c in enumerate(order):
+            out, lse = attention_function(query, k_chunks[c], v_chunks[c], dropout_p=dropout_p, is_causal=is_causal,
+                                          joint_attn_kwargs=joint_attn_kwargs, attention_kwargs=attention_kwargs)
+            merger.step(out, lse, final_step=(i == P - 1))
+        return merger.results()
+
+    def fused():
+        # every step is one launch: the kernel folds its block into the accumulator itself (same
+        # bits as the call + merge above); the joint keys/values join on the step the decorator
+        # would pick
+        AB._check_call(dropout_p, is_causal, attention_kwargs)
+        acc_out = torch.empty(query.shape, dtype=torch.float32, device=query.device)
+        acc_lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device)
+        final = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        for i, c in enumerate(order):
+            joint_kv = None
+            if joint_attn_kwargs is not None:
+                strategy = joint_attn_kwargs.get("joint_strategy", None)
+                step = joint_attn_kwargs.get("step", 0)
+                if (strategy == "front" and step == 0) or (strategy == "rear" and step == joint_attn_kwargs.get("total_steps", 1) - 1):
+                    joint_kv = (joint_attn_kwargs.get("joint_key", None), joint_attn_kwargs.get("joint_value", None), strategy)
+                joint_attn_kwargs["step"] = step + 1
+            k1, v1, k2, v2 = AB._split_joint(k_chunks[c], v_chunks[c], joint_kv)
+            last = i == P - 1
+            if torch.compiler.is_compiling():   # the same call as a registered custom op (traceable)
+                torch.ops.xdit_amd.attn_fwd_accumulate(query, k1, v1, k2, v2, acc_out, acc_lse, final if last else None,
+                                                       i == 0, last, scale)
+            else:
+                ops.attn_fwd_accumulate(query, k1, v1, acc_out, acc_lse, first=i == 0,
+                                        final_out=final if last else None, discard_acc_out=last,
+                                        softmax_scale=scale, k2=k2, v2=v2)
+        return final, acc_lse
+
+    call = fused if P > 1 and ops.fused_ring_step_supported(query) and ours else merged
+    if not grad:
+        return call()[0]
+    # one backward call over all keys that the steps take: the chunks, and the joint ones if a step is theirs
+    if len(order) != P:
+        raise ValueError(f"order has {len(order)} entries, expected {P}")
+    if sorted(order) != list(range(P)):   # a chunk twice, or not at all
+        key, value = (torch.cat([chunks[c] for c in order], dim=2) for chunks in (k_chunks, v_chunks))
+    step = joint.get("step", 0)
+    theirs = {"front": 0, "rear": joint.get("total_steps", 1) - 1}.get(joint.get("joint_strategy", None), -1)
+    taken = step <= theirs < step + P
+    return custom_ops.attn_in_steps(call, scale, False, query, key, value, joint.get("joint_key", None) if taken else None,
+                                    joint.get("joint_value", None) if taken else None)[0]
 
 
 def USP(query, key, value, dropout_p=0.0, is_causal=False, joint_query=None, joint_key=None,
