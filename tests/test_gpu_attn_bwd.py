@@ -181,6 +181,18 @@ def test_fp16_gradients_of_every_size(gpu, size):
     close(call(*t), *bounds(*t))
 
 
+def test_fp16_scores_stay_in_range(gpu):
+    """dS near fp16's end: values of 500 that all add up, and a gradient of the log-sum-exp far above dout."""
+    k, v = rand(gpu, 1, 1, 1, 2, 128).half(), torch.tensor([500.0, -500.0], device=gpu).view(1, 1, 2, 1).expand(1, 1, 2, 128).half().contiguous()
+    q, dout = (0.1 * rand(gpu, 2, 1, 1, 64, 128)).half(), torch.full((1, 1, 64, 128), 0.98, dtype=torch.float16, device=gpu)
+    out, lse = O.attn_fwd(q, k, v, 128 ** -0.5)
+    t = (q, k, v, None, None, dout, out.half(), lse.float())
+    close(call(*t), *bounds(*t))
+    t = inputs(gpu, 1, 2, 70, 3, 64, 0, "fp16", size=1e-3)
+    dlse = 50 * rand(gpu, 3, 1, 2, 70)
+    close(call(*t, dlse=dlse), *bounds(*t, dlse=dlse))
+
+
 def test_large_logits(gpu):
     """Rows whose probability is one key's."""
     q, k, v, _, _, dout, _, _ = inputs(gpu, 1, 2, 200, 190, 64)

@@ -151,6 +151,12 @@ def test_results_that_overlap(src, dst, dtypes):
     refused(_lib.lib().xdit_clip_grads, clip_args(s, d), BAD, "overlaps")
 
 
+@pytest.mark.parametrize("norm", [P, P + 36, 0x20000])
+def test_a_norm_inside_a_result(norm):
+    t = Table([(0x20000, 1), (P, 10)])
+    refused(_lib.lib().xdit_clip_grads, clip_args(t, t, norm=norm), BAD, "norm")
+
+
 @pytest.mark.parametrize("kw,needle", [(dict(struct_size=4), "struct_size"), (dict(count=-1), "count"), (dict(max_norm=-1.0), "max_norm"),
                                        (dict(max_norm=float("nan")), "max_norm"), (dict(max_norm=float("inf")), "max_norm"), (dict(norm=None), "norm"),
                                        (dict(norm=P + 2), "norm"), (dict(norm=None, norm_out=P + 2), "norm"), (dict(norm=None, norm_out=P, kind=3), "unknown norm"),

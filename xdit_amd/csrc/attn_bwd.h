@@ -34,7 +34,7 @@ struct AttnBwdParams {
   float scale;
   int sq_pad;         // Sq rounded up to whole tiles
   float* stats;       // workspace: per (batch, head) lse / ln 2 of every row (fp16: less kFp16Exponent), then -delta of every row, sq_pad of each
-  float* amax;        // workspace, fp16: largest |dout| of every block of kBwdStatRows rows of a (batch, head)
+  float* amax;        // workspace, fp16: of every block of kBwdStatRows rows of every (batch, head) the largest |dout|; then the largest |delta|; then |v|
   int tiles1;         // row tiles of the first segment of keys
   int step1;          // streamed tiles of the first segment of keys
   BwdRole keys;       // row tiles of keys, queries streamed: dk and dv
@@ -46,6 +46,11 @@ constexpr int kFp16Exponent = 13;
 constexpr int kBwdStatRows = 64;  // rows of a workgroup of the statistics kernel
 constexpr int kBwdWaves = 4;      // wavefronts of a workgroup, 32 owned rows each
 constexpr int kBwdRows = 32 * kBwdWaves;
+
+// Blocks of kBwdStatRows rows of a (batch, head)'s values, both segments.
+__host__ __device__ __forceinline__ int bwd_value_blocks(const AttnBwdParams& p) {
+  return (p.Sk + kBwdStatRows - 1) / kBwdStatRows + (p.Sk2 + kBwdStatRows - 1) / kBwdStatRows;
+}
 
 // A unit's tile (of all), part and slot of its partial result; false for the units that an XCD's last tiles do not have.
 struct BwdUnit {

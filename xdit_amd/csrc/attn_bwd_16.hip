@@ -52,20 +52,30 @@ template <int D> struct BwdGeom {
   static constexpr int STEP8 = 2 * PITCH;                        // +8 rows where bit 3 of the row is clear
 };
 
-// fp16: P is computed times 2^13 in the keys role, which is free: the exponent gets it.  dS is computed times 2^m, m between 0 and 13 so that 2^m
-// times the largest |dout| of the (batch, head) is below 16 (dS, about 16 sqrt(D) |v| P, is far below 65504 then).  The gradients are multiplied by 2^-13
-// and 2^-m at the end.
+// fp16: P is computed times 2^13 in the keys role, which is free: the exponent gets it.  dS is computed times 2^m, the largest
+// m up to 13 that keeps it below 2^15 whatever the signs:
+//   |dS_ij| = P_ij |dP_ij - delta_i| <= D max|dout| max|v| + max|delta|      (maxima of a (batch, head); of a chunk of a ring P_ij <= 1 too)
+// The gradients are multiplied by 2^-13 and 2^-m at the end.  The pass over v for its maximum is part of the statistics.
 __device__ __forceinline__ int fp16_exponent(const AttnBwdParams& p, int bh) {
-  __shared__ float tops[8];
-  float top = 0.f;
+  __shared__ float tops[3][kBwdWaves];
+  const int64_t heads = (int64_t)p.B * p.H;
   const int blocks = p.sq_pad / kBwdStatRows;
-  for (int i = threadIdx.x; i < blocks; i += blockDim.x) top = fmaxf(top, p.amax[(int64_t)bh * blocks + i]);
-  for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  float top[3] = {0.f, 0.f, 0.f};   // |dout|, |delta|, |v|
+#pragma unroll
+  for (int which = 0; which < 3; which++) {
+    const int n = which < 2 ? blocks : bwd_value_blocks(p);
+    const float* from = p.amax + which * heads * blocks + (int64_t)bh * n;
+    for (int i = threadIdx.x; i < n; i += 64 * kBwdWaves) top[which] = fmaxf(top[which], from[i]);
+    for (int m = 1; m < 64; m <<= 1) top[which] = fmaxf(top[which], __shfl_xor(top[which], m));
+    if ((threadIdx.x & 63) == 0) tops[which][threadIdx.x >> 6] = top[which];
+  }
   __syncthreads();
-  for (int i = 0; i < (int)blockDim.x >> 6; i++) top = fmaxf(top, tops[i]);
-  const int e = 130 - (int)(__float_as_uint(top) >> 23);   // 3 - floor(log2 top)
-  return __builtin_amdgcn_readfirstlane(e < 0 ? 0 : e > kFp16Exponent ? kFp16Exponent : e);
+#pragma unroll
+  for (int which = 0; which < 3; which++)
+    for (int i = 0; i < kBwdWaves; i++) top[which] = fmaxf(top[which], tops[which][i]);
+  const int e = (int)(__float_as_uint(p.D * top[0] * top[2] + top[1]) >> 23 & 255);   // the bound is below 2^(e - 126)
+  const int m = e == 255 ? 0 : 141 - e;   // (an infinity in dout or v: the rows that it does not reach keep the scale of ordinary ones)
+  return __builtin_amdgcn_readfirstlane(m > kFp16Exponent ? kFp16Exponent : m);
 }
 
 constexpr int kAhead = 4;  // LDS fragment reads in flight

@@ -137,6 +137,7 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   const int64_t bh = (int64_t)a->B * a->H;
   const int per_cu = f32 ? (a->D <= 96 ? 2 : 1) : a->D <= 64 ? 3 : 2;   // workgroups on a compute unit
   const int64_t cus = (xdit::resident_cus(a->cu_count) + 7) / 8;   // of an XCD
+  p.Sq = (int)a->Sq; p.Sk = (int)a->Sk; p.Sk2 = (int)a->Sk2;
   p.tiles1 = (int)((a->Sk + rows - 1) / rows);
   p.keys.tiles = p.tiles1 + (int)((a->Sk2 + rows - 1) / rows);
   p.keys.steps = (int)((a->Sq + step - 1) / step);
@@ -161,7 +162,7 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   plan_roles(p, cus, per_cu, cost);
   p.sq_pad = (int)((a->Sq + xdit::kBwdStatRows - 1) / xdit::kBwdStatRows * xdit::kBwdStatRows);
   plan.stats = align256(bh * 2 * p.sq_pad * 4);
-  plan.amax = a->dtype == XDIT_DTYPE_FP16 ? align256(bh * (p.sq_pad / xdit::kBwdStatRows) * 4) : 0;
+  plan.amax = a->dtype == XDIT_DTYPE_FP16 ? align256(bh * (2 * (p.sq_pad / xdit::kBwdStatRows) + xdit::bwd_value_blocks(p)) * 4) : 0;
   auto partial = [&](const xdit::BwdRole& r, int tensors) { return r.parts > 1 ? 8 * (int64_t)(r.per_xcd - r.whole) * r.parts * tensors * rows * dc * 4 : 0; };
   plan.keys = partial(p.keys, 2);
   plan.queries = partial(p.queries, 1);
@@ -298,7 +299,7 @@ int check_partials(int64_t n, const void* workspace, int64_t bytes) {
   return 0;
 }
 
-// Whether no destination overlaps another one, or a source other than itself.
+// Whether no destination overlaps another one, a source other than itself, or the norm.
 bool destinations_apart(const xdit_clip_grads_args* a) {
   struct Span { uintptr_t begin, end; int64_t i; };
   std::vector<Span> dst;
@@ -315,7 +316,9 @@ bool destinations_apart(const xdit_clip_grads_args* a) {
     for (; at != dst.end() && at->begin < end; ++at)
       if (at->i != i || at->begin != begin || a->src_dtype[i] != a->dst_dtype[i]) return false;
   }
-  return true;
+  const uintptr_t norm = reinterpret_cast<uintptr_t>(a->norm != nullptr ? a->norm : a->norm_out);   // every workgroup reads it
+  auto at = std::upper_bound(dst.begin(), dst.end(), norm, [](uintptr_t x, const Span& s) { return x < s.end; });
+  return at == dst.end() || at->begin >= norm + sizeof(float);
 }
 
 }  // namespace
@@ -357,8 +360,9 @@ int xdit_clip_grads(const xdit_clip_grads_args* a) {
     if ((rc = check_list("gradient", a->count, const_cast<void* const*>(a->src), a->numel, a->src_dtype))) return rc;
     if ((rc = check_list("result", a->count, a->dst, a->numel, a->dst_dtype))) return rc;
   }
+  if (!given && (rc = check_partials(partials_of(a->count, a->numel), a->workspace, a->workspace_bytes))) return rc;
   try {
-    if (!destinations_apart(a)) return api_fail(XDIT_ERR_INVALID_ARG, "a result overlaps another one, or a gradient other than its own");
+    if (!destinations_apart(a)) return api_fail(XDIT_ERR_INVALID_ARG, "a result overlaps another one, a gradient other than its own, or the norm");
   } catch (const std::bad_alloc&) {
     return api_fail(XDIT_ERR_INVALID_ARG, "no host memory for %lld tensors", (long long)a->count);
   }
@@ -373,7 +377,6 @@ int xdit_clip_grads(const xdit_clip_grads_args* a) {
   p.partials = 0;
   p.kind = a->kind;
   if (!given) {
-    if ((rc = check_partials(partials_of(a->count, a->numel), a->workspace, a->workspace_bytes))) return rc;
     const int64_t n = launch_partials(a->count, a->src, a->numel, a->src_dtype, a->kind, (double*)a->workspace, stream);
     if (n < 0) return (int)n;
     if (n == 0 || n > xdit::kClipPartials) {
@@ -477,7 +480,6 @@ int xdit_attn_bwd(const xdit_attn_bwd_args* a) {
   p.dlse = a->dlse;
   p.dl_b = a->dlse_stride.b; p.dl_h = a->dlse_stride.h; p.dl_s = a->dlse_stride.s;
   p.B = a->B; p.H = a->H; p.D = a->D;
-  p.Sq = (int)a->Sq; p.Sk = (int)a->Sk; p.Sk2 = (int)a->Sk2;
   p.scale = a->softmax_scale;
   unsigned char* ws = (unsigned char*)a->workspace;
   p.stats = (float*)ws;

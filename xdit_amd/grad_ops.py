@@ -224,7 +224,7 @@ def clip_grads(grads, max_norm, norm=None, norm_type=2.0, out=None):
 
     `norm` (an fp32 tensor without dimensions or with one element, e.g. joined over ranks) is computed by `grad_norm` where it is not given.
     out: as many tensors of the same sizes, in any of the three dtypes (e.g. the fp32 gradients that an optimizer steps on); none may share memory with
-    another, or with a gradient other than its own.  Products are fp32, rounded once; nothing waits for the GPU."""
+    another, with `norm`, or with a gradient other than its own.  Products are fp32, rounded once; nothing waits for the GPU."""
     kind = _kind(norm_type)
     g = _listed(grads)
     o = g if out is None else _listed(out)
