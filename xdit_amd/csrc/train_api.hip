@@ -59,19 +59,47 @@ struct StepCost {
   double part;                  // of a tensor's partial tile
 };
 
+// Where every unit has a place at once: the units of a compute unit are those whose numbers differ by the number of compute units, and what they do adds up, less
+// what they gain by running beside each other.
+double one_round_us(const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t cus, int per_cu, const StepCost& c) {
+  struct Group { int64_t end; double work, fixed; } g[4];
+  int n = 0;
+  int64_t units = 0;
+  for (int i = 0; i < 2; i++) {
+    const xdit::BwdRole& r = i ? q : k;
+    if (r.total == 0) continue;
+    if (r.whole) g[n++] = {units += r.whole, r.steps * c.alone[i], c.fixed[i]};
+    if (r.per_xcd > r.whole) g[n++] = {units += (int64_t)(r.per_xcd - r.whole) * r.parts, r.len * c.alone[i], c.fixed[i]};
+  }
+  double longest = 0.0;
+  for (int s = -1; s < n - 1; s++) {   // the compute units at which a group begins have the longest lists
+    double work = 0.0, fixed = 0.0, gain = 0.0;
+    int on = 0, at = 0;
+    for (int64_t u = (s < 0 ? 0 : g[s].end) % cus; u < units; u += cus, on++) {
+      while (u >= g[at].end) at++;
+      work += g[at].work;
+      fixed = std::max(fixed, g[at].fixed);
+      gain = (1.0 - c.shared[0] / (per_cu * c.alone[0])) * on / std::max(per_cu - 1, 1);
+    }
+    longest = std::max(longest, work * (1.0 - gain) + fixed);
+  }
+  return longest;
+}
+
 double launch_us(const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t cus, int per_cu, const StepCost& c) {
-  const bool alone = k.units + q.units <= cus;
+  const bool one_round = k.units + q.units <= cus * per_cu;
   Places p(cus * per_cu);
   double us = 0.0;
   for (int i = 0; i < 2; i++) {
     const xdit::BwdRole& r = i ? q : k;
-    const double step = (alone ? c.alone : c.shared)[i];
     if (r.total == 0) continue;
-    if (r.whole) p.run(r.whole, r.steps * step + c.fixed[i]);
-    if (r.per_xcd > r.whole) p.run((int64_t)(r.per_xcd - r.whole) * r.parts, r.len * step + c.fixed[i]);
+    if (!one_round) {
+      if (r.whole) p.run(r.whole, r.steps * c.shared[i] + c.fixed[i]);
+      if (r.per_xcd > r.whole) p.run((int64_t)(r.per_xcd - r.whole) * r.parts, r.len * c.shared[i] + c.fixed[i]);
+    }
     if (r.parts > 1) us += 8.0 * (r.per_xcd - r.whole) * r.parts * (2 - i) * c.part;
   }
-  return p.end() + us + (k.parts > 1 || q.parts > 1 ? 4.0 : 0.0);
+  return (one_round ? one_round_us(k, q, cus, per_cu, c) : p.end()) + us + (k.parts > 1 || q.parts > 1 ? 4.0 : 0.0);
 }
 
 void set_parts(xdit::BwdRole& r, int whole, int parts) {
@@ -150,9 +178,9 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
     r->per_xcd = (r->total + 7) / 8;
     set_parts(*r, r->per_xcd, 1);
   }
-  // measured: 8 and 16 heads of 16384 rows on 4096 and of 4096 on 16384, 3 of 1536 on 1536; fp32: 8 and 16 of 4096 at head_dims 64, 72 and 128, whose steps
+  // measured: 8 and 16 heads of 16384 rows on 4096 and of 4096 on 16384, 8 to 48 of 2048 on 2048 and 4096, 3 of 1536 on 1536; fp32: 8 and 16 of 4096 at head_dims 64, 72 and 128, whose steps
   // take what their matrix instructions do (over the columns that are contracted and those of the gradients)
-  StepCost cost = a->D <= 64 ? StepCost{{1.42, 1.2}, {2.99, 2.35}, {6.0, 5.0}, 0.0} : StepCost{{2.07, 1.77}, {3.56, 2.8}, {7.0, 5.5}, 0.0};
+  StepCost cost = a->D <= 64 ? StepCost{{1.15, 1.0}, {2.99, 2.35}, {6.0, 5.0}, 0.0} : StepCost{{1.95, 1.62}, {3.56, 2.8}, {7.0, 5.5}, 0.0};
   if (f32) {
     const int contracted = a->D > 64 && a->D <= 80 ? 80 : dc;
     const double k = 0.0158 * (2 * contracted + 2 * dc), q = 0.017 * (2 * contracted + dc);
