@@ -47,6 +47,9 @@ constexpr int kBwdStatRows = 64;  // rows of a workgroup of the statistics kerne
 constexpr int kBwdWaves = 4;      // wavefronts of a workgroup, 32 owned rows each
 constexpr int kBwdRows = 32 * kBwdWaves;
 
+// fp32: groups of 8 columns that a head_dim is computed with (72 is a model's own); its gradients have blocks of 16.
+inline int bwd_f32_groups(int D) { return D <= 32 ? 4 : D == 72 ? 9 : (D + 15) / 16 * 2; }
+
 // Blocks of kBwdStatRows rows of a (batch, head)'s values, both segments.
 __host__ __device__ __forceinline__ int bwd_value_blocks(const AttnBwdParams& p) {
   return (p.Sk + kBwdStatRows - 1) / kBwdStatRows + (p.Sk2 + kBwdStatRows - 1) / kBwdStatRows;

@@ -161,7 +161,7 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   BwdPlan plan;
   const bool f32 = a->dtype == XDIT_DTYPE_FP32;
   const int rows = xdit::kBwdRows, step = f32 ? 32 : 64;
-  const int dc = (a->D + 31) / 32 * 32;
+  const int dc = f32 ? (xdit::bwd_f32_groups(a->D) + 1) / 2 * 16 : (a->D + 31) / 32 * 32;   // computed columns of the gradients
   const int64_t bh = (int64_t)a->B * a->H;
   const int per_cu = f32 ? (a->D <= 96 ? 2 : 1) : a->D <= 64 ? 3 : 2;   // workgroups on a compute unit
   const int64_t cus = (xdit::resident_cus(a->cu_count) + 7) / 8;   // of an XCD
@@ -182,7 +182,7 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   // take what their matrix instructions do (over the columns that are contracted and those of the gradients)
   StepCost cost = a->D <= 64 ? StepCost{{1.15, 1.0}, {2.99, 2.35}, {6.0, 5.0}, 0.0} : StepCost{{1.95, 1.62}, {3.56, 2.8}, {7.0, 5.5}, 0.0};
   if (f32) {
-    const int contracted = a->D > 64 && a->D <= 80 ? 80 : dc;
+    const int contracted = 8 * xdit::bwd_f32_groups(a->D);
     const double k = 0.0158 * (2 * contracted + 2 * dc), q = 0.017 * (2 * contracted + dc);
     cost = StepCost{{k, q}, {per_cu * 0.94 * k, per_cu * 0.94 * q}, {8.0, 6.0}, 0.0};
   }
