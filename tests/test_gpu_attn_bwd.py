@@ -62,7 +62,7 @@ SHAPES = [(1, 1, 64, 64, 0), (1, 2, 64, 256, 0), (2, 3, 130, 77, 0), (1, 1, 1, 1
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("D", [8, 32, 40, 64, 72, 96, 104, 128])
+@pytest.mark.parametrize("D", [8, 32, 40, 64, 72, 80, 96, 104, 128])
 def test_head_dims(gpu, dtype, D):
     t = inputs(gpu, 1, 2, 200, 150, D, 40, dtype, "bshd")
     close(call(*t), *bounds(*t))
