@@ -4,6 +4,8 @@
 // one tensor and finds it by comparing its number with all first chunks at once (they are kernel arguments).  Sums are in 64
 // bits from the first square on (a square of a bf16 or fp32 gradient can leave fp32's range, and 1e9 of them its precision); the conversion
 // to it and the multiply-add take about half of the time that a compute unit waits for the element.  Partial sums are added by one workgroup, in a fixed order.
+// Measured: the norm of 0.89 GB of bf16 136 us (6.6 TB/s), of 2.0 GB of fp32 322 us (6.1); clipping 0.8 GB of bf16 into fp32 474 us, 2.0 GB of fp32 in place 769 us (5.1 either; a copy of
+// 1 GiB: 5.0).  Small lists are the host's: 84 tensors take 16.5 us a norm, 5 of them in the kernels.
 #include "grad_norm.h"
 #include "launchers.h"
 #include "row_ops.h"
