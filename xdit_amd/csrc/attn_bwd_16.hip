@@ -142,14 +142,14 @@ struct ColumnsProducts {
   }
 };
 
-// One unit of a role.  D: the head_dim of the LDS geometry, DC (a multiple of 32) the computed one; columns between the
-// tensors' head_dim and DC are zeros in F and G and in the LDS tiles.
-template <typename T, int D, int DC, bool KEYS>
+// One unit of a role.  D: the head_dim of the LDS geometry, DC (a multiple of 32) that of the gradients, DK (a multiple of 16) the contracted one; columns
+// between the tensors' head_dim and those are zeros in F and G and in the LDS tiles.
+template <typename T, int D, int DC, int DK, bool KEYS>
 __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n, unsigned char* smem) {
   typedef typename Mfma16<T>::vec8 vec8;
   typedef __attribute__((ext_vector_type(4))) T vec4;
   typedef BwdGeom<D> G;
-  constexpr int NW = kBwdWaves, KSTEPS = DC / 16, DBLOCKS = DC / 32, ROWS = kBwdRows;
+  constexpr int NW = kBwdWaves, KSTEPS = DK / 16, DBLOCKS = DC / 32, ROWS = kBwdRows;
 
   const BwdRole& R = KEYS ? p.keys : p.queries;
   BwdUnit unit;
@@ -394,34 +394,37 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
 }
 
 // Workgroup i runs on XCD i % 8: an XCD takes consecutive tiles, so that those of one (batch, head) stream the same rows through one L2.
-template <typename T, int D, int DC>
+template <typename T, int D, int DC, int DK>
 __global__ __launch_bounds__(64 * kBwdWaves, D == 64 ? 3 : 2) void attn_bwd_16_kernel(const AttnBwdParams p) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int xcd = blockIdx.x % 8, n = blockIdx.x / 8;
-  if (n < p.keys.units) bwd_role<T, D, DC, true>(p, xcd, n, smem);
-  else bwd_role<T, D, DC, false>(p, xcd, n - p.keys.units, smem);
+  if (n < p.keys.units) bwd_role<T, D, DC, DK, true>(p, xcd, n, smem);
+  else bwd_role<T, D, DC, DK, false>(p, xcd, n - p.keys.units, smem);
 }
 
-template <typename T, int D, int DC>
+template <typename T, int D, int DC, int DK = DC>
 hipError_t launch_kernels(const AttnBwdParams& p, hipStream_t stream) {
   static std::atomic<bool> lds_ready[kMaxDevices];
   constexpr int lds = 2 * BwdGeom<D>::BUF_BYTES;
   static_assert(lds >= kBwdWaves * kBwdStageBytes, "staging blocks");
   const int slot = current_device_slot();
   if (!lds_ready[slot].load(std::memory_order_relaxed)) {  // > 64 KiB of dynamic LDS must be enabled once per kernel and device
-    hipError_t e = hipFuncSetAttribute((const void*)attn_bwd_16_kernel<T, D, DC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipError_t e = hipFuncSetAttribute((const void*)attn_bwd_16_kernel<T, D, DC, DK>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     lds_ready[slot].store(true, std::memory_order_relaxed);
   }
   launch_bwd_stats<T>(p, stream);
-  hipLaunchKernelGGL((attn_bwd_16_kernel<T, D, DC>), dim3(8u * (unsigned)(p.keys.units + p.queries.units)), dim3(64 * kBwdWaves), lds, stream, p);
+  hipLaunchKernelGGL((attn_bwd_16_kernel<T, D, DC, DK>), dim3(8u * (unsigned)(p.keys.units + p.queries.units)), dim3(64 * kBwdWaves), lds, stream, p);
   return launch_bwd_fold<T, DC>(p, stream);
 }
 
+// (Contracting over 80 columns of 96 and 48 of 64: 16 heads of 4096 at head_dim 72 305 us instead of 318, 32 at 40 393 instead of 419.)
 template <typename T>
 hipError_t launch_typed(const AttnBwdParams& p, hipStream_t stream) {
   if (p.D <= 32) return launch_kernels<T, 64, 32>(p, stream);
+  if (p.D <= 48) return launch_kernels<T, 64, 64, 48>(p, stream);
   if (p.D <= 64) return launch_kernels<T, 64, 64>(p, stream);
+  if (p.D <= 80) return launch_kernels<T, 128, 96, 80>(p, stream);
   if (p.D <= 96) return launch_kernels<T, 128, 96>(p, stream);
   return launch_kernels<T, 128, 128>(p, stream);
 }
