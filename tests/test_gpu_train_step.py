@@ -5,12 +5,13 @@ between them: sqrt(8 * 0.036^2 + 0.05^2) = 0.11 relative to float32, held to 0.2
 roundings, each off by at most 2^-8: held to 2^-8."""
 import importlib.util
 import os
+import threading
 
 import pytest
 import torch
 
 from oracle import grad_oracle as O
-from xdit_amd import grad_ops, ops
+from xdit_amd import grad_ops, ops, usp
 
 spec = importlib.util.spec_from_file_location("dit_block", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "dit_block.py"))
 dit = importlib.util.module_from_spec(spec)
@@ -46,6 +47,40 @@ def test_training_step(gpu):
             p -= 0.01 * g
     _, after = dit.training_step(m, x, modulation, positions, r, max_norm=1e9)
     assert torch.isfinite(after) and not torch.equal(after, norm)
+
+
+@pytest.mark.parametrize("own_streams", [True, False])
+def test_two_threads_at_once(gpu, own_streams):
+    """Steps of two threads, of other sizes, on streams of their own or on one: the results of one after the other."""
+    def step(seed):
+        g = torch.Generator(device=gpu).manual_seed(seed)
+        q, k, v, dout = (torch.randn(1, 2 + seed, 500 + 100 * seed, 64, generator=g, device=gpu).half() for _ in range(4))
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        grads = list(torch.autograd.grad(usp.attention(*leaves), leaves, dout))
+        norm = grad_ops.clip_grads(grads, 0.5)
+        return [*grads, norm]
+
+    want = [step(s) for s in (0, 1)]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream() if own_streams else torch.cuda.default_stream()):
+                for _ in range(20):
+                    got[seed] = step(seed)
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for s in (0, 1) for a, b in zip(got[s], want[s]))
 
 
 def test_attention_forward_and_backward_in_one_graph(gpu):
