@@ -477,6 +477,8 @@ typedef struct {
   void* workspace;             /* 8-byte aligned, of the size below, private to the call until its kernels finish */
   int64_t workspace_bytes;
   void* stream;
+  uint32_t* counter;           /* device, 0 before the first call that is given it and left 0 by every one; as private as the workspace.  With it a
+                                  list of one dtype and few elements takes one launch, not two.  May be NULL */
 } xdit_grad_norm_args;
 
 int xdit_grad_norm(const xdit_grad_norm_args* args);

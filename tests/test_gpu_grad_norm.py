@@ -135,6 +135,28 @@ def test_matches_torch_on_a_model(gpu):
         assert bool(((a - p.grad).abs() <= 8 * EPS32 * p.grad.abs() + 1e-6 * p.grad.abs()).all())
 
 
+@pytest.mark.parametrize("kind", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("sizes,mixed", [([3], False), ([72] * 84, False), ([2041] * 184, False), ([2041] * 185, False), ([300000, 7], False), ([2097000], False),
+                                         ([2200000], False), ([50, 60], True), ([0, 5, 0], False)])
+def test_norm_in_one_launch(gpu, sizes, mixed, kind):
+    """Around the border between one launch and two, call after call: the same bits as in the clipping and in a graph, which take their sums another way."""
+    gs = grads(gpu, sizes)
+    gs = [t.bfloat16() if mixed and i else t.float() for i, t in enumerate(gs)]
+    norms = [grad_ops.grad_norm(gs, kind) for _ in range(5)]
+    norm_close(norms[0], O.grad_norm(gs, kind))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = grad_ops.grad_norm(gs, kind)
+    graph.replay()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        norms += [grad_ops.grad_norm(gs, kind) for _ in range(5)]
+    torch.cuda.current_stream().wait_stream(side)
+    clipped = grad_ops.clip_grads([t.clone() for t in gs], 1.0, norm_type=kind)
+    assert all(torch.equal(n, norms[0]) for n in (*norms, captured, clipped))
+
+
 def test_a_list_whose_tensors_move(gpu):
     t = [torch.ones(100, device=gpu), torch.ones(50, device=gpu)]
     g = grad_ops.GradList(t)

@@ -111,7 +111,7 @@ def clip_args(s, d, **kw):
 @pytest.mark.parametrize("kw,needle", [(dict(struct_size=4), "struct_size"), (dict(kind=3), "unknown norm"), (dict(kind=-1), "unknown norm"), (dict(count=-1), "count"),
                                        (dict(count=1 << 25), "count"), (dict(data=None), "table"), (dict(numel=None), "table"), (dict(dtype=None), "table"),
                                        (dict(norm=None), "norm"), (dict(norm=P + 2), "norm"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=8), "workspace"),
-                                       (dict(workspace=P + 4), "workspace")])
+                                       (dict(workspace=P + 4), "workspace"), (dict(counter=P + 2), "counter")])
 def test_norm_refusals(kw, needle):
     t = Table([(P, 5000), (0x9000, 10)])
     refused(_lib.lib().xdit_grad_norm, norm_args(t, **kw), BAD, needle)

@@ -65,6 +65,27 @@ def test_scratch_of_growing_calls(calls):
     assert sum(set(sizes)) < 2 * max(sizes)
 
 
+def test_norms_count_their_workgroups(calls, monkeypatch):
+    """One counter a stream, never one of a captured call's; the norm and the clipping of a list differ in what they are given."""
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+
+    monkeypatch.setattr(grad_ops, "_capturing", lambda device, stream: calls.capturing)
+    monkeypatch.setattr(grad_ops, "_COUNTERS", {})
+    ts = [torch.zeros(6).as_subclass(OnGpu)]
+    given = []
+    run = grad_ops._launch
+    monkeypatch.setattr(grad_ops, "_launch", lambda entry, a, *r, **k: (run(entry, a, *r, **k), given.append(getattr(a, "counter", None))))
+    grad_ops.grad_norm(ts)
+    grad_ops.grad_norm(ts, 1)
+    (c,) = grad_ops._COUNTERS.values()
+    assert given == [c.data_ptr()] * 2 and int(c) == 0
+    calls.capturing = True
+    grad_ops.grad_norm(ts)
+    grad_ops.clip_grads(ts, 1.0)
+    assert given[2:] == [None, None] and len(grad_ops._COUNTERS) == 1
+
+
 def test_gradients_that_are_asked_for(calls):
     q = torch.zeros(1, 2, 8, 64)
     k2 = torch.zeros(1, 2, 3, 64)

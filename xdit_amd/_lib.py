@@ -263,7 +263,7 @@ class AttnBwdArgs(ctypes.Structure):
 class GradNormArgs(ctypes.Structure):
     _fields_ = ([("struct_size", ctypes.c_uint32), ("kind", ctypes.c_int32), ("count", ctypes.c_int64)]
                 + [(n, ctypes.c_void_p) for n in ("data", "numel", "dtype", "norm", "workspace")]
-                + [("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)])
+                + [("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p), ("counter", ctypes.c_void_p)])
 
 
 class ClipGradsArgs(ctypes.Structure):

@@ -20,9 +20,11 @@ struct NormParams {
   int chunk;           // elements of a workgroup
   int kind;            // 0 maximum, 1 sum of sizes, 2 sum of squares
   double* partial;     // one per workgroup, from this launch's first on
+  unsigned* counter;   // not null: the launch's last workgroup to finish adds all partial sums up (there are no others), writes the norm and clears it
+  float* norm;
 };
 
-constexpr int kClipPartials = 1024;  // partial sums that the workgroups of a clipping launch add up by themselves
+constexpr int kClipPartials = 1024;  // partial sums that the workgroups of a clipping launch, or the last one of a norm's, add up by themselves
 
 struct ClipParams {
   GradTable<kClipTensors> t;

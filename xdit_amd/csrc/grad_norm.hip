@@ -5,7 +5,7 @@
 // bits from the first square on (a square of a bf16 or fp32 gradient can leave fp32's range, and 1e9 of them its precision); the conversion
 // to it and the multiply-add take about half of the time that a compute unit waits for the element.  Partial sums are added by one workgroup, in a fixed order.
 // Measured: the norm of 0.89 GB of bf16 136 us (6.6 TB/s), of 2.0 GB of fp32 322 us (6.1); clipping 0.8 GB of bf16 into fp32 474 us, 2.0 GB of fp32 in place 769 us (5.1 either; a copy of
-// 1 GiB: 5.0).  Small lists are the host's: 84 tensors take 16.5 us a norm, 5 of them in the kernels.
+// 1 GiB: 5.0).  Small lists are the host's: 84 tensors take 13.2 us a norm, 6 of them in the kernel.
 #include "grad_norm.h"
 #include "launchers.h"
 #include "row_ops.h"
@@ -62,6 +62,37 @@ __device__ __forceinline__ double workgroup_join(double v) {
   return v;
 }
 
+// The norm of n partial values, for thread 0 of 256 or (more than kClipPartials of them: four loads of each thread in flight; 7084 took 8.1 us with 256
+// threads and a load at a time) 1024; up to that count in the same order either way.
+template <int KIND, int THREADS, class Load>
+__device__ __forceinline__ float norm_of(Load load, int64_t n) {
+  double v = 0.;
+  int64_t i = threadIdx.x;
+  for (; i + 3 * THREADS < n; i += 4 * THREADS) {
+    double x[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = load(i + j * THREADS);
+#pragma unroll
+    for (int j = 0; j < 4; j++) v = norm_join<KIND>(v, x[j]);
+  }
+  for (; i < n; i += THREADS) v = norm_join<KIND>(v, load(i));
+  if constexpr (THREADS > 256) {
+    __shared__ double all[THREADS];
+    all[threadIdx.x] = v;
+    __syncthreads();
+    v = 0.;
+    if (threadIdx.x < 256)
+      for (int j = threadIdx.x; j < THREADS; j += 256) v = norm_join<KIND>(v, all[j]);
+  }
+  v = workgroup_join<KIND, THREADS / 64>(v);
+  return (float)(KIND == 2 ? __builtin_sqrt(v) : v);
+}
+template <int THREADS>
+__device__ __forceinline__ float norm_of(const double* partial, int64_t n, int kind) {
+  auto load = [&](int64_t i) { return partial[i]; };
+  return kind == 0 ? norm_of<0, THREADS>(load, n) : kind == 1 ? norm_of<1, THREADS>(load, n) : norm_of<2, THREADS>(load, n);
+}
+
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void grad_norm_kernel(const NormParams p) {
   const int which = tensor_of(p.t, blockIdx.x);
@@ -94,37 +125,27 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const NormParams p) {
     }
   }
   const double v = workgroup_join<KIND, 4>(norm_join<KIND>(norm_join<KIND>(acc[0], acc[1]), norm_join<KIND>(acc[2], acc[3])));
-  if (threadIdx.x == 0) p.partial[blockIdx.x] = v;
-}
-
-// The norm of n partial values, for thread 0 of 256 or (more than kClipPartials of them: four loads of each thread in flight; 7084 took 8.1 us with 256
-// threads and a load at a time) 1024; up to that count in the same order either way.
-template <int KIND, int THREADS>
-__device__ __forceinline__ float norm_of(const double* partial, int64_t n) {
-  double v = 0.;
-  int64_t i = threadIdx.x;
-  for (; i + 3 * THREADS < n; i += 4 * THREADS) {
-    double x[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) x[j] = partial[i + j * THREADS];
-#pragma unroll
-    for (int j = 0; j < 4; j++) v = norm_join<KIND>(v, x[j]);
+  if (p.counter == nullptr) {
+    if (threadIdx.x == 0) p.partial[blockIdx.x] = v;
+    return;
   }
-  for (; i < n; i += THREADS) v = norm_join<KIND>(v, partial[i]);
-  if constexpr (THREADS > 256) {
-    __shared__ double all[THREADS];
-    all[threadIdx.x] = v;
-    __syncthreads();
-    v = 0.;
-    if (threadIdx.x < 256)
-      for (int j = threadIdx.x; j < THREADS; j += 256) v = norm_join<KIND>(v, all[j]);
+  // The last workgroup to get here adds the sums up, which spares a small list the second launch (84 tensors: 16.5 -> 13.2 us a call, the host's).  Its
+  // accesses are device-scope ones, past the XCDs' caches; every workgroup waits for its store before it counts itself.
+  __shared__ bool latest;
+  if (threadIdx.x == 0) {
+    __hip_atomic_store((unsigned long long*)p.partial + blockIdx.x, __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    latest = __hip_atomic_fetch_add(p.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
   }
-  v = workgroup_join<KIND, THREADS / 64>(v);
-  return (float)(KIND == 2 ? __builtin_sqrt(v) : v);
-}
-template <int THREADS>
-__device__ __forceinline__ float norm_of(const double* partial, int64_t n, int kind) {
-  return kind == 0 ? norm_of<0, THREADS>(partial, n) : kind == 1 ? norm_of<1, THREADS>(partial, n) : norm_of<2, THREADS>(partial, n);
+  __syncthreads();
+  if (!latest) return;
+  const float norm = norm_of<KIND, 256>([&](int64_t i) {
+    return __builtin_bit_cast(double, __hip_atomic_load((const unsigned long long*)p.partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  }, gridDim.x);
+  if (threadIdx.x == 0) {
+    *p.norm = norm;
+    __hip_atomic_store(p.counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
 }
 
 __global__ __launch_bounds__(1024) void grad_norm_total_kernel(const double* partial, int64_t n, int kind, float* norm) {

@@ -281,13 +281,16 @@ int64_t chunk_elements(int64_t count, const int64_t* numel) {
 }
 int64_t chunks_of(int64_t numel, int64_t chunk) { return numel == 0 ? 0 : (numel + 7 + chunk - 1) / chunk; }   // up to 7 elements before its aligned start
 
-// The launches that leave a partial value of every chunk; their count, or a negative status.
-int64_t launch_partials(int64_t count, const void* const* data, const int64_t* numel, const int32_t* dtypes, int kind, double* partial, hipStream_t stream) {
+// The launches that leave a partial value of every chunk; their count, or a negative status.  With a counter and a norm there is one launch, which leaves the norm too.
+int64_t launch_partials(int64_t count, const void* const* data, const int64_t* numel, const int32_t* dtypes, int kind, double* partial, hipStream_t stream,
+                        unsigned* counter = nullptr, float* norm = nullptr) {
   const int64_t chunk = chunk_elements(count, numel);
   const double* const start = partial;
   xdit::NormParams p;
   p.chunk = (int)chunk;
   p.kind = kind;
+  p.counter = counter;
+  p.norm = norm;
   for (int dtype = XDIT_DTYPE_BF16; dtype <= XDIT_DTYPE_FP32; dtype++) {   // a launch holds tensors of one dtype
     int n = 0;
     int64_t chunks = 0;
@@ -319,6 +322,18 @@ int64_t partials_of(int64_t count, const int64_t* numel) {
   int64_t n = 0;
   for (int64_t i = 0; i < count; i++) n += chunks_of(numel[i], chunk);
   return n;
+}
+
+// Whether the norm of a list is one launch's, and its last workgroup can add the partial sums up: tensors of one dtype, as many as a launch takes, few chunks.
+bool one_launch(int64_t count, const int64_t* numel, const int32_t* dtypes, int64_t partials) {
+  int64_t tensors = 0;
+  int dtype = -1;
+  for (int64_t i = 0; i < count; i++) {
+    if (numel[i] == 0) continue;
+    if (tensors++ && dtypes[i] != dtype) return false;
+    dtype = dtypes[i];
+  }
+  return tensors > 0 && tensors <= xdit::kNormTensors && partials <= xdit::kClipPartials;
 }
 
 int check_partials(int64_t n, const void* workspace, int64_t bytes) {
@@ -363,10 +378,13 @@ int xdit_grad_norm(const xdit_grad_norm_args* a) {
   xdit::api_clear_error();
   if (int rc = check_norm_list(a)) return rc;
   if (a->norm == nullptr || reinterpret_cast<uintptr_t>(a->norm) & 3u) return api_fail(XDIT_ERR_INVALID_ARG, "norm is NULL or not 4-byte aligned");
-  if (int rc = check_partials(partials_of(a->count, a->numel), a->workspace, a->workspace_bytes)) return rc;
+  if (reinterpret_cast<uintptr_t>(a->counter) & 3u) return api_fail(XDIT_ERR_INVALID_ARG, "counter is not 4-byte aligned");
+  const int64_t partials = partials_of(a->count, a->numel);
+  if (int rc = check_partials(partials, a->workspace, a->workspace_bytes)) return rc;
   hipStream_t stream = (hipStream_t)a->stream;
-  const int64_t n = launch_partials(a->count, a->data, a->numel, a->dtype, a->kind, (double*)a->workspace, stream);
-  if (n < 0) return (int)n;
+  const bool one = a->counter != nullptr && one_launch(a->count, a->numel, a->dtype, partials);
+  const int64_t n = launch_partials(a->count, a->data, a->numel, a->dtype, a->kind, (double*)a->workspace, stream, one ? a->counter : nullptr, a->norm);
+  if (n < 0 || one) return n < 0 ? (int)n : XDIT_OK;
   const hipError_t e = xdit::launch_grad_norm_total((const double*)a->workspace, n, a->kind, a->norm, stream);
   if (e != hipSuccess) return api_fail(XDIT_ERR_LAUNCH, "gradient norm launch failed: %s", hipGetErrorString(e));
   return XDIT_OK;

@@ -11,7 +11,7 @@ import torch
 
 from . import _lib, ops
 from .block_ops import _plan, _ptr, _scratch
-from .ops import TUNING, _code, _on_device, _sig, _stream, _stream_lock, _strides
+from .ops import TUNING, _capturing, _code, _on_device, _sig, _stream, _stream_lock, _strides
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _GRADS = ("dq", "dk", "dv", "dk2", "dv2")
@@ -194,12 +194,28 @@ def _norm_need(g):
     return g.need
 
 
-def _launch(entry, a, device, need):
+_COUNTERS = {}
+
+
+def _counter(device, stream):
+    """The counter of a norm's workgroups, which every call leaves at zero: one per device and stream for eager calls; captured ones (whose graphs may run beside
+    each other) do without."""
+    if _capturing(device, stream):
+        return None
+    c = _COUNTERS.get((device, stream))
+    if c is None:
+        c = _COUNTERS[(device, stream)] = torch.zeros(1, dtype=torch.int32, device=device)
+    return c.data_ptr()
+
+
+def _launch(entry, a, device, need, counted=False):
     a.stream = stream = _stream(device)
     with _stream_lock(device, stream), _on_device(device):
         if need:
             scratch = _scratch(device, stream, need)
             a.workspace, a.workspace_bytes = scratch.data_ptr(), need
+            if counted:
+                a.counter = _counter(device, stream)
         rc = entry(ctypes.byref(a))
     if rc != 0:
         _lib.check(rc)
@@ -215,7 +231,7 @@ def grad_norm(grads, norm_type=2.0):
     norm = torch.empty((), dtype=torch.float32, device=g.device)
     a = _lib.GradNormArgs(ctypes.sizeof(_lib.GradNormArgs), kind, g.count, ctypes.addressof(g.ptr), ctypes.addressof(g.numel), ctypes.addressof(g.dtype),
                           norm.data_ptr())
-    _launch(_lib.lib().xdit_grad_norm, a, g.device, _norm_need(g))
+    _launch(_lib.lib().xdit_grad_norm, a, g.device, _norm_need(g), counted=True)
     return norm
 
 
