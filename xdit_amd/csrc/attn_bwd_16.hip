@@ -171,19 +171,23 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
   const int own_rows = KEYS ? (second ? p.Sk2 : p.Sk) : p.Sq;
   const int own0 = tile * ROWS + wave * 32;
   const int own = own0 + l32;
-  vec8 f[KSTEPS], g[KSTEPS];
+  // Whole rows side by side in a load; through LDS (below) every lane gets its own row.  (Each lane's own row by loads of 32 bytes a row: a unit of 40 heads of 32760 on 512 keys took 5.3 us to issue them, so 3.3;
+  // the call 1265 us, so 1240.)
+  constexpr int OWN_LOADS = D / 16;
+  vec8 raw_f[OWN_LOADS], raw_g[OWN_LOADS];
   {
-    const int r = own < own_rows ? own : own_rows - 1;
-    const T* fp = (const T*)F.p + b * F.b + h * F.h + (int64_t)r * F.s + hh * 8;
-    const T* gp = (const T*)Gt.p + b * Gt.b + h * Gt.h + (int64_t)r * Gt.s + hh * 8;
+    const int chunk = lane % G::LANES_PER_ROW;
+    const T* fp = (const T*)F.p + b * F.b + h * F.h + chunk * 8;
+    const T* gp = (const T*)Gt.p + b * Gt.b + h * Gt.h + chunk * 8;
 #pragma unroll
-    for (int ks = 0; ks < KSTEPS; ks++) {
-      if (ks * 16 + hh * 8 < p.D) {
-        f[ks] = *(const vec8*)(fp + ks * 16);
-        g[ks] = *(const vec8*)(gp + ks * 16);
-      } else {
+    for (int i = 0; i < OWN_LOADS; i++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[ks][e] = g[ks][e] = (T)0.f;
+      for (int e = 0; e < 8; e++) raw_f[i][e] = raw_g[i][e] = (T)0.f;
+      int r = own0 + (i * 64 + lane) / G::LANES_PER_ROW;
+      r = r < own_rows ? r : own_rows - 1;
+      if (chunk * 8 < p.D) {
+        raw_f[i] = *(const vec8*)(fp + (int64_t)r * F.s);
+        raw_g[i] = *(const vec8*)(gp + (int64_t)r * Gt.s);
       }
     }
   }
@@ -249,8 +253,36 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
     ld_left -= kTileRows;
     if (KEYS) ld_stats += kTileRows;
   };
+  aim(first);
+  issue(0);
+  // The owned rows through the second buffer, which is free until the first step: a wavefront's 32 rows in a block of its own, 16-byte columns exchanged by
+  // the row's number, so that neither the writes nor the reads meet a bank twice.
+  vec8 f[KSTEPS], g[KSTEPS];
+  {
+    XDIT_LDS unsigned char* const stage = (XDIT_LDS unsigned char*)smem + G::BUF_BYTES + wave * 32 * G::ROW_BYTES;
+    static_assert(NW * 32 * G::ROW_BYTES <= G::BUF_BYTES, "owned rows");
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+#pragma unroll
+      for (int i = 0; i < OWN_LOADS; i++) {
+        const int row = (i * 64 + lane) / G::LANES_PER_ROW, chunk = lane % G::LANES_PER_ROW;
+        *(XDIT_LDS vec8*)(stage + row * G::ROW_BYTES + (chunk ^ (row % G::LANES_PER_ROW)) * 16) = which ? raw_g[i] : raw_f[i];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ks++)
+        (which ? g : f)[ks] = *(const XDIT_LDS vec8*)(stage + l32 * G::ROW_BYTES + ((2 * ks + hh) ^ (l32 % G::LANES_PER_ROW)) * 16);
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  // Every wait for the owned rows is here: one inside the loop would be one for the tile loads too.
+#pragma unroll
+  for (int ks = 0; ks < KSTEPS; ks++) asm volatile("" : "+v"(f[ks]), "+v"(g[ks]));
   // Columns that the tensors do not have: zeros, once.
   if (DC > p.D) {
+    __syncthreads();   // all wavefronts have their owned rows
     typedef __attribute__((ext_vector_type(4))) int i32x4;
     const i32x4 zero = {0, 0, 0, 0};
     const int c0 = p.D / 8, n = DC / 8 - c0;
@@ -272,12 +304,6 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
       acc_f[db][e] = 0.f;
       if (KEYS) acc_g[KEYS ? db : 0][e] = 0.f;
     }
-  aim(first);
-  issue(0);
-  // The compiler accounts for the loads of the owned rows here: any wait for them inside the loop would be one for the tile loads too.
-#pragma unroll
-  for (int ks = 0; ks < KSTEPS; ks++) asm volatile("" : "+v"(f[ks]), "+v"(g[ks]));
-
   for (int t = first; t < last; t++) {
     const unsigned bo = ((t - first) & 1) * G::BUF_BYTES;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
