@@ -373,7 +373,7 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
   for (int which = 0; which < (KEYS ? 2 : 1); which++) {   // 0: gradient of F, 1: of G
     const float w = which ? __builtin_ldexpf(1.f, FP16 ? -kFp16Exponent : 0) : __builtin_ldexpf(p.scale, -m);
     if (unit.slot >= 0) {
-      float* prow = R.partial + ((unit.slot * (KEYS ? 2 : 1) + which) * ROWS + wave * 32 + l32) * DC + 4 * hh;
+      f32x4* to = (f32x4*)(R.partial + (unit.slot * (KEYS ? 2 : 1) + which) * ROWS * DC) + wave * (8 * DC) + lane;   // register by register: PartLayout
 #pragma unroll
       for (int db = 0; db < DBLOCKS; db++)
 #pragma unroll
@@ -381,7 +381,7 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
           f32x4 x;
 #pragma unroll
           for (int e = 0; e < 4; e++) x[e] = (which ? acc_g[KEYS ? db : 0] : acc_f[db])[4 * a + e] * w;
-          *(f32x4*)(prow + 32 * db + 8 * a) = x;
+          to[(4 * db + a) * 64] = x;
         }
     } else {
       // Through LDS, 64 columns at a time, so that a store covers whole 128-byte lines of 8 rows.
@@ -441,7 +441,7 @@ hipError_t launch_kernels(const AttnBwdParams& p, hipStream_t stream) {
   }
   launch_bwd_stats<T>(p, stream);
   hipLaunchKernelGGL((attn_bwd_16_kernel<T, D, DC, DK>), dim3(8u * (unsigned)(p.keys.units + p.queries.units)), dim3(64 * kBwdWaves), lds, stream, p);
-  return launch_bwd_fold<T, DC>(p, stream);
+  return launch_bwd_fold<T, DC, 32>(p, stream);
 }
 
 // (Contracting over 80 columns of 96 and 48 of 64: 16 heads of 4096 at head_dim 72 305 us instead of 318, 32 at 40 393 instead of 419.)

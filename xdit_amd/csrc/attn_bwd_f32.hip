@@ -247,12 +247,12 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
     for (int o = 0; o < 2; o++) {
       const int own = own0 + 16 * o;
       float* orow = (float*)O.p + b * O.b + h * O.h + (int64_t)own * O.s;
-      float* prow = R.partial + ((unit.slot * (KEYS ? 2 : 1) + which) * ROWS + wave * 32 + 16 * o + l16) * 16 * CB;
+      f32x4* to = (f32x4*)(R.partial + (unit.slot * (KEYS ? 2 : 1) + which) * ROWS * 16 * CB) + (wave * 2 + o) * (64 * CB) + lane;   // register by register: PartLayout
 #pragma unroll
       for (int cb = 0; cb < CB; cb++) {
         const int col = 16 * cb + 4 * qq;
         const f32x4 x = (which ? acc_g[KEYS ? cb : 0][o] : acc_f[cb][o]) * w;
-        if (unit.slot >= 0) *(f32x4*)(prow + col) = x;
+        if (unit.slot >= 0) to[cb * 64] = x;
         else if (own < own_rows && col < p.D) *(f32x4*)(orow + col) = x;
       }
     }
@@ -279,7 +279,7 @@ hipError_t launch_kernels(const AttnBwdParams& p, hipStream_t stream) {
   }
   launch_bwd_stats<float>(p, stream);
   hipLaunchKernelGGL((attn_bwd_f32_kernel<N8>), dim3(8u * (unsigned)(p.keys.units + p.queries.units)), dim3(64 * kBwdWaves), lds, stream, p);
-  return launch_bwd_fold<float, (N8 + 1) / 2 * 16>(p, stream);
+  return launch_bwd_fold<float, (N8 + 1) / 2 * 16, 16>(p, stream);
 }
 
 }  // namespace

@@ -119,15 +119,32 @@ void launch_bwd_stats(const AttnBwdParams& p, hipStream_t stream) {
   else hipLaunchKernelGGL((bwd_stats_kernel<T, 8>), grid, dim3(256), 0, stream, p);
 }
 
+// A part's result for 128 rows of DC columns, in units of four columns as the accumulators of its wavefronts hold them, so that a store covers 1 KiB (as rows, in
+// pieces of 32 bytes: 4 heads of 1024 32.1 us a call, so 31.2; 24 of 4608 772, so 770).  BLOCK: the columns and rows of an accumulator.
+template <int DC, int BLOCK> struct PartLayout {
+  static __device__ __forceinline__ void place(int i, int& row, int& col) {
+    constexpr int BLOCKS = DC / BLOCK;
+    const int lane = i & 63, m = i >> 6;
+    if (BLOCK == 32) {
+      row = m / (4 * BLOCKS) * 32 + (lane & 31);
+      col = m / 4 % BLOCKS * 32 + m % 4 * 8 + (lane >> 5) * 4;
+    } else {
+      row = m / BLOCKS * 16 + (lane & 15);
+      col = m % BLOCKS * 16 + (lane >> 4) * 4;
+    }
+  }
+};
+
 // Adds the parts of every row of the tiles that were cut up, in their order, and rounds.  Blocks of the keys role first, dk and dv of a tile
 // side by side, then those of the queries role.  The parts' reading bounds it: 63 MB (40 heads of 32760 on 512) 15.6 us, 38 MB (fp32, 16 heads of 1024 at head_dim 72) 8.2.
-template <typename T, int DC>
+template <typename T, int DC, int BLOCK>
 __global__ __launch_bounds__(256) void bwd_fold_kernel(const AttnBwdParams p) {
   typedef __attribute__((ext_vector_type(4))) T vec4;
   constexpr int BLOCKS = kBwdRows * (DC / 4) / 256;   // of a tile's gradient
   int n = blockIdx.x / BLOCKS;
   const int i = (blockIdx.x - n * BLOCKS) * 256 + threadIdx.x;
-  const int row = i / (DC / 4), col = (i % (DC / 4)) * 4;
+  int row, col;
+  PartLayout<DC, BLOCK>::place(i, row, col);
   const int from_keys = p.keys.parts > 1 ? 8 * (p.keys.per_xcd - p.keys.whole) * 2 : 0;
   const bool keys = n < from_keys;
   const BwdRole& R = keys ? p.keys : p.queries;
@@ -145,17 +162,17 @@ __global__ __launch_bounds__(256) void bwd_fold_kernel(const AttnBwdParams p) {
   const int rows = keys ? (second ? p.Sk2 : p.Sk) : p.Sq;
   const int own = tile * kBwdRows + row;
   if (own >= rows || col >= p.D) return;
-  const float* src = R.partial + ((int64_t)cut * R.parts * tensors + which) * kBwdRows * DC + (int64_t)row * DC + col;
+  const float* src = R.partial + ((int64_t)cut * R.parts * tensors + which) * kBwdRows * DC + i * 4;
   f32x4 x = *(const f32x4*)src;
   for (int k = 1; k < R.parts; k++) x += *(const f32x4*)(src + (int64_t)k * tensors * kBwdRows * DC);
   const BwdTensor& O = keys ? (which ? (second ? p.dv2 : p.dv) : (second ? p.dk2 : p.dk)) : p.dq;
   *(vec4*)((T*)O.p + b * O.b + h * O.h + (int64_t)own * O.s + col) = __builtin_convertvector(x, vec4);
 }
 
-template <typename T, int DC>
+template <typename T, int DC, int BLOCK>
 hipError_t launch_bwd_fold(const AttnBwdParams& p, hipStream_t stream) {
   const int tiles = (p.keys.parts > 1 ? 8 * (p.keys.per_xcd - p.keys.whole) * 2 : 0) + (p.queries.parts > 1 ? 8 * (p.queries.per_xcd - p.queries.whole) : 0);
-  if (tiles) hipLaunchKernelGGL((bwd_fold_kernel<T, DC>), dim3((unsigned)tiles * (kBwdRows * (DC / 4) / 256)), dim3(256), 0, stream, p);
+  if (tiles) hipLaunchKernelGGL((bwd_fold_kernel<T, DC, BLOCK>), dim3((unsigned)tiles * (kBwdRows * (DC / 4) / 256)), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
