@@ -165,6 +165,16 @@ def test_gradient_of_the_log_sum_exp(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("shape", [(1, 1, 4100, 3, 0), (1, 1, 5, 4000, 0), (3, 1, 2500, 9, 2), (1, 2, 1000, 1100, 0)])
+@pytest.mark.parametrize("D", [72, 128])
+def test_few_tiles_for_the_whole_chip(gpu, shape, D, dtype):
+    """Fewer tiles than XCDs, cut into many parts."""
+    B, H, Sq, Sk, Sk2 = shape
+    t = inputs(gpu, B, H, Sq, Sk, D, Sk2, dtype)
+    close(call(*t), *bounds(*t))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 def test_rows_that_attended_nothing(gpu, dtype):
     q, k, v, _, _, dout, out, lse = inputs(gpu, 1, 2, 150, 100, 64, 0, dtype)
     lse[:, 0, 10:20] = lse[:, 1, 149] = -math.inf

@@ -14,14 +14,18 @@ struct BwdTensor {  // a logical (B, H, S, D) tensor with a unit stride over D
 
 // The work of one role (see attn_bwd_16.hip).  Every (batch, head) has `tiles` row tiles that stream `steps` tiles each.  An XCD takes
 // `per_xcd` consecutive tiles of all (batch, head)s: the first `whole` of them are one unit each, the ranges of the others are cut into
-// `parts` units of `len` steps, whose fp32 results a launch of its own adds up.
+// `parts` units of `len` steps, whose fp32 results a launch of its own adds up.  Where all tiles are cut (`whole` 0), an XCD takes consecutive
+// units of them instead, so that a few tiles occupy all XCDs.
 struct BwdRole {
   int tiles, steps;
   int total;            // tiles of all (batch, head)s; 0: the role's gradients are not asked for
   int per_xcd, whole, parts, len;
   int units;            // per XCD
-  float* partial;       // [XCD][tile behind `whole`][part][tensor][row][column]
+  float* partial;       // [cut tile][part][tensor][128 rows of computed columns (PartLayout)]
 };
+
+// Tiles that are cut: all of them, or those behind every XCD's `whole` (some of the last XCD's may not exist).
+__host__ __device__ __forceinline__ int bwd_cut_tiles(const BwdRole& r) { return r.parts == 1 ? 0 : r.whole == 0 ? r.total : 8 * (r.per_xcd - r.whole); }
 
 struct AttnBwdParams {
   BwdTensor q, k, v, k2, v2, out, dout;
@@ -60,10 +64,17 @@ struct BwdUnit {
   int tile, part;
   int64_t slot;   // < 0: a whole tile
 };
-__device__ __forceinline__ bool bwd_unit(const BwdRole& r, int xcd, int n, BwdUnit& u) {
+__host__ __device__ __forceinline__ bool bwd_unit(const BwdRole& r, int xcd, int n, BwdUnit& u) {
   int t = n;
   u.part = 0;
   u.slot = -1;
+  if (r.whole == 0 && r.parts > 1) {
+    const int id = xcd * r.units + n;
+    u.tile = id / r.parts;
+    u.part = id - u.tile * r.parts;
+    u.slot = id;
+    return u.tile < r.total;
+  }
   if (n >= r.whole) {
     const int i = (n - r.whole) / r.parts;
     t = r.whole + i;

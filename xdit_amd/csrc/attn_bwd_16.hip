@@ -314,7 +314,7 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
       issue(G::BUF_BYTES - bo);
     }
 #pragma unroll 1
-    for (int hb = 0; hb < 2; hb++) {   // 32 streamed rows at a time
+    for (int hb = own0 < own_rows ? 0 : 2; hb < 2; hb++) {   // 32 streamed rows at a time (a wavefront without rows: none)
       const unsigned ra = row_addr + bo + hb * G::STEP32, ca = col_addr + bo + hb * G::STEP32;
       f32x16 s, dp;
       const XDIT_LDS f32x4* st = (const XDIT_LDS f32x4*)((XDIT_LDS unsigned char*)smem + bo + 2 * G::TENSOR_BYTES + hb * 128 + hh * 16);

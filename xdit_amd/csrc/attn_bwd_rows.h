@@ -145,14 +145,14 @@ __global__ __launch_bounds__(256) void bwd_fold_kernel(const AttnBwdParams p) {
   const int i = (blockIdx.x - n * BLOCKS) * 256 + threadIdx.x;
   int row, col;
   PartLayout<DC, BLOCK>::place(i, row, col);
-  const int from_keys = p.keys.parts > 1 ? 8 * (p.keys.per_xcd - p.keys.whole) * 2 : 0;
+  const int from_keys = bwd_cut_tiles(p.keys) * 2;
   const bool keys = n < from_keys;
   const BwdRole& R = keys ? p.keys : p.queries;
   const int tensors = keys ? 2 : 1;
   if (!keys) n -= from_keys;
   const int which = n % tensors, cut = n / tensors;
   const int xcd = cut / (R.per_xcd - R.whole), t = cut - xcd * (R.per_xcd - R.whole);
-  const int bt = xcd * R.per_xcd + R.whole + t;
+  const int bt = R.whole == 0 ? cut : xcd * R.per_xcd + R.whole + t;
   if (bt >= R.total) return;
   const int bh = bt / R.tiles;
   int tile = bt - bh * R.tiles;
@@ -164,6 +164,7 @@ __global__ __launch_bounds__(256) void bwd_fold_kernel(const AttnBwdParams p) {
   if (own >= rows || col >= p.D) return;
   const float* src = R.partial + ((int64_t)cut * R.parts * tensors + which) * kBwdRows * DC + i * 4;
   f32x4 x = *(const f32x4*)src;
+#pragma unroll 4
   for (int k = 1; k < R.parts; k++) x += *(const f32x4*)(src + (int64_t)k * tensors * kBwdRows * DC);
   const BwdTensor& O = keys ? (which ? (second ? p.dv2 : p.dv) : (second ? p.dk2 : p.dk)) : p.dq;
   *(vec4*)((T*)O.p + b * O.b + h * O.h + (int64_t)own * O.s + col) = __builtin_convertvector(x, vec4);
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(256) void bwd_fold_kernel(const AttnBwdParams p) {
 
 template <typename T, int DC, int BLOCK>
 hipError_t launch_bwd_fold(const AttnBwdParams& p, hipStream_t stream) {
-  const int tiles = (p.keys.parts > 1 ? 8 * (p.keys.per_xcd - p.keys.whole) * 2 : 0) + (p.queries.parts > 1 ? 8 * (p.queries.per_xcd - p.queries.whole) : 0);
+  const int tiles = bwd_cut_tiles(p.keys) * 2 + bwd_cut_tiles(p.queries);
   if (tiles) hipLaunchKernelGGL((bwd_fold_kernel<T, DC, BLOCK>), dim3((unsigned)tiles * (kBwdRows * (DC / 4) / 256)), dim3(256), 0, stream, p);
   return hipGetLastError();
 }

@@ -69,7 +69,7 @@ double one_round_us(const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t cus,
     const xdit::BwdRole& r = i ? q : k;
     if (r.total == 0) continue;
     if (r.whole) g[n++] = {units += r.whole, r.steps * c.alone[i], c.fixed[i]};
-    if (r.per_xcd > r.whole) g[n++] = {units += (int64_t)(r.per_xcd - r.whole) * r.parts, r.len * c.alone[i], c.fixed[i]};
+    if (r.per_xcd > r.whole) g[n++] = {units += r.units - r.whole, r.len * c.alone[i], c.fixed[i]};
   }
   double longest = 0.0;
   for (int s = -1; s < n - 1; s++) {   // the compute units at which a group begins have the longest lists
@@ -95,9 +95,9 @@ double launch_us(const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t cus, in
     if (r.total == 0) continue;
     if (!one_round) {
       if (r.whole) p.run(r.whole, r.steps * c.shared[i] + c.fixed[i]);
-      if (r.per_xcd > r.whole) p.run((int64_t)(r.per_xcd - r.whole) * r.parts, r.len * c.shared[i] + c.fixed[i]);
+      if (r.per_xcd > r.whole) p.run(r.units - r.whole, r.len * c.shared[i] + c.fixed[i]);
     }
-    if (r.parts > 1) us += 8.0 * (r.per_xcd - r.whole) * r.parts * (2 - i) * c.part;
+    us += (double)xdit::bwd_cut_tiles(r) * r.parts * (2 - i) * c.part;
   }
   return (one_round ? one_round_us(k, q, cus, per_cu, c) : p.end()) + us + (k.parts > 1 || q.parts > 1 ? 4.0 : 0.0);
 }
@@ -107,7 +107,7 @@ void set_parts(xdit::BwdRole& r, int whole, int parts) {
   r.len = (r.steps + parts - 1) / parts;
   r.parts = r.whole == r.per_xcd ? 1 : (r.steps + r.len - 1) / r.len;
   if (r.parts == 1) { r.whole = r.per_xcd; r.len = r.steps; }
-  r.units = r.total ? r.whole + (r.per_xcd - r.whole) * r.parts : 0;
+  r.units = r.total == 0 ? 0 : r.whole == 0 ? (r.total * r.parts + 7) / 8 : r.whole + (r.per_xcd - r.whole) * r.parts;
 }
 
 constexpr int kParts[] = {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
@@ -122,7 +122,7 @@ void plan_role(xdit::BwdRole& r, const xdit::BwdRole& k, const xdit::BwdRole& q,
     if (parts > r.steps) break;
     int64_t cut = r.per_xcd;
     for (int round = 0; cut > 0 && round < (last ? 4 : 1); round++) {
-      if (cut * parts <= 4 * cus * per_cu) {
+      if ((cut == r.per_xcd ? (int64_t)r.total * parts / 8 : cut * parts) <= 4 * cus * per_cu) {
         set_parts(r, r.per_xcd - (int)cut, parts);
         const double us = launch_us(k, q, cus, per_cu, c);
         if (us < best_us * 0.99) { best_us = us; best = r; }
@@ -191,7 +191,7 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   p.sq_pad = (int)((a->Sq + xdit::kBwdStatRows - 1) / xdit::kBwdStatRows * xdit::kBwdStatRows);
   plan.stats = align256(bh * 2 * p.sq_pad * 4);
   plan.amax = a->dtype == XDIT_DTYPE_FP16 ? align256(bh * (2 * (p.sq_pad / xdit::kBwdStatRows) + xdit::bwd_value_blocks(p)) * 4) : 0;
-  auto partial = [&](const xdit::BwdRole& r, int tensors) { return r.parts > 1 ? 8 * (int64_t)(r.per_xcd - r.whole) * r.parts * tensors * rows * dc * 4 : 0; };
+  auto partial = [&](const xdit::BwdRole& r, int tensors) { return (int64_t)xdit::bwd_cut_tiles(r) * r.parts * tensors * rows * dc * 4; };
   plan.keys = partial(p.keys, 2);
   plan.queries = partial(p.queries, 1);
   return plan;
