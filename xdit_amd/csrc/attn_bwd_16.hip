@@ -313,8 +313,9 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
       if (!KEYS && t + 1 == p.step1) aim(t + 1);   // the second segment's first tile
       issue(G::BUF_BYTES - bo);
     }
+    const int halves = own0 >= own_rows ? 0 : left > 32 ? 2 : 1;
 #pragma unroll 1
-    for (int hb = own0 < own_rows ? 0 : 2; hb < 2; hb++) {   // 32 streamed rows at a time (a wavefront without rows: none)
+    for (int hb = 0; hb < halves; hb++) {   // 32 streamed rows at a time, those that there are
       const unsigned ra = row_addr + bo + hb * G::STEP32, ca = col_addr + bo + hb * G::STEP32;
       f32x16 s, dp;
       const XDIT_LDS f32x4* st = (const XDIT_LDS f32x4*)((XDIT_LDS unsigned char*)smem + bo + 2 * G::TENSOR_BYTES + hb * 128 + hh * 16);
