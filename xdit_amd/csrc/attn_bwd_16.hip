@@ -16,8 +16,8 @@
 // Workgroups have four wavefronts, two of them share a compute unit (three at head_dim 64): with eight wavefronts in step 5 heads of 32760 tokens took
 // 3939 us in the queries role, with four 3596, 24 heads of 4250 x 2 at head_dim 64 1010 and 877 us in both.
 //
-// The matrix rate under the power limit bounds long rows: bf16, 5 heads of 32760 at head_dim 128 take 7.79 ms, 1.23 PFLOP/s over the seven products where a library
-// product of 8192^3 reaches 1.33 (matrix pipe busy 69 % at 1.6 GHz, no LDS bank conflicts); 24 heads of 4608 805 us, 1.13. fp16, 48 heads of 4250 at head_dim 64: 816 us, 0.95.
+// The matrix rate under the power limit bounds long rows: bf16, 5 heads of 32760 at head_dim 128 take 7.5 to 7.8 ms, 1.23 to 1.28 PFLOP/s over the seven products where a library
+// product of 8192^3 reaches 1.33 (matrix pipe busy 68 % at 1.7 GHz, no LDS bank conflicts); 24 heads of 4608 767 to 800 us, 1.14 to 1.19. fp16, 48 heads of 4250 at head_dim 64: 766 to 816 us.
 //
 // MFMA orientation (v_mfma_f32_32x32x16; A is 32x16, B is 16x32, lane l holds row/column l%32 and contraction elements
 // 8*(l/32)..+7; the result puts column l%32 and rows 8*(i/4) + 4*(l/32) + i%4, i = 0..15, in lane l).  X, Y: the streamed tensors
