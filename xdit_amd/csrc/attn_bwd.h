@@ -38,15 +38,15 @@ struct AttnBwdParams {
   float scale;
   int sq_pad;         // Sq rounded up to whole tiles
   float* stats;       // workspace: per (batch, head) lse / ln 2 of every row (fp16: less kFp16Exponent), then -delta of every row, sq_pad of each
-  float* amax;        // workspace, fp16: of every block of kBwdStatRows rows of every (batch, head) the largest |dout|; then the largest |delta|; then |v|
+  float* value_norms; // workspace, fp16: of every block of kBwdStatRows keys of every (batch, head) the largest norm of a row of v
   int tiles1;         // row tiles of the first segment of keys
   int step1;          // streamed tiles of the first segment of keys
   BwdRole keys;       // row tiles of keys, queries streamed: dk and dv
   BwdRole queries;    // row tiles of queries, keys streamed: dq
 };
 
-// fp16's numbers end at 2^-24, and P and dS are small: P is computed times 2^13 (it stays below 2^14) where it is rounded (attn_bwd_16.hip).
-constexpr int kFp16Exponent = 13;
+// fp16's numbers end at 2^-24, and P is small: it is computed times 2^15 (it stays below 65504, fp16's last number, up to 1.999) where it is rounded (attn_bwd_16.hip).
+constexpr int kFp16Exponent = 15;
 constexpr int kBwdStatRows = 64;  // rows of a workgroup of the statistics kernel
 constexpr int kBwdWaves = 4;      // wavefronts of a workgroup, 32 owned rows each
 constexpr int kBwdRows = 32 * kBwdWaves;

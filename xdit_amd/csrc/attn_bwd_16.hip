@@ -55,30 +55,50 @@ template <int D> struct BwdGeom {
   static constexpr int STEP8 = 2 * PITCH;                        // +8 rows where bit 3 of the row is clear
 };
 
-// fp16: P is computed times 2^13 in the keys role, which is free: the exponent gets it.  dS is computed times 2^m, the largest
-// m up to 13 that keeps it below 2^15 whatever the signs:
-//   |dS_ij| = P_ij |dP_ij - delta_i| <= D max|dout| max|v| + max|delta|      (maxima of a (batch, head); of a chunk of a ring P_ij <= 1 too)
-// The gradients are multiplied by 2^-13 and 2^-m at the end.  The pass over v for its maximum is part of the statistics.
-__device__ __forceinline__ int fp16_exponent(const AttnBwdParams& p, int bh) {
-  __shared__ float tops[3][kBwdWaves];
-  const int64_t heads = (int64_t)p.B * p.H;
-  const int blocks = p.sq_pad / kBwdStatRows;
-  float top[3] = {0.f, 0.f, 0.f};   // |dout|, |delta|, |v|
-#pragma unroll
-  for (int which = 0; which < 3; which++) {
-    const int n = which < 2 ? blocks : bwd_value_blocks(p);
-    const float* from = p.amax + which * heads * blocks + (int64_t)bh * n;
-    for (int i = threadIdx.x; i < n; i += 64 * kBwdWaves) top[which] = fmaxf(top[which], from[i]);
-    for (int m = 1; m < 64; m <<= 1) top[which] = fmaxf(top[which], __shfl_xor(top[which], m));
-    if ((threadIdx.x & 63) == 0) tops[which][threadIdx.x >> 6] = top[which];
-  }
+// fp16: numbers end at 2^-24 and 65504, and P and dS span more than that.  P is computed times 2^15 in the keys role, which is free: the exponent gets it.  dS
+// is computed times 2^m, and a lane owns one row of the result, so that m is the lane's own:
+//   queries role  the row's largest possible dS stays below 2^15, by
+//                 |dS_ij| = P_ij |dP_ij - delta_i| <= |dout_i| max_j |v_j| + |delta_i|      (norms; of a chunk of a ring P_ij <= 1 too)
+//   keys role     a key's dS are those of many queries, of any sizes, and P_ij may be far below 1: m starts at kFp16Most and is lowered (lower_exponent)
+//                 where a dS of the key would come to 2^15, so that this one comes to 2^2 .. 2^3.  What is off by a
+//                 denormal's 2^-25 afterwards is so by 2^-27 of the largest, whose own rounding is 2^-11.
+// (One m for a whole (batch, head), from a bound over all of its rows: 16384 keys at head_dim 128, a row of dout 4000 times the others and
+// a value of 50, the error of the other rows' dq was 1.2e-2 of them, 2.8e-4 with a row's own.  The maximum costs 48 heads of
+// 4250 at head_dim 64 805 us instead of 798.)
+constexpr int kFp16Most = 40;   // a dS of less than 2^-38 at most is below every fp16 result
+
+// The largest norm of a row of v.
+__device__ __forceinline__ float value_norm_of(const AttnBwdParams& p, int bh) {
+  __shared__ float tops[kBwdWaves];
+  const int n = bwd_value_blocks(p);
+  float top = 0.f;   // of the values' norms
+  for (int i = threadIdx.x; i < n; i += 64 * kBwdWaves) top = fmaxf(top, p.value_norms[(int64_t)bh * n + i]);
+  for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
+  for (int i = 0; i < kBwdWaves; i++) top = fmaxf(top, tops[i]);
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
+}
+
+// The queries role's m of a row whose dS stay at or below `most`.
+__device__ __forceinline__ int fp16_exponent(float most) {
+  const int e = (int)(__float_as_uint(most) >> 23 & 255);   // below 2^(e - 126)
+  const int m = e == 255 ? 0 : 141 - e;                     // (not finite: nor is the row)
+  return m > kFp16Most ? kFp16Most : m;
+}
+
+// Where a lane's dS come to 2^15: lowers the exponent of its key, whose other rows the lane 32 away has, and what has been added up.
+template <int DBLOCKS>
+__device__ __forceinline__ void lower_exponent(float top, float& p_to_ds, f32x16& ds, f32x16 (&acc)[DBLOCKS]) {
+  const int e = (int)(__float_as_uint(max_halves(top)) >> 23) - 127;
+  const float less = __builtin_ldexpf(1.f, e >= 15 && e < 128 ? 2 - e : 0);   // (an infinity stays one)
+  p_to_ds *= less;
 #pragma unroll
-  for (int which = 0; which < 3; which++)
-    for (int i = 0; i < kBwdWaves; i++) top[which] = fmaxf(top[which], tops[which][i]);
-  const int e = (int)(__float_as_uint(p.D * top[0] * top[2] + top[1]) >> 23 & 255);   // the bound is below 2^(e - 126)
-  const int m = e == 255 ? 0 : 141 - e;   // (an infinity in dout or v: the rows that it does not reach keep the scale of ordinary ones)
-  return __builtin_amdgcn_readfirstlane(m > kFp16Exponent ? kFp16Exponent : m);
+  for (int i = 0; i < 16; i++) ds[i] *= less;
+#pragma unroll
+  for (int db = 0; db < DBLOCKS; db++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) acc[db][i] *= less;
 }
 
 constexpr int kAhead = 4;  // LDS fragment reads in flight
@@ -194,11 +214,12 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
   const float c = p.scale * kLog2e;
   const float* stats = p.stats + (int64_t)bh * 2 * p.sq_pad;
   constexpr bool FP16 = __is_same(T, _Float16);
-  const int m = FP16 ? fp16_exponent(p, bh) : 0;
-  const float p_to_ds = FP16 && KEYS ? __builtin_ldexpf(1.f, m - kFp16Exponent) : 1.f;
+  const float value_norm = FP16 && !KEYS ? value_norm_of(p, bh) : 0.f;
+  int m = 0;   // fp16, queries role
+  float p_to_ds = FP16 && KEYS ? __builtin_ldexpf(1.f, kFp16Most - kFp16Exponent) : 1.f;
   float own_lse = 0.f, own_nd = 0.f;
   if constexpr (!KEYS) {
-    if (own < p.sq_pad) { own_lse = stats[own] + (FP16 ? (float)(kFp16Exponent - m) : 0.f); own_nd = stats[p.sq_pad + own]; }
+    if (own < p.sq_pad) { own_lse = stats[own]; own_nd = stats[p.sq_pad + own]; }
   }
 
   // ---- tile loads ----
@@ -280,6 +301,15 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
   // Every wait for the owned rows is here: one inside the loop would be one for the tile loads too.
 #pragma unroll
   for (int ks = 0; ks < KSTEPS; ks++) asm volatile("" : "+v"(f[ks]), "+v"(g[ks]));
+  if constexpr (FP16 && !KEYS) {
+    float squares = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ks++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) squares = __builtin_fmaf((float)g[ks][e], (float)g[ks][e], squares);
+    m = fp16_exponent(__builtin_sqrtf(sum_halves(squares)) * value_norm + __builtin_fabsf(own_nd));
+    own_lse += (float)(kFp16Exponent - m);
+  }
   // Columns that the tensors do not have: zeros, once.
   if (DC > p.D) {
     __syncthreads();   // all wavefronts have their owned rows
@@ -331,6 +361,20 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
       }
       rows_products<T, KSTEPS, G::TENSOR_BYTES>(s, dp, f, g, ra);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (FP16 && KEYS) {   // ahead of the other reads: none may be in flight where accumulators change
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          f32x4 x = st[2 * i];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            s[4 * i + e] = fast_exp2(__builtin_fmaf(s[4 * i + e], c, -x[e]));
+            dp[4 * i + e] *= s[4 * i + e] * p_to_ds;
+            top = fmaxf(top, __builtin_fabsf(dp[4 * i + e]));
+          }
+        }
+        if (__builtin_amdgcn_ballot_w64(top >= 32768.f)) lower_exponent(top, p_to_ds, dp, acc_f);
+      }
       ColumnsProducts<T, D, DBLOCKS, KEYS, G::TENSOR_BYTES> columns;
       columns.start(ca);
       vec8 pf[2], df[2];
@@ -346,15 +390,15 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         f32x4 pr, ds;
-        if constexpr (KEYS) {
+        if constexpr (KEYS && !FP16) {
           f32x4 x = st[2 * i];
 #pragma unroll
           for (int e = 0; e < 4; e++) pr[e] = fast_exp2(__builtin_fmaf(s[4 * i + e], c, -x[e]));
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          if (!KEYS) pr[e] = s[4 * i + e];
-          ds[e] = (FP16 && KEYS ? pr[e] * p_to_ds : pr[e]) * dp[4 * i + e];
+          if (!KEYS || FP16) pr[e] = s[4 * i + e];
+          ds[e] = FP16 && KEYS ? dp[4 * i + e] : pr[e] * dp[4 * i + e];
         }
         const vec4 a = __builtin_convertvector(pr, vec4), d = __builtin_convertvector(ds, vec4);
 #pragma unroll
@@ -372,7 +416,7 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
   if (unit.slot < 0) __syncthreads();   // the staging blocks lie over the tiles
 #pragma unroll
   for (int which = 0; which < (KEYS ? 2 : 1); which++) {   // 0: gradient of F, 1: of G
-    const float w = which ? __builtin_ldexpf(1.f, FP16 ? -kFp16Exponent : 0) : __builtin_ldexpf(p.scale, -m);
+    const float w = which ? __builtin_ldexpf(1.f, FP16 ? -kFp16Exponent : 0) : FP16 && KEYS ? p.scale * __builtin_ldexpf(1.f, -kFp16Exponent) / p_to_ds : __builtin_ldexpf(p.scale, -m);
     if (unit.slot >= 0) {
       f32x4* to = (f32x4*)(R.partial + (unit.slot * (KEYS ? 2 : 1) + which) * ROWS * DC) + wave * (8 * DC) + lane;   // register by register: PartLayout
 #pragma unroll

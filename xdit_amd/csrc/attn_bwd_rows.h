@@ -6,38 +6,25 @@
 namespace xdit {
 namespace {
 
-// lse / ln 2 and -delta of every row; rows up to the padded count get (infinity, 0), whose probabilities are zeros.  A row whose
-// log-sum-exp is -infinity attended nothing: the same.  fp16: also the largest |dout| and |delta| of the block's rows; further
-// blocks do so for the values.
-// Reading out and dout bounds it: all loads of a thread are asked for at once, `out`, which nothing reads again, past the caches' replacement order, and where the heads of
-// a token lie side by side, blocks that run together take all heads of their tokens (40 heads of 32760 x 128, BSHD: 139 us with two
-// loads at a time and head by head, 126 so).  LPR: lanes per row, 8 columns each.
-__device__ __forceinline__ void store_top(float top, float* dst) {
-  __shared__ float tops[4];
-  for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) *dst = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  __syncthreads();
-}
-
-// The largest |v| of block n of all (batch, head)s' values.
+// The largest norm of a row of block n of all (batch, head)s' values.
 template <typename T, int LPR>
-__device__ __forceinline__ void value_top(const AttnBwdParams& p, int n) {
+__device__ __forceinline__ void value_norm(const AttnBwdParams& p, int n) {
   constexpr int STEP = 256 / LPR, PASSES = kBwdStatRows / STEP;
   const int blocks = bwd_value_blocks(p), heads = p.B * p.H;
   const bool by_token = p.v.h < p.v.s;
   const int bh = by_token ? n % heads : n / blocks;
   int block = by_token ? n / heads : n - bh * blocks;
   const int b = bh / p.H, h = bh - b * p.H;
-  float* const dst = p.amax + 2 * (int64_t)heads * (p.sq_pad / kBwdStatRows) + (int64_t)bh * blocks + block;
+  float* const dst = p.value_norms + (int64_t)bh * blocks + block;
   const int blocks1 = (p.Sk + kBwdStatRows - 1) / kBwdStatRows;
   const bool second = block >= blocks1;
   if (second) block -= blocks1;
   const BwdTensor& V = second ? p.v2 : p.v;
   const int rows = second ? p.Sk2 : p.Sk, sub = threadIdx.x & (LPR - 1);
   const T* const vp = (const T*)V.p + b * V.b + h * V.h + sub * 8;
-  float top = 0.f;
+  float squares[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; i++) squares[i] = 0.f;
   if (sub * 8 < p.D) {
     Raw8<T> v[PASSES];
 #pragma unroll
@@ -49,18 +36,33 @@ __device__ __forceinline__ void value_top(const AttnBwdParams& p, int n) {
 #pragma unroll
     for (int i = 0; i < PASSES; i++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(v[i][e]));
+      for (int e = 0; e < 8; e++) squares[i] = __builtin_fmaf(v[i][e], v[i][e], squares[i]);
   }
-  store_top(top, dst);
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < PASSES; i++) {
+    for (int m = 1; m < LPR; m <<= 1) squares[i] += __shfl_xor(squares[i], m);
+    top = fmaxf(top, squares[i]);
+  }
+  __shared__ float tops[4];
+  for (int m = LPR; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) *dst = __builtin_sqrtf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
 }
 
+// lse / ln 2 and -delta of every row; rows up to the padded count get (infinity, 0), whose probabilities are zeros.  A row whose
+// log-sum-exp is -infinity attended nothing: the same.  fp16: further blocks look at the values (value_norm).
+// Reading out and dout bounds it: all loads of a thread are asked for at once, `out`, which nothing reads again, past the caches' replacement order, and where the heads of
+// a token lie side by side, blocks that run together take all heads of their tokens (40 heads of 32760 x 128, BSHD: 139 us with two
+// loads at a time and head by head, 126 so).  LPR: lanes per row, 8 columns each.
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void bwd_stats_kernel(const AttnBwdParams p) {
   constexpr int STEP = 256 / LPR, PASSES = kBwdStatRows / STEP;
   const int blocks = p.sq_pad / kBwdStatRows, heads = p.B * p.H;
   constexpr bool FP16 = __is_same(T, _Float16);
   if constexpr (FP16) {
-    if ((int)blockIdx.x >= heads * blocks) return value_top<T, LPR>(p, blockIdx.x - heads * blocks);
+    if ((int)blockIdx.x >= heads * blocks) return value_norm<T, LPR>(p, blockIdx.x - heads * blocks);
   }
   const bool by_token = p.dout.h < p.dout.s;
   const int bh = by_token ? blockIdx.x % heads : blockIdx.x / blocks;
@@ -87,28 +89,19 @@ __global__ __launch_bounds__(256) void bwd_stats_kernel(const AttnBwdParams p) {
     lse[i] = p.lse[b * p.ls_b + h * p.ls_h + row * p.ls_s];
     dlse[i] = p.dlse != nullptr ? p.dlse[b * p.dl_b + h * p.dl_h + row * p.dl_s] : 0.f;
   }
-  float top = 0.f, top_delta = 0.f;
 #pragma unroll
   for (int i = 0; i < PASSES; i++) {
     const int row = row0 + i * STEP;
     float dot = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      dot = __builtin_fmaf(o[i][e], g[i][e], dot);
-      top = fmaxf(top, __builtin_fabsf(g[i][e]));
-    }
+    for (int e = 0; e < 8; e++) dot = __builtin_fmaf(o[i][e], g[i][e], dot);
     for (int m = 1; m < LPR; m <<= 1) dot += __shfl_xor(dot, m);
     const bool live = row < p.Sq && lse[i] != -INFINITY;
-    if (live) top_delta = fmaxf(top_delta, __builtin_fabsf(dlse[i] - dot));
     if (sub == 0) {
       float* st = p.stats + (int64_t)bh * 2 * p.sq_pad + row;
       st[0] = live ? lse[i] * kLog2e - (FP16 ? (float)kFp16Exponent : 0.f) : INFINITY;
       st[p.sq_pad] = live ? dlse[i] - dot : 0.f;
     }
-  }
-  if constexpr (FP16) {
-    store_top(top, p.amax + (int64_t)bh * blocks + block);
-    store_top(top_delta, p.amax + ((int64_t)heads + bh) * blocks + block);
   }
 }
 

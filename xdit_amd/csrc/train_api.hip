@@ -153,8 +153,8 @@ void plan_roles(xdit::AttnBwdParams& p, int64_t cus, int per_cu, const StepCost&
 }
 
 struct BwdPlan {
-  int64_t stats, amax, keys, queries;   // bytes
-  int64_t need() const { return stats + amax + keys + queries; }
+  int64_t stats, norms, keys, queries;   // bytes
+  int64_t need() const { return stats + norms + keys + queries; }
 };
 
 BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
@@ -190,7 +190,7 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   plan_roles(p, cus, per_cu, cost);
   p.sq_pad = (int)((a->Sq + xdit::kBwdStatRows - 1) / xdit::kBwdStatRows * xdit::kBwdStatRows);
   plan.stats = align256(bh * 2 * p.sq_pad * 4);
-  plan.amax = a->dtype == XDIT_DTYPE_FP16 ? align256(bh * (2 * (p.sq_pad / xdit::kBwdStatRows) + xdit::bwd_value_blocks(p)) * 4) : 0;
+  plan.norms = a->dtype == XDIT_DTYPE_FP16 ? align256(bh * xdit::bwd_value_blocks(p) * 4) : 0;
   auto partial = [&](const xdit::BwdRole& r, int tensors) { return (int64_t)xdit::bwd_cut_tiles(r) * r.parts * tensors * rows * dc * 4; };
   plan.keys = partial(p.keys, 2);
   plan.queries = partial(p.queries, 1);
@@ -529,9 +529,9 @@ int xdit_attn_bwd(const xdit_attn_bwd_args* a) {
   p.scale = a->softmax_scale;
   unsigned char* ws = (unsigned char*)a->workspace;
   p.stats = (float*)ws;
-  if (plan.amax) p.amax = (float*)(ws + plan.stats);
-  p.keys.partial = (float*)(ws + plan.stats + plan.amax);
-  p.queries.partial = (float*)(ws + plan.stats + plan.amax + plan.keys);
+  if (plan.norms) p.value_norms = (float*)(ws + plan.stats);
+  p.keys.partial = (float*)(ws + plan.stats + plan.norms);
+  p.queries.partial = (float*)(ws + plan.stats + plan.norms + plan.keys);
   hipStream_t stream = (hipStream_t)a->stream;
   const hipError_t e = a->dtype == XDIT_DTYPE_FP32 ? xdit::launch_attn_bwd_f32(p, stream)
                                                    : xdit::launch_attn_bwd_16(p, a->dtype == XDIT_DTYPE_FP16, stream);
