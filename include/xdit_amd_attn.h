@@ -424,7 +424,8 @@ int xdit_qk_prologue_batch(const xdit_prologue_args* jobs, int32_t count);
  * bf16, fp16 or fp32, head_dim a multiple of 8 up to 128.  P and dS are rounded to dtype for the products, everything else is fp32, each gradient is
  * rounded once.  fp16: scaled by powers of two, dS by one of every query's own for dq and of every key's own for dk, so that neither a large row of dout nor a
  * large value takes bits of other rows; P by 2^15 (a probability below 2^-29 is off by up to 2^-40).  The same call gives the same bits.  dq, or dk and dv (then dk2 and dv2 too where Sk2 > 0), may be NULL: not computed.
- * Gradients must not overlap each other or an input.
+ * Gradients must not overlap each other or an input, which is checked (rows that interleave, as those of views of one buffer, are told apart; where
+ * strides are such that telling would take thousands of steps the call is refused).
  */
 typedef struct {
   uint32_t struct_size;        /* = sizeof(xdit_attn_bwd_args) */

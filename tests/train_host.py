@@ -1,0 +1,26 @@
+"""`train_host.hip` as a library, compiled once a session."""
+import atexit
+import ctypes
+import functools
+import os
+import shutil
+import subprocess
+import tempfile
+
+from xdit_amd import _lib
+from xdit_amd.build import _hipcc
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+@functools.lru_cache(maxsize=None)
+def host():
+    folder = tempfile.mkdtemp()
+    atexit.register(shutil.rmtree, folder, ignore_errors=True)
+    path = os.path.join(folder, "libtrain_host.so")
+    subprocess.check_call([_hipcc(), "-std=c++17", "-O1", "-fPIC", "-shared", "--offload-host-only", "-w", os.path.join(HERE, "train_host.hip"), "-o", path])
+    L = ctypes.CDLL(path)
+    L.host_message.restype = ctypes.c_char_p
+    for name, args in (("xdit_attn_bwd", _lib.AttnBwdArgs), ("xdit_grad_norm", _lib.GradNormArgs), ("xdit_clip_grads", _lib.ClipGradsArgs)):
+        getattr(L, name).argtypes = [ctypes.POINTER(args)]
+    return L

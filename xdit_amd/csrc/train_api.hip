@@ -230,6 +230,92 @@ int check_grad(const char* name, const void* p, const xdit_strides& st, int es, 
   return 0;
 }
 
+// The bytes of a (B, H, S) tensor of rows, from its first one on.
+struct Rows {
+  uintptr_t at;
+  int64_t width;
+  struct { int64_t n, stride; } axis[3];   // bytes
+  __int128 end() const {
+    __int128 e = (__int128)at + width;
+    for (const auto& a : axis) e += (__int128)a.stride * (a.n - 1);
+    return e;
+  }
+};
+
+Rows rows_of(const void* p, int64_t B, int64_t H, int64_t S, const xdit_strides& st, int64_t width, int es) {
+  return {reinterpret_cast<uintptr_t>(p), width * es, {{B, st.b * es}, {H, st.h * es}, {S, st.s * es}}};
+}
+
+// Whether a row of x and one of y share a byte: whether a sum of steps, at most those between two rows of either, leads from x to within a row of y.  Steps are
+// taken from the largest stride down, those only from which the smaller ones still reach: one or two a stride where rows lie as those of views of one buffer do.
+// Where they lie otherwise and 4096 sums were looked at, the answer is that they may.
+bool share_bytes(const Rows& x, const Rows& y) {
+  if ((__int128)x.at >= y.end() || (__int128)y.at >= x.end()) return false;
+  struct Step { __int128 stride; int64_t least, most; } step[6];
+  int n = 0;
+  for (int i = 0; i < 6; i++) {
+    const auto& a = i < 3 ? x.axis[i] : y.axis[i - 3];
+    if (a.n <= 1 || a.stride == 0) continue;
+    int k = 0;
+    while (k < n && step[k].stride != a.stride) k++;
+    if (k == n) step[n++] = {a.stride, 0, 0};
+    if (i < 3) step[k].least -= a.n - 1;
+    else step[k].most += a.n - 1;
+  }
+  std::sort(step, step + n, [](const Step& a, const Step& b) { return a.stride > b.stride; });
+  __int128 below[7], above[7];   // how far the steps from the k-th on lead back and forth
+  below[n] = above[n] = 0;
+  for (int k = n - 1; k >= 0; k--) {
+    below[k] = below[k + 1] + step[k].stride * step[k].least;
+    above[k] = above[k + 1] + step[k].stride * step[k].most;
+  }
+  int budget = 4096;
+  auto meet = [&](auto& self, int k, __int128 d) -> bool {   // d: from a row of x to one of y
+    if (--budget < 0) return true;
+    if (k == n) return d < x.width && -d < y.width;
+    const __int128 st = step[k].stride;
+    for (__int128 c = std::max<__int128>(step[k].least, (-y.width - d - above[k + 1]) / st - 1); c <= step[k].most; c++) {
+      const __int128 at = d + c * st;
+      if (at + above[k + 1] <= -y.width) continue;
+      if (at + below[k + 1] >= x.width) break;
+      if (self(self, k + 1, at)) return true;
+    }
+    return false;
+  };
+  return meet(meet, 0, (__int128)y.at - x.at);
+}
+
+// The same of all gradients and inputs, whatever part of them it is.
+int check_overlaps(const xdit_attn_bwd_args* a) {
+  const int es = a->dtype == XDIT_DTYPE_FP32 ? 4 : 2;
+  Rows in[9], out[5];
+  int inputs = 0, outputs = 0;
+  auto add = [&](Rows* list, int& n, const void* p, int64_t S, const xdit_strides& st) {
+    if (p != nullptr && S > 0) list[n++] = rows_of(p, a->B, a->H, S, st, a->D, es);
+  };
+  add(in, inputs, a->dout, a->Sq, a->dout_stride);
+  add(in, inputs, a->q, a->Sq, a->q_stride);
+  add(in, inputs, a->k, a->Sk, a->k_stride);
+  add(in, inputs, a->v, a->Sk, a->v_stride);
+  add(in, inputs, a->k2, a->Sk2, a->k2_stride);
+  add(in, inputs, a->v2, a->Sk2, a->v2_stride);
+  add(in, inputs, a->out, a->Sq, a->out_stride);
+  in[inputs++] = rows_of(a->lse, a->B, a->H, a->Sq, a->lse_stride, 1, 4);
+  if (a->dlse != nullptr) in[inputs++] = rows_of(a->dlse, a->B, a->H, a->Sq, a->dlse_stride, 1, 4);
+  add(out, outputs, a->dq, a->Sq, a->dq_stride);
+  add(out, outputs, a->dk, a->Sk, a->dk_stride);
+  add(out, outputs, a->dv, a->Sk, a->dv_stride);
+  add(out, outputs, a->dk2, a->Sk2, a->dk2_stride);
+  add(out, outputs, a->dv2, a->Sk2, a->dv2_stride);
+  for (int i = 0; i < outputs; i++) {
+    for (int j = 0; j < inputs; j++)
+      if (share_bytes(out[i], in[j])) return api_fail(XDIT_ERR_INVALID_ARG, "a gradient overlaps an input");
+    for (int j = 0; j < i; j++)
+      if (share_bytes(out[i], out[j])) return api_fail(XDIT_ERR_INVALID_ARG, "two gradients overlap");
+  }
+  return 0;
+}
+
 // A gradient in the place of an input, or two in one place: other workgroups still read what a workgroup writes.
 int check_places(const xdit_attn_bwd_args* a) {
   const void* in[] = {a->dout, a->q, a->k, a->v, a->out, a->lse, a->dlse, a->Sk2 > 0 ? a->k2 : nullptr, a->Sk2 > 0 ? a->v2 : nullptr};
@@ -507,6 +593,7 @@ int xdit_attn_bwd(const xdit_attn_bwd_args* a) {
   const int64_t need = plan.need();
   if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) || a->workspace_bytes < need)
     return api_fail(XDIT_ERR_INVALID_ARG, "workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
+  if ((rc = check_overlaps(a))) return rc;
   p.q = tensor(a->q, a->q_stride);
   p.k = tensor(a->k, a->k_stride);
   p.v = tensor(a->v, a->v_stride);
