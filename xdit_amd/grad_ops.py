@@ -117,7 +117,7 @@ _NORMS = {2.0: _lib.GRADNORM_L2, 1.0: _lib.GRADNORM_L1, math.inf: _lib.GRADNORM_
 
 class _Tables:
     """What the C entry points read of a list of gradients."""
-    __slots__ = ("device", "seen", "sizes", "nbytes", "ptr", "numel", "dtype", "need", "count")
+    __slots__ = ("device", "seen", "sizes", "dtypes", "ptr", "numel", "dtype", "need", "count")
 
     def __init__(self, ts):
         if not ts:
@@ -140,16 +140,15 @@ class _Tables:
         self.sizes = list(map(torch.Tensor.numel, ts))
         self.ptr = (ctypes.c_uint64 * n)(*self.seen)
         self.numel = (ctypes.c_int64 * n)(*self.sizes)
-        self.nbytes = [t.nbytes for t in ts]
-        self.dtype = (ctypes.c_int32 * n)(*(_code(t.dtype) for t in ts))
+        self.dtypes = [t.dtype for t in ts]
+        self.dtype = (ctypes.c_int32 * n)(*map(_code, self.dtypes))
         self.need = None   # workspace bytes of their norm
 
 
 class GradList(collections.abc.Sequence):
     """Gradients that stay where they are from step to step (views of a bucket, or kept by `zero_grad(set_to_none=False)`), with the
-    tables that `grad_norm` and `clip_grads` pass on.  Those of 84 tensors take 40 us of host time to make and 6 us to look whether a tensor has
-    another address or size in bytes than they say; they are made anew then.  (Looking for another order or 16-bit type at the same address and size would take 6 us
-    more: after such a change a new list is needed.)"""
+    tables that `grad_norm` and `clip_grads` pass on.  Those of 84 tensors take 40 us of host time to make and 12 us to look whether a tensor has
+    another address, size, type or order than they say; they are made anew then."""
 
     def __init__(self, tensors):
         if isinstance(tensors, torch.Tensor):
@@ -168,7 +167,8 @@ def _listed(grads):
     if not isinstance(grads, GradList):
         return GradList(grads)._tables
     tables, ts = grads._tables, grads._tensors
-    if list(map(torch.Tensor.data_ptr, ts)) != tables.seen or [t.nbytes for t in ts] != tables.nbytes:
+    if (list(map(torch.Tensor.data_ptr, ts)) != tables.seen or list(map(torch.Tensor.numel, ts)) != tables.sizes
+            or [t.dtype for t in ts] != tables.dtypes or not all(map(torch.Tensor.is_contiguous, ts))):
         tables = grads._tables = _Tables(ts)
     return tables
 
