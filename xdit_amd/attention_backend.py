@@ -172,13 +172,19 @@ def _mi355_fp8_attn_call(query, key, value, dropout_p, is_causal, attention_kwar
     q and k are Hadamard-rotated along head_dim inside the quantiser (block FP8_HADAMARD_BLOCK, or
     attention_kwargs["hadamard_block"]; 0 = off), as the AITER fp8 adapter does (:725-728).
     Inputs that are already float8_e4m3fn take their descales from attention_kwargs
-    ("q_descale", "k_descale", "v_descale")."""
+    ("q_descale", "k_descale", "v_descale").  There is no gradient: a backward pass through the result raises."""
     return _fp8_attn(query, None, key, value, dropout_p, is_causal, attention_kwargs, joint_kv)
 
 
 def _fp8_attn(query, query_tail, key, value, dropout_p, is_causal, attention_kwargs, joint_kv):
     """The adapter above on query rows that may lie in two tensors (16- or 32-bit ones, `query_tail` the
     later rows): the quantiser writes both into the rows of one fp8 tensor, with one scale."""
+    given = (query, query_tail, key, value, *(joint_kv[:2] if joint_kv is not None else ()))
+    return custom_ops.without_gradient(
+        "fp8 attention", lambda: _fp8_attn_fwd(query, query_tail, key, value, dropout_p, is_causal, attention_kwargs, joint_kv), *given)
+
+
+def _fp8_attn_fwd(query, query_tail, key, value, dropout_p, is_causal, attention_kwargs, joint_kv):
     _check_call(dropout_p, is_causal, attention_kwargs)
     kw = attention_kwargs or {}
     scale = query.shape[-1] ** -0.5

@@ -142,6 +142,25 @@ def attn_grad_wanted(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad and t.dtype in (torch.bfloat16, torch.float16, torch.float32) for t in tensors)
 
 
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, call, *tensors):
+        ctx.what = what
+        return call()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("%s has no gradient: call it on detached tensors, or under torch.no_grad()" % ctx.what)
+
+
+def without_gradient(what, call, *tensors):
+    """`call()`, new tensors made of `tensors` by kernels without a backward pass.  Where one of them asks for a gradient, the result's backward pass raises: it would
+    be left out in silence.  (Registered operators without a gradient do so by themselves.)"""
+    if torch.compiler.is_compiling() or not attn_grad_wanted(*tensors):
+        return call()
+    return _NoGradient.apply(what, call, *tensors)
+
+
 class RingAttention(torch.autograd.Function):
     """Attention over all of key, value [, key2, value2] that `call()` computes in its own steps -> (out, lse); the gradient is one backward
     call over the whole key range, from the merged output and log-sum-exp.  `bshd`: query, key, value and out are BSHD, lse is (B, H, Sq) either way."""

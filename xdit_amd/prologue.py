@@ -6,13 +6,15 @@ separate torch kernels (transformer_flux.py:116-147, 170-172; transformer_hunyua
 transformer_wan.py:99-122).  The functions here keep the call surfaces of the pieces they replace
 (diffusers' `apply_rotary_emb`, an RMSNorm module's forward) and add fused forms that do all of
 it in one pass and write straight into the BHSD tensor the attention kernel reads, text and image
-streams side by side (no torch.cat).
+streams side by side (no torch.cat).  They have no gradient: where a tensor asks for one, a backward pass through their result raises
+(`xdit_amd.block.axes_rope` is the differentiable norm and rotation).
 """
 import threading
 
 import torch
 
 from . import ops
+from .custom_ops import without_gradient
 
 
 def _as_bhsd(x, sequence_dim):
@@ -39,16 +41,23 @@ def apply_rotary_emb(x, freqs_cis, use_real=True, use_real_unbind_dim=-1, sequen
     else:
         raise ValueError(f"`use_real_unbind_dim={use_real_unbind_dim}` but should be -1 or -2.")
     xb = _as_bhsd(x, sequence_dim)
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    ops.qk_prologue(xb, rotary_emb=freqs_cis, rope=rope, out=_as_bhsd(out, sequence_dim))
-    return out
+
+    def call():
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        ops.qk_prologue(xb, rotary_emb=freqs_cis, rope=rope, out=_as_bhsd(out, sequence_dim))
+        return out
+
+    return without_gradient("apply_rotary_emb", call, x, *freqs_cis)
 
 
 def apply_rotary_emb_wan(hidden_states, freqs_cos, freqs_sin):
     """The local function of transformer_wan.py:108-120: hidden_states [B,S,H,D], freqs [1,S,1,D]."""
-    out = torch.empty_like(hidden_states, memory_format=torch.contiguous_format)
-    ops.qk_prologue(hidden_states.transpose(1, 2), rotary_emb=(freqs_cos, freqs_sin), rope="wan", out=out.transpose(1, 2))
-    return out
+    def call():
+        out = torch.empty_like(hidden_states, memory_format=torch.contiguous_format)
+        ops.qk_prologue(hidden_states.transpose(1, 2), rotary_emb=(freqs_cos, freqs_sin), rope="wan", out=out.transpose(1, 2))
+        return out
+
+    return without_gradient("apply_rotary_emb_wan", call, hidden_states, freqs_cos, freqs_sin)
 
 
 class RMSNorm(torch.nn.Module):
@@ -69,27 +78,33 @@ class RMSNorm(torch.nn.Module):
         if self.dim > 512:
             # a norm over the un-split projection (all heads of a token): rows of H*D elements
             raise NotImplementedError("use norm_rope(..., norm='token') for a norm across heads")
-        rows = x.reshape(1, 1, -1, self.dim)
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        w = None if self.weight is None else self.weight.detach()
-        ops.qk_prologue(rows, weight=w, eps=self.eps, norm="head", out=out.view(1, 1, -1, self.dim))
-        return out
+
+        def call():
+            rows = x.reshape(1, 1, -1, self.dim)
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            w = None if self.weight is None else self.weight.detach()
+            ops.qk_prologue(rows, weight=w, eps=self.eps, norm="head", out=out.view(1, 1, -1, self.dim))
+            return out
+
+        return without_gradient("prologue.RMSNorm", call, x, self.weight)
 
 
 def norm_rope(x, weight=None, eps=1e-6, freqs_cis=None, sequence_dim=1, norm="head", rope="interleaved",
               rope_row0=0, rope_rows=None, out=None, out_row0=0):
     """norm -> rotary embedding -> BHSD in ONE pass.  x is the head-split projection output
     [B,S,H,D] (sequence_dim=1) or [B,H,S,D] (2).  Writes rows [out_row0, out_row0 + S) of `out`
-    ([B,H,S_total,D]; a new BHSD-contiguous tensor of S rows when omitted) and returns `out`."""
+    ([B,H,S_total,D]; a new BHSD-contiguous tensor of S rows when omitted) and returns `out` (where a tensor
+    asks for a gradient a view of it)."""
     xb = _as_bhsd(x, sequence_dim)
     B, H, S, D = xb.shape
-    if out is None:
-        out = torch.empty((B, H, S, D), dtype=x.dtype, device=x.device)
-        out_row0 = 0
-    dst = out[:, :, out_row0:out_row0 + S]
-    ops.qk_prologue(xb, weight=weight, eps=eps, norm=norm, rotary_emb=freqs_cis, rope=rope,
-                    rope_row0=rope_row0, rope_rows=rope_rows, out=dst)
-    return out
+
+    def call():
+        o, row0 = (torch.empty((B, H, S, D), dtype=x.dtype, device=x.device), 0) if out is None else (out, out_row0)
+        ops.qk_prologue(xb, weight=weight, eps=eps, norm=norm, rotary_emb=freqs_cis, rope=rope,
+                        rope_row0=rope_row0, rope_rows=rope_rows, out=o[:, :, row0:row0 + S])
+        return o
+
+    return without_gradient("norm_rope", call, x, weight, out, *(freqs_cis or ()))
 
 
 _TLS = threading.local()   # cached argument structs are patched in place: one set per thread
@@ -103,6 +118,12 @@ def flux_joint_qkv(query, key, value, encoder_query, encoder_key, encoder_value,
     BHSD.  Inputs are the projection outputs [B,S_img,H*D] and [B,S_txt,H*D]; norm_* are the gain
     vectors (D entries, the tensors' dtype); image_rotary_emb = (cos, sin) of [S_txt+S_img, D].
     Returns q, k, v as BHSD-contiguous [B,H,S_txt+S_img,D]: ONE launch of six jobs, no intermediate tensor."""
+    given = (query, key, value, encoder_query, encoder_key, encoder_value, norm_q, norm_k, norm_added_q, norm_added_k, *image_rotary_emb)
+    return without_gradient("flux_joint_qkv", lambda: _flux_joint_qkv(*given[:6], heads, *given[6:10], image_rotary_emb, eps), *given)
+
+
+def _flux_joint_qkv(query, key, value, encoder_query, encoder_key, encoder_value, heads,
+                    norm_q, norm_k, norm_added_q, norm_added_k, image_rotary_emb, eps):
     srcs = (encoder_query, query, encoder_key, key, encoder_value, value)
     gains = (norm_added_q, norm_q, norm_added_k, norm_k)
     cos, sin = image_rotary_emb

@@ -75,9 +75,14 @@ def update_out_and_lse(out, lse, block_out, block_lse, slice_=None, final_out=No
     """Accumulator update of the ring loop.  block_out (B,S,H,D), block_lse (B,H,S) fp32;
     accumulator `out` fp32 (B,S,H,D) and `lse` fp32 (B,S,H,1).  The first call (out is None)
     creates the accumulator from the block.  `final_out`, if given, also receives the merged rows
-    cast to its dtype (fusing the `out.to(q.dtype)` epilogue)."""
+    cast to its dtype (fusing the `out.to(q.dtype)` epilogue).  Without a gradient: a backward pass through the
+    accumulator raises where a block asked for one (the ring's own call has it)."""
     if slice_ is not None:
         raise NotImplementedError("slice_ is not supported (xDiT never passes it)")
+    return custom_ops.without_gradient("update_out_and_lse", lambda: _update_out_and_lse(out, lse, block_out, block_lse, final_out), out, lse, block_out, block_lse)
+
+
+def _update_out_and_lse(out, lse, block_out, block_lse, final_out):
     B, S, H, D = block_out.shape
     first = out is None
     if first:

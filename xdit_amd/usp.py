@@ -87,16 +87,20 @@ class SDPAMerger:
     """Fold of per-chunk (out, lse) partials in BHSD, fp32 accumulators (torch _SDPAMerger:
     first block stored :161-163, later blocks merged :181-182, results cast back :215-223).
     Each step is one fused HIP pass; `results()` of the last step's cast is fused into that pass
-    when `final_step=True` is given to `step`."""
+    when `final_step=True` is given to `step`.  Without a gradient: a backward pass through the results raises
+    where a block asked for one (`ring_attn` has the gradient of the whole ring)."""
 
     def __init__(self):
         self._out = None
         self._lse = None
         self._final = None
         self._out_dtype = torch.float32
+        self._wanted = []   # blocks that ask for a gradient
 
     def step(self, out, lse, final_step=False):
         self._out_dtype = out.dtype
+        if torch.is_grad_enabled():
+            self._wanted += [t for t in (out, lse) if t.requires_grad]
         first = self._out is None
         if first:
             self._out = torch.empty(out.shape, dtype=torch.float32, device=out.device)
@@ -116,14 +120,14 @@ class SDPAMerger:
     def results(self):
         assert self._out is not None and self._lse is not None
         out = self._final if self._final is not None else self._out.to(self._out_dtype)
-        return out, self._lse
+        return custom_ops.without_gradient("SDPAMerger", lambda: (out, self._lse), *self._wanted)
 
 
 def ring_attn(attention_function, query, key, value, dropout_p=0.0, is_causal=False,
               joint_attn_kwargs=None, attention_kwargs=None, ring_chunks=1, order=None):
     """The ring schedule of usp.py:46-74 on one device.  K/V are split into `ring_chunks`
     contiguous chunks; `order` defaults to what rank 0 sees: [0, P-1, P-2, ..., 1].  On the 16- and 32-bit
-    backend the result is differentiable, joint tensors included."""
+    backend the result is differentiable, joint tensors included; on others a backward pass through it raises."""
     P = ring_chunks
     if key.shape[2] % P != 0:
         raise ValueError(f"key length {key.shape[2]} is not divisible by ring_chunks={P}")
@@ -135,8 +139,9 @@ def ring_attn(attention_function, query, key, value, dropout_p=0.0, is_causal=Fa
     decorated = _DECORATED.get(AttentionBackendType.MI355)
     ours = attention_function is mi355 or (decorated is not None and decorated[0] is mi355 and attention_function is decorated[1])
     joint = joint_attn_kwargs or {}
-    grad = ours and custom_ops.attn_grad_wanted(query, key, value, joint.get("joint_key", None), joint.get("joint_value", None))
-    if grad and P == 1:
+    given = (query, key, value, joint.get("joint_key", None), joint.get("joint_value", None))
+    wanted = custom_ops.attn_grad_wanted(*given)
+    if wanted and ours and P == 1:
         # one block: the merge is the identity, and the call itself has the gradient
         return attention_function(query, key, value, dropout_p=dropout_p, is_causal=is_causal,
                                   joint_attn_kwargs=joint_attn_kwargs, attention_kwargs=attention_kwargs)[0]
@@ -178,8 +183,10 @@ def ring_attn(attention_function, query, key, value, dropout_p=0.0, is_causal=Fa
         return final, acc_lse
 
     call = fused if P > 1 and ops.fused_ring_step_supported(query) and ours else merged
-    if not grad:
+    if not wanted:
         return call()[0]
+    if not ours:
+        return custom_ops.without_gradient("a ring on this attention function", call, *given)[0]
     # one backward call over all keys that the steps take: the chunks, and the joint ones if a step is theirs
     if len(order) != P:
         raise ValueError(f"order has {len(order)} entries, expected {P}")
