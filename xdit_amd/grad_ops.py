@@ -8,6 +8,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib, ops
 from .block_ops import _plan, _ptr, _scratch
@@ -109,6 +110,7 @@ def attn_bwd(dout, q, k, v, out, lse, softmax_scale=None, k2=None, v2=None, dlse
             rc = _lib.lib().xdit_attn_bwd(ctypes.byref(a))
         if rc != 0:
             _lib.check(rc)
+        increment_version([t for t in given.values() if t is not None])   # what autograd has saved of them is seen to have changed
     return tuple(result.get(name) for name in (_GRADS if k2 is not None else _GRADS[:3]))
 
 
@@ -117,7 +119,7 @@ _NORMS = {2.0: _lib.GRADNORM_L2, 1.0: _lib.GRADNORM_L1, math.inf: _lib.GRADNORM_
 
 class _Tables:
     """What the C entry points read of a list of gradients."""
-    __slots__ = ("device", "seen", "sizes", "dtypes", "ptr", "numel", "dtype", "need", "count")
+    __slots__ = ("tensors", "device", "seen", "sizes", "dtypes", "ptr", "numel", "dtype", "need", "count")
 
     def __init__(self, ts):
         if not ts:
@@ -125,6 +127,7 @@ class _Tables:
         for t in ts:
             if not isinstance(t, torch.Tensor):
                 raise ValueError("gradients must be tensors, not %s" % type(t).__name__)
+        self.tensors = ts
         self.device = ts[0].device
         for t in ts:
             if not t.is_cuda:
@@ -256,4 +259,5 @@ def clip_grads(grads, max_norm, norm=None, norm_type=2.0, out=None):
     a = _lib.ClipGradsArgs(ctypes.sizeof(_lib.ClipGradsArgs), float(max_norm), g.count, ctypes.addressof(g.ptr), ctypes.addressof(o.ptr),
                            ctypes.addressof(g.numel), ctypes.addressof(g.dtype), ctypes.addressof(o.dtype), _ptr(norm), result.data_ptr(), kind)
     _launch(_lib.lib().xdit_clip_grads, a, g.device, need)
+    increment_version(o.tensors)
     return result
