@@ -503,7 +503,7 @@ typedef struct {
   const float* norm;           /* device: one fp32; NULL: the norm of src, as xdit_grad_norm computes it */
   float* norm_out;             /* device: one fp32, receives the norm where `norm` is NULL */
   int32_t kind;                /* xdit_grad_norm_kind of that norm */
-  int32_t reserved0;
+  int32_t reserved0;           /* must be 0 */
   void* workspace;             /* for that norm, of the size that xdit_grad_norm_workspace_bytes gives for src */
   int64_t workspace_bytes;
   void* stream;

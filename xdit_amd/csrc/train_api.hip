@@ -482,6 +482,7 @@ int xdit_clip_grads(const xdit_clip_grads_args* a) {
   if (a->struct_size != sizeof(xdit_clip_grads_args))
     return api_fail(XDIT_ERR_INVALID_ARG, "struct_size %u != %zu (ABI mismatch)", a->struct_size, sizeof(xdit_clip_grads_args));
   if (a->count < 0 || a->count > (1 << 24)) return api_fail(XDIT_ERR_INVALID_ARG, "count %lld must lie between 0 and 2^24", (long long)a->count);
+  if (a->reserved0 != 0) return api_fail(XDIT_ERR_INVALID_ARG, "reserved0 must be 0");
   if (!(a->max_norm >= 0.f) || !std::isfinite(a->max_norm)) return api_fail(XDIT_ERR_INVALID_ARG, "max_norm must be finite and >= 0");
   const bool given = a->norm != nullptr;
   if (given ? reinterpret_cast<uintptr_t>(a->norm) & 3u : a->norm_out == nullptr || reinterpret_cast<uintptr_t>(a->norm_out) & 3u)
