@@ -420,7 +420,7 @@ int xdit_qk_prologue_batch(const xdit_prologue_args* jobs, int32_t count);
  *     dk_j = softmax_scale sum_i dS_ij q_i                dq_i = softmax_scale sum_j dS_ij k_j
  * `out` and `lse` are what the forward call gave for the same q, k, v and scale; `dlse` (may be NULL: zeros) is the gradient of lse.
  * With the out, lse and dout of a whole ring it gives one chunk's dk and dv, and that chunk's share of dq.  A row whose lse is
- * -infinity attended nothing: it gives and gets no gradient.
+ * -infinity attended nothing: it gives and gets no gradient, whatever its q, dout and out hold.
  * bf16, fp16 or fp32, head_dim a multiple of 8 up to 128.  P and dS are rounded to dtype for the products, everything else is fp32, each gradient is
  * rounded once.  fp16: scaled by powers of two, dS by one of every query's own for dq and of every key's own for dk, so that neither a large row of dout nor a
  * large value takes bits of other rows; P by 2^15 (a probability below 2^-29 is off by up to 2^-40).  The same call gives the same bits.  dq, or dk and dv (then dk2 and dv2 too where Sk2 > 0), may be NULL: not computed.

@@ -86,3 +86,24 @@ def test_a_row_that_is_not_finite(gpu, dtype, D, bad):
     w = v.clone()
     w[0, 1, 33, 5] = bad
     check(base.call(q, k, w, None, None, dout, out, lse), (every, 33, None))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D,layout", [(64, "bhsd"), (72, "bshd"), (128, "bshd")])
+@pytest.mark.parametrize("rows", [[70], [149], [0, 63, 64, 148, 149], list(range(64, 128)), list(range(150))])
+@pytest.mark.parametrize("cus", [0, 4096])
+def test_what_rows_hold_that_attended_nothing(gpu, dtype, D, layout, rows, cus, monkeypatch):
+    """Rows of q, dout and out whose log-sum-exp is -infinity need not be finite: the gradients have the bits that they have over any numbers there, those rows' own are zeros."""
+    monkeypatch.setitem(base.ops.TUNING, "cu_count", cus)
+    q, k, v, k2, v2, dout, out, lse = t = base.inputs(gpu, 1, 2, 150, 100, D, 30, dtype, layout)
+    lse[:, 1, rows] = -math.inf
+    clean = base.call(*t)
+    base.close(clean, *base.bounds(*t))
+    for bad in ((math.nan,) * 3, (1.0, math.inf, 1.0), (-math.inf, 1.0, math.nan), (1.0, math.nan, math.inf)):
+        fill = [x.clone() for x in (q, dout, out)]
+        for x, b in zip(fill, bad):
+            if b != 1.0:
+                x[:, 1, rows] = b
+        got = base.call(fill[0], k, v, k2, v2, fill[1], fill[2], lse)
+        assert all(torch.equal(a, b) for a, b in zip(got, clean))
+        assert not got[0][:, 1, rows].any()

@@ -144,6 +144,20 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (t + 1 < last) issue(t + 1, G::BUF_BYTES - bo);
+    if constexpr (KEYS) {   // queries that attended nothing, as in the 16-bit kernel
+      XDIT_LDS unsigned char* const buf = tiles + bo;
+      const int rows = p.Sq - t * kRows32;   // of the tensors, from this tile on
+      const unsigned none = (unsigned)__builtin_amdgcn_ballot_w64(((const XDIT_LDS float*)(buf + 2 * G::TENSOR_BYTES))[lane_now() & 31] == INFINITY);
+      if (none << (rows < kRows32 ? kRows32 - rows : 0)) {
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        for (unsigned rest = none; rest != 0; rest &= rest - 1) {
+          const int r = __builtin_ctz(rest), n = lane_now();
+          if (n < G::LANES_PER_ROW)
+            *(XDIT_LDS f32x4*)(buf + G::at(r) + n * 16) = *(XDIT_LDS f32x4*)(buf + G::at(r) + G::TENSOR_BYTES + n * 16) = zero;
+        }
+        __syncthreads();
+      }
+    }
     if (N8 <= 12 && tile * ROWS + wave * 32 >= own_rows) continue;   // a wavefront without rows leaves its SIMD to the other workgroup's (80 heads of 3291 on 3: 209 -> 155 us)
     int left = kRows32;
     if (!KEYS) {
@@ -252,7 +266,8 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
 #pragma unroll
       for (int cb = 0; cb < CB; cb++) {
         const int col = 16 * cb + 4 * qq;
-        const f32x4 x = (which ? acc_g[KEYS ? cb : 0][o] : acc_f[cb][o]) * w;
+        f32x4 x = (which ? acc_g[KEYS ? cb : 0][o] : acc_f[cb][o]) * w;
+        if (!KEYS && own_lse[o] == INFINITY) x = f32x4{0.f, 0.f, 0.f, 0.f};   // a query that attended nothing
         if (unit.slot >= 0) to[cb * 64] = x;
         else if (own < own_rows && col < p.D) *(f32x4*)(orow + col) = x;
       }
