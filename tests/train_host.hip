@@ -34,4 +34,7 @@ int host_share_bytes(const int64_t* x, const int64_t* y) {
   return share_bytes(rows(x), rows(y));
 }
 
+// Groups of 8 columns that an fp32 call of this head_dim is computed with.
+int host_f32_groups(int D) { return xdit::bwd_f32_groups(D); }
+
 }  // extern "C"

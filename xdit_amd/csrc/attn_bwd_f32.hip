@@ -194,8 +194,8 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
             s[r][o] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r][e], f[o][j][e], s[r][o], 0, 0, 0);
             dp[r][o] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[r][e], g[o][j][e], dp[r][o], 0, 0, 0);
           }
-      // (Wide heads: reads of later groups, taken ahead, spill 100 registers at head_dim 96 and cost 1 % at 128.)
-      if (N8 >= 12) __builtin_amdgcn_sched_barrier(0);
+      // (Wide heads: reads of later groups, taken ahead, spill 100 registers at head_dims 88 and 96 and cost 1 % at 128.)
+      if (N8 >= 11) __builtin_amdgcn_sched_barrier(0);
     }
     if (TAIL) {
       const XDIT_LDS unsigned char* const end = buf + G::at(l16) + 64 * WIDE + 8 * qq;
@@ -250,7 +250,7 @@ __device__ __forceinline__ void bwd_role_f32(const AttnBwdParams& p, int xcd, in
             if constexpr (KEYS) acc_g[cb][o] = __builtin_amdgcn_mfma_f32_16x16x4f32(xc[G::TENSOR_BYTES / 4 + 16 * cb], s[r][o][i], acc_g[cb][o], 0, 0, 0);
             acc_f[cb][o] = __builtin_amdgcn_mfma_f32_16x16x4f32(xc[16 * cb], dp[r][o][i], acc_f[cb][o], 0, 0, 0);
           }
-        if (N8 >= 12) __builtin_amdgcn_sched_barrier(0);
+        if (N8 >= 11) __builtin_amdgcn_sched_barrier(0);
       }
   }
 
@@ -303,12 +303,17 @@ hipError_t launch_kernels(const AttnBwdParams& p, hipStream_t stream) {
 hipError_t launch_attn_bwd_f32(const AttnBwdParams& p, hipStream_t stream) {
   switch (bwd_f32_groups(p.D)) {
     case 4: return launch_kernels<4>(p, stream);
+    case 5: return launch_kernels<5>(p, stream);
     case 6: return launch_kernels<6>(p, stream);
+    case 7: return launch_kernels<7>(p, stream);
     case 8: return launch_kernels<8>(p, stream);
     case 9: return launch_kernels<9>(p, stream);
     case 10: return launch_kernels<10>(p, stream);
+    case 11: return launch_kernels<11>(p, stream);
     case 12: return launch_kernels<12>(p, stream);
+    case 13: return launch_kernels<13>(p, stream);
     case 14: return launch_kernels<14>(p, stream);
+    case 15: return launch_kernels<15>(p, stream);
     default: return launch_kernels<16>(p, stream);
   }
 }
