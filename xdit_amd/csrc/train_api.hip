@@ -155,7 +155,13 @@ void plan_roles(xdit::AttnBwdParams& p, int64_t cus, int per_cu, const StepCost&
 struct BwdPlan {
   int64_t stats, norms, keys, queries;   // bytes
   int64_t need() const { return stats + norms + keys + queries; }
+  int64_t workgroups;                    // of the largest launch
 };
+
+// A launch has less than 2^32 threads, 256 of them in a workgroup.
+int check_launches(const BwdPlan& plan) {
+  return plan.workgroups >= (int64_t(1) << 24) ? api_fail(XDIT_ERR_INVALID_ARG, "B*H times the sequence length is too large for one launch") : 0;
+}
 
 BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   BwdPlan plan;
@@ -194,6 +200,9 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
   auto partial = [&](const xdit::BwdRole& r, int tensors) { return (int64_t)xdit::bwd_cut_tiles(r) * r.parts * tensors * rows * dc * 4; };
   plan.keys = partial(p.keys, 2);
   plan.queries = partial(p.queries, 1);
+  const int64_t stats = bh * (p.sq_pad / xdit::kBwdStatRows + (a->dtype == XDIT_DTYPE_FP16 ? xdit::bwd_value_blocks(p) : 0));
+  const int64_t fold = (int64_t)(2 * xdit::bwd_cut_tiles(p.keys) + xdit::bwd_cut_tiles(p.queries)) * (rows * dc / 1024);
+  plan.workgroups = std::max({stats, fold, 8 * (int64_t)(p.keys.units + p.queries.units)});
   return plan;
 }
 
@@ -555,6 +564,7 @@ int64_t xdit_attn_bwd_workspace_bytes(const xdit_attn_bwd_args* a) {
   xdit::AttnBwdParams p;
   std::memset(&p, 0, sizeof(p));
   const BwdPlan plan = plan_bwd(a, p);
+  if (int rc = check_launches(plan)) return rc;
   return plan.need();
 }
 
@@ -591,6 +601,7 @@ int xdit_attn_bwd(const xdit_attn_bwd_args* a) {
   xdit::AttnBwdParams p;
   std::memset(&p, 0, sizeof(p));
   const BwdPlan plan = plan_bwd(a, p);
+  if ((rc = check_launches(plan))) return rc;
   const int64_t need = plan.need();
   if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) || a->workspace_bytes < need)
     return api_fail(XDIT_ERR_INVALID_ARG, "workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
