@@ -37,4 +37,53 @@ int host_share_bytes(const int64_t* x, const int64_t* y) {
 // Groups of 8 columns that an fp32 call of this head_dim is computed with.
 int host_f32_groups(int D) { return xdit::bwd_f32_groups(D); }
 
+// How a call of attention's backward pass is cut up: for either role tiles of a (batch, head), steps, all tiles, tiles of an XCD, of those whole ones, parts, their
+// length, units of an XCD; then the workspace's bytes of partial results of either role.
+void host_plan(const xdit_attn_bwd_args* a, int64_t* out) {
+  xdit::AttnBwdParams p;
+  std::memset(&p, 0, sizeof(p));
+  const BwdPlan plan = plan_bwd(a, p);
+  for (const xdit::BwdRole* r : {&p.keys, &p.queries})
+    for (int64_t x : {r->tiles, r->steps, r->total, r->per_xcd, r->whole, r->parts, r->len, r->units}) *out++ = x;
+  *out++ = plan.keys;
+  *out++ = plan.queries;
+}
+
+// Walks through the units of a plan as the kernels do -> 0, or what is wrong with it first.
+int host_walk(const xdit_attn_bwd_args* a) {
+  xdit::AttnBwdParams p;
+  std::memset(&p, 0, sizeof(p));
+  const BwdPlan plan = plan_bwd(a, p);
+  const int dc = a->dtype == XDIT_DTYPE_FP32 ? (xdit::bwd_f32_groups(a->D) + 1) / 2 * 16 : (a->D + 31) / 32 * 32;
+  for (int role = 0; role < 2; role++) {
+    const xdit::BwdRole& r = role ? p.queries : p.keys;
+    if (r.total == 0) {
+      if (r.units) return 1;   // units of a role that is not asked for
+      continue;
+    }
+    const int64_t cut = xdit::bwd_cut_tiles(r), slots = cut * r.parts;
+    if ((role ? plan.queries : plan.keys) != slots * (2 - role) * xdit::kBwdRows * dc * 4) return 2;   // other than the slots take
+    std::vector<char> steps((size_t)r.total * r.steps, 0), written((size_t)slots, 0);
+    // the tile that the sum of the parts takes a cut one for
+    auto tile_of = [&](int64_t c) { return r.whole == 0 ? c : c / (r.per_xcd - r.whole) * r.per_xcd + r.whole + c % (r.per_xcd - r.whole); };
+    for (int xcd = 0; xcd < 8; xcd++)
+      for (int n = 0; n < r.units; n++) {
+        xdit::BwdUnit u;
+        if (!xdit::bwd_unit(r, xcd, n, u)) continue;
+        const int first = u.slot < 0 ? 0 : u.part * r.len, last = u.slot < 0 || first + r.len > r.steps ? r.steps : first + r.len;
+        if (u.tile < 0 || u.tile >= r.total || first >= last) return 3;   // nothing to do, or no such tile
+        if (u.slot >= slots || (u.slot >= 0 && written[u.slot]++)) return 4;   // a slot outside the workspace, or one twice
+        if (u.slot >= 0 && (tile_of(u.slot / r.parts) != u.tile || u.slot % r.parts != u.part)) return 5;   // added up as another's
+        for (int t = first; t < last; t++)
+          if (steps[(size_t)u.tile * r.steps + t]++) return 6;   // a step twice
+      }
+    for (char c : steps)
+      if (c != 1) return 7;   // a step left out
+    for (int64_t c = 0; c < cut; c++)
+      for (int k = 0; k < r.parts; k++)
+        if (tile_of(c) < r.total && !written[c * r.parts + k]) return 8;   // a part that is added up and that no unit writes
+  }
+  return 0;
+}
+
 }  // extern "C"
