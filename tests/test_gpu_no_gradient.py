@@ -62,3 +62,32 @@ def test_a_training_step_behind_the_prologue(gpu):
     with pytest.raises(RuntimeError, match="no gradient"):
         o.sum().backward()
     assert x.grad is None
+
+
+def traced_calls(gpu):
+    x, w = rand(gpu, 0, 1, 64, 2, 64), rand(gpu, 1, 64)
+    c, s = rand(gpu, 2, 64, 64, dtype=torch.float32), rand(gpu, 3, 64, 64, dtype=torch.float32)
+    m = prologue.RMSNorm(64, device=gpu, dtype=torch.bfloat16)
+    return x, {
+        "norm_rope": lambda x: prologue.norm_rope(2 * x, w, freqs_cis=(c, s)) + 1,
+        "apply_rotary_emb": lambda x: prologue.apply_rotary_emb(2 * x, (c, s), sequence_dim=1) + 1,
+        "apply_rotary_emb_wan": lambda x: prologue.apply_rotary_emb_wan(2 * x, c[None, :, None], s[None, :, None]) + 1,
+        "RMSNorm": lambda x: m(2 * x) + 1,
+        "flux_joint_qkv": lambda x: prologue.flux_joint_qkv(*[2 * x.flatten(2)] * 6, 2, w, w, w, w, (torch.cat((c, c)), torch.cat((s, s))))[0] + 1,
+        "ring": lambda x: usp.ring_attn(lambda q, k, v, **kw: (2 * q, torch.zeros(q.shape[:3], device=q.device)), x, x, x, ring_chunks=2) + 1,
+    }
+
+
+@pytest.mark.parametrize("name", ["norm_rope", "apply_rotary_emb", "apply_rotary_emb_wan", "RMSNorm", "flux_joint_qkv", "ring"])
+def test_traced_calls(gpu, name):
+    x, calls = traced_calls(gpu)
+    torch._dynamo.reset()
+    call = torch.compile(calls[name], backend="aot_eager")
+    with torch.no_grad():
+        plain = calls[name](x)
+        assert torch.equal(call(x), plain)
+    leaf = x.clone().requires_grad_()
+    got = call(leaf)
+    assert torch.equal(got, plain)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        got.float().sum().backward()

@@ -181,7 +181,7 @@ def _fp8_attn(query, query_tail, key, value, dropout_p, is_causal, attention_kwa
     later rows): the quantiser writes both into the rows of one fp8 tensor, with one scale."""
     given = (query, query_tail, key, value, *(joint_kv[:2] if joint_kv is not None else ()))
     return custom_ops.without_gradient(
-        "fp8 attention", lambda: _fp8_attn_fwd(query, query_tail, key, value, dropout_p, is_causal, attention_kwargs, joint_kv), *given)
+        "fp8 attention", lambda: _fp8_attn_fwd(query, query_tail, key, value, dropout_p, is_causal, attention_kwargs, joint_kv), *given, traced=True)
 
 
 def _fp8_attn_fwd(query, query_tail, key, value, dropout_p, is_causal, attention_kwargs, joint_kv):

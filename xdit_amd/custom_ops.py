@@ -153,12 +153,16 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError("%s has no gradient: call it on detached tensors, or under torch.no_grad()" % ctx.what)
 
 
-def without_gradient(what, call, *tensors):
+_refused = torch.compiler.disable(_NoGradient.apply)
+
+
+def without_gradient(what, call, *tensors, traced=False):
     """`call()`, new tensors made of `tensors` by kernels without a backward pass.  Where one of them asks for a gradient, the result's backward pass raises: it would
-    be left out in silence.  (Registered operators without a gradient do so by themselves.)"""
-    if torch.compiler.is_compiling() or not attn_grad_wanted(*tensors):
+    be left out in silence.  In traced code the call is left to Python then, unless it is one of registered operators (`traced`), which raise by themselves."""
+    compiling = torch.compiler.is_compiling()
+    if (compiling and traced) or not attn_grad_wanted(*tensors):
         return call()
-    return _NoGradient.apply(what, call, *tensors)
+    return (_refused if compiling else _NoGradient.apply)(what, call, *tensors)
 
 
 class RingAttention(torch.autograd.Function):
