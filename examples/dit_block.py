@@ -38,8 +38,9 @@ def grid_positions(frames, rows, cols, device):
 
 
 class DiTBlock(torch.nn.Module):
-    def __init__(self, heads, head_dim, mlp, dtype=torch.bfloat16, device="cuda", seed=0, train=False):
+    def __init__(self, heads, head_dim, mlp, dtype=torch.bfloat16, device="cuda", seed=0, train=False, fp32_attention=False):
         super().__init__()
+        self.fp32_attention = fp32_attention   # of a training step
         C = heads * head_dim
         g = torch.Generator(device=device).manual_seed(seed)
 
@@ -65,7 +66,9 @@ class DiTBlock(torch.nn.Module):
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
         q, k = block.axes_rope(q, k, positions, self.freq, self.pairs, norm=True, q_weight=self.q_gain, k_weight=self.k_gain)
         if train:
-            o = usp.attention(q, k, v).transpose(1, 2).reshape(B, S, C)
+            if self.fp32_attention:
+                q, k, v = q.float(), k.float(), v.float()
+            o = usp.attention(q, k, v).to(x.dtype).transpose(1, 2).reshape(B, S, C)
         else:
             o = torch.empty_like(x, memory_format=torch.contiguous_format)
             ops.attn_fwd(q, k, v, out=o.view(B, S, self.heads, self.head_dim).transpose(1, 2), return_lse=False)
@@ -159,9 +162,10 @@ def main():
     p.add_argument("--mlp", type=int, default=8192)
     p.add_argument("--batch", type=int, default=1)
     p.add_argument("--train", action="store_true", help="check the gradients and time a training step instead of the forward pass")
+    p.add_argument("--fp32-attention", action="store_true", help="attention of a training step in float32, forward and backward")
     p.add_argument("--no-check", action="store_true")
     a = p.parse_args()
-    m = DiTBlock(a.heads, a.head_dim, a.mlp, train=a.train)
+    m = DiTBlock(a.heads, a.head_dim, a.mlp, train=a.train, fp32_attention=a.fp32_attention)
     data = inputs(a.grid, a.heads, a.head_dim, a.batch)
     size = "%d tokens, %d heads of %d, MLP %d" % (data[0].shape[1], a.heads, a.head_dim, a.mlp)
     if a.train:
