@@ -1,5 +1,9 @@
 """Calls without a backward pass, next to those that have one: a gradient that is asked for through them is an error, never left out.  On the CPU, with kernels that write
 nothing but a number."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -160,3 +164,8 @@ def test_results_in_a_given_tensor(kernels):
     text = prologue.norm_rope(bshd().requires_grad_(), gain(), out=out)
     both = prologue.norm_rope(bshd().requires_grad_(), gain(), out=text, out_row0=S)
     assert both.data_ptr() == out.data_ptr() and both.requires_grad and not out.requires_grad
+
+
+def test_the_compiler_is_not_imported_for_it():
+    code = "import sys, torch, xdit_amd.attention_backend, xdit_amd.prologue, xdit_amd.ring, xdit_amd.usp; sys.exit('torch._dynamo' in sys.modules)"
+    assert subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__)))).returncode == 0

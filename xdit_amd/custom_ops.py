@@ -153,7 +153,9 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError("%s has no gradient: call it on detached tensors, or under torch.no_grad()" % ctx.what)
 
 
-_refused = torch.compiler.disable(_NoGradient.apply)
+@torch._disable_dynamo   # (torch.compiler.disable would import the compiler here, a second)
+def _untraced(what, call, *tensors):
+    return _NoGradient.apply(what, call, *tensors)
 
 
 def without_gradient(what, call, *tensors, traced=False):
@@ -162,7 +164,7 @@ def without_gradient(what, call, *tensors, traced=False):
     compiling = torch.compiler.is_compiling()
     if (compiling and traced) or not attn_grad_wanted(*tensors):
         return call()
-    return (_refused if compiling else _NoGradient.apply)(what, call, *tensors)
+    return (_untraced if compiling else _NoGradient.apply)(what, call, *tensors)
 
 
 class RingAttention(torch.autograd.Function):
