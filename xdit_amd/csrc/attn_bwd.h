@@ -45,15 +45,16 @@ struct AttnBwdParams {
   BwdRole queries;    // row tiles of queries, keys streamed: dq
 };
 
-// fp16's numbers end at 2^-24, and P is small: it is computed times 2^15 (it stays below 65504, fp16's last number, up to 1.999) where it is rounded (attn_bwd_16.hip).
+// fp16's numbers end at 2^-24, and P is small: it is computed times 2^15 (it stays below 65504, fp16's last number, up to 1.999) where it
+// is rounded (attn_bwd_16.hip).
 constexpr int kFp16Exponent = 15;
 constexpr int kBwdStatRows = 64;  // rows of a workgroup of the statistics kernel
 constexpr int kBwdWaves = 4;      // wavefronts of a workgroup, 32 owned rows each
 constexpr int kBwdRows = 32 * kBwdWaves;
 
-// fp32: groups of 8 columns that a head_dim is computed with, those that it has (up to 32: four, whose others are zeros); its gradients have blocks of 16.  An odd
-// number of them against the even one above it, 16 heads of 4096: head_dim 40 1225 against 1342 us, 56 1643 against 1756, 72 2053 against 2169, 88 2475 against 2600,
-// 104 3165 against 3255, 120 3570 against 3677.
+// fp32: groups of 8 columns that a head_dim is computed with, those that it has (up to 32: four, whose others are zeros); its gradients
+// have blocks of 16.  An odd number of them against the even one above it, 16 heads of 4096: head_dim 40 1225 against 1342 us, 56 1643
+// against 1756, 72 2053 against 2169, 88 2475 against 2600, 104 3165 against 3255, 120 3570 against 3677.
 inline int bwd_f32_groups(int D) { return D <= 32 ? 4 : D / 8; }
 
 // Blocks of kBwdStatRows rows of a (batch, head)'s values, both segments.

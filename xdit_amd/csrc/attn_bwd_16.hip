@@ -9,15 +9,16 @@
 // Work decomposition: bwd_stats_kernel writes lse / ln 2 and -delta of every row, then one launch has the units of two roles:
 //   keys     a workgroup owns 128 keys, wavefront w keys [32w, 32w+32); it streams the queries: dK and dV (four products)
 //   queries  a workgroup owns 128 queries; it streams the keys: dQ (three products)
-// Seven products instead of the five of a single pass: that one adds every workgroup's share of dQ up in memory, by
-// atomics (whose order changes the result) or through Sk / 128 fp32 copies of dQ, which cost as much time as the two products more.
-// The longer units, those of the keys, start first; the last units may be parts of tiles, which even out the end of the launch
-// and let few tiles fill the chip (BwdRole; the parts are added up by bwd_fold_kernel).
-// Workgroups have four wavefronts, two of them share a compute unit (three at head_dim 64): with eight wavefronts in step 5 heads of 32760 tokens took
-// 3939 us in the queries role, with four 3596, 24 heads of 4250 x 2 at head_dim 64 1010 and 877 us in both.
+// Seven products instead of the five of a single pass: that one adds every workgroup's share of dQ up in memory, by atomics (whose order
+// changes the result) or through Sk / 128 fp32 copies of dQ (5 heads of 32760: 21.5 GB written and read again, 8.5 ms at a copy's rate,
+// where the two products more take 2.1). The longer units, those of the keys, start first; the last units may be parts of tiles, which even
+// out the end of the launch and let few tiles fill the chip (BwdRole; the parts are added up by bwd_fold_kernel). Workgroups have four
+// wavefronts, two of them share a compute unit (three at head_dim 64): with eight wavefronts in step 5 heads of 32760 tokens took 3939 us
+// in the queries role, with four 3596, 24 heads of 4250 x 2 at head_dim 64 1010 and 877 us in both.
 //
-// The matrix rate under the power limit bounds long rows: bf16, 5 heads of 32760 at head_dim 128 take 7.5 to 7.8 ms, 1.23 to 1.28 PFLOP/s over the seven products where a library
-// product of 8192^3 reaches 1.33 (matrix pipe busy 68 % at 1.7 GHz, no LDS bank conflicts); 24 heads of 4608 767 to 800 us, 1.14 to 1.19. fp16, 48 heads of 4250 at head_dim 64: 766 to 816 us.
+// The matrix rate under the power limit bounds long rows: bf16, 5 heads of 32760 at head_dim 128 take 7.6 to 7.8 ms, 1.23 to 1.27 PFLOP/s
+// over the seven products where a library product of 8192^3 reaches 1.33 (matrix pipe busy 68 % at 1.7 GHz, no LDS bank conflicts); 24
+// heads of 4608 769 to 800 us, 1.14 to 1.19. fp16, 48 heads of 4250 at head_dim 64: 778 to 805 us.
 //
 // MFMA orientation (v_mfma_f32_32x32x16; A is 32x16, B is 16x32, lane l holds row/column l%32 and contraction elements
 // 8*(l/32)..+7; the result puts column l%32 and rows 8*(i/4) + 4*(l/32) + i%4, i = 0..15, in lane l).  X, Y: the streamed tensors
@@ -55,8 +56,8 @@ template <int D> struct BwdGeom {
   static constexpr int STEP8 = 2 * PITCH;                        // +8 rows where bit 3 of the row is clear
 };
 
-// fp16: numbers end at 2^-24 and 65504, and P and dS span more than that.  P is computed times 2^15 in the keys role, which is free: the exponent gets it.  dS
-// is computed times 2^m, and a lane owns one row of the result, so that m is the lane's own:
+// fp16: numbers end at 2^-24 and 65504, and P and dS span more than that.  P is computed times 2^15 in the keys role, which is free: the
+// exponent gets it.  dS is computed times 2^m, and a lane owns one row of the result, so that m is the lane's own:
 //   queries role  the row's largest possible dS stays below 2^15, by
 //                 |dS_ij| = P_ij |dP_ij - delta_i| <= |dout_i| max_j |v_j| + |delta_i|      (norms; of a chunk of a ring P_ij <= 1 too)
 //   keys role     a key's dS are those of many queries, of any sizes, and P_ij may be far below 1: m starts at kFp16Most and is lowered (lower_exponent)
@@ -128,8 +129,8 @@ __device__ __forceinline__ void rows_products(f32x16& s, f32x16& dp, const typen
   });
 }
 
-// Transposed products over the half's 32 rows, a sequence of fragment reads again: G_PRODUCTS: acc_g[db] += Y_half^T P, then acc_f[db] += X_half^T dS (pf, df:
-// two steps of 16 rows).  The first reads are started by `start`, ahead of the arithmetic that makes P and dS.
+// Transposed products over the half's 32 rows, a sequence of fragment reads again: G_PRODUCTS: acc_g[db] += Y_half^T P, then acc_f[db] +=
+// X_half^T dS (pf, df: two steps of 16 rows).  The first reads are started by `start`, ahead of the arithmetic that makes P and dS.
 template <typename T, int D, int DBLOCKS, bool G_PRODUCTS, int Y_OFF>
 struct ColumnsProducts {
   typedef typename Mfma16<T>::vec8 vec8;
@@ -162,8 +163,8 @@ struct ColumnsProducts {
   }
 };
 
-// One unit of a role.  D: the head_dim of the LDS geometry, DC (a multiple of 32) that of the gradients, DK (a multiple of 16) the contracted one; columns
-// between the tensors' head_dim and those are zeros in F and G and in the LDS tiles.
+// One unit of a role.  D: the head_dim of the LDS geometry, DC (a multiple of 32) that of the gradients, DK (a multiple of 16) the
+// contracted one; columns between the tensors' head_dim and those are zeros in F and G and in the LDS tiles.
 template <typename T, int D, int DC, int DK, bool KEYS>
 __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n, unsigned char* smem) {
   typedef typename Mfma16<T>::vec8 vec8;
@@ -191,8 +192,8 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
   const int own_rows = KEYS ? (second ? p.Sk2 : p.Sk) : p.Sq;
   const int own0 = tile * ROWS + wave * 32;
   const int own = own0 + l32;
-  // Whole rows side by side in a load; through LDS (below) every lane gets its own row.  (Each lane's own row by loads of 32 bytes a row: a unit of 40 heads of 32760 on 512 keys took 5.3 us to issue them, so 3.3;
-  // the call 1265 us, so 1240.)
+  // Whole rows side by side in a load; through LDS (below) every lane gets its own row.  (Each lane's own row by loads of 32 bytes a row: a
+  // unit of 40 heads of 32760 on 512 keys took 5.3 us to issue them, so 3.3; the call 1265 us, so 1240.)
   constexpr int OWN_LOADS = D / 16;
   vec8 raw_f[OWN_LOADS], raw_g[OWN_LOADS];
   {
@@ -276,8 +277,8 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
   };
   aim(first);
   issue(0);
-  // The owned rows through the second buffer, which is free until the first step: a wavefront's 32 rows in a block of its own, 16-byte columns exchanged by
-  // the row's number, so that neither the writes nor the reads meet a bank twice.
+  // The owned rows through the second buffer, which is free until the first step: a wavefront's 32 rows in a block of its own, 16-byte
+  // columns exchanged by the row's number, so that neither the writes nor the reads meet a bank twice.
   vec8 f[KSTEPS], g[KSTEPS];
   {
     XDIT_LDS unsigned char* const stage = (XDIT_LDS unsigned char*)smem + G::BUF_BYTES + wave * 32 * G::ROW_BYTES;
@@ -342,8 +343,8 @@ __device__ __forceinline__ void bwd_role(const AttnBwdParams& p, int xcd, int n,
       if (!KEYS && t + 1 == p.step1) aim(t + 1);   // the second segment's first tile
       issue(G::BUF_BYTES - bo);
     }
-    // Queries that attended nothing: zeros in place of rows that need not be finite, which a probability of zero does not undo.  (Looking at 64 log-sum-exps
-    // a tile: 5 heads of 32760 7543 -> 7590 us, 24 of 4608 766 -> 769.)
+    // Queries that attended nothing: zeros in place of rows that need not be finite, which a probability of zero does not undo.  (Looking
+    // at 64 log-sum-exps a tile: 5 heads of 32760 7543 -> 7590 us, 24 of 4608 766 -> 769.)
     if constexpr (KEYS) {
       XDIT_LDS unsigned char* const buf = (XDIT_LDS unsigned char*)smem + bo;
       const uint64_t none = __builtin_amdgcn_ballot_w64(((const XDIT_LDS float*)(buf + 2 * G::TENSOR_BYTES))[lane_now()] == INFINITY);

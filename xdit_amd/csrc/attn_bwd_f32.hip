@@ -2,14 +2,14 @@
 // (attn_bwd_16.hip) on v_mfma_f32_16x16x4_f32, with everything in fp32.
 //
 // Lane l of that instruction holds row/column l%16 and ONE contraction element, l/16; its result has column l%16 and rows 4*(l/16)..+3 in
-// lane l.  A wavefront's 32 owned rows are two groups of 16, a tile's 32 rows two groups as well.  Contraction over head_dim takes the columns
-// 16j + 4*(l/16) + 0..3 in four steps, so that a lane reads 16 bytes of its row at a time (8 at the end of an odd number of 8-column groups); contraction over
-// streamed rows takes rows 4*(l/16) + i in step i, which is where accumulator register i of P or dS has them.  (Blocks of 16 columns rather than the 32 of
-// v_mfma_f32_32x32x2_f32: head_dim 72 is 72 contracted columns and 80 of the gradients instead of 80 and 96, 16 heads of 4096 take 2055 us
-// instead of 2340; at head_dim 64 both take 1745 us, at 128 3650 and 3615.)
+// lane l.  A wavefront's 32 owned rows are two groups of 16, a tile's 32 rows two groups as well.  Contraction over head_dim takes the
+// columns 16j + 4*(l/16) + 0..3 in four steps, so that a lane reads 16 bytes of its row at a time (8 at the end of an odd number of
+// 8-column groups); contraction over streamed rows takes rows 4*(l/16) + i in step i, which is where accumulator register i of P or dS has
+// them.  (Blocks of 16 columns rather than the 32 of v_mfma_f32_32x32x2_f32: head_dim 72 is 72 contracted columns and 80 of the gradients
+// instead of 80 and 96, 16 heads of 4096 take 2055 us instead of 2340; at head_dim 64 both take 1745 us, at 128 3650 and 3615.)
 //
-// The instruction takes 32 clocks, which bounds the kernel; two workgroups of four wavefronts on a compute unit keep the matrix pipe fed (one at head_dims above 96, whose
-// operands and accumulators take more than 256 registers).
+// The instruction takes 32 clocks, which bounds the kernel; two workgroups of four wavefronts on a compute unit keep the matrix pipe fed
+// (one at head_dims above 96, whose operands and accumulators take more than 256 registers).
 #include "attn_bwd_rows.h"
 #include "attn_split.h"
 #include "attn_tiles.h"
@@ -19,8 +19,9 @@ namespace {
 
 constexpr int kRows32 = 32;   // streamed rows per LDS tile
 
-// LDS layout of a streamed tile, filled by 1 KiB pieces (a direct load writes lane i at 16 i) that lie 16 bytes more apart: rows that are read together (one
-// 16-byte column of 8 consecutive rows, one 64-byte column of rows 4 apart) sit in different pieces, on other banks.  N8: groups of 8 columns.
+// LDS layout of a streamed tile, filled by 1 KiB pieces (a direct load writes lane i at 16 i) that lie 16 bytes more apart: rows that are
+// read together (one 16-byte column of 8 consecutive rows, one 64-byte column of rows 4 apart) sit in different pieces, on other banks.
+// N8: groups of 8 columns.
 template <int N8> struct Geom32 {
   static constexpr int ROW_BYTES = N8 <= 8 ? 256 : 512;
   static constexpr int NG = kRows32 * ROW_BYTES / 1024;

@@ -52,10 +52,10 @@ __device__ __forceinline__ void value_norm(const AttnBwdParams& p, int n) {
 }
 
 // lse / ln 2 and -delta of every row; rows up to the padded count get (infinity, 0), whose probabilities are zeros.  A row whose
-// log-sum-exp is -infinity attended nothing: the same.  fp16: further blocks look at the values (value_norm).
-// Reading out and dout bounds it: all loads of a thread are asked for at once, `out`, which nothing reads again, past the caches' replacement order, and where the heads of
-// a token lie side by side, blocks that run together take all heads of their tokens (40 heads of 32760 x 128, BSHD: 139 us with two
-// loads at a time and head by head, 126 so).  LPR: lanes per row, 8 columns each.
+// log-sum-exp is -infinity attended nothing: the same.  fp16: further blocks look at the values (value_norm). Reading out and dout bounds
+// it: all loads of a thread are asked for at once, `out`, which nothing reads again, past the caches' replacement order, and where the
+// heads of a token lie side by side, blocks that run together take all heads of their tokens (40 heads of 32760 x 128, BSHD: 139 us with
+// two loads at a time and head by head, 126 so).  LPR: lanes per row, 8 columns each.
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void bwd_stats_kernel(const AttnBwdParams p) {
   constexpr int STEP = 256 / LPR, PASSES = kBwdStatRows / STEP;
@@ -112,8 +112,9 @@ void launch_bwd_stats(const AttnBwdParams& p, hipStream_t stream) {
   else hipLaunchKernelGGL((bwd_stats_kernel<T, 8>), grid, dim3(256), 0, stream, p);
 }
 
-// A part's result for 128 rows of DC columns, in units of four columns as the accumulators of its wavefronts hold them, so that a store covers 1 KiB (as rows, in
-// pieces of 32 bytes: 4 heads of 1024 32.1 us a call, so 31.2; 24 of 4608 772, so 770).  BLOCK: the columns and rows of an accumulator.
+// A part's result for 128 rows of DC columns, in units of four columns as the accumulators of its wavefronts hold them, so that a store
+// covers 1 KiB (as rows, in pieces of 32 bytes: 4 heads of 1024 32.1 us a call, so 31.2; 24 of 4608 772, so 770).  BLOCK: the columns and
+// rows of an accumulator.
 template <int DC, int BLOCK> struct PartLayout {
   static __device__ __forceinline__ void place(int i, int& row, int& col) {
     constexpr int BLOCKS = DC / BLOCK;
@@ -128,8 +129,9 @@ template <int DC, int BLOCK> struct PartLayout {
   }
 };
 
-// Adds the parts of every row of the tiles that were cut up, in their order, and rounds.  Blocks of the keys role first, dk and dv of a tile
-// side by side, then those of the queries role.  The parts' reading bounds it: 63 MB (40 heads of 32760 on 512) 15.6 us, 38 MB (fp32, 16 heads of 1024 at head_dim 72) 8.2.
+// Adds the parts of every row of the tiles that were cut up, in their order, and rounds.  Blocks of the keys role first, dk and dv of a
+// tile side by side, then those of the queries role.  The parts' reading bounds it: 63 MB (40 heads of 32760 on 512) 15.6 us, 38 MB (fp32,
+// 16 heads of 1024 at head_dim 72) 8.2.
 template <typename T, int DC, int BLOCK>
 __global__ __launch_bounds__(256) void bwd_fold_kernel(const AttnBwdParams p) {
   typedef __attribute__((ext_vector_type(4))) T vec4;

@@ -1,11 +1,12 @@
 // The norm of a list of gradients, and their clipping:  norm = (sum |g|^p)^(1/p) or max |g|,  g <- g min(1, max_norm / (norm + 1e-6)).
 //
-// Memory decides both: every element is read once for the norm, read and written once for the clipping.  A workgroup takes a chunk of
-// one tensor and finds it by comparing its number with all first chunks at once (they are kernel arguments).  Sums are in 64
-// bits from the first square on (a square of a bf16 or fp32 gradient can leave fp32's range, and 1e9 of them its precision); the conversion
-// to it and the multiply-add take about half of the time that a compute unit waits for the element.  Partial sums are added by one workgroup, in a fixed order.
-// Measured: the norm of 0.89 GB of bf16 136 us (6.6 TB/s), of 2.0 GB of fp32 322 us (6.1); clipping 0.8 GB of bf16 into fp32 474 us, 2.0 GB of fp32 in place 769 us (5.1 either; a copy of
-// 1 GiB: 5.0).  Small lists are the host's: 84 tensors take 13.2 us a norm, 6 of them in the kernel.
+// Memory decides both: every element is read once for the norm, read and written once for the clipping.  A workgroup takes a chunk of one
+// tensor and finds it by comparing its number with all first chunks at once (they are kernel arguments).  Sums are in 64 bits from the
+// first square on (a square of a bf16 or fp32 gradient can leave fp32's range, and 1e9 of them its precision); the conversion to it and the
+// multiply-add take about half of the time that a compute unit waits for the element.  Partial sums are added by one workgroup, in a fixed
+// order. Measured, a call among others: the norm of 0.89 GB of bf16 143 us (6.2 TB/s; the kernels alone 140), of 2.0 GB of fp32 312 us in
+// the kernel (6.3); clipping by it 0.8 GB of bf16 into fp32 475 us, 2.0 GB of fp32 in place 768 us (5.1 either; a copy of 1 GiB: 5.0).
+// Small lists are the host's: 84 tensors take 18 us a norm, 6 of them in the kernel.
 #include "grad_norm.h"
 #include "launchers.h"
 #include "row_ops.h"
@@ -38,8 +39,8 @@ __device__ __forceinline__ Raw8<T> stream_raw8(const T* p, int64_t off) {
   for (int i = 0; i < Raw8<T>::N; i++) r.x[i] = __builtin_nontemporal_load(v + i);
   return r;
 }
-// Groups of eight that a thread asks for at a time: 128 bytes (half of that: 152 us for 0.9 GB of bf16 where this takes 147; twice that: 2 GB of fp32 and their clipping
-// 1206 us, with this 1090).
+// Groups of eight that a thread asks for at a time: 128 bytes (half of that: 152 us for 0.9 GB of bf16 where this takes 147; twice that: 2
+// GB of fp32 and their clipping 1206 us, with this 1090).
 template <typename T> constexpr int kGroups = 16 / sizeof(T);
 
 template <int KIND>
@@ -62,8 +63,8 @@ __device__ __forceinline__ double workgroup_join(double v) {
   return v;
 }
 
-// The norm of n partial values, for thread 0 of 256 or (more than kClipPartials of them: four loads of each thread in flight; 7084 took 8.1 us with 256
-// threads and a load at a time) 1024; up to that count in the same order either way.
+// The norm of n partial values, for thread 0 of 256 or (more than kClipPartials of them: four loads of each thread in flight; 7084 took 8.1
+// us with 256 threads and a load at a time) 1024; up to that count in the same order either way.
 template <int KIND, int THREADS, class Load>
 __device__ __forceinline__ float norm_of(Load load, int64_t n) {
   double v = 0.;
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const NormParams p) {
     if (threadIdx.x == 0) p.partial[blockIdx.x] = v;
     return;
   }
-  // The last workgroup to get here adds the sums up, which spares a small list the second launch (84 tensors: 16.5 -> 13.2 us a call, the host's).  Its
+  // The last workgroup to get here adds the sums up, which spares a small list the second launch (84 tensors: 3.3 us a call less, the host's).  Its
   // accesses are device-scope ones, past the XCDs' caches; every workgroup waits for its store before it counts itself.
   __shared__ bool latest;
   if (threadIdx.x == 0) {
@@ -154,8 +155,9 @@ __global__ __launch_bounds__(1024) void grad_norm_total_kernel(const double* par
 }
 
 // A list of few chunks saves the launch between the norm and this one: every workgroup adds the partial sums up (84 tensors of a model's
-// gains: 6.5 us of host time less a call than with a launch of its own for the sum and a C call of its own for the norm).  Taking the chunks from the last to
-// the first, so that what the norm read last might still be in the memory-side cache, changed nothing (1097 us for 2 GB).
+// gains: 6.5 us of host time less a call than with a launch of its own for the sum and a C call of its own for the norm).  Taking the
+// chunks from the last to the first, so that what the norm read last might still be in the memory-side cache, changed nothing (1097 us for
+// 2 GB).
 template <typename S, typename D>
 __global__ __launch_bounds__(256) void grad_clip_kernel(const ClipParams p) {
   float norm;

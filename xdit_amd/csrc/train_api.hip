@@ -50,17 +50,17 @@ struct Places {
   double end() const { return g[used - 1].time; }
 };
 
-// Microseconds that a launch takes.  A unit's step (64 streamed rows; fp32: 32) takes `shared` beside the others that a compute unit holds and `alone`
-// where no compute unit has more than one; `fixed` are its operands, first tile and results.  Partial results are read back at 5 TB/s by a launch of 4 us
-// (they are written while other units compute).
+// Microseconds that a launch takes.  A unit's step (64 streamed rows; fp32: 32) takes `shared` beside the others that a compute unit holds
+// and `alone` where no compute unit has more than one; `fixed` are its operands, first tile and results.  Partial results are read back at
+// 5 TB/s by a launch of 4 us (they are written while other units compute).
 struct StepCost {
   double alone[2], shared[2];   // keys, queries
   double fixed[2];
   double part;                  // of a tensor's partial tile
 };
 
-// Where every unit has a place at once: the units of a compute unit are those whose numbers differ by the number of compute units, and what they do adds up, less
-// what they gain by running beside each other.
+// Where every unit has a place at once: the units of a compute unit are those whose numbers differ by the number of compute units, and what
+// they do adds up, less what they gain by running beside each other.
 double one_round_us(const xdit::BwdRole& k, const xdit::BwdRole& q, int64_t cus, int per_cu, const StepCost& c) {
   struct Group { int64_t end; double work, fixed; } g[4];
   int n = 0;
@@ -184,8 +184,9 @@ BwdPlan plan_bwd(const xdit_attn_bwd_args* a, xdit::AttnBwdParams& p) {
     r->per_xcd = (r->total + 7) / 8;
     set_parts(*r, r->per_xcd, 1);
   }
-  // measured: 8 and 16 heads of 16384 rows on 4096 and of 4096 on 16384, 8 to 48 of 2048 on 2048 and 4096, 3 of 1536 on 1536; fp32: 8 and 16 of 4096 at head_dims 64, 72 and 128, whose steps
-  // take what their matrix instructions do (over the columns that are contracted and those of the gradients)
+  // measured: 8 and 16 heads of 16384 rows on 4096 and of 4096 on 16384, 8 to 48 of 2048 on 2048 and 4096, 3 of 1536 on 1536; fp32: 8 and
+  // 16 of 4096 at head_dims 64, 72 and 128, whose steps take what their matrix instructions do (over the columns that are contracted and
+  // those of the gradients)
   StepCost cost = a->D <= 64 ? StepCost{{1.15, 1.0}, {2.99, 2.35}, {6.0, 5.0}, 0.0} : StepCost{{1.95, 1.62}, {3.56, 2.8}, {7.0, 5.5}, 0.0};
   if (f32) {
     const int contracted = 8 * xdit::bwd_f32_groups(a->D);
@@ -255,9 +256,9 @@ Rows rows_of(const void* p, int64_t B, int64_t H, int64_t S, const xdit_strides&
   return {reinterpret_cast<uintptr_t>(p), width * es, {{B, st.b * es}, {H, st.h * es}, {S, st.s * es}}};
 }
 
-// Whether a row of x and one of y share a byte: whether a sum of steps, at most those between two rows of either, leads from x to within a row of y.  Steps are
-// taken from the largest stride down, those only from which the smaller ones still reach: one or two a stride where rows lie as those of views of one buffer do.
-// Where they lie otherwise and 4096 sums were looked at, the answer is that they may.
+// Whether a row of x and one of y share a byte: whether a sum of steps, at most those between two rows of either, leads from x to within a
+// row of y.  Steps are taken from the largest stride down, those only from which the smaller ones still reach: one or two a stride where
+// rows lie as those of views of one buffer do. Where they lie otherwise and 4096 sums were looked at, the answer is that they may.
 bool share_bytes(const Rows& x, const Rows& y) {
   if ((__int128)x.at >= y.end() || (__int128)y.at >= x.end()) return false;
   struct Step { __int128 stride; int64_t least, most; } step[6];
@@ -376,7 +377,8 @@ int64_t chunk_elements(int64_t count, const int64_t* numel) {
 }
 int64_t chunks_of(int64_t numel, int64_t chunk) { return numel == 0 ? 0 : (numel + 7 + chunk - 1) / chunk; }   // up to 7 elements before its aligned start
 
-// The launches that leave a partial value of every chunk; their count, or a negative status.  With a counter and a norm there is one launch, which leaves the norm too.
+// The launches that leave a partial value of every chunk; their count, or a negative status.  With a counter and a norm there is one
+// launch, which leaves the norm too.
 int64_t launch_partials(int64_t count, const void* const* data, const int64_t* numel, const int32_t* dtypes, int kind, double* partial, hipStream_t stream,
                         unsigned* counter = nullptr, float* norm = nullptr) {
   const int64_t chunk = chunk_elements(count, numel);
@@ -419,7 +421,8 @@ int64_t partials_of(int64_t count, const int64_t* numel) {
   return n;
 }
 
-// Whether the norm of a list is one launch's, and its last workgroup can add the partial sums up: tensors of one dtype, as many as a launch takes, few chunks.
+// Whether the norm of a list is one launch's, and its last workgroup can add the partial sums up: tensors of one dtype, as many as a launch
+// takes, few chunks.
 bool one_launch(int64_t count, const int64_t* numel, const int32_t* dtypes, int64_t partials) {
   int64_t tensors = 0;
   int dtype = -1;
