@@ -17,7 +17,7 @@
 // in the queries role, with four 3596, 24 heads of 4250 x 2 at head_dim 64 1010 and 877 us in both.
 //
 // The matrix rate under the power limit bounds long rows: bf16, 5 heads of 32760 at head_dim 128 take 7.6 to 7.8 ms, 1.23 to 1.27 PFLOP/s
-// over the seven products where a library product of 8192^3 reaches 1.33 (matrix pipe busy 68 % at 1.7 GHz, no LDS bank conflicts); 24
+// over the seven products where a library product of 8192^3 reaches 1.33 (matrix pipe busy 65 % at 1.7 GHz, no LDS bank conflicts); 24
 // heads of 4608 769 to 800 us, 1.14 to 1.19. fp16, 48 heads of 4250 at head_dim 64: 778 to 805 us.
 //
 // MFMA orientation (v_mfma_f32_32x32x16; A is 32x16, B is 16x32, lane l holds row/column l%32 and contraction elements
