@@ -488,7 +488,7 @@ int64_t xdit_grad_norm_workspace_bytes(const xdit_grad_norm_args* args);  /* fro
 /*
  * Clipping by the gradients' own norm, or by one that is in device memory (e.g. of those of every rank):
  *     dst = src * min(1, max_norm / (norm + 1e-6))
- * in fp32, rounded once.  dst may be src itself; otherwise no dst may overlap another dst, a src or the norm.  Where the factor is 1 a dst
+ * in fp32, rounded once.  dst may be src itself; otherwise no dst may overlap another dst, a src or the norm, nor norm_out a src.  Where the factor is 1 a dst
  * that is its src is left as it is.  The tables are HOST arrays, read before the call returns.
  */
 typedef struct {

@@ -440,7 +440,7 @@ int check_partials(int64_t n, const void* workspace, int64_t bytes) {
   return 0;
 }
 
-// Whether no destination overlaps another one, a source other than itself, or the norm.
+// Whether no destination overlaps another one, a source other than itself, or the norm, and a norm that is written no source.
 bool destinations_apart(const xdit_clip_grads_args* a) {
   struct Span { uintptr_t begin, end; int64_t i; };
   std::vector<Span> dst;
@@ -450,14 +450,15 @@ bool destinations_apart(const xdit_clip_grads_args* a) {
   std::sort(dst.begin(), dst.end(), [](const Span& x, const Span& y) { return x.begin < y.begin; });
   for (size_t n = 1; n < dst.size(); n++)
     if (dst[n].begin < dst[n - 1].end) return false;
+  const uintptr_t norm = reinterpret_cast<uintptr_t>(a->norm != nullptr ? a->norm : a->norm_out);   // every workgroup reads it, or one writes it while others read gradients
   for (int64_t i = 0; i < a->count; i++) {
     if (a->numel[i] == 0) continue;
     const uintptr_t begin = reinterpret_cast<uintptr_t>(a->src[i]), end = begin + a->numel[i] * size_of(a->src_dtype[i]);
+    if (a->norm == nullptr && norm < end && norm + sizeof(float) > begin) return false;
     auto at = std::upper_bound(dst.begin(), dst.end(), begin, [](uintptr_t x, const Span& s) { return x < s.end; });   // the first that ends behind the source's start
     for (; at != dst.end() && at->begin < end; ++at)
       if (at->i != i || at->begin != begin || a->src_dtype[i] != a->dst_dtype[i]) return false;
   }
-  const uintptr_t norm = reinterpret_cast<uintptr_t>(a->norm != nullptr ? a->norm : a->norm_out);   // every workgroup reads it
   auto at = std::upper_bound(dst.begin(), dst.end(), norm, [](uintptr_t x, const Span& s) { return x < s.end; });
   return at == dst.end() || at->begin >= norm + sizeof(float);
 }
